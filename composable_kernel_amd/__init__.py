@@ -13,4 +13,5 @@ from .device_ops import (  # noqa: F401
     DeviceConv2dFwdInt8, DeviceConv2dFwdMultipleDInt8, DeviceConv2dFwdF16,
     DeviceConvNdFwdInt8, DeviceConvNdFwdF16,
     DeviceConv2dFwdBiasActivationF16, DeviceBatchedGemmGemmF16, DeviceBatchedGemmSoftmaxGemmF16,
+    KvCache8, DeviceBlockQuantizeF8, DeviceGemmBlockScaleF8, DeviceKvCacheTables, DeviceKvCacheStore8, DevicePagedAttention8,
 )

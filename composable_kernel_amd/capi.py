@@ -20,6 +20,7 @@ EPI_BILINEAR, EPI_ADD_ADD_FASTGELU = 8, 9    # fp16 GEMM: alpha * acc + beta * d
 (OP_GEMM_I8, OP_GEMM_F16, OP_CONV2D_FWD_I8, OP_CONV2D_FWD_F16, OP_BATCHED_GEMM_GEMM, OP_GEMM_SPLITK, OP_GEMM_BF16,
  OP_BATCHED_GEMM_SOFTMAX_GEMM) = range(8)
 INSTANCE_AUTO = -1
+TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_E4M3, TYPE_I8 = range(5)   # CKX_TYPE_*: the 8-bit serving operators
 STATIC_WORKSPACE_BYTES = 32 * 1024 * 1024   # CKX_STATIC_WORKSPACE_BYTES
 
 # every symbol include/ckx.h declares
@@ -36,6 +37,10 @@ SYMBOLS = [
     "ckx_convnd_fwd_is_supported", "ckx_convnd_fwd", "ckx_convnd_fwd_workspace_bytes",
     "ckx_batched_gemm_gemm_f16_is_supported", "ckx_batched_gemm_gemm_f16", "ckx_time_launches",
     "ckx_batched_gemm_softmax_gemm_f16_is_supported", "ckx_batched_gemm_softmax_gemm_f16",
+    "ckx_quantize_blocks_f8_is_supported", "ckx_quantize_blocks_f8",
+    "ckx_gemm_f8_blockscale_is_supported", "ckx_gemm_f8_blockscale", "ckx_gemm_f8_blockscale_workspace_bytes",
+    "ckx_kv_cache_tables_is_supported", "ckx_kv_cache_tables", "ckx_kv_cache_store8_is_supported", "ckx_kv_cache_store8",
+    "ckx_paged_attention8_is_supported", "ckx_paged_attention8", "ckx_paged_attention8_workspace_bytes",
     "ckx_gemm_plan", "ckx_conv2d_fwd_plan", "ckx_set_forced_k_runs", "ckx_set_big_tile_waves",
 ]
 
@@ -59,6 +64,13 @@ class ConvNdDesc(C.Structure):
         arr = lambda v: (C.c_int32 * 3)(*([int(x) for x in v] + [0] * (3 - nd)))
         return cls(nd, int(N), int(K), int(C_), arr(in_len), arr(filt), arr(out_len), arr(strides), arr(dilations),
                    arr(left_pads), arr(right_pads))
+
+
+class KvCache8Desc(C.Structure):
+    """ckx_kv_cache8"""
+    _fields_ = [("p_k", C.c_void_p), ("p_v", C.c_void_p), ("p_k_scale", C.c_void_p), ("p_v_scale", C.c_void_p)] + [
+        (n, C.c_int32) for n in ("type", "num_blocks", "block_size", "num_heads", "head_dim", "stride_head", "stride_token",
+                                 "stride_scale")] + [("stride_block", C.c_int64)]
 
 
 LAUNCH_FN = C.CFUNCTYPE(C.c_int, C.c_void_p)
@@ -140,6 +152,24 @@ def lib():
     gsg = [i32] * 9 + [i64] * 4 + [f32, C.c_int, C.c_int]
     L.ckx_batched_gemm_softmax_gemm_f16_is_supported.argtypes = gsg
     L.ckx_batched_gemm_softmax_gemm_f16.argtypes = [vp] * 4 + gsg + [vp]
+    quant = [i32] * 6 + [C.c_int]
+    L.ckx_quantize_blocks_f8_is_supported.argtypes = quant
+    L.ckx_quantize_blocks_f8.argtypes = [vp] * 3 + quant + [vp]
+    f8 = [i32] * 10 + [C.c_int]
+    L.ckx_gemm_f8_blockscale_is_supported.argtypes = f8
+    L.ckx_gemm_f8_blockscale.argtypes = [vp] * 5 + f8 + [vp, i64, vp]
+    L.ckx_gemm_f8_blockscale_workspace_bytes.restype = i64
+    L.ckx_gemm_f8_blockscale_workspace_bytes.argtypes = [i32] * 3
+    L.ckx_kv_cache_tables_is_supported.argtypes = [i32] * 6
+    L.ckx_kv_cache_tables.argtypes = [vp] * 8 + [i32] * 6 + [vp]
+    kvp = C.POINTER(KvCache8Desc)
+    L.ckx_kv_cache_store8_is_supported.argtypes = [kvp] + [i32] * 5 + [C.c_int]
+    L.ckx_kv_cache_store8.argtypes = [vp] * 3 + [kvp] + [i32] * 5 + [C.c_int, vp]
+    attn = [kvp] + [i32] * 10 + [f32, C.c_int, C.c_int]
+    L.ckx_paged_attention8_is_supported.argtypes = attn
+    L.ckx_paged_attention8.argtypes = [vp] * 5 + attn + [vp, i64, vp]
+    L.ckx_paged_attention8_workspace_bytes.restype = i64
+    L.ckx_paged_attention8_workspace_bytes.argtypes = [kvp] + [i32] * 5
     L.ckx_time_launches.argtypes = [LAUNCH_FN, vp, C.c_int, C.c_int, vp, C.POINTER(C.c_float)]
     ip = C.POINTER(C.c_int)
     L.ckx_gemm_plan.argtypes = [C.c_int] + shape + [C.c_int, i32, i64, ip, ip]

@@ -10,6 +10,7 @@
 #include <mutex>
 #include <string>
 
+#include "api_error.hpp"
 #include "ckx.h"
 #include "gemm_tile.hpp"
 #include "tile_launch.hpp"
@@ -1423,6 +1424,11 @@ int auto_conv3d_window(int op, const ckx_convnd_desc* d)
     ConvWindowArgs w;
     return conv_window_shape(es, d, pl, w);
 }
+} // namespace ckx
+
+namespace ckx {
+int api_fail(int code, const char* msg) { return ::fail(code, msg); }
+int api_hip_fail(hipError_t e, const char* what) { return ::hip_fail(e, what); }
 } // namespace ckx
 
 extern "C" {

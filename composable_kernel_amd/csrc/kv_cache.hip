@@ -1,0 +1,264 @@
+// The cache of 8-bit blocks: tables of a step from the requests' lengths, and the store of new tokens (formulas:
+// include/ckx.h, ckx_kv_cache_tables and ckx_kv_cache_store8).
+#include "f8.hpp"
+#include "serving.hpp"
+
+namespace ckx {
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------------- tables
+// One launch: every workgroup sums the lengths of all sequences for itself (8 bytes a sequence, out of L2 after the first
+// workgroup; 8192 at most, their two running sums in LDS), then takes its share of the tokens and of the new blocks and finds
+// the sequence of each by bisection. The alternative, one workgroup that sums and a second launch that fills, costs the second
+// launch. What bounds it is that latency: the bytes are few.
+constexpr int kTablesThreads = 256, kTokensPerGroup = 1024;
+
+__device__ __forceinline__ int blocks_of(int tokens, int shift) { return (int)(((int64_t)tokens + (1 << shift) - 1) >> shift); }
+
+// the last b in [0, n) with sums[b] <= x (sums ascending, sums[0] <= x)
+__device__ __forceinline__ int last_at_most(const int* sums, int n, int x)
+{
+    int lo = 0, hi = n;
+    while(hi - lo > 1)
+    {
+        const int mid = (lo + hi) >> 1;
+        if(sums[mid] <= x)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
+__global__ __launch_bounds__(kTablesThreads) void kv_tables_kernel(TablesArgs p)
+{
+    __shared__ int cu[kMaxTableSequences + 1], base[kMaxTableSequences + 1];
+    __shared__ int part[2][kTablesThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // a thread's stretch of sequences: its own sums, then those of the threads before it
+    const int per = (p.batch + kTablesThreads - 1) / kTablesThreads;
+    const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
+    int tokens = 0, blocks = 0;
+    for(int b = b0; b < b1; ++b)
+    {
+        const int c = max(p.context[b], 0), n = max(p.fresh[b], 0);
+        cu[b] = tokens, base[b] = blocks;
+        tokens += n;
+        blocks += blocks_of(c + n, p.block_shift) - blocks_of(c, p.block_shift);
+        if(blockIdx.x == 0)
+            p.kv_lens[b] = c + n;
+    }
+    int t = tokens, k = blocks;
+    for(int d = 1; d < 64; d *= 2)
+    {
+        const int tt = __shfl_up(t, d), kk = __shfl_up(k, d);
+        if(lane >= d)
+            t += tt, k += kk;
+    }
+    if(lane == 63)
+        part[0][wave] = t, part[1][wave] = k;
+    __syncthreads();
+    int t0 = t - tokens, k0 = k - blocks, all_tokens = 0, all_blocks = 0;
+    for(int w = 0; w < kTablesThreads / 64; ++w)
+    {
+        if(w < wave)
+            t0 += part[0][w], k0 += part[1][w];
+        all_tokens += part[0][w], all_blocks += part[1][w];
+    }
+    for(int b = b0; b < b1; ++b)
+    {
+        cu[b] += t0, base[b] += k0;
+        if(blockIdx.x == 0)
+            p.cu[b] = cu[b];
+    }
+    if(tid == 0)
+    {
+        cu[p.batch] = all_tokens, base[p.batch] = all_blocks;
+        if(blockIdx.x == 0)
+            p.cu[p.batch] = all_tokens, p.used[0] = all_blocks;
+    }
+    __syncthreads();
+
+    // the table's new columns: new block f of all belongs to sequence b
+    for(int f = blockIdx.x * kTablesThreads + tid; f < all_blocks && f < p.num_free; f += gridDim.x * kTablesThreads)
+    {
+        const int b   = last_at_most(base, p.batch, f);
+        const int col = blocks_of(max(p.context[b], 0), p.block_shift) + f - base[b];
+        if(col < p.max_blocks)
+            p.table[(int64_t)b * p.stride_table + col] = p.free[f];
+    }
+    // the slots; a new block comes from the free list itself, not from the table that another workgroup is writing
+    for(int i = 0; i < kTokensPerGroup / kTablesThreads; ++i)
+    {
+        const int x = blockIdx.x * kTokensPerGroup + i * kTablesThreads + tid;
+        if(x >= p.num_slots)
+            break;
+        int slot = -1;
+        if(x < all_tokens)
+        {
+            const int b = last_at_most(cu, p.batch, x);
+            const int c = max(p.context[b], 0), pos = c + x - cu[b], col = pos >> p.block_shift;
+            const int had = blocks_of(c, p.block_shift);
+            int block     = -1;
+            if(col < p.max_blocks)
+            {
+                if(col < had)
+                    block = p.table[(int64_t)b * p.stride_table + col];
+                else if(base[b] + col - had < p.num_free)
+                    block = p.free[base[b] + col - had];
+            }
+            if(block >= 0)
+                slot = (block << p.block_shift) + (pos & ((1 << p.block_shift) - 1));
+        }
+        p.slots[x] = slot;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- store
+// One wave takes a run (the new tokens of one block) of one head, keys or values: a pass for the maximum, the block's scale,
+// the older codes if the scale grew, and a pass that writes the codes; the second pass finds its 4 ... 32 KB in the caches. Which runs begin among a wave's
+// `span` tokens comes out of one comparison of neighbouring slots, so that no list of runs is needed. Memory bounds it
+// (2 bytes read, 1 written per element); few tokens, latency.
+template <typename T, int CODE>
+__global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs p, int span)
+{
+    const int lane  = threadIdx.x & 63;
+    const int64_t u = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int first = (int)(u * span);
+    if(u * span >= p.tokens)
+        return;
+    const int head   = blockIdx.y >> 1;
+    const bool value = blockIdx.y & 1;
+    const int shift = p.block_shift, size = 1 << shift;
+    const int64_t slots = (int64_t)p.cache.num_blocks << shift;
+    const T* x          = reinterpret_cast<const T*>(value ? p.v : p.k) + (int64_t)head * (value ? p.sv_h : p.sk_h);
+    const int64_t xt    = value ? p.sv_t : p.sk_t;
+    uint8_t* codes      = reinterpret_cast<uint8_t*>(value ? p.cache.p_v : p.cache.p_k) + (int64_t)head * p.cache.stride_head;
+    float* scales       = (value ? p.cache.p_v_scale : p.cache.p_k_scale) + head;
+    // block of token t's slot, -1 for a token that is skipped or not there
+    auto block_of = [&](int64_t t) {
+        if(t < 0 || t >= p.tokens)
+            return -1;
+        const int s = p.slots[t];
+        return s < 0 || s >= slots ? -1 : s >> shift;
+    };
+    const int own  = lane < span ? block_of((int64_t)first + lane) : -1;
+    uint64_t leads = __ballot(own >= 0 && own != block_of((int64_t)first + lane - 1));
+
+    const int per_token = p.cache.head_dim >> 3;      // lanes of eight elements
+    const int at_once   = 64 / per_token;             // tokens
+    const int my = lane / per_token, d = (lane - my * per_token) * 8;
+    const bool active = my < at_once;
+    while(leads)
+    {
+        const int i = __builtin_ctzll(leads);
+        leads &= leads - 1;
+        const int64_t t0 = (int64_t)first + i;
+        const int block  = __builtin_amdgcn_readfirstlane(__shfl(own, i));
+        const int begin  = p.slots[t0] & (size - 1);
+        int count        = 0; // tokens of the run, at most a block's
+        for(; count < size; count += 64)
+        {
+            const uint64_t out = __ballot(block_of(t0 + count + lane) != block);
+            if(out)
+            {
+                count += __builtin_ctzll(out);
+                break;
+            }
+        }
+        count = min(count, size);
+
+        float amax = kTinyAmax;
+        bool nan   = false;
+#pragma unroll 4
+        for(int n = 0; n < count; n += at_once)
+            if(active && n + my < count)
+            {
+                float v[8];
+                load8(x + (t0 + n + my) * xt + d, v);
+#pragma unroll
+                for(int j = 0; j < 8; ++j)
+                {
+                    amax = __builtin_fmaxf(amax, __builtin_fabsf(v[j]));
+                    nan |= v[j] != v[j];
+                }
+            }
+        for(int s = 1; s < 64; s *= 2)
+            amax = __builtin_fmaxf(amax, __shfl_xor(amax, s));
+        const float fresh = __any(nan) ? __builtin_nanf("") : amax / (CODE == CODE_E4M3 ? kE4m3Max : kI8Max);
+        float* const at   = scales + (int64_t)block * p.cache.stride_scale;
+        uint8_t* const to = codes + (int64_t)block * p.cache.stride_block;
+        float now         = fresh;
+        auto put = [&](int token, const float(&v)[8]) { // (a NaN has no code: the scale says it)
+            float w[8];
+#pragma unroll
+            for(int j = 0; j < 8; ++j)
+                w[j] = v[j] == v[j] ? v[j] : 0.0f;
+            *reinterpret_cast<u32x2*>(to + (int64_t)token * p.cache.stride_token + d) =
+                u32x2{codes_of<CODE>(w[0], w[1], w[2], w[3]), codes_of<CODE>(w[4], w[5], w[6], w[7])};
+        };
+        if(begin > 0)
+        {
+            const float old = *at;
+            now             = old != old || old >= fresh ? old : fresh;
+            if(now != old)
+            {
+                const float ratio = old / now;
+                for(int n = 0; n < begin; n += at_once)
+                    if(active && n + my < begin)
+                    {
+                        const u32x2 c = *reinterpret_cast<const u32x2*>(to + (int64_t)(n + my) * p.cache.stride_token + d);
+                        float v[8];
+#pragma unroll
+                        for(int j = 0; j < 8; ++j)
+                            v[j] = code_value<CODE>(c[j >> 2], j & 3) * ratio;
+                        put(n + my, v);
+                    }
+            }
+        }
+        if(lane == 0)
+            *at = now;
+        const float inv = 1.0f / now;
+#pragma unroll 4
+        for(int n = 0; n < count; n += at_once)
+            if(active && n + my < count)
+            {
+                float v[8];
+                load8(x + (t0 + n + my) * xt + d, v);
+#pragma unroll
+                for(int j = 0; j < 8; ++j)
+                    v[j] *= inv;
+                put(p.slots[t0 + n + my] & (size - 1), v);
+            }
+    }
+}
+
+template <typename T, int CODE>
+hipError_t launch_store(const StoreArgs& a, hipStream_t s)
+{
+    // tokens a wave looks at: one where the tokens are few (each its own run: a step's), 16 where they are many
+    const int span      = a.tokens <= 2048 ? 1 : 16;
+    const int64_t units = ((int64_t)a.tokens + span - 1) / span;
+    hipLaunchKernelGGL((kv_store_kernel<T, CODE>), dim3((unsigned)((units + 3) / 4), (unsigned)a.cache.num_heads * 2), dim3(256), 0, s,
+                       a, span);
+    return hipGetLastError();
+}
+
+} // namespace
+
+hipError_t kv_tables_launch(const TablesArgs& a, hipStream_t s)
+{
+    const int64_t groups = ((int64_t)a.num_slots + kTokensPerGroup - 1) / kTokensPerGroup;
+    hipLaunchKernelGGL(kv_tables_kernel, dim3((unsigned)(groups > 0 ? groups : 1)), dim3(kTablesThreads), 0, s, a);
+    return hipGetLastError();
+}
+
+hipError_t kv_store_launch(const StoreArgs& a, int x_type, hipStream_t s)
+{
+    if(a.cache.type == CKX_TYPE_E4M3)
+        return x_type == CKX_TYPE_F16 ? launch_store<_Float16, CODE_E4M3>(a, s) : launch_store<__bf16, CODE_E4M3>(a, s);
+    return x_type == CKX_TYPE_F16 ? launch_store<_Float16, CODE_I8>(a, s) : launch_store<__bf16, CODE_I8>(a, s);
+}
+
+} // namespace ckx

@@ -1,0 +1,375 @@
+// Attention over the 8-bit cache for few query rows per sequence (single tokens, a handful): the cache is read once, straight
+// into registers.
+//
+// One workgroup takes 16 query rows (the heads of one group, times as many tokens as fit) and a share of the cached tokens; its
+// four waves take 32 tokens each in turn with running maxima and sums of their own and are joined through LDS at the end.
+// Shares of one row are joined by a second launch.
+//   scores   S^T = K Q^T, v_mfma_f32_16x16x32: lane (row l % 16 of q, g = l / 16) gets tokens 4g .. 4g + 3 of each 16
+//   output   O^T = V^T P^T, the same instruction over 32 tokens: the lane's own probabilities are its operand, so V's lanes take tokens
+//            {4g .. 4g + 3, 16 + 4g .. + 3} as well, eight (four) neighbouring elements of d each, transposed by byte permutes
+//            in registers. MFMA j's row c stands for element c * E + j (E elements a lane): the lane ends with a contiguous
+//            stretch of the output row.
+// What bounds it is the cache's bytes: 64 bytes a lane and 16 tokens are on their way while the last ones are multiplied.
+#include "paged_attention.hpp"
+
+namespace ckx {
+
+namespace {
+
+constexpr int kWaves = 4;
+
+// 8 (4) bytes of each of four tokens -> per element the four tokens' bytes
+__device__ __forceinline__ void transpose4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t (&o)[4])
+{
+    const uint32_t ab0 = __builtin_amdgcn_perm(b, a, 0x05010400u), ab1 = __builtin_amdgcn_perm(b, a, 0x07030602u);
+    const uint32_t cd0 = __builtin_amdgcn_perm(d, c, 0x05010400u), cd1 = __builtin_amdgcn_perm(d, c, 0x07030602u);
+    o[0] = __builtin_amdgcn_perm(cd0, ab0, 0x05040100u), o[1] = __builtin_amdgcn_perm(cd0, ab0, 0x07060302u);
+    o[2] = __builtin_amdgcn_perm(cd1, ab1, 0x05040100u), o[3] = __builtin_amdgcn_perm(cd1, ab1, 0x07060302u);
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4 mfma_qk(const i32x4& k, const i32x4& q, const f32x4& c)
+{
+    if constexpr(std::is_same<T, __bf16>::value)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, k), __builtin_bit_cast(f16x8, q), c, 0, 0, 0);
+}
+
+// DP: head_dim rounded up to 64 or 128
+template <typename T, int CODE, int DP>
+__global__ __launch_bounds__(kWaves * 64) void attention_rows_kernel(AttentionArgs p)
+{
+    constexpr int KJ = DP / 64;  // 16-byte loads of a key row's lane
+    constexpr int E  = DP / 16;  // elements of a value row's lane
+    __shared__ float part[kWaves][16][DP + 4];
+    __shared__ float part_m[kWaves][16], part_l[kWaves][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const int D = p.cache.head_dim;
+
+    int id           = blockIdx.x;
+    const int split  = id % p.splits;
+    id /= p.splits;
+    const int head_tile = id % (p.cache.num_heads * p.head_tiles);
+    const TileOf tile   = tile_of(p, id / (p.cache.num_heads * p.head_tiles));
+    if(!tile.live)
+        return;
+    const int kvh = head_tile / p.head_tiles, h0 = (head_tile - kvh * p.head_tiles) * p.tile_heads;
+    // the lane's query row
+    const int rt = r / p.tile_heads, rh = h0 + (r - rt * p.tile_heads);
+    const bool row_live = rt < p.tile_tokens && tile.first + rt < tile.q_len && rh < p.group;
+    const int head      = kvh * p.group + rh;
+    const int64_t token = tile.q0 + tile.first + rt;
+    const int behind    = tile.q_len - 1 - (tile.first + rt); // query tokens behind the row's
+    const int see       = row_live ? (p.causal ? tile.kv - behind : tile.kv) : 0;
+    const int last      = min(tile.first + p.tile_tokens, tile.q_len) - 1;
+    const int most      = max(p.causal ? tile.kv - (tile.q_len - 1 - last) : tile.kv, 0); // what the tile's furthest row sees
+
+    // the share: whole steps of 32 tokens
+    const int steps = (most + 31) / 32, per = (steps + p.splits - 1) / p.splits;
+    const int step0 = min(split * per, steps), step1 = min(step0 + per, steps);
+
+    i32x4 qf[KJ][2];
+#pragma unroll
+    for(int j = 0; j < KJ; ++j)
+#pragma unroll
+        for(int h = 0; h < 2; ++h)
+        {
+            const int d = 64 * j + 16 * g + 8 * h;
+            qf[j][h]    = i32x4{0, 0, 0, 0};
+            if(row_live && d < D)
+                qf[j][h] = *reinterpret_cast<const i32x4*>(reinterpret_cast<const T*>(p.q) + token * p.sq_t + (int64_t)head * p.sq_h + d);
+        }
+
+    f32x4 acc[E];
+#pragma unroll
+    for(int j = 0; j < E; ++j)
+        acc[j] = f32x4{0, 0, 0, 0};
+    float m = -__builtin_inff(), l = 0.0f;
+    ValueScale unit;
+
+    const int* const table   = p.table + (int64_t)tile.b * p.stride_table;
+    const uint8_t* const kc  = reinterpret_cast<const uint8_t*>(p.cache.p_k) + (int64_t)kvh * p.cache.stride_head;
+    const uint8_t* const vc  = reinterpret_cast<const uint8_t*>(p.cache.p_v) + (int64_t)kvh * p.cache.stride_head;
+    const int in_block       = (1 << p.block_shift) - 1;
+
+    for(int step = step0 + wave; step < step1; step += kWaves)
+    {
+        const int t0 = step * 32;
+        u32x4 kb[2][KJ];
+        uint32_t vb[8][E / 4];
+        float ks[2], vs[2];
+        bool there[2];
+#pragma unroll
+        for(int h = 0; h < 2; ++h)
+        {
+            const int t   = t0 + 16 * h; // (16 tokens lie in one block)
+            int block     = t < most ? table[t >> p.block_shift] : -1;
+            there[h]      = block >= 0 && block < p.cache.num_blocks;
+            block         = there[h] ? block : 0;
+            const int64_t at = (int64_t)block * p.cache.stride_block;
+            ks[h] = vs[h] = 0.0f;
+            if(there[h])
+            {
+                ks[h] = p.cache.p_k_scale[(int64_t)block * p.cache.stride_scale + kvh];
+                vs[h] = p.cache.p_v_scale[(int64_t)block * p.cache.stride_scale + kvh];
+            }
+            const int kt = (t & in_block) + r;
+#pragma unroll
+            for(int j = 0; j < KJ; ++j)
+            {
+                kb[h][j] = u32x4{0, 0, 0, 0};
+                if(there[h] && 64 * j + 16 * g < D)
+                    kb[h][j] = *reinterpret_cast<const u32x4*>(kc + at + (int64_t)kt * p.cache.stride_token + 64 * j + 16 * g);
+            }
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+            {
+                // what lies behind the last token is no value: zero, whatever its bytes are
+                const bool live = there[h] && t + 4 * g + i < most && r * E < D;
+#pragma unroll
+                for(int e = 0; e < E / 4; ++e)
+                    vb[4 * h + i][e] = 0;
+                if(live)
+                {
+                    const uint8_t* v = vc + at + (int64_t)((t & in_block) + 4 * g + i) * p.cache.stride_token + r * E;
+                    if constexpr(E == 8)
+                    {
+                        const u32x2 x = *reinterpret_cast<const u32x2*>(v);
+                        vb[4 * h + i][0] = x[0], vb[4 * h + i][1] = x[1];
+                    }
+                    else
+                        vb[4 * h + i][0] = *reinterpret_cast<const uint32_t*>(v);
+                }
+            }
+        }
+        // scores
+        float s[8], top = -__builtin_inff();
+#pragma unroll
+        for(int h = 0; h < 2; ++h)
+        {
+            f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+            for(int j = 0; j < KJ; ++j)
+            {
+                x = mfma_qk<T>(codes8<CODE, T>(kb[h][j][0], kb[h][j][1]), qf[j][0], x);
+                x = mfma_qk<T>(codes8<CODE, T>(kb[h][j][2], kb[h][j][3]), qf[j][1], x);
+            }
+            const float c = ks[h] * p.scale;
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+            {
+                const bool seen = there[h] && t0 + 16 * h + 4 * g + i < see;
+                s[4 * h + i]    = seen ? x[i] * c : -__builtin_inff();
+                top             = __builtin_fmaxf(top, s[4 * h + i]);
+            }
+        }
+        const float now  = __builtin_fmaxf(m, max_over_rows(top));
+        const float zero = now == -__builtin_inff() ? 0.0f : now; // (nothing seen yet: exp2(-inf - 0) = 0)
+        const float keep = __builtin_amdgcn_exp2f(m - zero);
+        m                = now;
+        l *= keep;
+        const float keep_o = keep * unit.take(vs[0], vs[1]);
+#pragma unroll
+        for(int j = 0; j < E; ++j)
+            acc[j] *= keep_o;
+        const float w[2] = {unit.of(vs[0]), unit.of(vs[1])};
+        float pr[8];
+#pragma unroll
+        for(int i = 0; i < 8; ++i)
+        {
+            pr[i] = __builtin_amdgcn_exp2f(s[i] - zero);
+            l += pr[i];
+            // (masked: no value scale, which may be an infinity or NaN, gets into the sum)
+            pr[i] = s[i] == -__builtin_inff() ? 0.0f : pr[i] * w[i >> 2];
+        }
+        const i32x4 pf = {(int)pack_f16(pr[0], pr[1]), (int)pack_f16(pr[2], pr[3]), (int)pack_f16(pr[4], pr[5]),
+                          (int)pack_f16(pr[6], pr[7])};
+#pragma unroll
+        for(int e = 0; e < E / 4; ++e)
+        {
+            uint32_t lo[4], hi[4];
+            transpose4(vb[0][e], vb[1][e], vb[2][e], vb[3][e], lo);
+            transpose4(vb[4][e], vb[5][e], vb[6][e], vb[7][e], hi);
+#pragma unroll
+            for(int j = 0; j < 4; ++j)
+                acc[4 * e + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    __builtin_bit_cast(f16x8, (codes8<CODE, _Float16>(lo[j], hi[j]))), __builtin_bit_cast(f16x8, pf), acc[4 * e + j], 0, 0, 0);
+        }
+    }
+
+    // the four waves' sums. Lane (r, g) holds elements (4g + i) * E + j of row r at acc[j][i].
+    l = sum_over_rows(l);
+    if(g == 0)
+        part_m[wave][r] = m, part_l[wave][r] = l;
+#pragma unroll
+    for(int j = 0; j < E; ++j)
+#pragma unroll
+        for(int i = 0; i < 4; ++i)
+            part[wave][r][(4 * g + i) * E + j] = acc[j][i] * unit.top;
+    __syncthreads();
+    // thread (row, 16 of them a row) joins E elements
+    const int row = threadIdx.x >> 4, c = threadIdx.x & 15;
+    const int jt = row / p.tile_heads, jh = h0 + (row - jt * p.tile_heads);
+    if(jt >= p.tile_tokens || tile.first + jt >= tile.q_len || jh >= p.group || c * E >= D)
+        return;
+    float top = -__builtin_inff();
+#pragma unroll
+    for(int w = 0; w < kWaves; ++w)
+        top = __builtin_fmaxf(top, part_m[w][row]);
+    const float zero = top == -__builtin_inff() ? 0.0f : top;
+    float sum = 0.0f, o[E];
+#pragma unroll
+    for(int e = 0; e < E; ++e)
+        o[e] = 0.0f;
+#pragma unroll
+    for(int w = 0; w < kWaves; ++w)
+    {
+        const float f = __builtin_amdgcn_exp2f(part_m[w][row] - zero);
+        sum += part_l[w][row] * f;
+#pragma unroll
+        for(int e = 0; e < E; ++e)
+            o[e] += part[w][row][c * E + e] * f;
+    }
+    const int64_t out_token = tile.q0 + tile.first + jt, out_head = kvh * p.group + jh;
+    if(p.splits == 1)
+    {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum; // (a row that sees nothing: zero)
+        T* const to = reinterpret_cast<T*>(p.o) + out_token * p.so_t + out_head * p.so_h + c * E;
+        typedef T tx __attribute__((ext_vector_type(E)));
+        tx x;
+#pragma unroll
+        for(int e = 0; e < E; ++e)
+            x[e] = (T)(o[e] * inv);
+        *reinterpret_cast<tx*>(to) = x;
+    }
+    else
+    {
+        const int64_t at = (out_token * p.heads + out_head) * p.splits + split;
+        float* const to  = p.ws + at * DP + c * E;
+#pragma unroll
+        for(int e = 0; e < E; e += 4)
+            *reinterpret_cast<f32x4*>(to + e) = f32x4{o[e], o[e + 1], o[e + 2], o[e + 3]};
+        if(c == 0)
+        {
+            float* const ml = p.ws + attention_rows(p) * p.splits * DP + at * 2;
+            ml[0] = top, ml[1] = sum;
+        }
+    }
+}
+
+// joins the shares of a query row: 16 lanes a row. Rows outside the sequences (cu_q) are left alone.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs p)
+{
+    constexpr int E = DP / 16;
+    const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int c       = threadIdx.x & 15;
+    if(row >= attention_rows(p) || c * E >= p.cache.head_dim)
+        return;
+    const int64_t token = row / p.heads, head = row - token * p.heads;
+    if(token < p.cu_q[0] || token >= p.cu_q[p.batch])
+        return;
+    const float* const ml = p.ws + attention_rows(p) * p.splits * DP + row * p.splits * 2;
+    const float* const at = p.ws + row * p.splits * DP + c * E;
+    float top             = -__builtin_inff();
+    for(int s = 0; s < p.splits; ++s)
+        top = __builtin_fmaxf(top, ml[2 * s]);
+    const float zero = top == -__builtin_inff() ? 0.0f : top;
+    float sum = 0.0f, o[E];
+#pragma unroll
+    for(int e = 0; e < E; ++e)
+        o[e] = 0.0f;
+    for(int s = 0; s < p.splits; ++s)
+    {
+        const float f = __builtin_amdgcn_exp2f(ml[2 * s] - zero);
+        sum += ml[2 * s + 1] * f;
+#pragma unroll
+        for(int e = 0; e < E; e += 4)
+        {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(at + (int64_t)s * DP + e);
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+                o[e + i] += x[i] * f;
+        }
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    typedef T tx __attribute__((ext_vector_type(E)));
+    tx x;
+#pragma unroll
+    for(int e = 0; e < E; ++e)
+        x[e] = (T)(o[e] * inv);
+    *reinterpret_cast<tx*>(reinterpret_cast<T*>(p.o) + token * p.so_t + head * p.so_h + c * E) = x;
+}
+
+struct Plan
+{
+    int tile_tokens, tile_heads, head_tiles, tiles, splits;
+};
+
+Plan plan(const ckx_kv_cache8& c, int batch, int tokens, int heads, int max_kv, int max_blocks)
+{
+    Plan p;
+    const int group = heads / c.num_heads;
+    p.tile_heads  = group < 16 ? group : 16;
+    p.head_tiles  = (group + p.tile_heads - 1) / p.tile_heads;
+    p.tile_tokens = 16 / p.tile_heads;
+    p.tiles       = p.tile_tokens == 1 ? tokens : tokens / p.tile_tokens + batch;
+    // shares: about four workgroups a CU, none of under 256 tokens (two steps a wave)
+    const int64_t groups = (int64_t)(p.tile_tokens == 1 ? tokens : tokens < p.tiles ? tokens : p.tiles) * c.num_heads * p.head_tiles;
+    const int64_t most   = (int64_t)max_blocks * c.block_size;
+    const int64_t kv     = max_kv < most ? max_kv : most;
+    int64_t splits       = (1024 + groups - 1) / groups;
+    if(splits > kv / 256)
+        splits = kv / 256;
+    p.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
+    return p;
+}
+
+int padded(int head_dim) { return head_dim <= 64 ? 64 : 128; }
+
+template <typename T, int CODE, int DP>
+hipError_t launch(const AttentionArgs& a, hipStream_t s)
+{
+    const int64_t groups = (int64_t)a.tiles * a.cache.num_heads * a.head_tiles * a.splits;
+    hipLaunchKernelGGL((attention_rows_kernel<T, CODE, DP>), dim3((unsigned)groups), dim3(kWaves * 64), 0, s, a);
+    hipError_t e = hipGetLastError();
+    if(e != hipSuccess || a.splits == 1)
+        return e;
+    hipLaunchKernelGGL((attention_join_kernel<T, DP>), dim3((unsigned)((attention_rows(a) + 15) / 16)), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch(const AttentionArgs& a, hipStream_t s)
+{
+    const bool e4m3 = a.cache.type == CKX_TYPE_E4M3;
+    if(padded(a.cache.head_dim) == 64)
+        return e4m3 ? launch<T, CODE_E4M3, 64>(a, s) : launch<T, CODE_I8, 64>(a, s);
+    return e4m3 ? launch<T, CODE_E4M3, 128>(a, s) : launch<T, CODE_I8, 128>(a, s);
+}
+
+} // namespace
+
+// a launch has fewer than 2^32 threads
+bool attention_fits(const ckx_kv_cache8& c, int batch, int tokens, int heads, int max_kv, int max_blocks)
+{
+    const Plan p = plan(c, batch, tokens, heads, max_kv, max_blocks);
+    return (int64_t)p.tiles * c.num_heads * p.head_tiles * p.splits < (1ll << 32) / (kWaves * 64);
+}
+
+int64_t attention_workspace(const ckx_kv_cache8& c, int batch, int tokens, int heads, int max_kv, int max_blocks)
+{
+    const Plan p = plan(c, batch, tokens, heads, max_kv, max_blocks);
+    return p.splits == 1 ? 0 : (int64_t)tokens * heads * p.splits * (padded(c.head_dim) + 2) * 4;
+}
+
+hipError_t attention_launch(AttentionArgs a, int q_type, hipStream_t s)
+{
+    const Plan p  = plan(a.cache, a.batch, a.tokens, a.heads, a.max_kv, a.max_blocks);
+    a.tile_tokens = p.tile_tokens, a.tile_heads = p.tile_heads, a.head_tiles = p.head_tiles, a.tiles = p.tiles, a.splits = p.splits;
+    return q_type == CKX_TYPE_F16 ? launch<_Float16>(a, s) : launch<__bf16>(a, s);
+}
+
+} // namespace ckx

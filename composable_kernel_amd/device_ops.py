@@ -640,3 +640,172 @@ class DeviceBatchedGemmSoftmaxGemmF16(BaseOperator):
     def _launch(self, a, stream):
         return capi.lib().ckx_batched_gemm_softmax_gemm_f16(*a.ptrs, *a.dims, a.scale, int(self.mask), self.instance,
                                                             C.c_void_p(stream or 0))
+
+
+# ----------------------------------------------------------- 8-bit serving
+_TYPES = {"f32": capi.TYPE_F32, "f16": capi.TYPE_F16, "bf16": capi.TYPE_BF16}
+_TORCH_TYPES = {"torch.float32": "f32", "torch.float16": "f16", "torch.bfloat16": "bf16", "torch.float8_e4m3fn": "e4m3",
+                "torch.int8": "i8", "torch.int32": "i32"}
+
+
+def _typed(x, want, what):
+    """The address of a tensor of the wanted type ("bf16", "e4m3", "i32", ...); a bare address is taken as it is."""
+    if x is not None and not isinstance(x, int):
+        has = _TORCH_TYPES.get(str(x.dtype), str(x.dtype))
+        if has != want:
+            raise TypeError(f"{what}: {want} expected, {has} given")
+    return _ptr(x)
+
+
+class _ServingArgument(BaseArgument):
+    """dims: the arguments that IsSupportedArgument and the launch share; ptrs: the operands' addresses."""
+
+    def __init__(self, ptrs, dims, keep=None):
+        self.ptrs, self.dims, self._keep = ptrs, dims, keep
+
+
+class _ServingOperator(BaseOperator):
+    """One kernel choice per operator, made by the library: no instance list."""
+
+    def __init__(self):
+        super().__init__()
+
+    def GetTypeString(self):
+        return f"{type(self).__name__}<auto>"
+
+    @classmethod
+    def GetInstances(cls):
+        raise TypeError(f"{cls.__name__} has no instance list: the library chooses the kernel")
+
+
+class DeviceBlockQuantizeF8(_ServingOperator):
+    """x [M, K] -> e4m3 codes [M, K] and one fp32 scale per row and group of 128 columns (ckx_quantize_blocks_f8). XDataType:
+    "f32", "f16" or "bf16"."""
+
+    def __init__(self, XDataType="bf16"):
+        super().__init__()
+        self.x, self.x_type = XDataType, _TYPES[XDataType]
+
+    def MakeArgumentPointer(self, p_x, p_q, p_scale, M, K, StrideX, StrideQ, StrideScaleM, StrideScaleG):
+        return _ServingArgument((_typed(p_x, self.x, "x"), _typed(p_q, "e4m3", "q"), _typed(p_scale, "f32", "scale")),
+                                (int(M), int(K), int(StrideX), int(StrideQ), int(StrideScaleM), int(StrideScaleG), self.x_type))
+
+    def _supported(self, a):
+        return capi.lib().ckx_quantize_blocks_f8_is_supported(*a.dims)
+
+    def _launch(self, a, stream):
+        return capi.lib().ckx_quantize_blocks_f8(*a.ptrs, *a.dims, C.c_void_p(stream or 0))
+
+
+class DeviceGemmBlockScaleF8(_ServingOperator):
+    """C = sum over groups of 128 columns of scale_a * scale_b * (A_group B_group^T), e4m3 operands (ckx_gemm_f8_blockscale):
+    A [M, K], B [N, K]. StridesScaleA: of scale_a per row and per group; StridesScaleB: of scale_b per 128 columns of C and per
+    group. CDataType: "f32", "f16" or "bf16"."""
+
+    def __init__(self, CDataType="bf16"):
+        super().__init__()
+        self.c, self.c_type = CDataType, _TYPES[CDataType]
+
+    def MakeArgumentPointer(self, p_a, p_b, p_c, p_scale_a, p_scale_b, M, N, K, StrideA, StrideB, StrideC, StridesScaleA,
+                            StridesScaleB):
+        (sam, sag), (sbn, sbg) = StridesScaleA, StridesScaleB
+        ptrs = (_typed(p_a, "e4m3", "A"), _typed(p_b, "e4m3", "B"), _typed(p_c, self.c, "C"), _typed(p_scale_a, "f32", "scale_a"),
+                _typed(p_scale_b, "f32", "scale_b"))
+        return _ServingArgument(ptrs, tuple(int(x) for x in (M, N, K, StrideA, StrideB, StrideC, sam, sag, sbn, sbg, self.c_type)))
+
+    def _supported(self, a):
+        return capi.lib().ckx_gemm_f8_blockscale_is_supported(*a.dims)
+
+    def GetWorkSpaceSize(self, a):
+        return int(capi.lib().ckx_gemm_f8_blockscale_workspace_bytes(*a.dims[:3]))
+
+    def _launch(self, a, stream):
+        return capi.lib().ckx_gemm_f8_blockscale(*a.ptrs, *a.dims, a.p_workspace_ or 0, a.workspace_bytes_, C.c_void_p(stream or 0))
+
+
+class KvCache8:
+    """A cache of 8-bit blocks: k, v torch tensors [num_blocks, heads, block_size, head_dim] (any strides with neighbouring
+    elements; a cache laid out [num_blocks, block_size, heads, head_dim] is passed as its permute(0, 2, 1, 3)), both e4m3 or
+    both int8, and scales [num_blocks, heads]. The arguments made from it keep it alive."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        if k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.dim() != 4:
+            raise ValueError("keys and values: two tensors [num_blocks, heads, block_size, head_dim] of one type, shape and layout")
+        kind = {"e4m3": capi.TYPE_E4M3, "i8": capi.TYPE_I8}.get(_TORCH_TYPES.get(str(k.dtype)))
+        if kind is None:
+            raise TypeError("the cache holds e4m3 or int8 codes")
+        if k.stride(3) != 1 and k.shape[3] > 1:
+            raise ValueError("the elements of a head lie next to each other")
+        for s in (k_scale, v_scale):
+            _typed(s, "f32", "scales")
+            if tuple(s.shape) != tuple(k.shape[:2]) or s.stride() != k_scale.stride() or (s.shape[1] > 1 and s.stride(1) != 1):
+                raise ValueError("scales: [num_blocks, heads], the heads next to each other, keys and values alike")
+        n, heads, size, dim = k.shape
+        self.desc = capi.KvCache8Desc(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), kind, n, size, heads, dim, k.stride(1),
+                                      k.stride(2), k_scale.stride(0), k.stride(0))
+        self.tensors = (k, v, k_scale, v_scale)
+
+
+class DeviceKvCacheTables(_ServingOperator):
+    """Block tables, slots and lengths of a step from the requests' lengths (ckx_kv_cache_tables). int32 tensors."""
+
+    def MakeArgumentPointer(self, p_context_lens, p_new_lens, p_free_blocks, p_block_table, p_cu_new, p_kv_lens, p_slots, p_used, Batch,
+                            NumFree, MaxBlocks, StrideTable, NumSlots, BlockSize):
+        ptrs = tuple(_typed(x, "i32", "tables") for x in (p_context_lens, p_new_lens, p_free_blocks, p_block_table, p_cu_new, p_kv_lens,
+                                                          p_slots, p_used))
+        return _ServingArgument(ptrs, tuple(int(x) for x in (Batch, NumFree, MaxBlocks, StrideTable, NumSlots, BlockSize)))
+
+    def _supported(self, a):
+        return capi.lib().ckx_kv_cache_tables_is_supported(*a.dims)
+
+    def _launch(self, a, stream):
+        return capi.lib().ckx_kv_cache_tables(*a.ptrs, *a.dims, C.c_void_p(stream or 0))
+
+
+class DeviceKvCacheStore8(_ServingOperator):
+    """New keys and values into a KvCache8 (ckx_kv_cache_store8). StridesK / StridesV: of a token and of a head."""
+
+    def __init__(self, XDataType="bf16"):
+        super().__init__()
+        self.x, self.x_type = XDataType, _TYPES[XDataType]
+
+    def MakeArgumentPointer(self, p_k, p_v, p_slots, cache, NumTokens, StridesK, StridesV):
+        (kt, kh), (vt, vh) = StridesK, StridesV
+        ptrs = (_typed(p_k, self.x, "keys"), _typed(p_v, self.x, "values"), _typed(p_slots, "i32", "slots"))
+        return _ServingArgument(ptrs, (C.byref(cache.desc), int(NumTokens), int(kt), int(kh), int(vt), int(vh), self.x_type), cache)
+
+    def _supported(self, a):
+        return capi.lib().ckx_kv_cache_store8_is_supported(*a.dims)
+
+    def _launch(self, a, stream):
+        return capi.lib().ckx_kv_cache_store8(*a.ptrs, *a.dims, C.c_void_p(stream or 0))
+
+
+class DevicePagedAttention8(_ServingOperator):
+    """Attention of query tokens over a KvCache8 (ckx_paged_attention8), for single tokens and prompts. StridesQ / StridesO: of a
+    token and of a head."""
+
+    def __init__(self, QDataType="bf16", Causal=True):
+        super().__init__()
+        self.q, self.q_type, self.causal = QDataType, _TYPES[QDataType], int(bool(Causal))
+
+    def MakeArgumentPointer(self, p_q, p_o, p_block_table, p_cu_q, p_kv_lens, cache, Batch, NumTokens, NumHeads, MaxKvLen, MaxBlocks,
+                            StrideTable, StridesQ, StridesO, score_element_op=None):
+        if score_element_op is not None and not isinstance(score_element_op, (Scale, PassThrough)):
+            raise TypeError("the score operation is Scale or PassThrough")
+        scale = score_element_op.scale if isinstance(score_element_op, Scale) else 1.0
+        (qt, qh), (ot, oh) = StridesQ, StridesO
+        ptrs = (_typed(p_q, self.q, "q"), _typed(p_o, self.q, "o"), _typed(p_block_table, "i32", "block table"),
+                _typed(p_cu_q, "i32", "cu_q"), _typed(p_kv_lens, "i32", "lengths"))
+        dims = (C.byref(cache.desc), int(Batch), int(NumTokens), int(NumHeads), int(MaxKvLen), int(MaxBlocks), int(StrideTable), int(qt),
+                int(qh), int(ot), int(oh), scale, self.causal, self.q_type)
+        return _ServingArgument(ptrs, dims, cache)
+
+    def _supported(self, a):
+        return capi.lib().ckx_paged_attention8_is_supported(*a.dims)
+
+    def GetWorkSpaceSize(self, a):
+        return int(capi.lib().ckx_paged_attention8_workspace_bytes(*a.dims[:6]))
+
+    def _launch(self, a, stream):
+        return capi.lib().ckx_paged_attention8(*a.ptrs, *a.dims, a.p_workspace_ or 0, a.workspace_bytes_, C.c_void_p(stream or 0))

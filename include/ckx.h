@@ -415,6 +415,126 @@ int ckx_set_forced_k_runs(int k_runs);
  * before. The initial value is the environment variable CKX_BIG_TILE_WAVES, read once. */
 int ckx_set_big_tile_waves(int waves);
 
+/* ==== 8-bit serving ==============================================================================
+ * The linear and attention work of a decoder layer in 8 bits: activations to e4m3 in groups of 128, the product of two
+ * such operands, and attention over a cache of 8-bit blocks with the tables and the store that feed it. All entry points
+ * are asynchronous on `stream`, allocate nothing, can be captured into a graph, and read lengths, tables and slots on the
+ * device: a replay sees what they hold then. `stream`'s device has to be the current one.
+ *
+ * e4m3 is the OCP format (1-4-3, largest value 448, no infinities). */
+enum
+{
+    CKX_TYPE_F32  = 0,
+    CKX_TYPE_F16  = 1,
+    CKX_TYPE_BF16 = 2,
+    CKX_TYPE_E4M3 = 3,
+    CKX_TYPE_I8   = 4
+};
+
+/* ---- e4m3 codes of activations, one scale per row and group of 128 columns -----------------------
+ *   s[m, g] = max(max_{k in g} |x[m, k]|, 2^-100) / 448        (fp32; NaN does not count)
+ *   q[m, k] = e4m3(x[m, k] * (1 / s[m, k / 128]))              (fp32, round to nearest even)
+ * x [M, K] fp32, fp16 or bf16 (x_type), q [M, K] e4m3, rows stride_x / stride_q elements apart; the scale of row m, group g
+ * is p_scale[m * stride_scale_m + g * stride_scale_g]: (1, M) is the layout that ckx_gemm_f8_blockscale reads fastest. The last
+ * group is short where K is no multiple of 128. A NaN stays NaN; an infinity makes its group's scale infinite, and every
+ * value of the group NaN when it is read back. Any K, stride and address; 16-byte aligned rows run on wide loads. */
+int ckx_quantize_blocks_f8_is_supported(int32_t M, int32_t K, int32_t stride_x, int32_t stride_q, int32_t stride_scale_m,
+                                        int32_t stride_scale_g, int x_type);
+int ckx_quantize_blocks_f8(const void* p_x, void* p_q, float* p_scale, int32_t M, int32_t K, int32_t stride_x,
+                           int32_t stride_q, int32_t stride_scale_m, int32_t stride_scale_g, int x_type, void* stream);
+
+/* ---- GEMM, e4m3 operands with a scale for each block of 128 --------------------------------------
+ *   C[m, n] = round( sum_g sa[m, g] * sb[n / 128, g] * sum_{k in group g} A[m, k] * B[n, k] )
+ * A [M, K] row-major, B stored [N, K] (column-major K x N), C [M, N] row-major fp32, fp16 or bf16 (c_type), rounded once.
+ * sa[m, g] = p_scale_a[m * stride_sa_m + g * stride_sa_g], sb[j, g] = p_scale_b[j * stride_sb_n + g * stride_sb_g]. Products
+ * and sums are fp32. K == 0 gives zeros. Any extent, stride and address; K, lda, ldb multiples of 16 with 16-byte aligned A and B
+ * run on the vectorised kernels. Workspace (optional, ckx_gemm_f8_blockscale_workspace_bytes; 0 for most problems): lets few
+ * output tiles with a long K run side by side. */
+int ckx_gemm_f8_blockscale_is_supported(int32_t M, int32_t N, int32_t K, int32_t lda, int32_t ldb, int32_t ldc,
+                                        int32_t stride_sa_m, int32_t stride_sa_g, int32_t stride_sb_n, int32_t stride_sb_g,
+                                        int c_type);
+int64_t ckx_gemm_f8_blockscale_workspace_bytes(int32_t M, int32_t N, int32_t K);
+int ckx_gemm_f8_blockscale(const void* p_a, const void* p_b, void* p_c, const float* p_scale_a, const float* p_scale_b,
+                           int32_t M, int32_t N, int32_t K, int32_t lda, int32_t ldb, int32_t ldc, int32_t stride_sa_m,
+                           int32_t stride_sa_g, int32_t stride_sb_n, int32_t stride_sb_g, int c_type, void* p_workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/* ---- key / value cache in 8 bits -----------------------------------------------------------------
+ * Blocks of block_size tokens; the code of token t, head h, element d of block b is
+ * p_k[b * stride_block + h * stride_head + t * stride_token + d] (p_v alike), the value it stands for that code times
+ * p_k_scale[b * stride_scale + h]. Slot number = block * block_size + token. e4m3 or int8 codes; head_dim a multiple of
+ * 16 up to 128; block_size 16, 32, 64 or 128; strides multiples of 16, p_k and p_v 16-byte aligned. Codes are finite
+ * (ckx_kv_cache_store8 writes no others: it puts a NaN or infinity into the block's scale). Blocks with numbers outside
+ * [0, num_blocks) are neither read nor written. */
+typedef struct ckx_kv_cache8
+{
+    void* p_k;
+    void* p_v;
+    float* p_k_scale;
+    float* p_v_scale;
+    int32_t type; /* CKX_TYPE_E4M3 or CKX_TYPE_I8 */
+    int32_t num_blocks, block_size, num_heads, head_dim;
+    int32_t stride_head, stride_token;
+    int32_t stride_scale;
+    int64_t stride_block;
+} ckx_kv_cache8;
+
+/* Block tables and slots of one step, from the requests' lengths. Sequence b has p_context_lens[b] tokens in the cache and
+ * gets p_new_lens[b] more. All arrays are int32 on the device:
+ *   p_block_table [batch, max_blocks] (rows stride_table apart), in and out: the blocks that sequence b has already stand in
+ *       its first ceil(context / block_size) columns; the ones it needs beyond are taken from p_free_blocks in order,
+ *       sequence after sequence, and written behind them. Other columns are left alone.
+ *   p_cu_new [batch + 1]: sums of the new lengths before each sequence; p_kv_lens [batch]: context + new
+ *   p_slots [num_slots]: slot of every new token, sequence after sequence; -1 behind the last one, and where a token's
+ *       block is missing (free list too short, table too narrow)
+ *   p_used [1]: blocks needed; more than num_free says that the free list was too short
+ * Lengths under zero count as zero; their sums fit 31 bits. At most 8192 sequences. No output may lie on an input. */
+int ckx_kv_cache_tables_is_supported(int32_t batch, int32_t num_free, int32_t max_blocks, int32_t stride_table,
+                                     int32_t num_slots, int32_t block_size);
+int ckx_kv_cache_tables(const int32_t* p_context_lens, const int32_t* p_new_lens, const int32_t* p_free_blocks,
+                        int32_t* p_block_table, int32_t* p_cu_new, int32_t* p_kv_lens, int32_t* p_slots, int32_t* p_used,
+                        int32_t batch, int32_t num_free, int32_t max_blocks, int32_t stride_table, int32_t num_slots,
+                        int32_t block_size, void* stream);
+
+/* New keys and values into the cache. x: p_k / p_v [num_tokens, num_heads, head_dim] fp16 or bf16 (x_type), strides in
+ * elements (multiples of 8, 16-byte aligned), token t into slot p_slots[t]; slots outside the cache (-1) are skipped. A run =
+ * consecutive tokens whose slots lie in one block, slots ascending; a block occurs in one run of a call. With o the place
+ * of the run's first token in its block, Q = 448 (e4m3) or 127 (int8), per head, for keys and values alike:
+ *   new scale = max(max(max |x| over the run, 2^-100) / Q, o > 0 ? old scale : 0)
+ *   o > 0 and the scale grew: the codes of the tokens before o become round(code * (old / new))
+ *   codes of the run: round(x * (1 / new)), ties to even
+ * A block is filled in order: what lies behind the run counts as unwritten. A NaN or infinity among the run makes the
+ * scale NaN or infinite, so that the block's values are NaN until it is begun anew (o == 0). */
+int ckx_kv_cache_store8_is_supported(const ckx_kv_cache8* cache, int32_t num_tokens, int32_t stride_k_token,
+                                     int32_t stride_k_head, int32_t stride_v_token, int32_t stride_v_head, int x_type);
+int ckx_kv_cache_store8(const void* p_k, const void* p_v, const int32_t* p_slots, const ckx_kv_cache8* cache,
+                        int32_t num_tokens, int32_t stride_k_token, int32_t stride_k_head, int32_t stride_v_token,
+                        int32_t stride_v_head, int x_type, void* stream);
+
+/* Attention of query tokens over the cache, fp16 or bf16 (q_type): sequence b has the query rows
+ * p_cu_q[b] ... p_cu_q[b + 1] - 1 of p_q [num_tokens, num_q_heads, head_dim] and the p_kv_lens[b] cached tokens that row b
+ * of p_block_table [batch, max_blocks] names (rows stride_table apart). Query head h reads cache head
+ * h / (num_q_heads / num_heads).
+ *   O[t, h] = sum_j softmax_j(scale * q[t, h] . k[j, h']) * v[j, h']
+ * over all cached tokens of the sequence, or with `causal` those up to the token's own place (the last query row sees all
+ * of them, the one before it one less). A row that sees nothing is 0. Rows of p_o outside p_cu_q's are left alone. Scores, softmax
+ * and sums are fp32; probability times value scale is rounded to fp16 (relative to the row's largest value scale) before the
+ * second product. max_kv_len (an upper bound that a
+ * program knows) steers how the work is cut and no result depends on its being right; num_tokens bounds the rows that are
+ * read and written. Token and head strides of q and o: elements, multiples of 8, 16-byte aligned.
+ * Workspace (ckx_paged_attention8_workspace_bytes): required where that is not 0; launches that share one must not overlap. */
+int ckx_paged_attention8_is_supported(const ckx_kv_cache8* cache, int32_t batch, int32_t num_tokens, int32_t num_q_heads,
+                                      int32_t max_kv_len, int32_t max_blocks, int32_t stride_table, int32_t stride_q_token,
+                                      int32_t stride_q_head, int32_t stride_o_token, int32_t stride_o_head, float scale,
+                                      int causal, int q_type);
+int64_t ckx_paged_attention8_workspace_bytes(const ckx_kv_cache8* cache, int32_t batch, int32_t num_tokens,
+                                             int32_t num_q_heads, int32_t max_kv_len, int32_t max_blocks);
+int ckx_paged_attention8(const void* p_q, void* p_o, const int32_t* p_block_table, const int32_t* p_cu_q,
+                         const int32_t* p_kv_lens, const ckx_kv_cache8* cache, int32_t batch, int32_t num_tokens,
+                         int32_t num_q_heads, int32_t max_kv_len, int32_t max_blocks, int32_t stride_table,
+                         int32_t stride_q_token, int32_t stride_q_head, int32_t stride_o_token, int32_t stride_o_head,
+                         float scale, int causal, int q_type, void* p_workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- timing helper --------------------------------------------------------
  * launch_and_time_kernel (include/ck/device_utility/kernel_launch.hpp:13-74):
  * `fn(user)` is called n_warmup times untimed, then n_repeat times between two

@@ -1,0 +1,193 @@
+"""DevicePagedAttention8 against attention in 64 bits (bound: serving_plain.attention_bound)."""
+import pytest
+import torch
+
+import composable_kernel_amd as ck
+import serving_plain as sp
+
+pytestmark = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "f16": torch.float16}
+
+
+class Problem:
+    def __init__(self, news, kvs, heads, H, D, size, code=torch.float8_e4m3fn, xt="bf16", layout="bhsd", seed=0, causal=True, scale=None,
+                 spare=0):
+        g = sp.gen(seed + heads + D + size + sum(kvs))
+        self.news, self.kvs, self.heads, self.D, self.size, self.xt, self.causal = news, kvs, heads, D, size, xt, causal
+        self.scale = D ** -0.5 if scale is None else scale
+        self.cu = [0]
+        for n in news:
+            self.cu.append(self.cu[-1] + n)
+        each = [-(-kv // size) for kv in kvs]
+        blocks = sum(each) + 3
+        self.cache = list(sp.random_cache(g, blocks, H, size, D, code, layout))
+        order, at = torch.randperm(blocks, generator=g).tolist(), 0
+        self.table = torch.full((len(news), max(each + [1]) + 1), -1, dtype=torch.int32)
+        for b, n in enumerate(each):
+            self.table[b, :n] = torch.tensor(order[at:at + n])
+            at += n
+        self.T = self.cu[-1] + spare
+        self.q = sp.normal(g, (self.T, heads, D), DT[xt])
+
+    def run(self, max_kv=None, tokens=None, o=None, sync=True):
+        kc, vc, ks, vs = (x.cuda() for x in self.cache)
+        self.dev = [kc, vc, ks, vs, self.table.cuda(), torch.tensor(self.cu, dtype=torch.int32, device="cuda"),
+                    torch.tensor(self.kvs, dtype=torch.int32, device="cuda")]
+        # queries as columns of a fused projection, outputs with a gap behind every token
+        qkv = torch.zeros(self.T, (self.heads + 3) * self.D, dtype=DT[self.xt], device="cuda")
+        q = qkv[:, :self.heads * self.D].view(self.T, self.heads, self.D)
+        q.copy_(self.q)
+        out = torch.full((self.T, self.heads * self.D + 8), 5.0, dtype=DT[self.xt], device="cuda")
+        o = out[:, :self.heads * self.D].view(self.T, self.heads, self.D)
+        op = ck.DevicePagedAttention8(self.xt, Causal=self.causal)
+        arg = op.MakeArgumentPointer(q, o, self.dev[4], self.dev[5], self.dev[6], ck.KvCache8(kc, vc, ks, vs), len(self.news), self.T,
+                                     self.heads, max(self.kvs + [0]) if max_kv is None else max_kv, self.table.shape[1],
+                                     self.table.shape[1], q.stride()[:2], o.stride()[:2], ck.Scale(self.scale))
+        assert op.IsSupportedArgument(arg), ck.capi.last_error()
+        need = op.GetWorkSpaceSize(arg)
+        if need:
+            op.SetWorkSpacePointer(arg, torch.full((need,), 0x7F, device="cuda", dtype=torch.uint8))
+        op.MakeInvokerPointer().Run(arg, ck.StreamConfig(torch.cuda.current_stream().cuda_stream))
+        torch.cuda.synchronize()
+        assert bool((out[:, self.heads * self.D:] == 5).all()) and bool((out[self.cu[-1]:] == 5).all()), "wrote outside the rows"
+        return o.cpu()[:self.cu[-1]]
+
+    def check(self, **kw):
+        got = self.run(**kw).double()
+        kc, vc, ks, vs = self.cache
+        want, mag, big = sp.attention(self.q[:self.cu[-1]], self.table, self.cu, self.kvs, kc, vc, ks, vs, self.scale, self.causal)
+        bound = sp.attention_bound(want, mag, big, DT[self.xt], self.D, max(self.kvs + [0]))
+        bad = ~((got - want).abs() <= bound)
+        assert not bool(bad.any()), (float((got - want).abs().max()), bad.nonzero()[:4].tolist(), int(bad.sum()))
+        return got
+
+
+@pytest.mark.parametrize("code", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("xt", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,H,D,size", [(4, 1, 64, 16), (8, 2, 128, 16), (7, 1, 80, 32), (3, 3, 16, 64), (32, 2, 112, 128), (20, 1, 96, 16)])
+def test_single_tokens(code, xt, heads, H, D, size):
+    Problem([1, 1, 1, 1, 1], [1, 15, 33, 64, 300], heads, H, D, size, code, xt).check()
+
+
+@pytest.mark.parametrize("kv", [1, 2, 16, 31, 32, 33, 127, 128, 129, 255, 257, 511, 1000, 2049, 5000])
+def test_lengths(kv):
+    Problem([1], [kv], 8, 2, 64, 16).check()
+
+
+@pytest.mark.parametrize("code", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,H,D,size", [(4, 1, 64, 16), (8, 2, 128, 32), (6, 6, 48, 16), (14, 2, 80, 64), (48, 2, 64, 16)])
+def test_prompts(code, causal, heads, H, D, size):
+    Problem([5, 1, 17, 40], [5, 9, 50, 100], heads, H, D, size, code, "bf16", causal=causal).check()
+    Problem([33, 70], [33, 200], heads, H, D, size, code, "f16", causal=causal).check()
+
+
+@pytest.mark.parametrize("news,kvs", [([130], [130]), ([200, 3], [333, 3]), ([64, 128, 256], [64, 129, 300]), ([1, 257], [400, 257])])
+@pytest.mark.parametrize("heads,H,D", [(4, 1, 128), (2, 2, 64), (7, 1, 64)])
+def test_longer_prompts(news, kvs, heads, H, D):
+    Problem(news, kvs, heads, H, D, 16).check()
+    Problem(news, kvs, heads, H, D, 32, torch.int8, "f16", causal=False).check()
+
+
+def test_rows_that_see_nothing_are_zero():
+    # a sequence without cached tokens, one with fewer than it has queries (its first rows see none), one without queries
+    p = Problem([2, 5, 0, 1], [0, 3, 40, 20], 8, 2, 64, 16)
+    got = p.check()
+    assert bool((got[:4] == 0).all()) and bool((got[4:] != 0).any())
+    p = Problem([2, 70, 0, 1], [0, 3, 40, 20], 8, 2, 64, 16)
+    got = p.check()
+    assert bool((got[:69] == 0).all())
+    p = Problem([2, 5, 0, 1], [0, 3, 40, 20], 8, 2, 64, 16, causal=False)
+    assert bool((p.check()[:2] == 0).all())
+
+
+def test_no_sequence_and_no_token():
+    assert Problem([], [], 4, 1, 64, 16, spare=3).run().shape[0] == 0
+    assert Problem([0, 0], [5, 0], 4, 1, 64, 16, spare=2).run().shape[0] == 0
+
+
+def test_rows_behind_the_last_sequence_stay():
+    Problem([1, 3, 1], [40, 50, 600], 8, 2, 64, 16, spare=7).check()
+    Problem([90, 40], [90, 600], 8, 2, 64, 16, spare=200).check()
+
+
+@pytest.mark.parametrize("layout", ["bhsd", "bshd"])
+def test_cache_layouts(layout):
+    Problem([1, 4], [77, 300], 8, 2, 64, 32, layout=layout).check()
+    Problem([100], [300], 8, 2, 128, 32, torch.int8, layout=layout).check()
+
+
+@pytest.mark.parametrize("news", [[1, 1, 1], [1, 2, 3], [80, 1, 30]])
+def test_stale_codes_scales_and_table_entries_do_not_matter(news):
+    """Behind the last token of a block: NaN codes; blocks that no sequence has: NaN codes and scales; table columns behind the
+    last block: numbers of those blocks, and numbers outside the cache."""
+    p = Problem(news, [17, 100, 47], 8, 2, 64, 16)
+    want = p.run()
+    kc, vc, ks, vs = p.cache
+    nan = torch.tensor(float("nan")).to(torch.float8_e4m3fn)
+    used = set()
+    for b, kv in enumerate(p.kvs):
+        for c in range(-(-kv // 16)):
+            used.add(int(p.table[b, c]))
+        for x in (kc, vc):
+            if kv % 16:
+                x[int(p.table[b, kv // 16]), :, kv % 16:] = nan
+    free = [i for i in range(kc.shape[0]) if i not in used]
+    for i in free:
+        kc[i], vc[i], ks[i], vs[i] = nan, nan, float("nan"), float("inf")
+    for b, kv in enumerate(p.kvs):
+        p.table[b, -(-kv // 16):] = free[b % len(free)]
+    p.table[0, -1], p.table[1, -1] = 1 << 30, -(1 << 31)
+    assert torch.equal(p.run(), want)
+
+
+@pytest.mark.parametrize("bad", [-1, 1 << 30, -(1 << 31)])
+@pytest.mark.parametrize("news", [[1, 1], [60, 2]])
+def test_blocks_outside_the_cache_count_as_not_there(news, bad):
+    p = Problem(news, [90, 64], 8, 2, 64, 16)
+    p.table[0, 1], p.table[1, 3], p.table[1, 0] = bad, bad, bad
+    p.check()
+    p = Problem(news, [90, 64], 8, 2, 64, 16)
+    p.table[:] = bad
+    assert bool((p.check() == 0).all())
+
+
+def test_lengths_past_the_table_end_with_it():
+    p = Problem([1, 2], [60, 40], 4, 1, 64, 16)
+    p.kvs = [10000, 10000]
+    p.table[p.table < 0] = 0
+    p.check(max_kv=64)
+
+
+@pytest.mark.parametrize("max_kv", [0, 1, 300, 5000, 100000])
+def test_the_bound_on_the_lengths_does_not_change_results(max_kv):
+    Problem([1, 1], [1500, 300], 8, 2, 64, 16).check(max_kv=max_kv)
+
+
+def test_a_poisoned_block_reaches_only_rows_that_see_it():
+    p = Problem([1, 40, 1], [64, 64, 64], 8, 2, 64, 16)
+    first = int(p.table[1, 3])                     # tokens 48 ... 63 of the sequence with 40 queries (24 ... 63)
+    p.cache[3][first] = float("nan")
+    p.cache[1][first] = 0.0
+    got = p.run()
+    assert bool(got[0].isfinite().all()) and bool(got[41].isfinite().all())
+    assert bool(got[1:25].isfinite().all()) and bool(got[25:41].isnan().all())
+    p = Problem([1, 40, 1], [64, 64, 64], 8, 2, 64, 16)
+    p.cache[2][int(p.table[1, 3])] = float("nan")
+    got = p.run()
+    assert bool(got[1:25].isfinite().all()) and bool(got[25:41].isnan().all()) and bool(got[41].isfinite().all())
+
+
+def test_large_scores_and_uneven_scales():
+    p = Problem([1, 50], [500, 200], 8, 2, 64, 16, scale=3.0)
+    p.check()
+    p = Problem([1, 50], [500, 200], 8, 2, 64, 16, torch.int8)
+    p.cache[3] *= torch.exp2(torch.randint(-6, 7, p.cache[3].shape, generator=sp.gen(1)).float())
+    p.cache[2] *= torch.exp2(torch.randint(-3, 2, p.cache[2].shape, generator=sp.gen(2)).float())
+    p.check()
+    Problem([3, 70], [90, 70], 8, 2, 64, 16, scale=-0.2).check()
+
+
+def test_the_same_call_twice_gives_the_same_bits():
+    p = Problem([1, 1, 130], [3000, 2000, 700], 8, 2, 128, 16)
+    assert torch.equal(p.run(), p.run())
