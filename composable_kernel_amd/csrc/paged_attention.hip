@@ -17,15 +17,8 @@ namespace ckx {
 namespace {
 
 constexpr int kWaves = 4;
-
-// 8 (4) bytes of each of four tokens -> per element the four tokens' bytes
-__device__ __forceinline__ void transpose4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t (&o)[4])
-{
-    const uint32_t ab0 = __builtin_amdgcn_perm(b, a, 0x05010400u), ab1 = __builtin_amdgcn_perm(b, a, 0x07030602u);
-    const uint32_t cd0 = __builtin_amdgcn_perm(d, c, 0x05010400u), cd1 = __builtin_amdgcn_perm(d, c, 0x07030602u);
-    o[0] = __builtin_amdgcn_perm(cd0, ab0, 0x05040100u), o[1] = __builtin_amdgcn_perm(cd0, ab0, 0x07060302u);
-    o[2] = __builtin_amdgcn_perm(cd1, ab1, 0x05040100u), o[3] = __builtin_amdgcn_perm(cd1, ab1, 0x07060302u);
-}
+// query rows of a sequence (tokens x heads of a group), on average, past which the kernel for prompts takes over
+constexpr int kPromptRows = 32;
 
 template <typename T>
 __device__ __forceinline__ f32x4 mfma_qk(const i32x4& k, const i32x4& q, const f32x4& c)
@@ -306,21 +299,27 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs p)
 struct Plan
 {
     int tile_tokens, tile_heads, head_tiles, tiles, splits;
+    bool prompt;
 };
 
 Plan plan(const ckx_kv_cache8& c, int batch, int tokens, int heads, int max_kv, int max_blocks)
 {
     Plan p;
     const int group = heads / c.num_heads;
-    p.tile_heads  = group < 16 ? group : 16;
-    p.head_tiles  = (group + p.tile_heads - 1) / p.tile_heads;
-    p.tile_tokens = 16 / p.tile_heads;
-    p.tiles       = p.tile_tokens == 1 ? tokens : tokens / p.tile_tokens + batch;
+    p.prompt        = (int64_t)tokens * group > (int64_t)kPromptRows * batch;
+    const int rows  = p.prompt ? 128 : 16, most_heads = p.prompt ? 32 : 16;
+    p.tile_heads    = group < most_heads ? group : most_heads;
+    p.head_tiles    = (group + p.tile_heads - 1) / p.tile_heads;
+    p.tile_tokens   = rows / p.tile_heads;
+    p.tiles         = p.tile_tokens == 1 ? tokens : tokens / p.tile_tokens + batch;
+    p.splits        = 1;
+    if(p.prompt)
+        return p;
     // shares: about four workgroups a CU, none of under 256 tokens (two steps a wave)
-    const int64_t groups = (int64_t)(p.tile_tokens == 1 ? tokens : tokens < p.tiles ? tokens : p.tiles) * c.num_heads * p.head_tiles;
-    const int64_t most   = (int64_t)max_blocks * c.block_size;
-    const int64_t kv     = max_kv < most ? max_kv : most;
-    int64_t splits       = (1024 + groups - 1) / groups;
+    const int64_t groups = (int64_t)(tokens < p.tiles ? tokens : p.tiles) * c.num_heads * p.head_tiles;
+    const int64_t longest = (int64_t)max_blocks * c.block_size;
+    const int64_t kv      = max_kv < longest ? max_kv : longest;
+    int64_t splits        = (1024 + groups - 1) / groups;
     if(splits > kv / 256)
         splits = kv / 256;
     p.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
@@ -369,6 +368,8 @@ hipError_t attention_launch(AttentionArgs a, int q_type, hipStream_t s)
 {
     const Plan p  = plan(a.cache, a.batch, a.tokens, a.heads, a.max_kv, a.max_blocks);
     a.tile_tokens = p.tile_tokens, a.tile_heads = p.tile_heads, a.head_tiles = p.head_tiles, a.tiles = p.tiles, a.splits = p.splits;
+    if(p.prompt)
+        return attention_tile_launch(a, q_type, s);
     return q_type == CKX_TYPE_F16 ? launch<_Float16>(a, s) : launch<__bf16>(a, s);
 }
 

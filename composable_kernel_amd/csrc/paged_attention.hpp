@@ -61,6 +61,15 @@ struct ValueScale
     __device__ __forceinline__ float of(float x) const { return x * inv; }
 };
 
+// four bytes of each of four tokens -> per element the four tokens' bytes
+__device__ __forceinline__ void transpose4(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t (&o)[4])
+{
+    const uint32_t ab0 = __builtin_amdgcn_perm(b, a, 0x05010400u), ab1 = __builtin_amdgcn_perm(b, a, 0x07030602u);
+    const uint32_t cd0 = __builtin_amdgcn_perm(d, c, 0x05010400u), cd1 = __builtin_amdgcn_perm(d, c, 0x07030602u);
+    o[0] = __builtin_amdgcn_perm(cd0, ab0, 0x05040100u), o[1] = __builtin_amdgcn_perm(cd0, ab0, 0x07060302u);
+    o[2] = __builtin_amdgcn_perm(cd1, ab1, 0x05040100u), o[3] = __builtin_amdgcn_perm(cd1, ab1, 0x07060302u);
+}
+
 // What a tile is about: its sequence, its tokens and how far they see. The sequence is found by all lanes at once: sequence b's
 // tiles begin at cu[b] / tile_tokens + b (cu[b] with one token a tile), which leaves every sequence enough of them.
 struct TileOf
@@ -98,5 +107,7 @@ __device__ __forceinline__ TileOf tile_of(const AttentionArgs& p, int tile)
 
 // sums of one share of the cached tokens, per query row: what the second pass joins
 __host__ __device__ inline int64_t attention_rows(const AttentionArgs& p) { return (int64_t)p.tokens * p.heads; }
+
+hipError_t attention_tile_launch(const AttentionArgs& a, int q_type, hipStream_t s); // paged_attention_tile.hip
 
 } // namespace ckx
