@@ -10,7 +10,7 @@
 //            d) are ordered so that a lane ends with 16 neighbouring elements of each 32.
 // LDS rows of 16-byte chunks, chunk c of row r at c ^ (r & 15) (keys of 128), c ^ (r & 7) (keys of 64), c ^ ((r ^ r / 4) & 7)
 // (values): eight neighbouring rows never meet on a bank, neither for the writes nor for the reads.
-// What bounds it are vector instructions: 8 a score (the exponential counts four), about as many cycles as the matrix
+// What bounds it are vector instructions: 7 a score (the exponential counts four), about as many cycles as the matrix
 // instructions take, and the two share the SIMD's issue.
 #include "paged_attention.hpp"
 
@@ -81,18 +81,22 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
         qf[k] = i32x4{0, 0, 0, 0};
         if(row_live && 16 * k < D)
             qf[k] = *reinterpret_cast<const i32x4*>(reinterpret_cast<const T*>(p.q) + token * p.sq_t + (int64_t)head * p.sq_h + 16 * k + 8 * h);
+        // (a negative score scale: its sign goes here, so that the largest score is the largest product)
+        if(p.scale < 0.0f)
+            qf[k] ^= (int)0x80008000;
     }
 
-    // uniform loads through the scalar cache
-    typedef const __attribute__((address_space(4))) int* int_ptr;
-    typedef const __attribute__((address_space(4))) float* float_ptr;
-    const int_ptr table  = (int_ptr)(p.table + (int64_t)tile.b * p.stride_table);
-    const float_ptr ksp = (float_ptr)(p.cache.p_k_scale + kvh), vsp = (float_ptr)(p.cache.p_v_scale + kvh);
-    // number of the block that holds token t, -1 for none
-    auto block_of = [&](int t) {
+    // Block numbers and scales of a step: lane b (and 4 + b) has those of its b-th 16 tokens, keys (values). They are asked for a
+    // step, the numbers two steps ahead, in front of the codes' loads: through the scalar cache every wait for an LDS read would
+    // wait for them as well.
+    const int* const table = p.table + (int64_t)tile.b * p.stride_table;
+    const float* const scales = (lane & 4 ? p.cache.p_v_scale : p.cache.p_k_scale) + kvh;
+    auto blocks_of = [&](int step) {
+        const int t = step * kStep + 16 * (lane & 3);
         const int b = t < most ? table[t >> p.block_shift] : -1;
-        return b >= 0 && b < p.cache.num_blocks ? b : -1;
+        return b >= 0 && b < p.cache.num_blocks ? b : -1; // (-1: no such block)
     };
+    auto scales_of = [&](int blocks) { return blocks >= 0 ? scales[(int64_t)blocks * p.cache.stride_scale] : 0.0f; };
     const uint8_t* const kc = reinterpret_cast<const uint8_t*>(p.cache.p_k) + (int64_t)kvh * p.cache.stride_head;
     const uint8_t* const vc = reinterpret_cast<const uint8_t*>(p.cache.p_v) + (int64_t)kvh * p.cache.stride_head;
     const int in_block      = (1 << p.block_shift) - 1;
@@ -105,35 +109,42 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
     uint32_t vb[8];
     const int kt = lane >> 2, kq = lane & 3;
     const int vh = lane / VL, vd = (lane % VL) * 4;     // half, element
+    // (columns behind head_dim repeat its last ones: q is zero there, and no one stores such an element of the output)
+    uint32_t k_off[KB];
+#pragma unroll
+    for(int j = 0; j < KB; ++j)
+        k_off[j] = (uint32_t)kt * p.cache.stride_token + min(kq * (DP / 4) + 16 * j, D - 16);
+    const uint32_t v_off = (uint32_t)(4 * (vh & 1)) * p.cache.stride_token + min(vd, D - 4);
     auto fetch = [&](int step, int block) {
-        const int t = step * kStep + wave * 16;
+        if(block < 0)
+        {
+#pragma unroll
+            for(int j = 0; j < KB; ++j)
+                kb[j] = u32x4{0, 0, 0, 0};
+#pragma unroll
+            for(int i = 0; i < 8; ++i)
+                vb[i] = 0;
+            return;
+        }
+        const int64_t at       = (int64_t)block * p.cache.stride_block + (int64_t)((step * kStep + wave * 16) & in_block) * p.cache.stride_token;
+        const uint8_t* const k = kc + at;
+        const uint8_t* const v = vc + at;
 #pragma unroll
         for(int j = 0; j < KB; ++j)
-            kb[j] = u32x4{0, 0, 0, 0};
+            kb[j] = *reinterpret_cast<const u32x4*>(k + k_off[j]);
 #pragma unroll
         for(int i = 0; i < 8; ++i)
-            vb[i] = 0;
-        if(block < 0)
-            return;
-        const uint8_t* const k = kc + (int64_t)block * p.cache.stride_block + (int64_t)((t & in_block) + kt) * p.cache.stride_token;
-        const uint8_t* const v = vc + (int64_t)block * p.cache.stride_block + (int64_t)(t & in_block) * p.cache.stride_token + vd;
-#pragma unroll
-        for(int j = 0; j < KB; ++j)
-            if(kq * (DP / 4) + 16 * j < D)
-                kb[j] = *reinterpret_cast<const u32x4*>(k + kq * (DP / 4) + 16 * j);
-        if(vh < 2 && vd < D)
+            vb[i] = *reinterpret_cast<const uint32_t*>(v + (int64_t)(8 * (i >> 2) + (i & 3)) * p.cache.stride_token + v_off);
+    };
+    auto deposit = [&](int step) {
+        const int t = step * kStep + wave * 16;
+        if(t + 16 > most) // (what lies behind the last token is no value: zero, whatever its bytes are)
         {
 #pragma unroll
             for(int i = 0; i < 8; ++i)
-            {
-                const int at = 8 * (i >> 2) + 4 * vh + (i & 3);
-                if(t + at < most) // (what lies behind the last token is no value: zero, whatever its bytes are)
-                    vb[i] = *reinterpret_cast<const uint32_t*>(v + (int64_t)at * p.cache.stride_token);
-            }
+                vb[i] = t + 8 * (i >> 2) + 4 * vh + (i & 3) < most ? vb[i] : 0;
         }
-    };
-    auto deposit = [&](int stage) {
-        uint8_t* const kl = lds + stage * STAGE;
+        uint8_t* const kl = lds + (step & 1) * STAGE;
         uint8_t* const vl = kl + K_TILE;
         const int krow    = wave * 16 + kt;
 #pragma unroll
@@ -168,54 +179,56 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
     float m = -__builtin_inff(), l = 0.0f;
     ValueScale unit;
 
-    int mine = block_of(wave * 16);
-    fetch(0, mine);
-    mine = block_of(kStep + wave * 16);
+    auto lane_of = [](auto x, int from) {
+        return __builtin_bit_cast(decltype(x), __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), from));
+    };
+    int blocks = blocks_of(0), blocks_next = blocks_of(1);
+    float scale = scales_of(blocks), scale_next = 0.0f;
+    fetch(0, lane_of(blocks, wave));
     deposit(0);
     __syncthreads();
     for(int step = 0; step < steps; ++step)
     {
         const bool more = step + 1 < steps;
+        const uint32_t there = (uint32_t)__ballot(blocks >= 0) & 15u; // (a bit for each 16 tokens)
         if(more)
         {
-            fetch(step + 1, mine);
-            mine = block_of((step + 2) * kStep + wave * 16);
+            blocks     = blocks_next;
+            scale_next = scales_of(blocks);
+            fetch(step + 1, lane_of(blocks, wave));
+            blocks_next = blocks_of(step + 2);
         }
         const int t0 = step * kStep;
         if(t0 < furthest)
         {
             const uint8_t* const kl = lds + (step & 1) * STAGE;
             const uint8_t* const vl = kl + K_TILE;
-            float c[4], vs[4];
-            bool whole = t0 + kStep <= least;
-            bool there[4];
+            // The value scales relative to the largest so far go into the exponent, exp2(score - m + log2 w), which saves a multiplication a
+            // score; the sum of the probabilities takes them out again, 16 tokens at a time. (The least: no 1 / w is infinite.)
+            float keep_v = 1.0f;
+            if(__any((lane & 4) && scale > unit.top))
+                keep_v = unit.take(lane_of(scale, 4), lane_of(scale, 5)) * unit.take(lane_of(scale, 6), lane_of(scale, 7));
+            const float rel = unit.of(scale), wl = rel < kTinyAmax ? kTinyAmax : rel;
+            const float wl_log = __builtin_amdgcn_logf(wl), wl_inv = __builtin_amdgcn_rcpf(wl);
+            float c[4], w_log[4], w_inv[4];
 #pragma unroll
             for(int b = 0; b < 4; ++b)
             {
-                const int block = block_of(t0 + 16 * b);
-                there[b]        = block >= 0;
-                whole &= there[b];
-                c[b]  = there[b] ? ksp[(int64_t)block * p.cache.stride_scale] * p.scale : 0.0f;
-                vs[b] = there[b] ? vsp[(int64_t)block * p.cache.stride_scale] : 0.0f;
+                c[b]     = lane_of(scale, b) * __builtin_fabsf(p.scale);
+                w_log[b] = lane_of(wl_log, 4 + b);
+                w_inv[b] = lane_of(wl_inv, 4 + b);
             }
+            const bool whole = t0 + kStep <= least && there == 15u;
             f32x16 s[2];
 #pragma unroll
             for(int u = 0; u < 2; ++u)
             {
-#pragma unroll
-                for(int i = 0; i < 16; ++i)
-                    s[u][i] = 0.0f;
                 const int krow = 32 * u + r;
 #pragma unroll
                 for(int k = 0; k < KK; ++k)
-                    s[u] = mfma32<T>(*reinterpret_cast<const i32x4*>(kl + krow * (DP * 2) + (((2 * k + h) ^ (krow & (KC - 1))) << 4)), qf[k], s[u]);
+                    s[u] = mfma32<T>(*reinterpret_cast<const i32x4*>(kl + krow * (DP * 2) + (((2 * k + h) ^ (krow & (KC - 1))) << 4)), qf[k],
+                                     k == 0 ? f32x16(0.0f) : s[u]);
             }
-            float top = -__builtin_inff();
-#pragma unroll
-            for(int u = 0; u < 2; ++u)
-#pragma unroll
-                for(int i = 0; i < 16; ++i)
-                    s[u][i] *= c[2 * u + (i >> 3)];
             if(!whole)
             {
 #pragma unroll
@@ -224,52 +237,57 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
                     for(int i = 0; i < 16; ++i)
                     {
                         const int t = t0 + 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
-                        s[u][i]     = there[2 * u + (i >> 3)] && t < see ? s[u][i] : -__builtin_inff();
+                        s[u][i]     = (there >> (2 * u + (i >> 3)) & 1) && t < see ? s[u][i] : -__builtin_inff();
                     }
             }
+            // (the maximum is there for the range only: of the unscaled scores of 16 tokens, then scaled; and it is raised only by
+            // leaps, 2^6 or more, so that the sums are seldom rescaled: no probability exceeds 2^6 then)
+            float top = -__builtin_inff();
 #pragma unroll
-            for(int u = 0; u < 2; ++u)
+            for(int b = 0; b < 4; ++b)
+            {
+                float x = s[b >> 1][8 * (b & 1)];
 #pragma unroll
-                for(int i = 0; i < 16; ++i)
-                    top = __builtin_fmaxf(top, s[u][i]);
-            const float now  = __builtin_fmaxf(m, over_halves(top, [](float a, float b) { return __builtin_fmaxf(a, b); }));
-            const float zero = now == -__builtin_inff() ? 0.0f : now; // (nothing seen yet: exp2(-inf - 0) = 0)
-            const float keep = __builtin_amdgcn_exp2f(m - zero);
-            m                = now;
-            const float keep_o = keep * unit.take(vs[0], vs[1]) * unit.take(vs[2], vs[3]);
+                for(int i = 1; i < 8; ++i)
+                    x = __builtin_fmaxf(x, s[b >> 1][8 * (b & 1) + i]);
+                top = __builtin_fmaxf(top, x == -__builtin_inff() ? x : x * c[b]);
+            }
+            top = over_halves(top, [](float a, float b) { return __builtin_fmaxf(a, b); });
+            float keep_o = keep_v;
+            if(__any(top > m + 6.0f))
+            {
+                const float now = __builtin_fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - (now == -__builtin_inff() ? 0.0f : now));
+                m = now;
+                l *= keep;
+                keep_o *= keep;
+            }
             if(__any(keep_o != 1.0f))
             {
-                l *= keep;
 #pragma unroll
                 for(int j = 0; j < DT; ++j)
                     o[j] *= keep_o;
             }
-            float w[4];
-#pragma unroll
-            for(int b = 0; b < 4; ++b)
-                w[b] = unit.of(vs[b]);
+            const float zero = m == -__builtin_inff() ? 0.0f : m; // (nothing seen yet)
             i32x4 pf[4];
 #pragma unroll
-            for(int u = 0; u < 2; ++u)
+            for(int b = 0; b < 4; ++b)
             {
-                float pr[16];
+                const float bias = w_log[b] - zero;
+                float pr[8], sum = 0.0f;
 #pragma unroll
-                for(int i = 0; i < 16; ++i)
-                {
-                    pr[i] = __builtin_amdgcn_exp2f(s[u][i] - zero);
-                    l += pr[i];
-                    pr[i] *= w[2 * u + (i >> 3)];
-                }
-                if(!whole) // (masked: no value scale, which may be an infinity or NaN, gets into the sum)
+                for(int i = 0; i < 8; ++i)
+                    pr[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b >> 1][8 * (b & 1) + i], c[b], bias));
+                if(!whole) // (masked: zero, whatever the scales are)
                 {
 #pragma unroll
-                    for(int i = 0; i < 16; ++i)
-                        pr[i] = s[u][i] == -__builtin_inff() ? 0.0f : pr[i];
+                    for(int i = 0; i < 8; ++i)
+                        pr[i] = s[b >> 1][8 * (b & 1) + i] == -__builtin_inff() ? 0.0f : pr[i];
                 }
 #pragma unroll
-                for(int k = 0; k < 2; ++k)
-                    pf[2 * u + k] = i32x4{(int)pack_f16(pr[8 * k], pr[8 * k + 1]), (int)pack_f16(pr[8 * k + 2], pr[8 * k + 3]),
-                                          (int)pack_f16(pr[8 * k + 4], pr[8 * k + 5]), (int)pack_f16(pr[8 * k + 6], pr[8 * k + 7])};
+                for(int i = 0; i < 8; ++i)
+                    sum += pr[i];
+                l = !whole && sum == 0.0f ? l : __builtin_fmaf(sum, w_inv[b], l);
+                pf[b] = i32x4{(int)pack_f16(pr[0], pr[1]), (int)pack_f16(pr[2], pr[3]), (int)pack_f16(pr[4], pr[5]), (int)pack_f16(pr[6], pr[7])};
             }
 #pragma unroll
             for(int j = 0; j < DT; ++j)
@@ -282,7 +300,8 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
             }
         }
         if(more)
-            deposit((step + 1) & 1);
+            deposit(step + 1);
+        scale = scale_next;
         __syncthreads();
     }
 

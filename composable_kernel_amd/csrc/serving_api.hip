@@ -36,6 +36,8 @@ int check_cache(const ckx_kv_cache8* c)
         return api_fail(CKX_UNSUPPORTED, "slot numbers are 32-bit: at most 2^31 - 1 slots");
     if(c->stride_block % 16 || c->stride_head % 16 || c->stride_token % 16)
         return api_fail(CKX_UNSUPPORTED, "cache strides are multiples of 16");
+    if((int64_t)c->block_size * c->stride_token > 0x7fffffffll)
+        return api_fail(CKX_UNSUPPORTED, "the tokens of a block span 2 GiB");
     if(c->stride_block < 0 || c->stride_head < 0 || c->stride_token < c->head_dim || c->stride_scale < 0)
         return api_fail(CKX_UNSUPPORTED, "cache strides: tokens at least head_dim apart, none negative");
     // every (block, head, token) has bytes of its own: the three strides nest, heads and tokens in either order

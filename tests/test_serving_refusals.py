@@ -116,6 +116,7 @@ BAD_CACHES = [
     (dict(head=512), capi.UNSUPPORTED),              # heads on each other
     (dict(block=1024), capi.UNSUPPORTED),
     (dict(scale=1), capi.UNSUPPORTED),
+    (dict(heads=1, token=1 << 27, head=0, block=1 << 32), capi.UNSUPPORTED),
     (dict(blocks=1 << 28), capi.UNSUPPORTED),        # slot numbers past 31 bits
 ]
 
