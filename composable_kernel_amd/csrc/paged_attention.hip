@@ -312,41 +312,46 @@ Plan plan(const ckx_kv_cache8& c, int batch, int tokens, int heads, int max_kv, 
     p.head_tiles    = (group + p.tile_heads - 1) / p.tile_heads;
     p.tile_tokens   = rows / p.tile_heads;
     p.tiles         = p.tile_tokens == 1 ? tokens : tokens / p.tile_tokens + batch;
-    p.splits        = 1;
-    if(p.prompt)
-        return p;
-    // shares: about four workgroups a CU, none of under 256 tokens (two steps a wave)
-    const int64_t groups = (int64_t)(tokens < p.tiles ? tokens : p.tiles) * c.num_heads * p.head_tiles;
+    // Shares of the cached tokens, joined by a second launch, where the tiles alone leave CUs without work: about four workgroups a
+    // CU and none of under 256 tokens (two steps a wave); prompts: two a CU (what fits on one) and none of under 512 (eight steps)
+    const int64_t groups  = (int64_t)(tokens < p.tiles ? tokens : p.tiles) * c.num_heads * p.head_tiles;
     const int64_t longest = (int64_t)max_blocks * c.block_size;
     const int64_t kv      = max_kv < longest ? max_kv : longest;
-    int64_t splits        = (1024 + groups - 1) / groups;
-    if(splits > kv / 256)
-        splits = kv / 256;
+    int64_t splits        = p.prompt ? 512 / groups : (1024 + groups - 1) / groups;
+    const int64_t least   = p.prompt ? 512 : 256;
+    if(splits > kv / least)
+        splits = kv / least;
     p.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
     return p;
 }
 
 int padded(int head_dim) { return head_dim <= 64 ? 64 : 128; }
 
-template <typename T, int CODE, int DP>
-hipError_t launch(const AttentionArgs& a, hipStream_t s)
+template <typename T, int CODE>
+hipError_t launch_rows(const AttentionArgs& a, hipStream_t s)
 {
-    const int64_t groups = (int64_t)a.tiles * a.cache.num_heads * a.head_tiles * a.splits;
-    hipLaunchKernelGGL((attention_rows_kernel<T, CODE, DP>), dim3((unsigned)groups), dim3(kWaves * 64), 0, s, a);
-    hipError_t e = hipGetLastError();
-    if(e != hipSuccess || a.splits == 1)
-        return e;
-    hipLaunchKernelGGL((attention_join_kernel<T, DP>), dim3((unsigned)((attention_rows(a) + 15) / 16)), dim3(256), 0, s, a);
+    const dim3 grid((unsigned)((int64_t)a.tiles * a.cache.num_heads * a.head_tiles * a.splits));
+    if(padded(a.cache.head_dim) == 64)
+        hipLaunchKernelGGL((attention_rows_kernel<T, CODE, 64>), grid, dim3(kWaves * 64), 0, s, a);
+    else
+        hipLaunchKernelGGL((attention_rows_kernel<T, CODE, 128>), grid, dim3(kWaves * 64), 0, s, a);
     return hipGetLastError();
 }
 
 template <typename T>
-hipError_t launch(const AttentionArgs& a, hipStream_t s)
+hipError_t launch(const AttentionArgs& a, bool prompt, hipStream_t s)
 {
-    const bool e4m3 = a.cache.type == CKX_TYPE_E4M3;
+    hipError_t e = prompt ? attention_tile_launch(a, std::is_same<T, _Float16>::value, s)
+                   : a.cache.type == CKX_TYPE_E4M3 ? launch_rows<T, CODE_E4M3>(a, s)
+                                                   : launch_rows<T, CODE_I8>(a, s);
+    if(e != hipSuccess || a.splits == 1)
+        return e;
+    const dim3 grid((unsigned)((attention_rows(a) + 15) / 16));
     if(padded(a.cache.head_dim) == 64)
-        return e4m3 ? launch<T, CODE_E4M3, 64>(a, s) : launch<T, CODE_I8, 64>(a, s);
-    return e4m3 ? launch<T, CODE_E4M3, 128>(a, s) : launch<T, CODE_I8, 128>(a, s);
+        hipLaunchKernelGGL((attention_join_kernel<T, 64>), grid, dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((attention_join_kernel<T, 128>), grid, dim3(256), 0, s, a);
+    return hipGetLastError();
 }
 
 } // namespace
@@ -368,9 +373,7 @@ hipError_t attention_launch(AttentionArgs a, int q_type, hipStream_t s)
 {
     const Plan p  = plan(a.cache, a.batch, a.tokens, a.heads, a.max_kv, a.max_blocks);
     a.tile_tokens = p.tile_tokens, a.tile_heads = p.tile_heads, a.head_tiles = p.head_tiles, a.tiles = p.tiles, a.splits = p.splits;
-    if(p.prompt)
-        return attention_tile_launch(a, q_type, s);
-    return q_type == CKX_TYPE_F16 ? launch<_Float16>(a, s) : launch<__bf16>(a, s);
+    return q_type == CKX_TYPE_F16 ? launch<_Float16>(a, p.prompt, s) : launch<__bf16>(a, p.prompt, s);
 }
 
 } // namespace ckx

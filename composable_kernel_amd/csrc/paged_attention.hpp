@@ -108,6 +108,6 @@ __device__ __forceinline__ TileOf tile_of(const AttentionArgs& p, int tile)
 // sums of one share of the cached tokens, per query row: what the second pass joins
 __host__ __device__ inline int64_t attention_rows(const AttentionArgs& p) { return (int64_t)p.tokens * p.heads; }
 
-hipError_t attention_tile_launch(const AttentionArgs& a, int q_type, hipStream_t s); // paged_attention_tile.hip
+hipError_t attention_tile_launch(const AttentionArgs& a, bool f16, hipStream_t s); // paged_attention_tile.hip
 
 } // namespace ckx

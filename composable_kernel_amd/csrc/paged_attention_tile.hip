@@ -53,6 +53,8 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
 
     // the last tiles first: with the causal mask they have the most to do
     int id              = (int)(gridDim.x - 1 - blockIdx.x);
+    const int split     = id % p.splits;
+    id /= p.splits;
     const int per_tile  = p.cache.num_heads * p.head_tiles;
     const int head_tile = id % per_tile;
     const TileOf tile   = tile_of(p, id / per_tile);
@@ -66,7 +68,9 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
     const int see       = row_live ? (p.causal ? tile.kv - (tile.q_len - 1 - (tile.first + rt)) : tile.kv) : 0;
     const int last      = min(tile.first + p.tile_tokens, tile.q_len) - 1;
     const int most      = max(p.causal ? tile.kv - (tile.q_len - 1 - last) : tile.kv, 0);
-    const int steps     = (most + kStep - 1) / kStep;
+    // the share of the cached tokens: an even number of steps
+    const int all_steps = (most + kStep - 1) / kStep, per = ((all_steps + p.splits - 1) / p.splits + 1) & ~1;
+    const int begin = min(split * per, (all_steps + 1) & ~1), steps = min(begin + per, all_steps);
     // the least and the most that a live row of this wave sees
     int least = row_live ? see : 0x7fffffff, furthest = see;
 #pragma unroll
@@ -105,8 +109,8 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
     // tokens (as above) times four (two) elements
     constexpr int KB = DP / 64, VL = DP / 4;            // 16-byte loads of a lane's quarter; lanes of a value row's four elements
     constexpr int VG = 64 / VL;                         // token halves side by side in a wave (DP 128: 2; DP 64: 4, two of them idle)
-    u32x4 kb[KB];
-    uint32_t vb[8];
+    u32x4 kb[2][KB]; // (of even and odd steps)
+    uint32_t vb[2][8];
     const int kt = lane >> 2, kq = lane & 3;
     const int vh = lane / VL, vd = (lane % VL) * 4;     // half, element
     // (columns behind head_dim repeat its last ones: q is zero there, and no one stores such an element of the output)
@@ -115,15 +119,16 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
     for(int j = 0; j < KB; ++j)
         k_off[j] = (uint32_t)kt * p.cache.stride_token + min(kq * (DP / 4) + 16 * j, D - 16);
     const uint32_t v_off = (uint32_t)(4 * (vh & 1)) * p.cache.stride_token + min(vd, D - 4);
-    auto fetch = [&](int step, int block) {
+    auto fetch = [&](int step, int block, auto odd) {
+        constexpr int S = decltype(odd)::value;
         if(block < 0)
         {
 #pragma unroll
             for(int j = 0; j < KB; ++j)
-                kb[j] = u32x4{0, 0, 0, 0};
+                kb[S][j] = u32x4{0, 0, 0, 0};
 #pragma unroll
             for(int i = 0; i < 8; ++i)
-                vb[i] = 0;
+                vb[S][i] = 0;
             return;
         }
         const int64_t at       = (int64_t)block * p.cache.stride_block + (int64_t)((step * kStep + wave * 16) & in_block) * p.cache.stride_token;
@@ -131,45 +136,48 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
         const uint8_t* const v = vc + at;
 #pragma unroll
         for(int j = 0; j < KB; ++j)
-            kb[j] = *reinterpret_cast<const u32x4*>(k + k_off[j]);
+            kb[S][j] = *reinterpret_cast<const u32x4*>(k + k_off[j]);
 #pragma unroll
         for(int i = 0; i < 8; ++i)
-            vb[i] = *reinterpret_cast<const uint32_t*>(v + (int64_t)(8 * (i >> 2) + (i & 3)) * p.cache.stride_token + v_off);
+            vb[S][i] = *reinterpret_cast<const uint32_t*>(v + (int64_t)(8 * (i >> 2) + (i & 3)) * p.cache.stride_token + v_off);
     };
-    auto deposit = [&](int step) {
+    // element 32 j + 16 a + 4 x + y lies in row 32 j + 8 x + 4 a + y
+    const int krow = wave * 16 + kt, vrow = (vd & ~31) + (((vd >> 2) & 3) << 3) + (((vd >> 4) & 1) << 2);
+    const uint32_t k_write = krow * (DP * 2) + (((kq * (KC / 4)) ^ (krow & (KC - 1))) << 4);
+    const uint32_t v_write = K_TILE + vrow * (kStep * 2) + (((2 * wave + vh) ^ ((vrow ^ (vrow >> 2)) & 7)) << 4);
+    auto deposit = [&](int step, auto odd) {
+        constexpr int S = decltype(odd)::value;
         const int t = step * kStep + wave * 16;
         if(t + 16 > most) // (what lies behind the last token is no value: zero, whatever its bytes are)
         {
 #pragma unroll
             for(int i = 0; i < 8; ++i)
-                vb[i] = t + 8 * (i >> 2) + 4 * vh + (i & 3) < most ? vb[i] : 0;
+                vb[S][i] = t + 8 * (i >> 2) + 4 * vh + (i & 3) < most ? vb[S][i] : 0;
         }
-        uint8_t* const kl = lds + (step & 1) * STAGE;
-        uint8_t* const vl = kl + K_TILE;
-        const int krow    = wave * 16 + kt;
+        uint32_t k_to = k_write + (step & 1) * STAGE, v_to = v_write + (step & 1) * STAGE;
+        asm volatile("" : "+v"(k_to), "+v"(v_to));
 #pragma unroll
         for(int j = 0; j < KB; ++j)
 #pragma unroll
             for(int e = 0; e < 2; ++e)
             {
-                const int c = kq * (KC / 4) + 2 * j + e;
-                *reinterpret_cast<i32x4*>(kl + krow * (DP * 2) + ((c ^ (krow & (KC - 1))) << 4)) = codes8<CODE, T>(kb[j][2 * e], kb[j][2 * e + 1]);
+                const int c = 2 * j + e; // (+ kq * KC / 4, whose bits are higher ones)
+                *reinterpret_cast<i32x4*>(lds + (k_to ^ (uint32_t)(c << 4))) = codes8<CODE, T>(kb[S][j][2 * e], kb[S][j][2 * e + 1]);
             }
         if(vh < 2)
         {
             uint32_t lo[4], hi[4];
-            transpose4(vb[0], vb[1], vb[2], vb[3], lo);
-            transpose4(vb[4], vb[5], vb[6], vb[7], hi);
+            transpose4(vb[S][0], vb[S][1], vb[S][2], vb[S][3], lo);
+            transpose4(vb[S][4], vb[S][5], vb[S][6], vb[S][7], hi);
 #pragma unroll
             for(int i = 0; i < 4; ++i)
             {
-                // element 32 j + 16 a + 4 x + y lies in row 32 j + 8 x + 4 a + y
-                const int vrow = (vd & ~31) + (((vd >> 2) & 3) << 3) + (((vd >> 4) & 1) << 2) + i, c = 2 * wave + vh;
-                *reinterpret_cast<i32x4*>(vl + vrow * (kStep * 2) + ((c ^ ((vrow ^ (vrow >> 2)) & 7)) << 4)) = codes8<CODE, _Float16>(lo[i], hi[i]);
+                *reinterpret_cast<i32x4*>(lds + (v_to ^ (uint32_t)(i << 4)) + i * (kStep * 2)) = codes8<CODE, _Float16>(lo[i], hi[i]);
             }
         }
     };
 
+    const uint32_t k_read = r * (DP * 2) + ((h ^ (r & (KC - 1))) << 4), v_read = K_TILE + r * (kStep * 2) + ((h ^ ((r ^ (r >> 2)) & 7)) << 4);
     f32x16 o[DT];
 #pragma unroll
     for(int j = 0; j < DT; ++j)
@@ -182,27 +190,27 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
     auto lane_of = [](auto x, int from) {
         return __builtin_bit_cast(decltype(x), __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), from));
     };
-    int blocks = blocks_of(0), blocks_next = blocks_of(1);
-    float scale = scales_of(blocks), scale_next = 0.0f;
-    fetch(0, lane_of(blocks, wave));
-    deposit(0);
+    std::integral_constant<int, 0> even;
+    std::integral_constant<int, 1> odd;
+    // of this step and the two behind it; their codes are fetched two steps ahead
+    int blocks = blocks_of(begin), blocks1 = blocks_of(begin + 1), blocks2 = blocks_of(begin + 2);
+    float scale = scales_of(blocks), scale1 = scales_of(blocks1);
+    fetch(begin, lane_of(blocks, wave), even);
+    fetch(begin + 1, lane_of(blocks1, wave), odd);
+    deposit(begin, even);
     __syncthreads();
-    for(int step = 0; step < steps; ++step)
-    {
-        const bool more = step + 1 < steps;
+    auto one_step = [&](int step, auto mine, auto other) {
         const uint32_t there = (uint32_t)__ballot(blocks >= 0) & 15u; // (a bit for each 16 tokens)
-        if(more)
-        {
-            blocks     = blocks_next;
-            scale_next = scales_of(blocks);
-            fetch(step + 1, lane_of(blocks, wave));
-            blocks_next = blocks_of(step + 2);
-        }
+        // (behind the last step: no block, nothing read)
+        const float scale2 = scales_of(blocks2);
+        const int blocks3  = blocks_of(step + 3);
+        fetch(step + 2, lane_of(blocks2, wave), mine);
         const int t0 = step * kStep;
-        if(t0 < furthest)
-        {
-            const uint8_t* const kl = lds + (step & 1) * STAGE;
-            const uint8_t* const vl = kl + K_TILE;
+        auto multiply = [&](bool whole) {
+            // chunk 2 k + h of a row: k's bits flip those of k = 0. (Worked out in every step: kept over the loop, the addresses are
+            // twelve registers that the kernel has not got.)
+            uint32_t k_at = k_read + (step & 1) * STAGE, v_at = v_read + (step & 1) * STAGE;
+            asm volatile("" : "+v"(k_at), "+v"(v_at));
             // The value scales relative to the largest so far go into the exponent, exp2(score - m + log2 w), which saves a multiplication a
             // score; the sum of the probabilities takes them out again, 16 tokens at a time. (The least: no 1 / w is infinite.)
             float keep_v = 1.0f;
@@ -215,29 +223,44 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
             for(int b = 0; b < 4; ++b)
             {
                 c[b]     = lane_of(scale, b) * __builtin_fabsf(p.scale);
+                c[b]     = c[b] < kTinyAmax ? kTinyAmax : c[b]; // (no -inf times zero; NaN stays)
                 w_log[b] = lane_of(wl_log, 4 + b);
                 w_inv[b] = lane_of(wl_inv, 4 + b);
             }
-            const bool whole = t0 + kStep <= least && there == 15u;
             f32x16 s[2];
+            constexpr int DQ = 2; // fragments DQ pairs of instructions ahead: an LDS read takes about as long as three of them
+            i32x4 kf[DQ + 1][2];
+            auto read_k = [&](int k) {
 #pragma unroll
-            for(int u = 0; u < 2; ++u)
+                for(int u = 0; u < 2; ++u)
+                    kf[k % (DQ + 1)][u] = *reinterpret_cast<const i32x4*>(lds + (k_at ^ (uint32_t)(k << 5)) + u * 32 * DP * 2);
+            };
+#pragma unroll
+            for(int k = 0; k < DQ; ++k)
+                read_k(k);
+#pragma unroll
+            for(int k = 0; k < KK; ++k)
             {
-                const int krow = 32 * u + r;
+                if(k + DQ < KK)
+                    read_k(k + DQ);
 #pragma unroll
-                for(int k = 0; k < KK; ++k)
-                    s[u] = mfma32<T>(*reinterpret_cast<const i32x4*>(kl + krow * (DP * 2) + (((2 * k + h) ^ (krow & (KC - 1))) << 4)), qf[k],
-                                     k == 0 ? f32x16(0.0f) : s[u]);
+                for(int u = 0; u < 2; ++u)
+                    s[u] = mfma32<T>(kf[k % (DQ + 1)][u], qf[k], k == 0 ? f32x16(0.0f) : s[u]);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            const int reach = see - t0 - 4 * h;
             if(!whole)
             {
+                // (a branch: without these the compiler masks every step)
+                asm volatile("" : "+v"(s[0]));
+                asm volatile("" : "+v"(s[1]));
 #pragma unroll
                 for(int u = 0; u < 2; ++u)
 #pragma unroll
                     for(int i = 0; i < 16; ++i)
                     {
-                        const int t = t0 + 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
-                        s[u][i]     = (there >> (2 * u + (i >> 3)) & 1) && t < see ? s[u][i] : -__builtin_inff();
+                        const int t = 32 * u + 8 * (i >> 2) + (i & 3);
+                        s[u][i]     = (there >> (2 * u + (i >> 3)) & 1) && t < reach ? s[u][i] : -__builtin_inff();
                     }
             }
             // (the maximum is there for the range only: of the unscaled scores of 16 tokens, then scaled; and it is raised only by
@@ -249,10 +272,12 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
                 float x = s[b >> 1][8 * (b & 1)];
 #pragma unroll
                 for(int i = 1; i < 8; ++i)
-                    x = __builtin_fmaxf(x, s[b >> 1][8 * (b & 1) + i]);
-                top = __builtin_fmaxf(top, x == -__builtin_inff() ? x : x * c[b]);
+                    x = __builtin_elementwise_maximum(x, s[b >> 1][8 * (b & 1) + i]);
+                top = __builtin_elementwise_maximum(top, x == -__builtin_inff() ? x : x * c[b]); // (-inf: nothing seen, whatever the scale is)
             }
-            top = over_halves(top, [](float a, float b) { return __builtin_fmaxf(a, b); });
+            // (maximum, which a NaN wins: one instruction for three values where fmaxf makes every one a quiet number first. A row with a NaN
+            // among its scores raises no maximum any more; it is NaN.)
+            top = over_halves(top, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
             float keep_o = keep_v;
             if(__any(top > m + 6.0f))
             {
@@ -268,46 +293,75 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
                     o[j] *= keep_o;
             }
             const float zero = m == -__builtin_inff() ? 0.0f : m; // (nothing seen yet)
+            i32x4 vf[2][DT];
+            auto read_v = [&](int k) {
+#pragma unroll
+                for(int j = 0; j < DT; ++j)
+                    vf[k & 1][j] = *reinterpret_cast<const i32x4*>(lds + (v_at ^ (uint32_t)(k << 5)) + j * 32 * kStep * 2);
+            };
             i32x4 pf[4];
 #pragma unroll
             for(int b = 0; b < 4; ++b)
             {
-                const float bias = w_log[b] - zero;
+                // a masked score is -inf and its probability zero, but for scales that are no numbers: they are kept from rows
+                // that see none of the lane's eight tokens
+                const bool sees  = whole || reach > 16 * b;
+                const float cb   = sees ? c[b] : 1.0f, bias = sees ? w_log[b] - zero : 0.0f;
                 float pr[8], sum = 0.0f;
 #pragma unroll
                 for(int i = 0; i < 8; ++i)
-                    pr[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b >> 1][8 * (b & 1) + i], c[b], bias));
-                if(!whole) // (masked: zero, whatever the scales are)
                 {
-#pragma unroll
-                    for(int i = 0; i < 8; ++i)
-                        pr[i] = s[b >> 1][8 * (b & 1) + i] == -__builtin_inff() ? 0.0f : pr[i];
-                }
-#pragma unroll
-                for(int i = 0; i < 8; ++i)
+                    pr[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b >> 1][8 * (b & 1) + i], cb, bias));
                     sum += pr[i];
-                l = !whole && sum == 0.0f ? l : __builtin_fmaf(sum, w_inv[b], l);
+                }
+                l     = __builtin_fmaf(sum, sees ? w_inv[b] : 0.0f, l);
                 pf[b] = i32x4{(int)pack_f16(pr[0], pr[1]), (int)pack_f16(pr[2], pr[3]), (int)pack_f16(pr[4], pr[5]), (int)pack_f16(pr[6], pr[7])};
             }
+            read_v(0);
 #pragma unroll
-            for(int j = 0; j < DT; ++j)
+            for(int k = 0; k < 4; ++k)
             {
-                const int vrow = 32 * j + r;
+                if(k < 3)
+                    read_v(k + 1);
 #pragma unroll
-                for(int k = 0; k < 4; ++k)
-                    o[j] = mfma32<_Float16>(*reinterpret_cast<const i32x4*>(vl + vrow * (kStep * 2) + (((2 * k + h) ^ ((vrow ^ (vrow >> 2)) & 7)) << 4)),
-                                            pf[k], o[j]);
+                for(int j = 0; j < DT; ++j)
+                    o[j] = mfma32<_Float16>(vf[k & 1][j], pf[k], o[j]);
             }
-        }
-        if(more)
-            deposit(step + 1);
-        scale = scale_next;
+        };
+        if(t0 < furthest)
+            multiply(t0 + kStep <= least && there == 15u);
+        if(step + 1 < steps)
+            deposit(step + 1, other);
+        blocks = blocks1, blocks1 = blocks2, blocks2 = blocks3;
+        scale = scale1, scale1 = scale2;
         __syncthreads();
+    };
+    for(int step = begin; step < steps; step += 2)
+    {
+        one_step(step, even, odd);
+        if(step + 1 < steps)
+            one_step(step + 1, odd, even);
     }
 
     l = over_halves(l, [](float a, float b) { return a + b; });
     if(!row_live)
         return;
+    if(p.splits > 1)
+    {
+        const int64_t at = (token * p.heads + head) * p.splits + split;
+#pragma unroll
+        for(int j = 0; j < DT; ++j)
+#pragma unroll
+            for(int e = 0; e < 16; e += 4)
+                *reinterpret_cast<f32x4*>(p.ws + at * DP + 32 * j + 16 * h + e) =
+                    f32x4{o[j][e] * unit.top, o[j][e + 1] * unit.top, o[j][e + 2] * unit.top, o[j][e + 3] * unit.top};
+        if(h == 0)
+        {
+            float* const ml = p.ws + attention_rows(p) * p.splits * DP + at * 2;
+            ml[0] = m, ml[1] = l;
+        }
+        return;
+    }
     const float f = l == 0.0f ? 0.0f : unit.top / l; // (a row that sees nothing: zero)
     T* const to   = reinterpret_cast<T*>(p.o) + token * p.so_t + (int64_t)head * p.so_h;
     typedef T tx8 __attribute__((ext_vector_type(8)));
@@ -329,7 +383,7 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
 template <typename T, int CODE>
 hipError_t launch(const AttentionArgs& a, hipStream_t s)
 {
-    const dim3 grid((unsigned)(a.tiles * a.cache.num_heads * a.head_tiles));
+    const dim3 grid((unsigned)((int64_t)a.tiles * a.cache.num_heads * a.head_tiles * a.splits));
     if(a.cache.head_dim <= 64)
         hipLaunchKernelGGL((attention_tile_kernel<T, CODE, 64>), grid, dim3(256), 0, s, a);
     else
@@ -339,11 +393,11 @@ hipError_t launch(const AttentionArgs& a, hipStream_t s)
 
 } // namespace
 
-hipError_t attention_tile_launch(const AttentionArgs& a, int q_type, hipStream_t s)
+hipError_t attention_tile_launch(const AttentionArgs& a, bool f16, hipStream_t s)
 {
     if(a.cache.type == CKX_TYPE_E4M3)
-        return q_type == CKX_TYPE_F16 ? launch<_Float16, CODE_E4M3>(a, s) : launch<__bf16, CODE_E4M3>(a, s);
-    return q_type == CKX_TYPE_F16 ? launch<_Float16, CODE_I8>(a, s) : launch<__bf16, CODE_I8>(a, s);
+        return f16 ? launch<_Float16, CODE_E4M3>(a, s) : launch<__bf16, CODE_E4M3>(a, s);
+    return f16 ? launch<_Float16, CODE_I8>(a, s) : launch<__bf16, CODE_I8>(a, s);
 }
 
 } // namespace ckx

@@ -191,3 +191,11 @@ def test_large_scores_and_uneven_scales():
 def test_the_same_call_twice_gives_the_same_bits():
     p = Problem([1, 1, 130], [3000, 2000, 700], 8, 2, 128, 16)
     assert torch.equal(p.run(), p.run())
+
+
+@pytest.mark.parametrize("code", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("news,kvs", [([64], [3000]), ([33, 40], [2100, 700]), ([100], [4097])])
+def test_prompts_over_long_caches(news, kvs, code):
+    """Few tiles, many cached tokens: the shares of the cached tokens are joined, some of them empty."""
+    Problem(news, kvs, 4, 1, 64, 16, code).check()
+    Problem(news, kvs, 2, 2, 128, 64, code, "f16", causal=False).check()
