@@ -12,7 +12,7 @@ namespace {
 // workgroup; 8192 at most, their two running sums in LDS), then takes its share of the tokens and of the new blocks and finds
 // the sequence of each by bisection. The alternative, one workgroup that sums and a second launch that fills, costs the second
 // launch. What bounds it is that latency: the bytes are few.
-constexpr int kTablesThreads = 256, kTokensPerGroup = 1024;
+constexpr int kTablesThreads = 256, kTokensPerGroup = 4 * kTablesThreads;
 
 __device__ __forceinline__ int blocks_of(int tokens, int shift) { return (int)(((int64_t)tokens + (1 << shift) - 1) >> shift); }
 
@@ -88,17 +88,23 @@ __global__ __launch_bounds__(kTablesThreads) void kv_tables_kernel(TablesArgs p)
         if(col < p.max_blocks)
             p.table[(int64_t)b * p.stride_table + col] = p.free[f];
     }
-    // the slots; a new block comes from the free list itself, not from the table that another workgroup is writing
-    for(int i = 0; i < kTokensPerGroup / kTablesThreads; ++i)
+    // the slots, four neighbours a thread, whose sequence is looked for once; a new block comes from the free list itself, not from
+    // the table that another workgroup is writing
+    const int64_t x0 = (int64_t)blockIdx.x * kTokensPerGroup + tid * 4;
+    if(x0 >= p.num_slots)
+        return;
+    int b = x0 < all_tokens ? last_at_most(cu, p.batch, (int)x0) : 0;
+    int slot[4];
+#pragma unroll
+    for(int i = 0; i < 4; ++i)
     {
-        const int x = blockIdx.x * kTokensPerGroup + i * kTablesThreads + tid;
-        if(x >= p.num_slots)
-            break;
-        int slot = -1;
+        const int64_t x = x0 + i;
+        slot[i]         = -1;
         if(x < all_tokens)
         {
-            const int b = last_at_most(cu, p.batch, x);
-            const int c = max(p.context[b], 0), pos = c + x - cu[b], col = pos >> p.block_shift;
+            while(cu[b + 1] <= (int)x)
+                ++b;
+            const int c = max(p.context[b], 0), pos = c + (int)x - cu[b], col = pos >> p.block_shift;
             const int had = blocks_of(c, p.block_shift);
             int block     = -1;
             if(col < p.max_blocks)
@@ -109,17 +115,26 @@ __global__ __launch_bounds__(kTablesThreads) void kv_tables_kernel(TablesArgs p)
                     block = p.free[base[b] + col - had];
             }
             if(block >= 0)
-                slot = (block << p.block_shift) + (pos & ((1 << p.block_shift) - 1));
+                slot[i] = (block << p.block_shift) + (pos & ((1 << p.block_shift) - 1));
         }
-        p.slots[x] = slot;
     }
+    if(x0 + 4 <= p.num_slots)
+        reinterpret_cast<AnyAlign<i32x4>*>(p.slots + x0)->v = i32x4{slot[0], slot[1], slot[2], slot[3]};
+    else
+#pragma unroll
+        for(int i = 0; i < 3; ++i)
+            if(x0 + i < p.num_slots)
+                p.slots[x0 + i] = slot[i];
 }
 
 // ---------------------------------------------------------------------------------------------------- store
 // One wave takes a run (the new tokens of one block) of one head, keys or values: a pass for the maximum, the block's scale,
-// the older codes if the scale grew, and a pass that writes the codes; the second pass finds its 4 ... 32 KB in the caches. Which runs begin among a wave's
-// `span` tokens comes out of one comparison of neighbouring slots, so that no list of runs is needed. Memory bounds it
+// the older codes if the scale grew, and a pass that writes the codes. Which runs begin among a wave's
+// `span` tokens comes out of one comparison of neighbouring slots, so that no list of runs is needed. The first 16 (32) tokens of
+// a run stay in registers between the passes. Memory bounds it
 // (2 bytes read, 1 written per element); few tokens, latency.
+constexpr int kKept = 4; // vectors a lane keeps
+
 template <typename T, int CODE>
 __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs p, int span)
 {
@@ -143,8 +158,10 @@ __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs p, int span)
         const int s = p.slots[t];
         return s < 0 || s >= slots ? -1 : s >> shift;
     };
-    const int own  = lane < span ? block_of((int64_t)first + lane) : -1;
-    uint64_t leads = __ballot(own >= 0 && own != block_of((int64_t)first + lane - 1));
+    // lane l: the block of token first - 1 + l
+    const int near = block_of((int64_t)first - 1 + lane);
+    const int before = __shfl_up(near, 1); // (by all lanes: one that takes no part gives nothing)
+    uint64_t leads   = __ballot(lane >= 1 && lane <= span && near >= 0 && near != before);
 
     const int per_token = p.cache.head_dim >> 3;      // lanes of eight elements
     const int at_once   = 64 / per_token;             // tokens
@@ -152,38 +169,52 @@ __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs p, int span)
     const bool active = my < at_once;
     while(leads)
     {
-        const int i = __builtin_ctzll(leads);
+        const int i = __builtin_ctzll(leads); // (the lane)
         leads &= leads - 1;
-        const int64_t t0 = (int64_t)first + i;
-        const int block  = __builtin_amdgcn_readfirstlane(__shfl(own, i));
+        const int64_t t0 = (int64_t)first - 1 + i;
+        const int block  = __builtin_amdgcn_readfirstlane(__shfl(near, i));
         const int begin  = p.slots[t0] & (size - 1);
-        int count        = 0; // tokens of the run, at most a block's
-        for(; count < size; count += 64)
-        {
-            const uint64_t out = __ballot(block_of(t0 + count + lane) != block);
-            if(out)
+        // tokens of the run, at most a block's: as far as the lanes see, then on from there
+        int count = __builtin_ctzll(~(__ballot(near == block) >> i)); // (i >= 1: the shift brings zeros)
+        if(count >= 64 - i)
+            for(count = 64 - i; count < size; count += 64)
             {
-                count += __builtin_ctzll(out);
-                break;
+                const uint64_t out = __ballot(block_of(t0 + count + lane) != block);
+                if(out)
+                {
+                    count += __builtin_ctzll(out);
+                    break;
+                }
             }
-        }
         count = min(count, size);
 
         float amax = kTinyAmax;
         bool nan   = false;
-#pragma unroll 4
-        for(int n = 0; n < count; n += at_once)
-            if(active && n + my < count)
-            {
-                float v[8];
-                load8(x + (t0 + n + my) * xt + d, v);
+        typedef T tx8 __attribute__((ext_vector_type(8)));
+        tx8 kept[kKept];
 #pragma unroll
-                for(int j = 0; j < 8; ++j)
-                {
-                    amax = __builtin_fmaxf(amax, __builtin_fabsf(v[j]));
-                    nan |= v[j] != v[j];
-                }
+        for(int c = 0; c < kKept; ++c)
+        {
+            const int n = c * at_once + my;
+            kept[c]     = tx8{0, 0, 0, 0, 0, 0, 0, 0};
+            if(active && n < count)
+                kept[c] = *reinterpret_cast<const tx8*>(x + (t0 + n) * xt + d);
+        }
+        auto look = [&](const tx8& v) {
+#pragma unroll
+            for(int j = 0; j < 8; ++j)
+            {
+                amax = __builtin_fmaxf(amax, __builtin_fabsf((float)v[j]));
+                nan |= v[j] != v[j];
             }
+        };
+#pragma unroll
+        for(int c = 0; c < kKept; ++c)
+            look(kept[c]);
+#pragma unroll 4
+        for(int n = kKept * at_once; n < count; n += at_once)
+            if(active && n + my < count)
+                look(*reinterpret_cast<const tx8*>(x + (t0 + n + my) * xt + d));
         for(int s = 1; s < 64; s *= 2)
             amax = __builtin_fmaxf(amax, __shfl_xor(amax, s));
         const float fresh = __any(nan) ? __builtin_nanf("") : amax / (CODE == CODE_E4M3 ? kE4m3Max : kI8Max);
@@ -220,17 +251,21 @@ __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs p, int span)
         if(lane == 0)
             *at = now;
         const float inv = 1.0f / now;
-#pragma unroll 4
-        for(int n = 0; n < count; n += at_once)
-            if(active && n + my < count)
-            {
-                float v[8];
-                load8(x + (t0 + n + my) * xt + d, v);
+        auto write = [&](int n, const tx8& raw) {
+            float v[8];
 #pragma unroll
-                for(int j = 0; j < 8; ++j)
-                    v[j] *= inv;
-                put(p.slots[t0 + n + my] & (size - 1), v);
-            }
+            for(int j = 0; j < 8; ++j)
+                v[j] = (float)raw[j] * inv;
+            put(p.slots[t0 + n] & (size - 1), v);
+        };
+#pragma unroll
+        for(int c = 0; c < kKept; ++c)
+            if(active && c * at_once + my < count)
+                write(c * at_once + my, kept[c]);
+#pragma unroll 4
+        for(int n = kKept * at_once; n < count; n += at_once)
+            if(active && n + my < count)
+                write(n + my, *reinterpret_cast<const tx8*>(x + (t0 + n + my) * xt + d));
     }
 }
 

@@ -2,23 +2,27 @@
 // into registers.
 //
 // One workgroup takes 16 query rows (the heads of one group, times as many tokens as fit) and a share of the cached tokens; its
-// four waves take 32 tokens each in turn with running maxima and sums of their own and are joined through LDS at the end.
+// waves take 32 tokens each in turn with running maxima and sums of their own and are joined through LDS at the end.
 // Shares of one row are joined by a second launch.
 //   scores   S^T = K Q^T, v_mfma_f32_16x16x32: lane (row l % 16 of q, g = l / 16) gets tokens 4g .. 4g + 3 of each 16
 //   output   O^T = V^T P^T, the same instruction over 32 tokens: the lane's own probabilities are its operand, so V's lanes take tokens
 //            {4g .. 4g + 3, 16 + 4g .. + 3} as well, eight (four) neighbouring elements of d each, transposed by byte permutes
 //            in registers. MFMA j's row c stands for element c * E + j (E elements a lane): the lane ends with a contiguous
 //            stretch of the output row.
-// What bounds it is the cache's bytes: 64 bytes a lane and 16 tokens are on their way while the last ones are multiplied.
+// What bounds it is the cache's bytes. The next 32 tokens' codes (8 KB a wave for heads of 128) are on their way while the present
+// ones are multiplied; block numbers and scales of 32 such turns are fetched at once, a lane each.
 #include "paged_attention.hpp"
 
 namespace ckx {
 
 namespace {
 
-constexpr int kWaves = 4;
 // query rows of a sequence (tokens x heads of a group), on average, past which the kernel for prompts takes over
-constexpr int kPromptRows = 32;
+#ifndef PROWS
+#define PROWS 32
+#endif
+constexpr int kPromptRows = PROWS;
+constexpr int NW          = 8; // waves (four, with three workgroups a CU: 64 sequences of 8192 170 us against 159)
 
 template <typename T>
 __device__ __forceinline__ f32x4 mfma_qk(const i32x4& k, const i32x4& q, const f32x4& c)
@@ -31,12 +35,12 @@ __device__ __forceinline__ f32x4 mfma_qk(const i32x4& k, const i32x4& q, const f
 
 // DP: head_dim rounded up to 64 or 128
 template <typename T, int CODE, int DP>
-__global__ __launch_bounds__(kWaves * 64) void attention_rows_kernel(AttentionArgs p)
+__global__ __launch_bounds__(NW * 64, 2) void attention_rows_kernel(AttentionArgs p)
 {
     constexpr int KJ = DP / 64;  // 16-byte loads of a key row's lane
     constexpr int E  = DP / 16;  // elements of a value row's lane
-    __shared__ float part[kWaves][16][DP + 4];
-    __shared__ float part_m[kWaves][16], part_l[kWaves][16];
+    __shared__ float part[NW][16][DP + 4];
+    __shared__ float part_m[NW][16], part_l[NW][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r = lane & 15, g = lane >> 4;
     const int D = p.cache.head_dim;
@@ -59,10 +63,91 @@ __global__ __launch_bounds__(kWaves * 64) void attention_rows_kernel(AttentionAr
     const int last      = min(tile.first + p.tile_tokens, tile.q_len) - 1;
     const int most      = max(p.causal ? tile.kv - (tile.q_len - 1 - last) : tile.kv, 0); // what the tile's furthest row sees
 
-    // the share: whole steps of 32 tokens
+    // the share: whole steps of 32 tokens; the wave's turns among them
     const int steps = (most + 31) / 32, per = (steps + p.splits - 1) / p.splits;
     const int step0 = min(split * per, steps), step1 = min(step0 + per, steps);
+    const int turns = max(step1 - step0 - wave + NW - 1, 0) / NW;
 
+    const int* const table  = p.table + (int64_t)tile.b * p.stride_table;
+    const uint8_t* const kc = reinterpret_cast<const uint8_t*>(p.cache.p_k) + (int64_t)kvh * p.cache.stride_head;
+    const uint8_t* const vc = reinterpret_cast<const uint8_t*>(p.cache.p_v) + (int64_t)kvh * p.cache.stride_head;
+    const int in_block      = (1 << p.block_shift) - 1;
+    auto first_of           = [&](int turn) { return (step0 + wave + NW * turn) * 32; }; // token
+    // lane 2 x + h: block and scales of the 16 tokens h of turn (32 n + x); -1: no such block
+    int blocks  = -1;
+    float ks_of = 0.0f, vs_of = 0.0f;
+    auto look_up = [&](int turn) {
+        const int t = first_of(turn + (lane >> 1)) + 16 * (lane & 1);
+        blocks      = turn + (lane >> 1) < turns && t < most ? table[t >> p.block_shift] : -1;
+        blocks      = blocks < p.cache.num_blocks ? blocks : -1;
+        ks_of = vs_of = 0.0f;
+        if(blocks >= 0)
+        {
+            ks_of = p.cache.p_k_scale[(int64_t)blocks * p.cache.stride_scale + kvh];
+            vs_of = p.cache.p_v_scale[(int64_t)blocks * p.cache.stride_scale + kvh];
+        }
+    };
+    // (columns behind head_dim repeat its last ones: q is zero there, and no one stores such an element of the output)
+    uint32_t k_off[KJ];
+#pragma unroll
+    for(int j = 0; j < KJ; ++j)
+        k_off[j] = (uint32_t)r * p.cache.stride_token + min(64 * j + 16 * g, D - 16);
+    const uint32_t v_off = (uint32_t)(4 * g) * p.cache.stride_token + min(r * E, D - E);
+    struct Turn
+    {
+        u32x4 kb[2][KJ];
+        uint32_t vb[8][E / 4];
+        float ks[2], vs[2];
+        bool there[2];
+    };
+    auto lane_of = [](auto x, int from) {
+        return __builtin_bit_cast(decltype(x), __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), from));
+    };
+    auto fetch = [&](Turn& x, int turn) {
+        if((turn & 31) == 0)
+            look_up(turn);
+#pragma unroll
+        for(int h = 0; h < 2; ++h)
+        {
+            const int from  = 2 * (turn & 31) + h;
+            const int block = lane_of(blocks, from);
+            x.there[h] = block >= 0, x.ks[h] = lane_of(ks_of, from), x.vs[h] = lane_of(vs_of, from);
+            if(block < 0)
+            {
+#pragma unroll
+                for(int j = 0; j < KJ; ++j)
+                    x.kb[h][j] = u32x4{0, 0, 0, 0};
+#pragma unroll
+                for(int i = 0; i < 4; ++i)
+#pragma unroll
+                    for(int e = 0; e < E / 4; ++e)
+                        x.vb[4 * h + i][e] = 0;
+                continue;
+            }
+            const int64_t at       = (int64_t)block * p.cache.stride_block + (int64_t)((first_of(turn) + 16 * h) & in_block) * p.cache.stride_token;
+            const uint8_t* const k = kc + at;
+            const uint8_t* const v = vc + at;
+#pragma unroll
+            for(int j = 0; j < KJ; ++j)
+                x.kb[h][j] = *reinterpret_cast<const u32x4*>(k + k_off[j]);
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+            {
+                const uint8_t* const vi = v + (int64_t)i * p.cache.stride_token + v_off;
+                if constexpr(E == 8)
+                {
+                    const u32x2 y = *reinterpret_cast<const u32x2*>(vi);
+                    x.vb[4 * h + i][0] = y[0], x.vb[4 * h + i][1] = y[1];
+                }
+                else
+                    x.vb[4 * h + i][0] = *reinterpret_cast<const uint32_t*>(vi);
+            }
+        }
+    };
+
+    Turn even, odd;
+    if(turns > 0)
+        fetch(even, 0);
     i32x4 qf[KJ][2];
 #pragma unroll
     for(int j = 0; j < KJ; ++j)
@@ -82,92 +167,56 @@ __global__ __launch_bounds__(kWaves * 64) void attention_rows_kernel(AttentionAr
     float m = -__builtin_inff(), l = 0.0f;
     ValueScale unit;
 
-    const int* const table   = p.table + (int64_t)tile.b * p.stride_table;
-    const uint8_t* const kc  = reinterpret_cast<const uint8_t*>(p.cache.p_k) + (int64_t)kvh * p.cache.stride_head;
-    const uint8_t* const vc  = reinterpret_cast<const uint8_t*>(p.cache.p_v) + (int64_t)kvh * p.cache.stride_head;
-    const int in_block       = (1 << p.block_shift) - 1;
-
-    for(int step = step0 + wave; step < step1; step += kWaves)
-    {
-        const int t0 = step * 32;
-        u32x4 kb[2][KJ];
-        uint32_t vb[8][E / 4];
-        float ks[2], vs[2];
-        bool there[2];
-#pragma unroll
-        for(int h = 0; h < 2; ++h)
+    auto multiply = [&](Turn& x, int turn) {
+        const int t0 = first_of(turn);
+        if(t0 + 32 > most) // (what lies behind the last token is no value: zero, whatever its bytes are)
         {
-            const int t   = t0 + 16 * h; // (16 tokens lie in one block)
-            int block     = t < most ? table[t >> p.block_shift] : -1;
-            there[h]      = block >= 0 && block < p.cache.num_blocks;
-            block         = there[h] ? block : 0;
-            const int64_t at = (int64_t)block * p.cache.stride_block;
-            ks[h] = vs[h] = 0.0f;
-            if(there[h])
-            {
-                ks[h] = p.cache.p_k_scale[(int64_t)block * p.cache.stride_scale + kvh];
-                vs[h] = p.cache.p_v_scale[(int64_t)block * p.cache.stride_scale + kvh];
-            }
-            const int kt = (t & in_block) + r;
 #pragma unroll
-            for(int j = 0; j < KJ; ++j)
-            {
-                kb[h][j] = u32x4{0, 0, 0, 0};
-                if(there[h] && 64 * j + 16 * g < D)
-                    kb[h][j] = *reinterpret_cast<const u32x4*>(kc + at + (int64_t)kt * p.cache.stride_token + 64 * j + 16 * g);
-            }
-#pragma unroll
-            for(int i = 0; i < 4; ++i)
-            {
-                // what lies behind the last token is no value: zero, whatever its bytes are
-                const bool live = there[h] && t + 4 * g + i < most && r * E < D;
+            for(int i = 0; i < 8; ++i)
 #pragma unroll
                 for(int e = 0; e < E / 4; ++e)
-                    vb[4 * h + i][e] = 0;
-                if(live)
-                {
-                    const uint8_t* v = vc + at + (int64_t)((t & in_block) + 4 * g + i) * p.cache.stride_token + r * E;
-                    if constexpr(E == 8)
-                    {
-                        const u32x2 x = *reinterpret_cast<const u32x2*>(v);
-                        vb[4 * h + i][0] = x[0], vb[4 * h + i][1] = x[1];
-                    }
-                    else
-                        vb[4 * h + i][0] = *reinterpret_cast<const uint32_t*>(v);
-                }
-            }
+                    x.vb[i][e] = t0 + 16 * (i >> 2) + 4 * g + (i & 3) < most ? x.vb[i][e] : 0;
         }
-        // scores
         float s[8], top = -__builtin_inff();
 #pragma unroll
         for(int h = 0; h < 2; ++h)
         {
-            f32x4 x = {0, 0, 0, 0};
+            f32x4 y = {0, 0, 0, 0};
 #pragma unroll
             for(int j = 0; j < KJ; ++j)
             {
-                x = mfma_qk<T>(codes8<CODE, T>(kb[h][j][0], kb[h][j][1]), qf[j][0], x);
-                x = mfma_qk<T>(codes8<CODE, T>(kb[h][j][2], kb[h][j][3]), qf[j][1], x);
+                y = mfma_qk<T>(codes8<CODE, T>(x.kb[h][j][0], x.kb[h][j][1]), qf[j][0], y);
+                y = mfma_qk<T>(codes8<CODE, T>(x.kb[h][j][2], x.kb[h][j][3]), qf[j][1], y);
             }
-            const float c = ks[h] * p.scale;
+            const float c = x.ks[h] * p.scale;
 #pragma unroll
             for(int i = 0; i < 4; ++i)
             {
-                const bool seen = there[h] && t0 + 16 * h + 4 * g + i < see;
-                s[4 * h + i]    = seen ? x[i] * c : -__builtin_inff();
+                const bool seen = x.there[h] && t0 + 16 * h + 4 * g + i < see;
+                s[4 * h + i]    = seen ? y[i] * c : -__builtin_inff();
                 top             = __builtin_fmaxf(top, s[4 * h + i]);
             }
         }
-        const float now  = __builtin_fmaxf(m, max_over_rows(top));
-        const float zero = now == -__builtin_inff() ? 0.0f : now; // (nothing seen yet: exp2(-inf - 0) = 0)
-        const float keep = __builtin_amdgcn_exp2f(m - zero);
-        m                = now;
-        l *= keep;
-        const float keep_o = keep * unit.take(vs[0], vs[1]);
+        top = max_over_rows(top);
+        // (the maximum is there for the range only and raised only by leaps, 2^6 or more: the sums are seldom rescaled)
+        float keep_o = 1.0f;
+        if(__any((lane == 0) && (x.vs[0] > unit.top || x.vs[1] > unit.top)))
+            keep_o = unit.take(x.vs[0], x.vs[1]);
+        if(__any(top > m + 6.0f))
+        {
+            const float now = __builtin_fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - (now == -__builtin_inff() ? 0.0f : now));
+            m = now;
+            l *= keep;
+            keep_o *= keep;
+        }
+        if(__any(keep_o != 1.0f))
+        {
 #pragma unroll
-        for(int j = 0; j < E; ++j)
-            acc[j] *= keep_o;
-        const float w[2] = {unit.of(vs[0]), unit.of(vs[1])};
+            for(int j = 0; j < E; ++j)
+                acc[j] *= keep_o;
+        }
+        const float zero = m == -__builtin_inff() ? 0.0f : m; // (nothing seen yet: exp2(-inf - 0) = 0)
+        const float w[2] = {unit.of(x.vs[0]), unit.of(x.vs[1])};
         float pr[8];
 #pragma unroll
         for(int i = 0; i < 8; ++i)
@@ -183,16 +232,26 @@ __global__ __launch_bounds__(kWaves * 64) void attention_rows_kernel(AttentionAr
         for(int e = 0; e < E / 4; ++e)
         {
             uint32_t lo[4], hi[4];
-            transpose4(vb[0][e], vb[1][e], vb[2][e], vb[3][e], lo);
-            transpose4(vb[4][e], vb[5][e], vb[6][e], vb[7][e], hi);
+            transpose4(x.vb[0][e], x.vb[1][e], x.vb[2][e], x.vb[3][e], lo);
+            transpose4(x.vb[4][e], x.vb[5][e], x.vb[6][e], x.vb[7][e], hi);
 #pragma unroll
             for(int j = 0; j < 4; ++j)
                 acc[4 * e + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                     __builtin_bit_cast(f16x8, (codes8<CODE, _Float16>(lo[j], hi[j]))), __builtin_bit_cast(f16x8, pf), acc[4 * e + j], 0, 0, 0);
         }
+    };
+    for(int turn = 0; turn < turns; turn += 2)
+    {
+        if(turn + 1 < turns)
+            fetch(odd, turn + 1);
+        multiply(even, turn);
+        if(turn + 2 < turns)
+            fetch(even, turn + 2);
+        if(turn + 1 < turns)
+            multiply(odd, turn + 1);
     }
 
-    // the four waves' sums. Lane (r, g) holds elements (4g + i) * E + j of row r at acc[j][i].
+    // the waves' sums. Lane (r, g) holds elements (4g + i) * E + j of row r at acc[j][i].
     l = sum_over_rows(l);
     if(g == 0)
         part_m[wave][r] = m, part_l[wave][r] = l;
@@ -203,13 +262,15 @@ __global__ __launch_bounds__(kWaves * 64) void attention_rows_kernel(AttentionAr
             part[wave][r][(4 * g + i) * E + j] = acc[j][i] * unit.top;
     __syncthreads();
     // thread (row, 16 of them a row) joins E elements
+    if(threadIdx.x >= 256)
+        return;
     const int row = threadIdx.x >> 4, c = threadIdx.x & 15;
     const int jt = row / p.tile_heads, jh = h0 + (row - jt * p.tile_heads);
     if(jt >= p.tile_tokens || tile.first + jt >= tile.q_len || jh >= p.group || c * E >= D)
         return;
     float top = -__builtin_inff();
 #pragma unroll
-    for(int w = 0; w < kWaves; ++w)
+    for(int w = 0; w < NW; ++w)
         top = __builtin_fmaxf(top, part_m[w][row]);
     const float zero = top == -__builtin_inff() ? 0.0f : top;
     float sum = 0.0f, o[E];
@@ -217,7 +278,7 @@ __global__ __launch_bounds__(kWaves * 64) void attention_rows_kernel(AttentionAr
     for(int e = 0; e < E; ++e)
         o[e] = 0.0f;
 #pragma unroll
-    for(int w = 0; w < kWaves; ++w)
+    for(int w = 0; w < NW; ++w)
     {
         const float f = __builtin_amdgcn_exp2f(part_m[w][row] - zero);
         sum += part_l[w][row] * f;
@@ -267,6 +328,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs p)
     const float* const ml = p.ws + attention_rows(p) * p.splits * DP + row * p.splits * 2;
     const float* const at = p.ws + row * p.splits * DP + c * E;
     float top             = -__builtin_inff();
+#pragma unroll 8
     for(int s = 0; s < p.splits; ++s)
         top = __builtin_fmaxf(top, ml[2 * s]);
     const float zero = top == -__builtin_inff() ? 0.0f : top;
@@ -274,6 +336,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs p)
 #pragma unroll
     for(int e = 0; e < E; ++e)
         o[e] = 0.0f;
+#pragma unroll 8
     for(int s = 0; s < p.splits; ++s)
     {
         const float f = __builtin_amdgcn_exp2f(ml[2 * s] - zero);
@@ -312,12 +375,13 @@ Plan plan(const ckx_kv_cache8& c, int batch, int tokens, int heads, int max_kv, 
     p.head_tiles    = (group + p.tile_heads - 1) / p.tile_heads;
     p.tile_tokens   = rows / p.tile_heads;
     p.tiles         = p.tile_tokens == 1 ? tokens : tokens / p.tile_tokens + batch;
-    // Shares of the cached tokens, joined by a second launch, where the tiles alone leave CUs without work: about four workgroups a
-    // CU and none of under 256 tokens (two steps a wave); prompts: two a CU (what fits on one) and none of under 512 (eight steps)
+    // Shares of the cached tokens, joined by a second launch, where the tiles alone leave CUs without work. Single tokens: one
+    // workgroup a CU (what fits on one), none of under 256 tokens, a turn for each wave; 8 sequences of 8192: 30.5 us, 32.7 with two
+    // a CU, 38.3 with three. Prompts: two a CU and none of under 512 tokens, eight steps.
     const int64_t groups  = (int64_t)(tokens < p.tiles ? tokens : p.tiles) * c.num_heads * p.head_tiles;
     const int64_t longest = (int64_t)max_blocks * c.block_size;
     const int64_t kv      = max_kv < longest ? max_kv : longest;
-    int64_t splits        = p.prompt ? 512 / groups : (1024 + groups - 1) / groups;
+    int64_t splits        = p.prompt ? 512 / groups : (256 + groups - 1) / groups;
     const int64_t least   = p.prompt ? 512 : 256;
     if(splits > kv / least)
         splits = kv / least;
@@ -332,9 +396,9 @@ hipError_t launch_rows(const AttentionArgs& a, hipStream_t s)
 {
     const dim3 grid((unsigned)((int64_t)a.tiles * a.cache.num_heads * a.head_tiles * a.splits));
     if(padded(a.cache.head_dim) == 64)
-        hipLaunchKernelGGL((attention_rows_kernel<T, CODE, 64>), grid, dim3(kWaves * 64), 0, s, a);
+        hipLaunchKernelGGL((attention_rows_kernel<T, CODE, 64>), grid, dim3(NW * 64), 0, s, a);
     else
-        hipLaunchKernelGGL((attention_rows_kernel<T, CODE, 128>), grid, dim3(kWaves * 64), 0, s, a);
+        hipLaunchKernelGGL((attention_rows_kernel<T, CODE, 128>), grid, dim3(NW * 64), 0, s, a);
     return hipGetLastError();
 }
 
@@ -360,7 +424,7 @@ hipError_t launch(const AttentionArgs& a, bool prompt, hipStream_t s)
 bool attention_fits(const ckx_kv_cache8& c, int batch, int tokens, int heads, int max_kv, int max_blocks)
 {
     const Plan p = plan(c, batch, tokens, heads, max_kv, max_blocks);
-    return (int64_t)p.tiles * c.num_heads * p.head_tiles * p.splits < (1ll << 32) / (kWaves * 64);
+    return (int64_t)p.tiles * c.num_heads * p.head_tiles * p.splits < (1ll << 32) / (NW * 64);
 }
 
 int64_t attention_workspace(const ckx_kv_cache8& c, int batch, int tokens, int heads, int max_kv, int max_blocks)
