@@ -17,11 +17,10 @@ namespace ckx {
 
 namespace {
 
-// query rows of a sequence (tokens x heads of a group), on average, past which the kernel for prompts takes over
-#ifndef PROWS
-#define PROWS 32
-#endif
-constexpr int kPromptRows = PROWS;
+// query rows of a sequence (tokens x heads of a group), on average, past which the kernel for prompts takes over; it / this one, us:
+// 16 sequences of 4096, 32 / 8 heads of 128: 48 rows 82 / 59, 72 rows 82 / 80, 120 rows 89 / 114; 64 of 1000, 96 rows 65 / 131;
+// 16 of 2000, 16 / 16 heads of 64: 96 rows 66 / 56, 192 rows 93 / 101
+constexpr int kPromptRows = 80;
 constexpr int NW          = 8; // waves (four, with three workgroups a CU: 64 sequences of 8192 170 us against 159)
 
 template <typename T>

@@ -23,6 +23,11 @@
 //                     alpha beta [nrepeat]   (profiler/src/profile_gemm_bilinear.cpp:28-66)
 //   ckx_profiler gemm_add_add_fastgelu <dtype 1> <layout 0..3> <verify> <init> <log> <time> M N K StrideA StrideB
 //                     StrideD0 StrideD1 StrideE [nrepeat]   (profiler/src/profile_gemm_add_add_fastgelu.cpp:29-62)
+//   ckx_profiler gemm_f8_blockscale <c type 1:fp16 2:bf16> <verify> <init> <log> <time> M N K [nrepeat]
+//                     (fp16 activations through DeviceBlockQuantizeF8, then DeviceGemmBlockScaleF8; weights with 128 x 128 scales)
+//   ckx_profiler paged_attention8 <cache 1:e4m3 2:int8> <verify> <init> <log> <time> Batch Context New QHeads KvHeads HeadDim
+//                     BlockSize [causal 0|1] [nrepeat]   (a step of a decoder: DeviceKvCacheTables, DeviceKvCacheStore8,
+//                     DevicePagedAttention8, fp16; the cached tokens are stored by a step of their own first)
 //
 // Every instance of the family is run (DeviceOperationInstanceFactory), one "Perf:" line each
 // and a final "Best Perf:" line, in the reference's format (profile_gemm_impl.hpp:176-177,
@@ -38,6 +43,7 @@
 
 #include "ckx/device_ops.hpp"
 #include "ckx/host_tensor.hpp"
+#include "ckx/serving_ops.hpp"
 
 using namespace ck;
 using namespace ck::tensor_operation;
@@ -882,6 +888,164 @@ int profile_gemm_softmax_gemm(int argc, char* argv[])
                 : profile_gemm_softmax_gemm_t<false>(verify, init, time_kernel, M, N, K, O, G, scale, nrepeat);
 }
 
+// timed (a "Perf:" line) or untimed launch of an operator that has one kernel choice of its own
+template <typename Op>
+void run_one(Op& op, const typename Op::Argument& arg, const char* what, bool time_kernel, int nrepeat, double flop, double bytes, bool i8)
+{
+    if(!op.IsSupportedArgument(arg))
+        throw std::runtime_error(std::string(what) + " is not supported: " + ckx_last_error());
+    const float ms = op.MakeInvoker().Run(arg, StreamConfig{nullptr, time_kernel, nrepeat, 1});
+    ckx::hip_check(hipDeviceSynchronize());
+    if(time_kernel)
+        report("Perf: ", ms, flop, bytes, op.GetTypeString(), i8);
+}
+
+template <typename T>
+int profile_gemm_f8_t(bool time_kernel, int M, int N, int K, int nrepeat)
+{
+    const int groups = (K + 127) / 128, nb = (N + 127) / 128;
+    std::vector<half_t> x((std::size_t)M * K);
+    ckx::fill_uniform_f16(x, -1.f, 1.f, 0xC0FFEE + 10);
+    // weights: every finite code; scales of 2^-9 ... 2^-6
+    std::vector<uint8_t> w((std::size_t)N * K);
+    for(std::size_t i = 0; i < w.size(); ++i)
+    {
+        w[i] = (uint8_t)(ckx::splitmix64(0xC0FFEE + 11, i) >> 56);
+        w[i] = (w[i] & 127) == 127 ? 0 : w[i];
+    }
+    std::vector<float> sw((std::size_t)nb * groups);
+    for(std::size_t i = 0; i < sw.size(); ++i)
+        sw[i] = 1.0f / (float)(64 << (ckx::splitmix64(0xC0FFEE + 12, i) >> 62));
+    ckx::DeviceMem dx(x.size() * 2), dq(x.size()), ds((std::size_t)M * groups * 4), dw(w.size()), dsw(sw.size() * 4),
+        dc((std::size_t)M * N * sizeof(T));
+    dx.ToDevice(x.data());
+    dw.ToDevice(w.data());
+    dsw.ToDevice(sw.data());
+    device::DeviceBlockQuantizeF8<half_t> quantize;
+    run_one(quantize,
+            quantize.MakeArgument(static_cast<const half_t*>(dx.GetDeviceBuffer()), static_cast<f8_t*>(dq.GetDeviceBuffer()),
+                                  static_cast<float*>(ds.GetDeviceBuffer()), M, K, K, K, 1, M),
+            "the quantiser", time_kernel, nrepeat, 3.0 * M * K, 3.0 * M * K + 4.0 * M * groups, false);
+    device::DeviceGemmBlockScaleF8<T> gemm;
+    auto arg = gemm.MakeArgument(static_cast<const f8_t*>(dq.GetDeviceBuffer()), static_cast<const f8_t*>(dw.GetDeviceBuffer()),
+                                 static_cast<T*>(dc.GetDeviceBuffer()), static_cast<const float*>(ds.GetDeviceBuffer()),
+                                 static_cast<const float*>(dsw.GetDeviceBuffer()), M, N, K, K, K, N, 1, M, groups, 1);
+    ckx::DeviceMem ws(gemm.GetWorkSpaceSize(&arg));
+    if(ws.GetBufferSize() > 0)
+        gemm.SetWorkSpacePointer(&arg, ws.GetDeviceBuffer());
+    run_one(gemm, arg, "the product", time_kernel, nrepeat, 2.0 * M * N * K, (double)M * K + (double)N * K + 2.0 * M * N, true);
+    if(const char* path = std::getenv("CKX_PROFILER_DUMP"))
+    {
+        std::vector<T> out((std::size_t)M * N);
+        dc.FromDevice(out.data());
+        ckx::dump_to_file(path, out);
+    }
+    return 0;
+}
+
+int profile_gemm_f8(int argc, char* argv[])
+{
+    if(argc < 10)
+    {
+        std::printf("arg1: tensor operation (gemm_f8_blockscale)\narg2: type of C (1: fp16, 2: bf16)\narg3: verification\n"
+                    "arg4: initialization\narg5: print tensor value\narg6: time kernel\narg7 to 9: M, N, K\nlast: nrepeat\n");
+        return 1;
+    }
+    const int M = std::atoi(argv[7]), N = std::atoi(argv[8]), K = std::atoi(argv[9]), nrepeat = argc > 10 ? std::atoi(argv[10]) : 10;
+    if(M < 1 || N < 1 || K < 1)
+        throw std::runtime_error("M, N and K are at least 1");
+    return std::atoi(argv[2]) == 2 ? profile_gemm_f8_t<bhalf_t>(std::atoi(argv[6]), M, N, K, nrepeat)
+                                   : profile_gemm_f8_t<half_t>(std::atoi(argv[6]), M, N, K, nrepeat);
+}
+
+template <bool Causal>
+int profile_attention8_t(int type, bool time_kernel, int B, int ctx, int fresh, int heads, int kv_heads, int D, int bs, int nrepeat)
+{
+    const int width = (ctx + fresh + bs - 1) / bs, blocks = B * width;
+    const std::size_t codes = (std::size_t)blocks * kv_heads * bs * D;
+    ckx::DeviceMem dk(codes), dv(codes), dks((std::size_t)blocks * kv_heads * 4), dvs((std::size_t)blocks * kv_heads * 4);
+    ckx_kv_cache8 cache{};
+    cache.p_k = dk.GetDeviceBuffer(), cache.p_v = dv.GetDeviceBuffer();
+    cache.p_k_scale = static_cast<float*>(dks.GetDeviceBuffer()), cache.p_v_scale = static_cast<float*>(dvs.GetDeviceBuffer());
+    cache.type = type, cache.num_blocks = blocks, cache.block_size = bs, cache.num_heads = kv_heads, cache.head_dim = D;
+    cache.stride_head = bs * D, cache.stride_token = D, cache.stride_scale = kv_heads, cache.stride_block = (int64_t)kv_heads * bs * D;
+    // the free list: all blocks, every other one first
+    std::vector<index_t> free, zero(B, 0), context(B, ctx), news(B, fresh);
+    for(int i = 0; i < blocks; i += 2)
+        free.push_back(i);
+    for(int i = 1; i < blocks; i += 2)
+        free.push_back(i);
+    ckx::DeviceMem dfree(free.size() * 4), dzero(B * 4), dctx(B * 4), dnew(B * 4), dtable((std::size_t)B * width * 4), dcu((B + 1) * 4),
+        dkv(B * 4), dused(4), dslots((std::size_t)B * (ctx > fresh ? ctx : fresh) * 4);
+    dfree.ToDevice(free.data()), dzero.ToDevice(zero.data()), dctx.ToDevice(context.data()), dnew.ToDevice(news.data());
+    auto ints = [](ckx::DeviceMem& m) { return static_cast<index_t*>(m.GetDeviceBuffer()); };
+    device::DeviceKvCacheTables tables;
+    device::DeviceKvCacheStore8<half_t> store;
+    device::DevicePagedAttention8<half_t, Causal> attention;
+    const int row = (heads + 2 * kv_heads) * D;
+    index_t taken = 0;
+    // a step: `n` new tokens of every sequence behind `before`; queries, keys and values as columns of one matrix
+    auto step = [&](ckx::DeviceMem& dqkv, ckx::DeviceMem& before, ckx::DeviceMem& lens, int n, bool time) {
+        auto targ = tables.MakeArgument(ints(before), ints(lens), ints(dfree) + taken, ints(dtable), ints(dcu), ints(dkv), ints(dslots),
+                                        ints(dused), B, (index_t)free.size() - taken, width, width, B * n, bs);
+        run_one(tables, targ, "the tables", time, nrepeat, (double)B * n, 4.0 * B * (4 + n), false);
+        index_t used = 0;
+        dused.FromDevice(&used);
+        taken += used;
+        const half_t* qkv = static_cast<const half_t*>(dqkv.GetDeviceBuffer());
+        auto sarg = store.MakeArgument(qkv + heads * D, qkv + (heads + kv_heads) * D, ints(dslots), cache, B * n, row, D, row, D);
+        run_one(store, sarg, "the store", time, nrepeat, 6.0 * B * n * kv_heads * D, 6.0 * B * n * kv_heads * D, false);
+    };
+    auto filled = [&](int n, uint64_t seed) {
+        std::vector<half_t> v((std::size_t)B * n * row);
+        ckx::fill_uniform_f16(v, -1.f, 1.f, seed);
+        auto m = std::make_unique<ckx::DeviceMem>(v.size() * 2);
+        m->ToDevice(v.data());
+        return m;
+    };
+    if(ctx > 0)
+        step(*filled(ctx, 0xC0FFEE + 13), dzero, dctx, ctx, false);
+    auto dqkv = filled(fresh, 0xC0FFEE + 14);
+    step(*dqkv, dctx, dnew, fresh, time_kernel);
+    ckx::DeviceMem dout((std::size_t)B * fresh * heads * D * 2);
+    auto arg = attention.MakeArgument(static_cast<const half_t*>(dqkv->GetDeviceBuffer()), static_cast<half_t*>(dout.GetDeviceBuffer()),
+                                      ints(dtable), ints(dcu), ints(dkv), cache, B, B * fresh, heads, ctx + fresh, width, width, row, D,
+                                      heads * D, D, element_wise::Scale{1.0f / std::sqrt((float)D)});
+    ckx::DeviceMem ws(attention.GetWorkSpaceSize(&arg));
+    if(ws.GetBufferSize() > 0)
+        attention.SetWorkSpacePointer(&arg, ws.GetDeviceBuffer());
+    run_one(attention, arg, "the attention", time_kernel, nrepeat, 4.0 * B * fresh * heads * D * (Causal ? ctx + (fresh + 1) / 2.0 : ctx + fresh),
+            2.0 * B * (double)(ctx + fresh) * kv_heads * D + 4.0 * B * fresh * heads * D, false);
+    if(const char* path = std::getenv("CKX_PROFILER_DUMP"))
+    {
+        std::vector<half_t> out((std::size_t)B * fresh * heads * D);
+        dout.FromDevice(out.data());
+        ckx::dump_to_file(path, out);
+    }
+    return 0;
+}
+
+int profile_attention8(int argc, char* argv[])
+{
+    if(argc < 14)
+    {
+        std::printf("arg1: tensor operation (paged_attention8)\narg2: cache (1: e4m3, 2: int8)\narg3: verification\n"
+                    "arg4: initialization\narg5: print tensor value\narg6: time kernel\n"
+                    "arg7 to 13: Batch, Context, New, QHeads, KvHeads, HeadDim, BlockSize\n"
+                    "arg14: causal (0 | 1)\nlast: nrepeat\n");
+        return 1;
+    }
+    int p[7];
+    for(int i = 0; i < 7; ++i)
+        p[i] = std::atoi(argv[7 + i]);
+    if(p[0] < 1 || p[1] < 0 || p[2] < 1 || p[3] < 1 || p[4] < 1 || p[5] < 1 || p[6] < 1)
+        throw std::runtime_error("sizes are at least 1, the context at least 0");
+    const bool causal = argc > 14 ? std::atoi(argv[14]) != 0 : true;
+    const int nrepeat = argc > 15 ? std::atoi(argv[15]) : 10, type = std::atoi(argv[2]) == 2 ? CKX_TYPE_I8 : CKX_TYPE_E4M3;
+    auto* run         = causal ? &profile_attention8_t<true> : &profile_attention8_t<false>;
+    return run(type, std::atoi(argv[6]) != 0, p[0], p[1], p[2], p[3], p[4], p[5], p[6], nrepeat);
+}
+
 } // namespace
 
 int main(int argc, char* argv[])
@@ -914,6 +1078,10 @@ int main(int argc, char* argv[])
             return profile_gemm_bilinear(argc, argv);
         if(argc >= 2 && std::strcmp(argv[1], "gemm_add_add_fastgelu") == 0)
             return profile_gemm_add_add_fastgelu(argc, argv);
+        if(argc >= 2 && std::strcmp(argv[1], "gemm_f8_blockscale") == 0)
+            return profile_gemm_f8(argc, argv);
+        if(argc >= 2 && std::strcmp(argv[1], "paged_attention8") == 0)
+            return profile_attention8(argc, argv);
         std::printf("arg1: tensor operation (gemm: GEMM\n"
                     "                        conv2d_fwd: NHWC/KYXC/NHWK forward convolution\n"
                     "                        batched_gemm_gemm: batched fused GEMM+GEMM\n"
@@ -923,7 +1091,9 @@ int main(int argc, char* argv[])
                     "                        conv_fwd_bias_relu_add: ForwardConvolution+Bias+ReLU+Add\n"
                     "                        batched_gemm: Batched GEMM\n"
                     "                        gemm_splitk: Split-K GEMM\n"
-                    "                        gemm_bias_relu: GEMM+Bias+ReLU)\n");
+                    "                        gemm_bias_relu: GEMM+Bias+ReLU\n"
+                    "                        gemm_f8_blockscale: quantiser and GEMM, e4m3 with a scale for each block of 128\n"
+                    "                        paged_attention8: tables, store and attention over a cache of 8-bit blocks)\n");
         return 1;
     }
     catch(const std::exception& e)

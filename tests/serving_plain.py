@@ -124,6 +124,14 @@ def attention_bound(o, mag, big, dtype, D, kv):
     return HALF_STEP[dtype] * o.abs() + mag * (2.0 ** -11 + 2 * (D + 4) * 2.0 ** -23 * big[:, :, None] + 2 * (kv + 16) * 2.0 ** -23) + 1e-30
 
 
+def small_products(scale, dtype, kv):
+    """What fp16's subnormal numbers cost, for scores far apart, where attention_bound's relative terms alone do not hold: a
+    probability (at most 1 beside the row's largest) times a value scale relative to the largest value scale is off by at most half
+    of fp16's smallest step, 2^-25; the sum of up to kv of them, times codes of at most QMAX and that scale, is divided by a sum of
+    probabilities of at least 1."""
+    return kv * 2.0 ** -25 * QMAX[dtype] * float(scale.abs().max())
+
+
 def random_cache(g, blocks, heads, size, D, dtype, layout="bhsd"):
     shape = (blocks, heads, size, D) if layout == "bhsd" else (blocks, size, heads, D)
     def codes():

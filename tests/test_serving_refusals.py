@@ -226,3 +226,22 @@ def test_python_operators_check_types():
         ck.KvCache8(k, k[:3], s, s)
     with pytest.raises(ValueError):
         ck.KvCache8(k, k, s, s[:, :1])
+
+
+def test_python_operators_refuse_host_memory_and_wide_sizes():
+    import torch
+    x = torch.zeros(4, 256)
+    q, scale = torch.zeros(4, 256, dtype=torch.float8_e4m3fn), torch.zeros(4, 2)
+    op = ck.DeviceBlockQuantizeF8("f32")
+    host = op.MakeArgumentPointer(x, q, scale, 4, 256, 256, 256, 2, 1)
+    assert op.IsSupportedArgument(host)
+    with pytest.raises(ValueError, match="one GPU"):
+        op.MakeInvokerPointer().Run(host)
+    mixed = op.MakeArgumentPointer(torch.zeros(4, 256, device="meta"), q, scale, 4, 256, 256, 256, 2, 1)
+    with pytest.raises(ValueError, match="one GPU"):
+        op.MakeInvokerPointer().Run(mixed)
+    for wide in (2 ** 31, 2 ** 32 + 4, -2 ** 31 - 1):
+        with pytest.raises(OverflowError):
+            op.MakeArgumentPointer(0, 0, 0, wide, 256, 256, 256, 1, 4)
+        with pytest.raises(OverflowError):
+            ck.DeviceKvCacheTables().MakeArgumentPointer(*[0] * 8, 4, 8, 4, 4, wide, 16)
