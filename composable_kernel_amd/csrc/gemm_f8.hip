@@ -550,6 +550,13 @@ hipError_t launch(GemmF8Args& a, int64_t workspace_bytes, hipStream_t s)
 
 } // namespace
 
+// a launch has fewer than 2^32 threads, 512 a workgroup at most: one for 16 columns (up to 32 rows) or for 64 x 128 outputs
+bool gemm_f8_fits(int M, int N)
+{
+    const int64_t m = M <= 32 ? 2 : ((int64_t)M + 63) / 64, n = ((int64_t)N + (M <= 32 ? 15 : 127)) / (M <= 32 ? 16 : 128);
+    return m * n < (1ll << 32) / 512;
+}
+
 int64_t gemm_f8_workspace(int M, int N, int K)
 {
     const Plan p = plan(M, N, K, false, INT64_MAX);

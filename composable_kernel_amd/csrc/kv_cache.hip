@@ -85,7 +85,7 @@ __global__ __launch_bounds__(kTablesThreads) void kv_tables_kernel(TablesArgs p)
     {
         const int b   = last_at_most(base, p.batch, f);
         const int col = blocks_of(max(p.context[b], 0), p.block_shift) + f - base[b];
-        if(col < p.max_blocks)
+        if((unsigned)col < (unsigned)p.max_blocks) // (unsigned: sums past 31 bits lead nowhere outside)
             p.table[(int64_t)b * p.stride_table + col] = p.free[f];
     }
     // the slots, four neighbours a thread, whose sequence is looked for once; a new block comes from the free list itself, not from
@@ -107,14 +107,14 @@ __global__ __launch_bounds__(kTablesThreads) void kv_tables_kernel(TablesArgs p)
             const int c = max(p.context[b], 0), pos = c + (int)x - cu[b], col = pos >> p.block_shift;
             const int had = blocks_of(c, p.block_shift);
             int block     = -1;
-            if(col < p.max_blocks)
+            if((unsigned)col < (unsigned)p.max_blocks)
             {
                 if(col < had)
                     block = p.table[(int64_t)b * p.stride_table + col];
-                else if(base[b] + col - had < p.num_free)
+                else if((unsigned)(base[b] + col - had) < (unsigned)p.num_free)
                     block = p.free[base[b] + col - had];
             }
-            if(block >= 0)
+            if(block >= 0 && block <= 0x7fffffff >> p.block_shift) // (a number without a 32-bit slot is no block)
                 slot[i] = (block << p.block_shift) + (pos & ((1 << p.block_shift) - 1));
         }
     }

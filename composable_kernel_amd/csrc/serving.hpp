@@ -29,6 +29,7 @@ struct GemmF8Args
     int groups, ksplit, per; // groups of 128 along K; runs they are cut into, groups a run
     float* ws;               // ksplit > 1: [ksplit][M][N] sums
 };
+bool gemm_f8_fits(int M, int N);
 int64_t gemm_f8_workspace(int M, int N, int K);
 hipError_t gemm_f8_launch(GemmF8Args a, int c_type, int64_t workspace_bytes, hipStream_t s);
 

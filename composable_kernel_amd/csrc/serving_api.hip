@@ -15,6 +15,9 @@ bool float_type(int t) { return t == CKX_TYPE_F32 || half_type(t); }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 
+constexpr float kLog2e        = 1.4426950408889634f;
+constexpr int64_t kMostCached = 0x7fff0000; // (token numbers are rounded up to whole steps in 32 bits)
+
 int block_shift(int size)
 {
     return size == 16 ? 4 : size == 32 ? 5 : size == 64 ? 6 : size == 128 ? 7 : -1;
@@ -123,6 +126,10 @@ int ckx_gemm_f8_blockscale_is_supported(int32_t M, int32_t N, int32_t K, int32_t
         return api_fail(CKX_UNSUPPORTED, "leading dimension smaller than the row");
     if(lda < 0 || ldb < 0 || ldc < 0 || stride_sa_m < 0 || stride_sa_g < 0 || stride_sb_n < 0 || stride_sb_g < 0)
         return api_fail(CKX_UNSUPPORTED, "negative stride");
+    if(K > 1 << 30)
+        return api_fail(CKX_UNSUPPORTED, "K is at most 2^30");
+    if(!ckx::gemm_f8_fits(M, N))
+        return api_fail(CKX_UNSUPPORTED, "more output tiles than one launch takes");
     // the rows of one tile (256 at most) are addressed through 32-bit offsets
     if((int64_t)lda * 256 > 0x7fff0000ll || (int64_t)ldb * 256 > 0x7fff0000ll)
         return api_fail(CKX_UNSUPPORTED, "256 rows of A or B span 2 GiB");
@@ -227,6 +234,8 @@ int ckx_kv_cache_store8_is_supported(const ckx_kv_cache8* cache, int32_t num_tok
         return api_fail(CKX_UNSUPPORTED, "key / value strides: multiples of 8, heads at least head_dim and tokens a whole row apart");
     if(cache->num_heads > 32767)
         return api_fail(CKX_UNSUPPORTED, "at most 32767 heads");
+    if(num_tokens > 1 << 29)
+        return api_fail(CKX_UNSUPPORTED, "at most 2^29 tokens a call");
     return CKX_OK;
 }
 
@@ -266,14 +275,14 @@ int ckx_paged_attention8_is_supported(const ckx_kv_cache8* cache, int32_t batch,
         return api_fail(CKX_INVALID_VALUE, "queries and outputs are fp16 or bf16");
     if(causal != 0 && causal != 1)
         return api_fail(CKX_INVALID_VALUE, "causal is 0 or 1");
-    if(!std::isfinite(scale))
-        return api_fail(CKX_INVALID_VALUE, "the score scale must be finite");
+    if(!std::isfinite(scale * kLog2e))
+        return api_fail(CKX_INVALID_VALUE, "the score scale (times log2 e) must be finite");
     if(num_q_heads > 0 && (cache->num_heads == 0 || num_q_heads % cache->num_heads))
         return api_fail(CKX_UNSUPPORTED, "query heads are a multiple of the cache's heads");
     if(batch > 1 && stride_table < max_blocks)
         return api_fail(CKX_UNSUPPORTED, "table rows overlap");
-    if((int64_t)max_blocks * cache->block_size > 0x7fffffffll)
-        return api_fail(CKX_UNSUPPORTED, "a sequence has at most 2^31 - 1 tokens");
+    if((int64_t)max_blocks * cache->block_size > kMostCached)
+        return api_fail(CKX_UNSUPPORTED, "a sequence has at most 2^31 - 65536 tokens");
     if(!rows_apart(stride_q_token, stride_q_head, num_q_heads, cache->head_dim) ||
        !rows_apart(stride_o_token, stride_o_head, num_q_heads, cache->head_dim))
         return api_fail(CKX_UNSUPPORTED, "query / output strides: multiples of 8, heads at least head_dim and tokens a whole row apart");
@@ -289,7 +298,7 @@ int64_t ckx_paged_attention8_workspace_bytes(const ckx_kv_cache8* cache, int32_t
 {
     if(check_cache(cache) != CKX_OK || batch <= 0 || num_tokens <= 0 || num_q_heads <= 0 || max_kv_len < 0 || max_blocks < 0 ||
        cache->num_heads <= 0 || num_q_heads % cache->num_heads || batch > 0x3fffffff ||
-       (int64_t)num_tokens * num_q_heads > 0x3fffffffll || (int64_t)max_blocks * cache->block_size > 0x7fffffffll)
+       (int64_t)num_tokens * num_q_heads > 0x3fffffffll || (int64_t)max_blocks * cache->block_size > kMostCached)
         return 0;
     return ckx::attention_workspace(*cache, batch, num_tokens, num_q_heads, max_kv_len, max_blocks);
 }
@@ -324,7 +333,7 @@ int ckx_paged_attention8(const void* p_q, void* p_o, const int32_t* p_block_tabl
     a.max_kv = max_kv_len, a.max_blocks = max_blocks, a.stride_table = stride_table;
     a.block_shift = block_shift(cache->block_size);
     a.sq_t = stride_q_token, a.sq_h = stride_q_head, a.so_t = stride_o_token, a.so_h = stride_o_head;
-    a.scale  = scale * 1.4426950408889634f; // (the kernels work in powers of two)
+    a.scale  = scale * kLog2e; // (the kernels work in powers of two)
     a.causal = causal;
     a.ws     = static_cast<float*>(p_workspace);
     hipError_t e = ckx::attention_launch(a, q_type, (hipStream_t)stream);

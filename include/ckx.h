@@ -447,7 +447,8 @@ int ckx_quantize_blocks_f8(const void* p_x, void* p_q, float* p_scale, int32_t M
  *   C[m, n] = round( sum_g sa[m, g] * sb[n / 128, g] * sum_{k in group g} A[m, k] * B[n, k] )
  * A [M, K] row-major, B stored [N, K] (column-major K x N), C [M, N] row-major fp32, fp16 or bf16 (c_type), rounded once.
  * sa[m, g] = p_scale_a[m * stride_sa_m + g * stride_sa_g], sb[j, g] = p_scale_b[j * stride_sb_n + g * stride_sb_g]. Products
- * and sums are fp32. K == 0 gives zeros. Any extent, stride and address; K, lda, ldb multiples of 16 with 16-byte aligned A and B
+ * and sums are fp32. K == 0 gives zeros. Any stride and address; K <= 2^30, 256 rows of A or of B within 2 GiB, and fewer
+ * than 2^23 output tiles (64 x 128; up to 32 rows 32 x 16). K, lda, ldb multiples of 16 with 16-byte aligned A and B
  * run on the vectorised kernels. Workspace (optional, ckx_gemm_f8_blockscale_workspace_bytes; 0 for most problems): lets few
  * output tiles with a long K run side by side. */
 int ckx_gemm_f8_blockscale_is_supported(int32_t M, int32_t N, int32_t K, int32_t lda, int32_t ldb, int32_t ldc,
@@ -463,7 +464,7 @@ int ckx_gemm_f8_blockscale(const void* p_a, const void* p_b, void* p_c, const fl
  * Blocks of block_size tokens; the code of token t, head h, element d of block b is
  * p_k[b * stride_block + h * stride_head + t * stride_token + d] (p_v alike), the value it stands for that code times
  * p_k_scale[b * stride_scale + h]. Slot number = block * block_size + token. e4m3 or int8 codes; head_dim a multiple of
- * 16 up to 128; block_size 16, 32, 64 or 128; strides multiples of 16, p_k and p_v 16-byte aligned. Codes are finite
+ * 16 up to 128; block_size 16, 32, 64 or 128; strides multiples of 16, p_k and p_v 16-byte aligned, block_size * stride_token under 2 GiB. Codes are finite
  * (ckx_kv_cache_store8 writes no others: it puts a NaN or infinity into the block's scale). Blocks with numbers outside
  * [0, num_blocks) are neither read nor written. */
 typedef struct ckx_kv_cache8
@@ -486,7 +487,7 @@ typedef struct ckx_kv_cache8
  *       sequence after sequence, and written behind them. Other columns are left alone.
  *   p_cu_new [batch + 1]: sums of the new lengths before each sequence; p_kv_lens [batch]: context + new
  *   p_slots [num_slots]: slot of every new token, sequence after sequence; -1 behind the last one, and where a token's
- *       block is missing (free list too short, table too narrow)
+ *       block is missing (free list too short, table too narrow) or has no 32-bit slot number
  *   p_used [1]: blocks needed; more than num_free says that the free list was too short
  * Lengths under zero count as zero; their sums fit 31 bits. At most 8192 sequences. No output may lie on an input. */
 int ckx_kv_cache_tables_is_supported(int32_t batch, int32_t num_free, int32_t max_blocks, int32_t stride_table,
@@ -497,7 +498,7 @@ int ckx_kv_cache_tables(const int32_t* p_context_lens, const int32_t* p_new_lens
                         int32_t block_size, void* stream);
 
 /* New keys and values into the cache. x: p_k / p_v [num_tokens, num_heads, head_dim] fp16 or bf16 (x_type), strides in
- * elements (multiples of 8, 16-byte aligned), token t into slot p_slots[t]; slots outside the cache (-1) are skipped. A run =
+ * elements (multiples of 8, 16-byte aligned), at most 2^29 tokens, token t into slot p_slots[t]; slots outside the cache (-1) are skipped. A run =
  * consecutive tokens whose slots lie in one block, slots ascending; a block occurs in one run of a call. With o the place
  * of the run's first token in its block, Q = 448 (e4m3) or 127 (int8), per head, for keys and values alike:
  *   new scale = max(max(max |x| over the run, 2^-100) / Q, o > 0 ? old scale : 0)
@@ -519,9 +520,10 @@ int ckx_kv_cache_store8(const void* p_k, const void* p_v, const int32_t* p_slots
  * over all cached tokens of the sequence, or with `causal` those up to the token's own place (the last query row sees all
  * of them, the one before it one less). A row that sees nothing is 0. Rows of p_o outside p_cu_q's are left alone. Scores, softmax
  * and sums are fp32; probability times value scale is rounded to fp16 (relative to the row's largest value scale) before the
- * second product. max_kv_len (an upper bound that a
+ * second product: an error of 2^-11 of each summand and, under 2^-14 of the largest, of 2^-25 of the row's largest value. max_kv_len (an upper bound that a
  * program knows) steers how the work is cut and no result depends on its being right; num_tokens bounds the rows that are
  * read and written. Token and head strides of q and o: elements, multiples of 8, 16-byte aligned.
+ * At most 2^31 - 65536 cached tokens a sequence (max_blocks * block_size); what p_kv_lens says beyond the table is not there.
  * Workspace (ckx_paged_attention8_workspace_bytes): required where that is not 0; launches that share one must not overlap. */
 int ckx_paged_attention8_is_supported(const ckx_kv_cache8* cache, int32_t batch, int32_t num_tokens, int32_t num_q_heads,
                                       int32_t max_kv_len, int32_t max_blocks, int32_t stride_table, int32_t stride_q_token,

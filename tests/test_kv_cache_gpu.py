@@ -220,3 +220,12 @@ def test_a_cache_past_32_bit_offsets():
     assert int(flat.count_nonzero()) == int(want[0][0].count_nonzero() + want[1][0].count_nonzero())
     ref, mag, big = sp.attention(q.cpu(), torch.zeros(1, 1), [0, 2], [2], want[0][0], want[1][0], want[0][1], want[1][1], 0.125, True)
     assert bool(((o.cpu().double() - ref).abs() <= sp.attention_bound(ref, mag, big, torch.bfloat16, D, 2)).all())
+
+
+def test_tables_block_numbers_without_a_slot():
+    """Numbers past 2^31 / block_size, in the table or the free list, would wrap to another block's slots."""
+    top = 2 ** 31 // 16
+    table = np.array([[top + 3, 5, -1], [top - 1, 2 ** 31 - 1, -1]])
+    got = run_tables([16, 31], [18, 3], [top, 9, top - 2], table, 21, 16)
+    want = [-1] * 16 + [9 * 16, 9 * 16 + 1] + [-1, (top - 2) * 16, (top - 2) * 16 + 1]
+    assert got[1] == [0, 18, 21] and got[4] == 3 and got[3].tolist() == want

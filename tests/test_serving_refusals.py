@@ -245,3 +245,18 @@ def test_python_operators_refuse_host_memory_and_wide_sizes():
             op.MakeArgumentPointer(0, 0, 0, wide, 256, 256, 256, 1, 4)
         with pytest.raises(OverflowError):
             ck.DeviceKvCacheTables().MakeArgumentPointer(*[0] * 8, 4, 8, 4, 4, wide, 16)
+
+
+def test_largest_sizes():
+    gemm = lambda M, N, K, lda=16, ldb=16, ldc=0: L.ckx_gemm_f8_blockscale_is_supported(M, N, K, lda, ldb, max(ldc, N), 1, M, 1, 1, capi.TYPE_BF16)
+    assert gemm(1, 1, 1 << 30) == capi.OK and gemm(1, 1, (1 << 30) + 16) == capi.UNSUPPORTED
+    assert gemm(1, (1 << 26) - 16, 16) == capi.OK and gemm(1, 1 << 26, 16) == capi.UNSUPPORTED
+    assert gemm(1 << 28, 128, 16) == capi.OK and gemm(1 << 29, 128, 16) == capi.UNSUPPORTED
+    c = cache()
+    store = lambda n: L.ckx_kv_cache_store8_is_supported(C.byref(c), n, 128, 64, 128, 64, capi.TYPE_F16)
+    assert store(1 << 29) == capi.OK and store((1 << 29) + 1) == capi.UNSUPPORTED
+    attend = lambda **k: L.ckx_paged_attention8_is_supported(C.byref(c), *{**GOOD, **k}.values())
+    most = 0x7fff0000 // 16
+    assert attend(blocks=most, st=most) == capi.OK and attend(blocks=most + 1, st=most + 1) == capi.UNSUPPORTED
+    assert L.ckx_paged_attention8_workspace_bytes(C.byref(c), 1, 1, 4, 1 << 20, most + 1) == 0
+    assert attend(scale=3e38) == capi.INVALID_VALUE and attend(scale=2e38) == capi.OK
