@@ -81,27 +81,27 @@ struct TileOf
 __device__ __forceinline__ TileOf tile_of(const AttentionArgs& p, int tile)
 {
     const int lane = threadIdx.x & 63;
-    auto start     = [&](int b) {
-        const int c = min(max(p.cu_q[b], 0), p.tokens);
-        return p.tile_tokens == 1 ? c : c / p.tile_tokens + b;
-    };
-    int count = 0; // sequences that begin at or before the tile
+    TileOf t;
+    t.b = 0, t.live = false, t.q0 = t.q_len = t.first = t.kv = 0;
     for(int b0 = 0; b0 < p.batch; b0 += 64)
     {
-        const int b   = b0 + lane;
-        const int n   = __popcll(__ballot(b < p.batch && start(b) <= tile));
-        count += n;
+        // all three at once: what the sequence's lane has is handed on, not loaded again
+        const int b = b0 + lane, at = min(b, p.batch - 1);
+        const int begin = p.cu_q[at], end = p.cu_q[at + 1], kv = p.kv_lens[at];
+        const int c = min(max(begin, 0), p.tokens), start = p.tile_tokens == 1 ? c : c / p.tile_tokens + b;
+        const int n = __popcll(__ballot(b < p.batch && start <= tile)); // sequences that begin at or before the tile
+        if(n > 0)
+        {
+            t.b     = b0 + n - 1;
+            t.q0    = __builtin_amdgcn_readlane(c, n - 1);
+            t.q_len = min(max(__builtin_amdgcn_readlane(end, n - 1), t.q0), p.tokens) - t.q0;
+            t.first = (tile - __builtin_amdgcn_readlane(start, n - 1)) * p.tile_tokens;
+            t.live  = t.first >= 0 && t.first < t.q_len;
+            t.kv    = min(max(__builtin_amdgcn_readlane(kv, n - 1), 0), p.max_blocks << p.block_shift);
+        }
         if(n < 64)
             break;
     }
-    TileOf t;
-    t.b    = __builtin_amdgcn_readfirstlane(max(count - 1, 0));
-    t.live = count > 0;
-    t.q0   = min(max(p.cu_q[t.b], 0), p.tokens);
-    t.q_len = min(max(p.cu_q[t.b + 1], t.q0), p.tokens) - t.q0;
-    t.first = (tile - start(t.b)) * p.tile_tokens;
-    t.live  = t.live && t.first >= 0 && t.first < t.q_len;
-    t.kv    = min(max(p.kv_lens[t.b], 0), p.max_blocks << p.block_shift);
     return t;
 }
 
