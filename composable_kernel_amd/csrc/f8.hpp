@@ -85,13 +85,38 @@ __device__ __forceinline__ uint32_t codes_of(float a, float b, float c, float d)
                                          (int)__builtin_rintf(d));
 }
 
-// eight consecutive elements of T as floats
+// x * f / d, the quotient rounded once: a multiplication by 1 / d leaves it up to two roundings off, which turns codes over where it
+// lies half way between two of them, and with x of 16 bits that is no rarity (x = 0.75 of the group's largest is such a place). The
+// remainder of the first quotient is exact, so that the second is the nearest. f is a few bits long: x * f is exact for 16-bit types,
+// its rest is added for fp32 (EXACT false). d infinite: 0 (NaN for an infinite x); d NaN: NaN.
+struct Quotient
+{
+    float f, d, inv;
+    __device__ __forceinline__ Quotient(float f_, float d_) : f(f_), d(__builtin_isinf(d_) ? 0.0f : d_), inv(1.0f / d_) {}
+    template <bool EXACT>
+    __device__ __forceinline__ float of(float x) const
+    {
+        const float y = x * f, q = y * inv;
+        float rest = __builtin_fmaf(-q, d, y);
+        if constexpr(!EXACT)
+            rest += __builtin_fmaf(x, f, -y);
+        return __builtin_fmaf(rest, inv, q);
+    }
+};
+// x * Q / amax with Q the largest code: both brought down by a power of two, so that nothing overflows
+template <int CODE>
+__device__ __forceinline__ Quotient quotient_of(float amax)
+{
+    return CODE == CODE_E4M3 ? Quotient(kE4m3Max / 512, amax * (1.0f / 512)) : Quotient(kI8Max / 128, amax * (1.0f / 128));
+}
+
+// eight consecutive elements of T as floats, at any address
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&x)[8])
 {
     if constexpr(sizeof(T) == 4)
     {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+        const f32x4 a = load_vec<f32x4>(p), b = load_vec<f32x4>(p + 4);
 #pragma unroll
         for(int i = 0; i < 4; ++i)
             x[i] = a[i], x[4 + i] = b[i];
@@ -99,7 +124,7 @@ __device__ __forceinline__ void load8(const T* p, float (&x)[8])
     else
     {
         typedef T tx8 __attribute__((ext_vector_type(8)));
-        const tx8 a = *reinterpret_cast<const tx8*>(p);
+        const tx8 a = load_vec<tx8>(p);
 #pragma unroll
         for(int i = 0; i < 8; ++i)
             x[i] = (float)a[i];

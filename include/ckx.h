@@ -433,7 +433,7 @@ enum
 
 /* ---- e4m3 codes of activations, one scale per row and group of 128 columns -----------------------
  *   s[m, g] = max(max_{k in g} |x[m, k]|, 2^-100) / 448        (fp32; NaN does not count)
- *   q[m, k] = e4m3(x[m, k] * (1 / s[m, k / 128]))              (fp32, round to nearest even)
+ *   q[m, k] = e4m3(x[m, k] * 448 / max(max |x|, 2^-100))       (the quotient rounded to fp32, then to nearest even)
  * x [M, K] fp32, fp16 or bf16 (x_type), q [M, K] e4m3, rows stride_x / stride_q elements apart; the scale of row m, group g
  * is p_scale[m * stride_scale_m + g * stride_scale_g]: (1, M) is the layout that ckx_gemm_f8_blockscale reads fastest. The last
  * group is short where K is no multiple of 128. A NaN stays NaN; an infinity makes its group's scale infinite, and every
@@ -503,7 +503,8 @@ int ckx_kv_cache_tables(const int32_t* p_context_lens, const int32_t* p_new_lens
  * of the run's first token in its block, Q = 448 (e4m3) or 127 (int8), per head, for keys and values alike:
  *   new scale = max(max(max |x| over the run, 2^-100) / Q, o > 0 ? old scale : 0)
  *   o > 0 and the scale grew: the codes of the tokens before o become round(code * (old / new))
- *   codes of the run: round(x * (1 / new)), ties to even
+ *   codes of the run: round(x * Q / max(max |x|, 2^-100)) where the run set the scale, round(x / old) where it did not; the
+ *   quotient rounded to fp32, then ties to even
  * A block is filled in order: what lies behind the run counts as unwritten. A NaN or infinity among the run makes the
  * scale NaN or infinite, so that the block's values are NaN until it is begun anew (o == 0). */
 int ckx_kv_cache_store8_is_supported(const ckx_kv_cache8* cache, int32_t num_tokens, int32_t stride_k_token,

@@ -21,16 +21,16 @@ def to_code(x32, dtype):
 
 
 def quantize(x):
-    """(codes, scales [M, groups]) by the formula's own fp32 steps."""
+    """(codes, scales [M, groups]): fp32 scales, codes of the quotient in 64 bits rounded to fp32 first, as the formula says."""
     M, K = x.shape
     groups = -(-K // 128)
     pad = torch.zeros((M, groups * 128))
     pad[:, :K] = x.float()
     pad = pad.view(M, groups, 128)
     amax = torch.where(pad.isnan(), torch.zeros_like(pad), pad).abs().amax(dim=2)
-    scale = torch.clamp(amax, min=TINY) / 448.0
-    q = (pad * (1.0 / scale)[:, :, None]).view(M, groups * 128)[:, :K].to(torch.float8_e4m3fn)
-    return q, scale
+    amax = torch.clamp(amax, min=TINY)
+    q = (pad.double() * 448.0 / amax.double()[:, :, None]).float().view(M, groups * 128)[:, :K].to(torch.float8_e4m3fn)
+    return q, amax / 448.0
 
 
 def gemm(a, b, sa, sb):
@@ -65,7 +65,9 @@ def store(cache, scale, x, slots):
         new = x[t:end].float()
         for h in range(cache.shape[1]):
             v = new[:, h]
-            s = torch.tensor(float("nan")) if v.isnan().any() else torch.clamp(v.abs().max(), min=TINY) / q
+            amax = torch.clamp(v.abs().max(), min=TINY)
+            s = torch.tensor(float("nan")) if v.isnan().any() else amax / q
+            quotient = (v.double() * q / amax.double()).float()
             if begin > 0:
                 old = scale[block, h].clone()
                 if not old.isnan() and not old >= s:
@@ -73,8 +75,9 @@ def store(cache, scale, x, slots):
                     cache[block, h, :begin] = to_code(torch.nan_to_num(codes, nan=0.0), cache.dtype)
                 else:
                     s = old
+                    quotient = (v.double() / s.double()).float()
             scale[block, h] = s
-            codes = to_code(torch.nan_to_num(v * (1.0 / s), nan=0.0), cache.dtype)
+            codes = to_code(torch.nan_to_num(quotient, nan=0.0), cache.dtype)
             for i in range(t, end):
                 cache[block, h, slots[i] % size] = codes[i - t]
         t = end

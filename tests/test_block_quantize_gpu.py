@@ -77,3 +77,21 @@ def test_nan_and_infinity():
     assert bool(back[0, 5].isnan()) and int(back[0].isnan().sum()) == 1
     assert bool(back[1, 128:].isnan().all()) and not bool(back[1, :128].isnan().any())
     assert bool(back[3, :128].isnan().all()) and not bool(back[3, 128:].isnan().any())
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_values_half_way_between_codes(kind):
+    """x * 448 / amax with 8 (11) bits in x and amax lies on the middle of two codes or 2^-16 and more away from it: every code is the
+    one that 64 bits round to. Rows of every mantissa of amax; x = 0.75 amax, 0.65625 amax, ... where they have a bit pattern."""
+    bits = 7 if kind == "bf16" else 10
+    amax = (1 + torch.arange(2 ** bits) / 2 ** bits)[:, None].double()
+    part = torch.tensor([(17 + 2 * i) * 2.0 ** -j / 28 * s for i in range(8) for j in range(1, 7) for s in (1, -1)]).double()
+    x = torch.cat([amax, (amax * part).to(DT[kind]).double().clamp(-amax, amax), torch.zeros(2 ** bits, 31)], dim=1).to(DT[kind])
+    assert x.shape[1] == 128
+    q, s = run(x, kind)
+    want = x.double() * 448 / amax
+    step = torch.exp2(torch.floor(torch.log2(want.abs().clamp(min=2.0 ** -6))) - 3)
+    ties = ((want / step) % 1 == 0.5).sum()
+    assert int(ties) > 2 ** bits
+    assert torch.equal(q.double(), torch.round(want / step) * step)
+    check(x, kind)
