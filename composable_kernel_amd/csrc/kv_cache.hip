@@ -274,8 +274,10 @@ __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs p, int span)
 template <typename T, int CODE>
 hipError_t launch_store(const StoreArgs& a, hipStream_t s)
 {
-    // tokens a wave looks at: one where the tokens are few (each its own run: a step's), 16 where they are many
-    const int span      = a.tokens <= 2048 ? 1 : 16;
+    // Tokens a wave looks at, us with 1 / 4 / 16 of them (8 heads of 128). Single tokens of as many sequences: 64 5.0 / 6.9 / 22, 512
+    // 7.6 / 8.2 / 21, 1024 12.1 / 10.9 / 21, 4096 43 / 35 / 37; prompts: 512 5.2 / 4.8 / 5.7, 1024 9.5 / 4.8 / 5.4, 4096 14.3 / 9.6 / 8.8,
+    // 4 of 4096 37 / 25 / 19
+    const int span      = a.tokens <= 512 ? 1 : a.tokens <= 4096 ? 4 : 16;
     const int64_t units = ((int64_t)a.tokens + span - 1) / span;
     hipLaunchKernelGGL((kv_store_kernel<T, CODE>), dim3((unsigned)((units + 3) / 4), (unsigned)a.cache.num_heads * 2), dim3(256), 0, s,
                        a, span);

@@ -11,7 +11,10 @@
 // LDS rows of 16-byte chunks, chunk c of row r at c ^ (r & 15) (keys of 128), c ^ (r & 7) (keys of 64), c ^ ((r ^ r / 4) & 7)
 // (values): eight neighbouring rows never meet on a bank, neither for the writes nor for the reads.
 // What bounds it are vector instructions: 7 a score (the exponential counts four), about as many cycles as the matrix
-// instructions take, and the two share the SIMD's issue.
+// instructions take, and the two share the SIMD's issue: 4 sequences of 4096 and 1024 new tokens, 32 / 8 heads of 128, int8, 309 us,
+// 0.65 PFLOP/s (counters before the last steps: matrix instructions busy 33 %, vector instructions 56 %). Codes two steps ahead
+// instead of one, and scales one ahead, were the last steps that gave; a copy of the loop without masks gives heads of 64 a tenth and
+// spills at 128.
 #include "paged_attention.hpp"
 
 namespace ckx {

@@ -147,18 +147,19 @@ def test_store(code, xt, H, D, size, layout):
     check_store(k, v, slots, cache, xt)
 
 
-def test_store_of_many_tokens():
-    """More tokens than one wave looks at one by one, runs that begin anywhere, skipped tokens between and inside them."""
+@pytest.mark.parametrize("tokens", [300, 700, 2600, 5200])
+def test_store_of_many_tokens(tokens):
+    """One token, four and sixteen a wave, runs that begin anywhere, skipped tokens between and inside them."""
     g = sp.gen(8)
-    cache = sp.random_cache(g, 300, 2, 16, 64, torch.float8_e4m3fn)
-    order = torch.randperm(300, generator=g).tolist()
+    blocks = tokens // 8
+    cache = sp.random_cache(g, blocks, 2, 16, 64, torch.float8_e4m3fn)
+    order = torch.randperm(blocks, generator=g).tolist()
     slots, at = [], 0
-    while len(slots) < 2600 and at < 280:
+    while len(slots) < tokens:
         first, n = int(torch.randint(0, 16, (1,), generator=g)), int(torch.randint(1, 60, (1,), generator=g))
-        blocks = order[at:at + -(-(first + n) // 16)]
-        at += len(blocks)
-        slots += [blocks[(first + i) // 16] * 16 + (first + i) % 16 for i in range(n)] + [-1] * int(torch.randint(0, 3, (1,), generator=g))
-    assert len(slots) > 2048
+        mine = order[at:at + -(-(first + n) // 16)]
+        at += len(mine)
+        slots += [mine[(first + i) // 16] * 16 + (first + i) % 16 for i in range(n)] + [-1] * int(torch.randint(0, 3, (1,), generator=g))
     k, v = sp.normal(g, (len(slots), 2, 64), torch.bfloat16, 2.0), sp.normal(g, (len(slots), 2, 64), torch.bfloat16, 0.2)
     check_store(k, v, slots, cache, "bf16")
 
