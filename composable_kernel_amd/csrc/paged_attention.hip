@@ -377,14 +377,18 @@ Plan plan(const ckx_kv_cache8& c, int batch, int tokens, int heads, int max_kv, 
     p.tiles         = p.tile_tokens == 1 ? tokens : tokens / p.tile_tokens + batch;
     // Shares of the cached tokens, joined by a second launch, where the tiles alone leave CUs without work. Single tokens: one
     // workgroup a CU (what fits on one), none of under 256 tokens, a turn for each wave; 8 sequences of 8192: 30.5 us, 32.7 with two
-    // a CU, 38.3 with three. Prompts: two a CU and none of under 512 tokens, eight steps.
+    // a CU, 38.3 with three. Prompts: up to two a CU, none of under 128 tokens, two steps, and none under 1024 cached tokens, where the
+    // second launch costs what the shares give (whole / shares of 128, heads of 128: 1 x 512 new 21.0 / 25.9 us, 1 x 1024 34.8 / 34.5,
+    // 4 x (1000 + 100) 26.8 / 20.5; shares of 256 22.0).
     const int64_t groups  = (int64_t)(tokens < p.tiles ? tokens : p.tiles) * c.num_heads * p.head_tiles;
     const int64_t longest = (int64_t)max_blocks * c.block_size;
     const int64_t kv      = max_kv < longest ? max_kv : longest;
     int64_t splits        = p.prompt ? 512 / groups : (256 + groups - 1) / groups;
-    const int64_t least   = p.prompt ? 512 : 256;
+    const int64_t least   = p.prompt ? 128 : 256;
     if(splits > kv / least)
         splits = kv / least;
+    if(p.prompt && kv < 1024)
+        splits = 1;
     p.splits = (int)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
     return p;
 }

@@ -199,3 +199,11 @@ def test_prompts_over_long_caches(news, kvs, code):
     """Few tiles, many cached tokens: the shares of the cached tokens are joined, some of them empty."""
     Problem(news, kvs, 4, 1, 64, 16, code).check()
     Problem(news, kvs, 2, 2, 128, 64, code, "f16", causal=False).check()
+
+
+@pytest.mark.parametrize("max_kv", [0, 1023, 1024, 1500, 100000])
+@pytest.mark.parametrize("causal", [True, False])
+def test_shares_of_prompts(max_kv, causal):
+    """Shares of two steps and more, most of them empty for the short sequences; the bound only steers how many there are."""
+    Problem([60, 40, 70], [1500, 30, 70], 4, 1, 80, 16, causal=causal).check(max_kv=max_kv)
+    Problem([200], [1100], 8, 2, 128, 32, torch.int8, "f16", causal=causal).check(max_kv=max_kv)
