@@ -11,9 +11,9 @@
 // LDS rows of 16-byte chunks, chunk c of row r at c ^ (r & 15) (keys of 128), c ^ (r & 7) (keys of 64), c ^ ((r ^ r / 4) & 7)
 // (values): eight neighbouring rows never meet on a bank, neither for the writes nor for the reads.
 // What bounds it are vector instructions: 7 a score (the exponential counts four), about as many cycles as the matrix
-// instructions take, and the two share the SIMD's issue: 4 sequences of 4096 and 1024 new tokens, 32 / 8 heads of 128, int8, 309 us,
-// 0.65 PFLOP/s (counters before the last steps: matrix instructions busy 33 %, vector instructions 56 %). Codes two steps ahead
-// instead of one, and scales one ahead, were the last steps that gave; a copy of the loop without masks gives heads of 64 a tenth and
+// instructions take, and the two share the SIMD's issue: 4 sequences of 4096 and 1024 new tokens, 32 / 8 heads of 128, int8, 306 us,
+// 0.65 PFLOP/s (counters some steps earlier: matrix instructions busy 33 %, vector instructions 56 %; LDS is read at about 60 % of its
+// rate). Fragments further ahead, and the output's matrix instructions between the exponentials, are level; a copy of the loop without masks gives heads of 64 a tenth and
 // spills at 128.
 #include "paged_attention.hpp"
 
@@ -148,7 +148,10 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
     const int krow = wave * 16 + kt, vrow = (vd & ~31) + (((vd >> 2) & 3) << 3) + (((vd >> 4) & 1) << 2);
     const uint32_t k_write = krow * (DP * 2) + (((kq * (KC / 4)) ^ (krow & (KC - 1))) << 4);
     const uint32_t v_write = K_TILE + vrow * (kStep * 2) + (((2 * wave + vh) ^ ((vrow ^ (vrow >> 2)) & 7)) << 4);
-    auto deposit = [&](int step, auto odd) {
+    // In pieces (2 KB chunks of keys, 4 of values), so that a wave converts the next step's between the matrix instructions of its scores:
+    // heads of 64, 8 x (1024 + 256) 50.9 -> 44.3 us, heads of 128, 4 x (4096 + 1024) 292 -> 285. The stage was last read a step ago.
+    uint32_t k_to, v_to, v_lo[4], v_hi[4];
+    auto deposit_begin = [&](int step, auto odd) {
         constexpr int S = decltype(odd)::value;
         const int t = step * kStep + wave * 16;
         if(t + 16 > most) // (what lies behind the last token is no value: zero, whatever its bytes are)
@@ -157,27 +160,31 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
             for(int i = 0; i < 8; ++i)
                 vb[S][i] = t + 8 * (i >> 2) + 4 * vh + (i & 3) < most ? vb[S][i] : 0;
         }
-        uint32_t k_to = k_write + (step & 1) * STAGE, v_to = v_write + (step & 1) * STAGE;
+        k_to = k_write + (step & 1) * STAGE, v_to = v_write + (step & 1) * STAGE;
         asm volatile("" : "+v"(k_to), "+v"(v_to));
-#pragma unroll
-        for(int j = 0; j < KB; ++j)
-#pragma unroll
-            for(int e = 0; e < 2; ++e)
-            {
-                const int c = 2 * j + e; // (+ kq * KC / 4, whose bits are higher ones)
-                *reinterpret_cast<i32x4*>(lds + (k_to ^ (uint32_t)(c << 4))) = codes8<CODE, T>(kb[S][j][2 * e], kb[S][j][2 * e + 1]);
-            }
-        if(vh < 2)
+    };
+    constexpr int PIECES = 2 * KB + 4;
+    auto deposit_piece = [&](int n, auto odd) {
+        constexpr int S = decltype(odd)::value;
+        if(n < 2 * KB) // (+ kq * KC / 4, whose bits are higher ones)
+            *reinterpret_cast<i32x4*>(lds + (k_to ^ (uint32_t)(n << 4))) =
+                codes8<CODE, T>(kb[S][n / 2][2 * (n & 1)], kb[S][n / 2][2 * (n & 1) + 1]);
+        else if(DP == 128 || vh < 2)
         {
-            uint32_t lo[4], hi[4];
-            transpose4(vb[S][0], vb[S][1], vb[S][2], vb[S][3], lo);
-            transpose4(vb[S][4], vb[S][5], vb[S][6], vb[S][7], hi);
-#pragma unroll
-            for(int i = 0; i < 4; ++i)
+            const int i = n - 2 * KB;
+            if(i == 0)
             {
-                *reinterpret_cast<i32x4*>(lds + (v_to ^ (uint32_t)(i << 4)) + i * (kStep * 2)) = codes8<CODE, _Float16>(lo[i], hi[i]);
+                transpose4(vb[S][0], vb[S][1], vb[S][2], vb[S][3], v_lo);
+                transpose4(vb[S][4], vb[S][5], vb[S][6], vb[S][7], v_hi);
             }
+            *reinterpret_cast<i32x4*>(lds + (v_to ^ (uint32_t)(i << 4)) + i * (kStep * 2)) = codes8<CODE, _Float16>(v_lo[i], v_hi[i]);
         }
+    };
+    auto deposit = [&](int step, auto odd) {
+        deposit_begin(step, odd);
+#pragma unroll
+        for(int n = 0; n < PIECES; ++n)
+            deposit_piece(n, odd);
     };
 
     const uint32_t k_read = r * (DP * 2) + ((h ^ (r & (KC - 1))) << 4), v_read = K_TILE + r * (kStep * 2) + ((h ^ ((r ^ (r >> 2)) & 7)) << 4);
@@ -230,6 +237,7 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
                 w_log[b] = lane_of(wl_log, 4 + b);
                 w_inv[b] = lane_of(wl_inv, 4 + b);
             }
+            deposit_begin(step + 1, other);
             f32x16 s[2];
             constexpr int DQ = 2; // fragments DQ pairs of instructions ahead: an LDS read takes about as long as three of them
             i32x4 kf[DQ + 1][2];
@@ -249,6 +257,9 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
 #pragma unroll
                 for(int u = 0; u < 2; ++u)
                     s[u] = mfma32<T>(kf[k % (DQ + 1)][u], qf[k], k == 0 ? f32x16(0.0f) : s[u]);
+#pragma unroll
+                for(int n = k * PIECES / KK; n < (k + 1) * PIECES / KK; ++n)
+                    deposit_piece(n, other);
                 __builtin_amdgcn_sched_barrier(0);
             }
             const int reach = see - t0 - 4 * h;
@@ -333,7 +344,7 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
         };
         if(t0 < furthest)
             multiply(t0 + kStep <= least && there == 15u);
-        if(step + 1 < steps)
+        else
             deposit(step + 1, other);
         blocks = blocks1, blocks1 = blocks2, blocks2 = blocks3;
         scale = scale1, scale1 = scale2;
