@@ -103,7 +103,13 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_rows_kernel(AttentionArg
     auto lane_of = [](auto x, int from) {
         return __builtin_bit_cast(decltype(x), __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), from));
     };
-    auto fetch = [&](Turn& x, int turn) {
+    // (the first turn's codes are asked for before its scales are waited for; in the loop that order costs registers and 6 % for int8)
+    auto scales_to = [&](Turn& x, int turn) {
+#pragma unroll
+        for(int h = 0; h < 2; ++h)
+            x.ks[h] = lane_of(ks_of, 2 * (turn & 31) + h), x.vs[h] = lane_of(vs_of, 2 * (turn & 31) + h);
+    };
+    auto fetch = [&](Turn& x, int turn, auto first) {
         if((turn & 31) == 0)
             look_up(turn);
 #pragma unroll
@@ -111,7 +117,9 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_rows_kernel(AttentionArg
         {
             const int from  = 2 * (turn & 31) + h;
             const int block = lane_of(blocks, from);
-            x.there[h] = block >= 0, x.ks[h] = lane_of(ks_of, from), x.vs[h] = lane_of(vs_of, from);
+            x.there[h]      = block >= 0;
+            if constexpr(!decltype(first)::value)
+                x.ks[h] = lane_of(ks_of, from), x.vs[h] = lane_of(vs_of, from);
             if(block < 0)
             {
 #pragma unroll
@@ -143,11 +151,16 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_rows_kernel(AttentionArg
                     x.vb[4 * h + i][0] = *reinterpret_cast<const uint32_t*>(vi);
             }
         }
+        if constexpr(decltype(first)::value)
+        {
+            __builtin_amdgcn_sched_barrier(0);
+            scales_to(x, turn);
+        }
     };
 
     Turn even, odd;
     if(turns > 0)
-        fetch(even, 0);
+        fetch(even, 0, std::true_type{});
     i32x4 qf[KJ][2];
 #pragma unroll
     for(int j = 0; j < KJ; ++j)
@@ -243,10 +256,10 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_rows_kernel(AttentionArg
     for(int turn = 0; turn < turns; turn += 2)
     {
         if(turn + 1 < turns)
-            fetch(odd, turn + 1);
+            fetch(odd, turn + 1, std::false_type{});
         multiply(even, turn);
         if(turn + 2 < turns)
-            fetch(even, turn + 2);
+            fetch(even, turn + 2, std::false_type{});
         if(turn + 1 < turns)
             multiply(odd, turn + 1);
     }
