@@ -207,3 +207,10 @@ def test_shares_of_prompts(max_kv, causal):
     """Shares of two steps and more, most of them empty for the short sequences; the bound only steers how many there are."""
     Problem([60, 40, 70], [1500, 30, 70], 4, 1, 80, 16, causal=causal).check(max_kv=max_kv)
     Problem([200], [1100], 8, 2, 128, 32, torch.int8, "f16", causal=causal).check(max_kv=max_kv)
+
+
+@pytest.mark.parametrize("code", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("D,size", [(64, 16), (128, 64)])
+def test_one_share_of_a_long_cache(code, D, size):
+    """Over 8192 tokens a share: the block numbers and scales of a wave's 32 turns are fetched anew."""
+    Problem([1, 2, 1], [8193, 20000, 8192], 4, 1, D, size, code).check(max_kv=0)
