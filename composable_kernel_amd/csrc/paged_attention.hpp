@@ -3,7 +3,7 @@
 // The scales stay out of the products: a block's key scale multiplies the finished score q . codes, its value scale the
 // probability, so that the matrix instructions run on the codes themselves, converted exactly to 16 bits (keys to the type of q,
 // values to fp16). What is rounded is probability * value scale, to fp16 (2^-11 of each summand, independent from token to
-// token), taken relative to the largest value scale met so far: without that, a scale of 2^-10 would put most of a row's products
+// token), taken relative to the largest value scale that the row has met so far: without that, a scale of 2^-10 would put most of a row's products
 // under fp16's normal numbers; bf16 would not need it, but rounds by 2^-8. Products under 2^-14 of that largest scale lose bits one by
 // one, 2^-25 of it at most.
 #pragma once
@@ -41,8 +41,9 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b)
     return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
 }
 
-// The value scale that the output sums are relative to: the largest finite one so far. take() returns what the sums so far
-// are to be multiplied by, of() a scale relative to it (an infinity or NaN stays one).
+// The value scale that a row's output sums are relative to: the largest finite one of the blocks that the row has seen so far (a block
+// that it does not see, however large, would cost it bits). take() returns what the sums so far are to be multiplied by, of() a
+// scale relative to it (an infinity or NaN stays one).
 struct ValueScale
 {
     float top = kLeast, inv = 1.0f / kLeast;

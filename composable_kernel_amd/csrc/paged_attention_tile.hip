@@ -195,7 +195,10 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
         for(int i = 0; i < 16; ++i)
             o[j][i] = 0.0f;
     float m = -__builtin_inff(), l = 0.0f;
-    ValueScale unit;
+    // The value scale that the row's sums are relative to, the largest finite one that it has seen, and its logarithm; `low`: the least of
+    // them among the wave's rows (steps that all rows see whole leave them one), under which no scale raises any.
+    constexpr float kLeast = 1.9259299443872359e-34f; // (2^-112: a score's sum relative to it stays finite)
+    float top = kLeast, top_log = -112.0f, low = kLeast;
 
     auto lane_of = [](auto x, int from) {
         return __builtin_bit_cast(decltype(x), __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), from));
@@ -221,22 +224,34 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
             // twelve registers that the kernel has not got.)
             uint32_t k_at = k_read + (step & 1) * STAGE, v_at = v_read + (step & 1) * STAGE;
             asm volatile("" : "+v"(k_at), "+v"(v_at));
-            // The value scales relative to the largest so far go into the exponent, exp2(score - m + log2 w), which saves a multiplication a
-            // score; the sum of the probabilities takes them out again, 16 tokens at a time. (The least: no 1 / w is infinite.)
+            // The value scales go into the exponent, exp2(score - m + log2(scale / top)), which saves a multiplication a score; the
+            // sum of the probabilities takes them out again, 16 tokens at a time.
             float keep_v = 1.0f;
-            if(__any((lane & 4) && scale > unit.top))
-                keep_v = unit.take(lane_of(scale, 4), lane_of(scale, 5)) * unit.take(lane_of(scale, 6), lane_of(scale, 7));
-            const float rel = unit.of(scale), wl = rel < kTinyAmax ? kTinyAmax : rel;
-            const float wl_log = __builtin_amdgcn_logf(wl), wl_inv = __builtin_amdgcn_rcpf(wl);
+            if(__any((lane & 4) && scale > low))
+            {
+                float next = top;
+#pragma unroll
+                for(int b = 0; b < 4; ++b)
+                {
+                    const float v = lane_of(scale, 4 + b);
+                    next          = __builtin_fmaxf(next, __builtin_isfinite(v) && see - t0 > 16 * b ? v : 0.0f);
+                }
+                keep_v = top / next;
+                top = next, top_log = __builtin_amdgcn_logf(next);
+                float x = see > t0 ? next : __builtin_inff(); // (rows that are through do not count)
+#pragma unroll
+                for(int d = 1; d < 32; d *= 2)
+                    x = __builtin_fminf(x, __shfl_xor(x, d));
+                low = lane_of(x, 0);
+            }
+            // (The least: no 1 / w is infinite.)
+            const float least_w = __builtin_fmaxf(low * 0x1p-100f, 0x1p-125f), w = scale < least_w ? least_w : scale;
+            const float w_logs = __builtin_amdgcn_logf(w), w_invs = __builtin_amdgcn_rcpf(w);
+            const float cs = scale * __builtin_fabsf(p.scale), c_least = cs < kTinyAmax ? kTinyAmax : cs; // (no -inf times zero; NaN stays)
             float c[4], w_log[4], w_inv[4];
 #pragma unroll
             for(int b = 0; b < 4; ++b)
-            {
-                c[b]     = lane_of(scale, b) * __builtin_fabsf(p.scale);
-                c[b]     = c[b] < kTinyAmax ? kTinyAmax : c[b]; // (no -inf times zero; NaN stays)
-                w_log[b] = lane_of(wl_log, 4 + b);
-                w_inv[b] = lane_of(wl_inv, 4 + b);
-            }
+                c[b] = lane_of(c_least, b), w_log[b] = lane_of(w_logs, 4 + b), w_inv[b] = lane_of(w_invs, 4 + b);
             deposit_begin(step + 1, other);
             f32x16 s[2];
             constexpr int DQ = 2; // fragments DQ pairs of instructions ahead: an LDS read takes about as long as three of them
@@ -279,7 +294,7 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
             }
             // (the maximum is there for the range only: of the unscaled scores of 16 tokens, then scaled; and it is raised only by
             // leaps, 2^6 or more, so that the sums are seldom rescaled: no probability exceeds 2^6 then)
-            float top = -__builtin_inff();
+            float most_s = -__builtin_inff();
 #pragma unroll
             for(int b = 0; b < 4; ++b)
             {
@@ -287,15 +302,15 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
 #pragma unroll
                 for(int i = 1; i < 8; ++i)
                     x = __builtin_elementwise_maximum(x, s[b >> 1][8 * (b & 1) + i]);
-                top = __builtin_elementwise_maximum(top, x == -__builtin_inff() ? x : x * c[b]); // (-inf: nothing seen, whatever the scale is)
+                most_s = __builtin_elementwise_maximum(most_s, x == -__builtin_inff() ? x : x * c[b]); // (-inf: nothing seen, whatever the scale is)
             }
             // (maximum, which a NaN wins: one instruction for three values where fmaxf makes every one a quiet number first. A row with a NaN
             // among its scores raises no maximum any more; it is NaN.)
-            top = over_halves(top, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+            most_s = over_halves(most_s, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
             float keep_o = keep_v;
-            if(__any(top > m + 6.0f))
+            if(__any(most_s > m + 6.0f))
             {
-                const float now = __builtin_fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - (now == -__builtin_inff() ? 0.0f : now));
+                const float now = __builtin_fmaxf(m, most_s), keep = __builtin_amdgcn_exp2f(m - (now == -__builtin_inff() ? 0.0f : now));
                 m = now;
                 l *= keep;
                 keep_o *= keep;
@@ -306,7 +321,7 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
                 for(int j = 0; j < DT; ++j)
                     o[j] *= keep_o;
             }
-            const float zero = m == -__builtin_inff() ? 0.0f : m; // (nothing seen yet)
+            const float zero = (m == -__builtin_inff() ? 0.0f : m) + top_log; // (nothing seen yet)
             i32x4 vf[2][DT];
             auto read_v = [&](int k) {
 #pragma unroll
@@ -314,6 +329,7 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
                     vf[k & 1][j] = *reinterpret_cast<const i32x4*>(lds + (v_at ^ (uint32_t)(k << 5)) + j * 32 * kStep * 2);
             };
             i32x4 pf[4];
+            float sums = 0.0f; // over top
 #pragma unroll
             for(int b = 0; b < 4; ++b)
             {
@@ -328,9 +344,10 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
                     pr[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b >> 1][8 * (b & 1) + i], cb, bias));
                     sum += pr[i];
                 }
-                l     = __builtin_fmaf(sum, sees ? w_inv[b] : 0.0f, l);
+                sums  = __builtin_fmaf(sum, sees ? w_inv[b] : 0.0f, sums);
                 pf[b] = i32x4{(int)pack_f16(pr[0], pr[1]), (int)pack_f16(pr[2], pr[3]), (int)pack_f16(pr[4], pr[5]), (int)pack_f16(pr[6], pr[7])};
             }
+            l = __builtin_fmaf(sums, top, l);
             read_v(0);
 #pragma unroll
             for(int k = 0; k < 4; ++k)
@@ -368,7 +385,7 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
 #pragma unroll
             for(int e = 0; e < 16; e += 4)
                 *reinterpret_cast<f32x4*>(p.ws + at * DP + 32 * j + 16 * h + e) =
-                    f32x4{o[j][e] * unit.top, o[j][e + 1] * unit.top, o[j][e + 2] * unit.top, o[j][e + 3] * unit.top};
+                    f32x4{o[j][e] * top, o[j][e + 1] * top, o[j][e + 2] * top, o[j][e + 3] * top};
         if(h == 0)
         {
             float* const ml = p.ws + attention_rows(p) * p.splits * DP + at * 2;
@@ -376,7 +393,7 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
         }
         return;
     }
-    const float f = l == 0.0f ? 0.0f : unit.top / l; // (a row that sees nothing: zero)
+    const float f = l == 0.0f ? 0.0f : top / l; // (a row that sees nothing: zero)
     T* const to   = reinterpret_cast<T*>(p.o) + token * p.so_t + (int64_t)head * p.so_h;
     typedef T tx8 __attribute__((ext_vector_type(8)));
 #pragma unroll

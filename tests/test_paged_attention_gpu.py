@@ -214,3 +214,40 @@ def test_shares_of_prompts(max_kv, causal):
 def test_one_share_of_a_long_cache(code, D, size):
     """Over 8192 tokens a share: the block numbers and scales of a wave's 32 turns are fetched anew."""
     Problem([1, 2, 1], [8193, 20000, 8192], 4, 1, D, size, code).check(max_kv=0)
+
+
+def _rows_largest_scale(p):
+    """[rows]: the largest value scale among the blocks that a row sees."""
+    top = torch.zeros(p.cu[-1], dtype=torch.float64)
+    for b, (n, kv) in enumerate(zip(p.news, p.kvs)):
+        for i in range(n):
+            see = kv - n + i + 1 if p.causal else kv
+            blocks = [int(x) for x in p.table[b, :-(-max(see, 0) // p.size)]]
+            top[p.cu[b] + i] = max([float(p.cache[3][x].abs().max()) for x in blocks] + [0.0])
+    return top
+
+
+def _check_to_each_rows_own_scale(p, **kw):
+    """attention_bound, and what probabilities under fp16's normal numbers cost (serving_plain.small_products), row by row."""
+    got = p.run(**kw).double()
+    kc, vc, ks, vs = p.cache
+    want, mag, big = sp.attention(p.q, p.table, p.cu, p.kvs, kc, vc, ks, vs, p.scale, p.causal)
+    small = max(p.kvs) * 2.0 ** -25 * sp.QMAX[vc.dtype] * _rows_largest_scale(p)
+    bound = sp.attention_bound(want, mag, big, DT[p.xt], p.D, max(p.kvs)) + small[:, None, None]
+    bad = ~((got - want).abs() <= bound)
+    assert not bool(bad.any()), (float(((got - want).abs() / bound).nan_to_num(nan=1e9).max()), bad.nonzero()[:4].tolist(), int(bad.sum()))
+
+
+@pytest.mark.parametrize("code", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("up", [10, 30])
+@pytest.mark.parametrize("news,kvs,heads,H,D", [([5], [50], 8, 2, 64), ([7, 9], [50, 70], 6, 3, 128), ([40], [64], 8, 2, 64),
+                                                ([100, 33], [200, 40], 8, 2, 128), ([70, 60], [1500, 70], 4, 1, 80)])
+def test_a_value_scale_reaches_only_rows_that_see_its_block(news, kvs, heads, H, D, up, code):
+    """Value scales that grow 2^up-fold from block to block over the new tokens: a row that sees the first of them keeps its own
+    precision, whatever the scales of the blocks behind it are."""
+    p = Problem(news, kvs, heads, H, D, 16, code)
+    for b, (n, kv) in enumerate(zip(news, kvs)):
+        first = (kv - n) // 16
+        for c in range(first + 1, -(-kv // 16)):
+            p.cache[3][int(p.table[b, c])] *= 2.0 ** min(up * (c - first), 90)
+    _check_to_each_rows_own_scale(p)
