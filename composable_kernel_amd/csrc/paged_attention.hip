@@ -218,7 +218,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_rows_kernel(AttentionArg
             keep_o = unit.take(v0, v1);
         if(__any(top > m + 6.0f))
         {
-            const float now = __builtin_fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - (now == -__builtin_inff() ? 0.0f : now));
+            // (the rows that leap, no others: a row's bits are its own)
+            const float now = top > m + 6.0f ? top : m, keep = __builtin_amdgcn_exp2f(m - (now == -__builtin_inff() ? 0.0f : now));
             m = now;
             l *= keep;
             keep_o *= keep;

@@ -310,7 +310,8 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
             float keep_o = keep_v;
             if(__any(most_s > m + 6.0f))
             {
-                const float now = __builtin_fmaxf(m, most_s), keep = __builtin_amdgcn_exp2f(m - (now == -__builtin_inff() ? 0.0f : now));
+                // (the rows that leap, no others: a row's bits are its own)
+                const float now = most_s > m + 6.0f ? most_s : m, keep = __builtin_amdgcn_exp2f(m - (now == -__builtin_inff() ? 0.0f : now));
                 m = now;
                 l *= keep;
                 keep_o *= keep;

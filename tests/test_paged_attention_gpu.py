@@ -251,3 +251,19 @@ def test_a_value_scale_reaches_only_rows_that_see_its_block(news, kvs, heads, H,
         for c in range(first + 1, -(-kv // 16)):
             p.cache[3][int(p.table[b, c])] *= 2.0 ** min(up * (c - first), 90)
     _check_to_each_rows_own_scale(p)
+
+
+@pytest.mark.parametrize("code", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("news,kvs,heads,H,D", [([5], [50], 8, 2, 64), ([10, 9], [311, 70], 8, 2, 128), ([40], [64], 8, 2, 64),
+                                                ([100, 33], [250, 40], 8, 2, 128), ([70, 60], [1524, 70], 4, 1, 80)])
+def test_blocks_that_a_row_does_not_see_change_none_of_its_bits(news, kvs, heads, H, D, code):
+    """Large key and value scales in the last block of every sequence, which only the last rows see."""
+    p = Problem(news, kvs, heads, H, D, 16, code)
+    want, blind = p.run(), []
+    for b, (n, kv) in enumerate(zip(news, kvs)):
+        last = (kv - 1) // 16
+        for x in p.cache[2:]:
+            x[int(p.table[b, last])] *= 2.0 ** 6
+        blind += [p.cu[b] + i for i in range(n) if kv - n + i < last * 16]
+    got = p.run()
+    assert len(blind) >= 3 and torch.equal(got[blind], want[blind]) and not torch.equal(got, want)
