@@ -244,8 +244,9 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
                     x = __builtin_fminf(x, __shfl_xor(x, d));
                 low = lane_of(x, 0);
             }
-            // (The least: no 1 / w is infinite.)
-            const float least_w = __builtin_fmaxf(low * 0x1p-100f, 0x1p-125f), w = scale < least_w ? least_w : scale;
+            // (Under 2^-40 of a row's top every product is zero in fp16. Lifted to that, no probability sinks under fp32's normal numbers
+            // on the way to the sum, and no 1 / w is infinite.)
+            const float least_w = __builtin_fmaxf(low * 0x1p-40f, 0x1p-125f), w = scale < least_w ? least_w : scale;
             const float w_logs = __builtin_amdgcn_logf(w), w_invs = __builtin_amdgcn_rcpf(w);
             const float cs = scale * __builtin_fabsf(p.scale), c_least = cs < kTinyAmax ? kTinyAmax : cs; // (no -inf times zero; NaN stays)
             float c[4], w_log[4], w_inv[4];

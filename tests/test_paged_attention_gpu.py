@@ -1,4 +1,6 @@
 """DevicePagedAttention8 against attention in 64 bits (bound: serving_plain.attention_bound)."""
+import math
+
 import pytest
 import torch
 
@@ -267,3 +269,25 @@ def test_blocks_that_a_row_does_not_see_change_none_of_its_bits(news, kvs, heads
         blind += [p.cu[b] + i for i in range(n) if kv - n + i < last * 16]
     got = p.run()
     assert len(blind) >= 3 and torch.equal(got[blind], want[blind]) and not torch.equal(got, want)
+
+
+def test_no_probability_is_lost_beside_a_value_scale_far_below_the_others():
+    """One token whose value is 1, and 80000 behind it whose values are zero (their blocks' scales are what the store makes of zeros),
+    with scores 26.5 powers of two under the first one's: the output is 1 / (1 + sum of their probabilities). Off by half a step of
+    fp16 under 1 (2^-12), by 2^-24 for each of the 5000 additions of eight probabilities to a sum near 1 (a lane has every other
+    eight), and 2^-18 for the exponents (26.5 and 109 rounded to fp32, twice)."""
+    size, D, heads, kv, below = 16, 64, 4, 80000, 26.5
+    p = Problem([30], [kv], heads, 1, D, size, torch.int8, "f16", causal=False, scale=1.0)
+    kc, vc, ks, vs = p.cache
+    p.q.zero_()
+    p.q[:, :, 0] = 1.0
+    for x in (kc, vc):
+        x.zero_()
+    ks.fill_(below * math.log(2.0) / 127)
+    vs.fill_(2.0 ** -100 / 127)
+    first = int(p.table[0, 0])
+    kc[first, 0, 0, 0], vc[first, 0, 0], vs[first] = 127, 127, 1 / 127
+    got = p.run(max_kv=0).double()   # (one share)
+    want = 1 / (1 + (kv - 1) * 2.0 ** -below)
+    assert bool(((got - want).abs() <= 2.0 ** -12 + 5000 * 2.0 ** -24 + 2.0 ** -18).all()), (float(got.min()), float(got.max()), want)
+
