@@ -219,7 +219,9 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_rows_kernel(AttentionArg
         if(__any(top > m + 6.0f))
         {
             // (the rows that leap, no others: a row's bits are its own)
-            const float now = top > m + 6.0f ? top : m, keep = __builtin_amdgcn_exp2f(m - (now == -__builtin_inff() ? 0.0f : now));
+            float now = top > m + 6.0f ? top : m;
+            asm volatile("" : "+v"(now)); // (in the branch: left to itself the compiler chooses outside of it, every turn)
+            const float keep = __builtin_amdgcn_exp2f(m - (now == -__builtin_inff() ? 0.0f : now));
             m = now;
             l *= keep;
             keep_o *= keep;

@@ -312,7 +312,9 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
             if(__any(most_s > m + 6.0f))
             {
                 // (the rows that leap, no others: a row's bits are its own)
-                const float now = most_s > m + 6.0f ? most_s : m, keep = __builtin_amdgcn_exp2f(m - (now == -__builtin_inff() ? 0.0f : now));
+                float now = most_s > m + 6.0f ? most_s : m;
+                asm volatile("" : "+v"(now)); // (in the branch: left to itself the compiler chooses outside of it, every step)
+                const float keep = __builtin_amdgcn_exp2f(m - (now == -__builtin_inff() ? 0.0f : now));
                 m = now;
                 l *= keep;
                 keep_o *= keep;
