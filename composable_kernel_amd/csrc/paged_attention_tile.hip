@@ -248,7 +248,8 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
             // on the way to the sum, and no 1 / w is infinite.)
             const float least_w = __builtin_fmaxf(low * 0x1p-40f, 0x1p-125f), w = scale < least_w ? least_w : scale;
             const float w_logs = __builtin_amdgcn_logf(w), w_invs = __builtin_amdgcn_rcpf(w);
-            const float cs = scale * __builtin_fabsf(p.scale), c_least = cs < kTinyAmax ? kTinyAmax : cs; // (no -inf times zero; NaN stays)
+            // (fp32's least number in place of zero: no -inf times zero, and no score of a tiny scale changes. NaN stays.)
+            const float cs = scale * __builtin_fabsf(p.scale), c_least = cs < 0x1p-149f ? 0x1p-149f : cs;
             float c[4], w_log[4], w_inv[4];
 #pragma unroll
             for(int b = 0; b < 4; ++b)

@@ -291,3 +291,27 @@ def test_no_probability_is_lost_beside_a_value_scale_far_below_the_others():
     want = 1 / (1 + (kv - 1) * 2.0 ** -below)
     assert bool(((got - want).abs() <= 2.0 ** -12 + 5000 * 2.0 ** -24 + 2.0 ** -18).all()), (float(got.min()), float(got.max()), want)
 
+
+
+@pytest.mark.parametrize("code", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("news,kvs", [([1, 3], [300, 77]), ([60, 40], [90, 1100])])
+def test_tiny_key_scales_under_large_queries(news, kvs, code):
+    """Keys 2^-100 and queries 2^100 times as large, exact in bf16 and fp32: the same scores, and the same bits."""
+    p = Problem(news, kvs, 8, 2, 64, 16, code)
+    want = p.check()
+    p.cache[2] *= 2.0 ** -100
+    p.q *= 2.0 ** 100
+    assert torch.equal(p.run().double(), want)
+
+
+@pytest.mark.parametrize("news,kvs", [([1, 3], [300, 77]), ([60, 40], [90, 1100])])
+def test_key_scales_of_zero(news, kvs):
+    """All scores zero, masked ones apart, whatever the codes: the mean of the values that a row sees."""
+    p = Problem(news, kvs, 8, 2, 64, 16)
+    p.cache[2].zero_()
+    p.q *= 2.0 ** 100
+    p.check()
+    p.cache[2].fill_(0.1)
+    p.q *= 2.0 ** -100
+    p.scale = 0.0
+    p.check()
