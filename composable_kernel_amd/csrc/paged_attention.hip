@@ -213,7 +213,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_rows_kernel(AttentionArg
         top = max_over_rows(top);
         // (the maximum is there for the range only and raised only by leaps, 2^6 or more: the sums are seldom rescaled)
         float keep_o   = 1.0f;
-        const float v0 = t0 < see ? x.vs[0] : 0.0f, v1 = t0 + 16 < see ? x.vs[1] : 0.0f; // (no block: zero)
+        const float v0 = t0 < see ? __builtin_fabsf(x.vs[0]) : 0.0f, v1 = t0 + 16 < see ? __builtin_fabsf(x.vs[1]) : 0.0f; // (no block: zero)
         if(__any(v0 > unit.top || v1 > unit.top))
             keep_o = unit.take(v0, v1);
         if(__any(top > m + 6.0f))

@@ -41,7 +41,7 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b)
     return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
 }
 
-// The value scale that a row's output sums are relative to: the largest finite one of the blocks that the row has seen so far (a block
+// The value scale that a row's output sums are relative to: the largest finite one, by its size, of the blocks that the row has seen so far (a block
 // that it does not see, however large, would cost it bits). take() returns what the sums so far are to be multiplied by, of() a
 // scale relative to it (an infinity or NaN stays one).
 struct ValueScale

@@ -187,6 +187,24 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
             deposit_piece(n, odd);
     };
 
+    // A block with a negative scale: what the wave has put of it into LDS changes sign (exactly: 16-bit floats), the scale counts by its
+    // size. Behind the step's work, where the branch parts nothing that is scheduled together.
+    auto negate = [&](int step, float scales) {
+        const uint32_t mine = (uint32_t)__ballot(scales < 0.0f) >> wave; // bit 0: keys, 4: values
+        if((mine & 0x11u) == 0)
+            return;
+        uint32_t k_old = k_write + (step & 1) * STAGE, v_old = v_write + (step & 1) * STAGE;
+        asm volatile("" : "+v"(k_old), "+v"(v_old)); // (worked out here, not kept)
+        if(mine & 1u)
+#pragma unroll
+            for(int n = 0; n < 2 * KB; ++n)
+                *reinterpret_cast<i32x4*>(lds + (k_old ^ (uint32_t)(n << 4))) ^= (int)0x80008000;
+        if((mine & 16u) && (DP == 128 || vh < 2))
+#pragma unroll
+            for(int i = 0; i < 4; ++i)
+                *reinterpret_cast<i32x4*>(lds + (v_old ^ (uint32_t)(i << 4)) + i * (kStep * 2)) ^= (int)0x80008000;
+    };
+
     const uint32_t k_read = r * (DP * 2) + ((h ^ (r & (KC - 1))) << 4), v_read = K_TILE + r * (kStep * 2) + ((h ^ ((r ^ (r >> 2)) & 7)) << 4);
     f32x16 o[DT];
 #pragma unroll
@@ -195,7 +213,7 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
         for(int i = 0; i < 16; ++i)
             o[j][i] = 0.0f;
     float m = -__builtin_inff(), l = 0.0f;
-    // The value scale that the row's sums are relative to, the largest finite one that it has seen, and its logarithm; `low`: the least of
+    // The value scale that the row's sums are relative to, the largest finite one (by its size) that it has seen, and its logarithm; `low`: the least of
     // them among the wave's rows (steps that all rows see whole leave them one), under which no scale raises any.
     constexpr float kLeast = 1.9259299443872359e-34f; // (2^-112: a score's sum relative to it stays finite)
     float top = kLeast, top_log = -112.0f, low = kLeast;
@@ -211,6 +229,7 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
     fetch(begin, lane_of(blocks, wave), even);
     fetch(begin + 1, lane_of(blocks1, wave), odd);
     deposit(begin, even);
+    negate(begin, scale);
     __syncthreads();
     auto one_step = [&](int step, auto mine, auto other) {
         const uint32_t there = (uint32_t)__ballot(blocks >= 0) & 15u; // (a bit for each 16 tokens)
@@ -225,15 +244,17 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
             uint32_t k_at = k_read + (step & 1) * STAGE, v_at = v_read + (step & 1) * STAGE;
             asm volatile("" : "+v"(k_at), "+v"(v_at));
             // The value scales go into the exponent, exp2(score - m + log2(scale / top)), which saves a multiplication a score; the
-            // sum of the probabilities takes them out again, 16 tokens at a time.
-            float keep_v = 1.0f;
-            if(__any((lane & 4) && scale > low))
+            // sum of the probabilities takes them out again, 16 tokens at a time. All scales enter by
+            // their size (negate).
+            const float size = __builtin_fabsf(scale);
+            float keep_v     = 1.0f;
+            if(__any((lane & 4) && size > low))
             {
                 float next = top;
 #pragma unroll
                 for(int b = 0; b < 4; ++b)
                 {
-                    const float v = lane_of(scale, 4 + b);
+                    const float v = lane_of(size, 4 + b);
                     next          = __builtin_fmaxf(next, __builtin_isfinite(v) && see - t0 > 16 * b ? v : 0.0f);
                 }
                 keep_v = top / next;
@@ -246,10 +267,10 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
             }
             // (Under 2^-40 of a row's top every product is zero in fp16. Lifted to that, no probability sinks under fp32's normal numbers
             // on the way to the sum, and no 1 / w is infinite.)
-            const float least_w = __builtin_fmaxf(low * 0x1p-40f, 0x1p-125f), w = scale < least_w ? least_w : scale;
+            const float least_w = __builtin_fmaxf(low * 0x1p-40f, 0x1p-125f), w = size < least_w ? least_w : size;
             const float w_logs = __builtin_amdgcn_logf(w), w_invs = __builtin_amdgcn_rcpf(w);
             // (fp32's least number in place of zero: no -inf times zero, and no score of a tiny scale changes. NaN stays.)
-            const float cs = scale * __builtin_fabsf(p.scale), c_least = cs < 0x1p-149f ? 0x1p-149f : cs;
+            const float cs = size * __builtin_fabsf(p.scale), c_least = cs < 0x1p-149f ? 0x1p-149f : cs;
             float c[4], w_log[4], w_inv[4];
 #pragma unroll
             for(int b = 0; b < 4; ++b)
@@ -368,6 +389,7 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
             multiply(t0 + kStep <= least && there == 15u);
         else
             deposit(step + 1, other);
+        negate(step + 1, scale1);
         blocks = blocks1, blocks1 = blocks2, blocks2 = blocks3;
         scale = scale1, scale1 = scale2;
         __syncthreads();

@@ -463,7 +463,7 @@ int ckx_gemm_f8_blockscale(const void* p_a, const void* p_b, void* p_c, const fl
 /* ---- key / value cache in 8 bits -----------------------------------------------------------------
  * Blocks of block_size tokens; the code of token t, head h, element d of block b is
  * p_k[b * stride_block + h * stride_head + t * stride_token + d] (p_v alike), the value it stands for that code times
- * p_k_scale[b * stride_scale + h]. Slot number = block * block_size + token. e4m3 or int8 codes; head_dim a multiple of
+ * p_k_scale[b * stride_scale + h], a scale of either sign. Slot number = block * block_size + token. e4m3 or int8 codes; head_dim a multiple of
  * 16 up to 128; block_size 16, 32, 64 or 128; strides multiples of 16, p_k and p_v 16-byte aligned, block_size * stride_token under 2 GiB. Codes are finite
  * (ckx_kv_cache_store8 writes no others: it puts a NaN or infinity into the block's scale). Blocks with numbers outside
  * [0, num_blocks) are neither read nor written. */

@@ -315,3 +315,22 @@ def test_key_scales_of_zero(news, kvs):
     p.q *= 2.0 ** -100
     p.scale = 0.0
     p.check()
+
+
+@pytest.mark.parametrize("code", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("news,kvs,D", [([1, 3], [300, 77], 64), ([1], [5000], 128), ([60, 40], [90, 1100], 64), ([120, 7], [333, 30], 128)])
+@pytest.mark.parametrize("which", ["keys", "values", "both", "all values", "all keys"])
+def test_scales_of_either_sign(which, news, kvs, D, code):
+    p = Problem(news, kvs, 8, 2, D, 16, code)
+    g = sp.gen(12)
+    signs = lambda x: torch.randint(0, 2, x.shape, generator=g) * 2.0 - 1
+    if which in ("keys", "both"):
+        p.cache[2] *= signs(p.cache[2])
+    if which in ("values", "both"):
+        p.cache[3] *= signs(p.cache[3])
+    if which.startswith("all"):
+        p.cache[2 if which == "all keys" else 3].neg_()
+    p.check()
+    if which == "both":
+        p.scale = -p.scale
+        p.check()
