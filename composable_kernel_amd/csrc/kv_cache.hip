@@ -233,7 +233,7 @@ __global__ __launch_bounds__(256) void kv_store_kernel(StoreArgs p, int span)
         if(begin > 0)
         {
             const float old = *at;
-            now             = old != old || old >= fresh ? old : fresh;
+            now             = old != old || __builtin_fabsf(old) >= fresh ? old : fresh; // (a scale of either sign, by its size)
             if(now == old || old != old)
                 by = Quotient(1.0f, old);
             else

@@ -501,7 +501,7 @@ int ckx_kv_cache_tables(const int32_t* p_context_lens, const int32_t* p_new_lens
  * elements (multiples of 8, 16-byte aligned), at most 2^29 tokens, token t into slot p_slots[t]; slots outside the cache (-1) are skipped. A run =
  * consecutive tokens whose slots lie in one block, slots ascending; a block occurs in one run of a call. With o the place
  * of the run's first token in its block, Q = 448 (e4m3) or 127 (int8), per head, for keys and values alike:
- *   new scale = max(max(max |x| over the run, 2^-100) / Q, o > 0 ? old scale : 0)
+ *   new scale = max(max |x| over the run, 2^-100) / Q, or with o > 0 the old scale where its size is at least that
  *   o > 0 and the scale grew: the codes of the tokens before o become round(code * (old / new))
  *   codes of the run: round(x * Q / max(max |x|, 2^-100)) where the run set the scale, round(x / old) where it did not; the
  *   quotient rounded to fp32, then ties to even

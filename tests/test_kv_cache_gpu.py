@@ -230,3 +230,23 @@ def test_tables_block_numbers_without_a_slot():
     got = run_tables([16, 31], [18, 3], [top, 9, top - 2], table, 21, 16)
     want = [-1] * 16 + [9 * 16, 9 * 16 + 1] + [-1, (top - 2) * 16, (top - 2) * 16 + 1]
     assert got[1] == [0, 18, 21] and got[4] == 3 and got[3].tolist() == want
+
+
+@pytest.mark.parametrize("code", [torch.float8_e4m3fn, torch.int8])
+def test_a_started_block_with_a_negative_scale(code):
+    """Blocks that hold (-codes, -scales) instead of (codes, scales) stand for the same values, and go on doing so: where the scale
+    stays, the new codes are the negative ones, where it grows, codes and scale are the same in both."""
+    g = sp.gen(21)
+    cache = sp.random_cache(g, 8, 2, 16, 64, code)
+    turned = [(-x.float()).to(code) for x in cache[:2]] + [-x for x in cache[2:]]
+    slots = [b * 16 + i for b, (o, n) in enumerate(((0, 4), (1, 3), (7, 1), (15, 1), (3, 13), (9, 2), (4, 1), (0, 16))) for i in range(o, o + n)]
+    # blocks 1, 3, 5: tokens small enough for the scale to stay; 2, 4, 6: large ones
+    size = torch.tensor([4.0 if (s // 16) % 2 == 0 else 0.05 for s in slots])[:, None, None]
+    k, v = ((sp.normal(g, (len(slots), 2, 64)) * size).to(torch.bfloat16) for _ in range(2))
+    want, got = run_store(k, v, slots, cache, "bf16"), run_store(k, v, slots, turned, "bf16")
+    value = lambda c, s, i: c[i].float() * s[i][:, None, None]
+    for i in range(2):
+        assert torch.equal(want[2 + i][1::2][:3], cache[2 + i][1::2][:3])
+        for b in range(8):
+            end = max(s for s in slots if s // 16 == b) % 16 + 1    # (what lies behind the run is unwritten)
+            assert torch.equal(value(got[i], got[2 + i], b)[:, :end], value(want[i], want[2 + i], b)[:, :end]), (i, b)
