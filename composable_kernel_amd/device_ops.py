@@ -771,8 +771,10 @@ class KvCache8:
             if tuple(s.shape) != tuple(k.shape[:2]) or s.stride() != k_scale.stride() or (s.shape[1] > 1 and s.stride(1) != 1):
                 raise ValueError("scales: [num_blocks, heads], the heads next to each other, keys and values alike")
         n, heads, size, dim = k.shape
-        self.desc = capi.KvCache8Desc(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), kind, n, size, heads, dim, k.stride(1),
-                                      k.stride(2), k_scale.stride(0), k.stride(0))
+        # (the stride of a single head, or block's scales, is never used)
+        strides = (k.stride(1) if heads > 1 else 0, k.stride(2), k_scale.stride(0) if n > 1 else 0)
+        self.desc = capi.KvCache8Desc(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), kind, *map(_i32, (n, size, heads, dim) + strides),
+                                      k.stride(0))
         self.tensors = (k, v, k_scale, v_scale)
 
 

@@ -260,3 +260,22 @@ def test_largest_sizes():
     assert attend(blocks=most, st=most) == capi.OK and attend(blocks=most + 1, st=most + 1) == capi.UNSUPPORTED
     assert L.ckx_paged_attention8_workspace_bytes(C.byref(c), 1, 1, 4, 1 << 20, most + 1) == 0
     assert attend(scale=3e38) == capi.INVALID_VALUE and attend(scale=2e38) == capi.OK
+
+
+def test_cache_strides_past_32_bits_are_refused():
+    """Heads (or scales) further apart than the descriptor's 32 bits say: cut to them, a kernel would read and write elsewhere."""
+    import torch
+    blank = lambda shape, strides, t: torch.empty_strided(shape, strides, dtype=t, device="meta")
+    scale = blank((2, 2), (2, 1), torch.float32)
+    codes = lambda head, token=64: blank((2, 2, 16, 64), (1 << 45, head, token, 1), torch.int8)
+    for k in (codes((1 << 32) + 1024), codes(1 << 31), codes(1 << 40, (1 << 32) + 64)):
+        with pytest.raises(OverflowError):
+            ck.KvCache8(k, k, scale, scale)
+    wide = blank((2, 2), ((1 << 32) + 2, 1), torch.float32)
+    with pytest.raises(OverflowError):
+        ck.KvCache8(codes(1024), codes(1024), wide, wide)
+    far = ck.KvCache8(codes((1 << 31) - 16), codes((1 << 31) - 16), scale, scale)       # (blocks have 64 bits)
+    assert far.desc.stride_head == (1 << 31) - 16 and far.desc.stride_block == 1 << 45
+    one = blank((2, 1, 16, 64), (1 << 45, 1 << 40, 64, 1), torch.int8)                  # (a single head's stride is never used)
+    assert L.ckx_kv_cache_store8_is_supported(C.byref(ck.KvCache8(one, one, scale[:, :1], scale[:, :1]).desc), 4, 64, 64, 64, 64,
+                                              capi.TYPE_BF16) == capi.OK
