@@ -446,8 +446,12 @@ int ckx_quantize_blocks_f8(const void* p_x, void* p_q, float* p_scale, int32_t M
 /* ---- GEMM, e4m3 operands with a scale for each block of 128 --------------------------------------
  *   C[m, n] = round( sum_g sa[m, g] * sb[n / 128, g] * sum_{k in group g} A[m, k] * B[n, k] )
  * A [M, K] row-major, B stored [N, K] (column-major K x N), C [M, N] row-major fp32, fp16 or bf16 (c_type), rounded once.
- * sa[m, g] = p_scale_a[m * stride_sa_m + g * stride_sa_g], sb[j, g] = p_scale_b[j * stride_sb_n + g * stride_sb_g]. Products
- * and sums are fp32. K == 0 gives zeros. Any stride and address; K <= 2^30, 256 rows of A or of B within 2 GiB, and fewer
+ * sa[m, g] = p_scale_a[m * stride_sa_m + g * stride_sa_g], sb[j, g] = p_scale_b[j * stride_sb_n + g * stride_sb_g].
+ * fp32 outputs: products are exact, sums fp32. 16-bit outputs: so are the sums of groups, scales and eights, but the products of eight
+ * neighbours of K (8i ... 8i + 7) are first cut, towards zero, to a grid of 2^-13 of the power of two under the largest of them.
+ * A product within 2^5 of the largest loses nothing, another less than 2^-13 of the largest: with normal operands 1.5e-5 of C in
+ * the 2-norm. Where large products cancel, the loss is measured by them and not by C: 448 * 448 - 448 * 448 + six times 1 gives
+ * 0. A caller with such operands takes fp32 outputs. K == 0 gives zeros. Any stride and address; K <= 2^30, 256 rows of A or of B within 2 GiB, and fewer
  * than 2^23 output tiles (64 x 128; up to 32 rows 32 x 16). K, lda, ldb multiples of 16 with 16-byte aligned A and B
  * run on the vectorised kernels. Workspace (optional, ckx_gemm_f8_blockscale_workspace_bytes; 0 for most problems): lets few
  * output tiles with a long K run side by side. */

@@ -136,3 +136,54 @@ def test_exact_sums_come_out_exactly():
         assert torch.equal(run(a, b, sa, sb, "f32").double(), want)
         # (products within 2^-4 ... 9 of each other: nothing lies under the 8-bit instruction's grid either)
         assert torch.equal(run(a, b, sa, sb, "bf16"), want.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("M,K", [(5, 256), (20, 256), (100, 512), (70, 264)])
+def test_products_that_cancel(M, K):
+    """Eights of +P, -P and six products of 1, scales 1. fp32 outputs: exactly 6 an eight. 16-bit outputs: the same where 1 lies on the
+    grid (P = 64: 2^-7); for P = 448^2 (16) each 1 is lost, less than 2^-13 P."""
+    ones = lambda n: torch.ones(n, -(-K // 128))
+    for p in (8.0, 448.0):
+        a, b = torch.ones(M, K), torch.ones(40, K)
+        a[:, ::8], a[:, 1::8], b[:, ::8], b[:, 1::8] = p, p, p, -p
+        a, b = a.to(torch.float8_e4m3fn), b.to(torch.float8_e4m3fn)
+        want = 6.0 * (K // 8)
+        assert bool((run(a, b, ones(M), ones(1), "f32") == want).all())
+        for out in ("bf16", "f16"):
+            got = run(a, b, ones(M), ones(1), out).float()
+            rounded = float(torch.tensor(want).to(DT[out]))
+            assert bool((got == rounded).all() if p == 8.0 else ((got >= 0) & (got <= rounded)).all()), (p, out, got.unique())
+
+
+def check_norm(M, N, K, out):
+    """The 2-norm of the error, over outputs of normal operands: half a step of each output, fp32's roundings as in check, and of the
+    cut products the root of their squares' sum (seven of an eight by less than 2^-13 of its largest; a cut goes towards zero, so that its sign is
+    the product's own, and these are independent)."""
+    a, b, sa, sb = operands(M, N, K, M + N + K)
+    got = run(a, b, sa, sb, out).double()
+    want, mag, _ = sp.gemm(a, b, sa, sb)
+    wide = lambda x, s: (x.double() * s)[:, :K // 8 * 8].view(x.shape[0], -1, 8).abs().amax(dim=2) ** 2
+    cut = 7 * 2.0 ** -26 * (wide(a, sa.repeat_interleave(128, dim=1)[:, :K]) @
+                            wide(b, sb.repeat_interleave(128, dim=1)[:, :K].repeat_interleave(128, dim=0)[:N]).t())
+    bound = sp.HALF_STEP[DT[out]] * want.norm() + (128 + sa.shape[1] + 4) * 2.0 ** -23 * mag.norm()
+    if out != "f32":
+        bound += cut.sum().sqrt()
+    assert float((got - want).norm()) <= float(bound), (float((got - want).norm() / want.norm()), float(bound / want.norm()))
+
+
+@pytest.mark.parametrize("out", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("M,N,K", [(9, 700, 1024), (30, 300, 512), (200, 300, 512), (40, 200, 2048), (100, 200, 1000)])
+def test_error_in_the_2_norm(M, N, K, out):
+    check_norm(M, N, K, out)
+
+
+@pytest.mark.parametrize("out", ["f16", "bf16"])
+@pytest.mark.parametrize("M", [6, 30, 150])
+def test_nan_and_infinite_scales_in_16_bit_outputs(M, out):
+    a, b, sa, sb = operands(M, 140, 384, 78)
+    a[3, 130] = float("nan")
+    sa[5, 1] = float("inf")
+    c = run(a, b, sa, sb, out)
+    assert bool(c[3].isnan().all()) and not bool(c[5].isfinite().any())
+    rest = [i for i in range(M) if i not in (3, 5)]
+    assert bool(c[rest].isfinite().all())
