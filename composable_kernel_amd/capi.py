@@ -39,6 +39,7 @@ SYMBOLS = [
     "ckx_batched_gemm_softmax_gemm_f16_is_supported", "ckx_batched_gemm_softmax_gemm_f16",
     "ckx_quantize_blocks_f8_is_supported", "ckx_quantize_blocks_f8",
     "ckx_gemm_f8_blockscale_is_supported", "ckx_gemm_f8_blockscale", "ckx_gemm_f8_blockscale_workspace_bytes",
+    "ckx_gemm_f8_blockscale_plan",
     "ckx_kv_cache_tables_is_supported", "ckx_kv_cache_tables", "ckx_kv_cache_store8_is_supported", "ckx_kv_cache_store8",
     "ckx_paged_attention8_is_supported", "ckx_paged_attention8", "ckx_paged_attention8_workspace_bytes",
     "ckx_gemm_plan", "ckx_conv2d_fwd_plan", "ckx_set_forced_k_runs", "ckx_set_big_tile_waves",
@@ -160,6 +161,7 @@ def lib():
     L.ckx_gemm_f8_blockscale.argtypes = [vp] * 5 + f8 + [vp, i64, vp]
     L.ckx_gemm_f8_blockscale_workspace_bytes.restype = i64
     L.ckx_gemm_f8_blockscale_workspace_bytes.argtypes = [i32] * 3
+    L.ckx_gemm_f8_blockscale_plan.argtypes = [i32] * 6 + [C.c_int, i64] + [C.POINTER(C.c_int)] * 3
     L.ckx_kv_cache_tables_is_supported.argtypes = [i32] * 6
     L.ckx_kv_cache_tables.argtypes = [vp] * 8 + [i32] * 6 + [vp]
     kvp = C.POINTER(KvCache8Desc)
@@ -208,6 +210,15 @@ def gemm_plan(op, M, N, K, sa=None, sb=None, sc=None, a_layout=ROW_MAJOR, b_layo
     check(lib().ckx_gemm_plan(op, M, N, K, sa, sb, sc, a_layout, b_layout, ROW_MAJOR, epilogue, batch, int(workspace_bytes),
                               C.byref(inst), C.byref(runs)))
     return inst.value, runs.value
+
+
+def gemm_f8_plan(M, N, K, lda=None, ldb=None, ldc=None, c_type=TYPE_BF16, workspace_bytes=0):
+    """(tile rows, tile columns, K runs) a launch of this block-scaled GEMM would use (ckx_gemm_f8_blockscale_plan); 0 runs: the kernel
+    for any K and stride."""
+    out = [C.c_int(0) for _ in range(3)]
+    check(lib().ckx_gemm_f8_blockscale_plan(M, N, K, K if lda is None else lda, K if ldb is None else ldb, N if ldc is None else ldc, c_type,
+                                            int(workspace_bytes), *map(C.byref, out)))
+    return tuple(x.value for x in out)
 
 
 def conv2d_fwd_plan(op, desc, epilogue=EPI_PASSTHROUGH, workspace_bytes=0, instance=INSTANCE_AUTO):

@@ -487,9 +487,16 @@ hipError_t launch_direct(GemmF8Args& a, hipStream_t s)
 // Up to 32 rows the direct kernel: one row of 11008 x 4096 9.7 us (the weights' 9.1), 64 x 128 tiles 18.5.
 struct Plan
 {
-    int kind; // 0: direct, up to 16 rows; 1: direct, up to 32; 2, 3, 4: the tiles above
+    int kind; // 0: direct, up to 16 rows; 1: direct, up to 32; 2, 3, 4: the tiles above; kRagged
     int ksplit, per;
 };
+constexpr int kRagged = -1;
+
+// whether the kernels of 16-byte vectors take K and the strides; `addresses`: those of A and B, or-ed
+bool whole_vectors(int M, int N, int K, int lda, int ldb, uintptr_t addresses)
+{
+    return K > 0 && ((addresses | (uintptr_t)K | (uintptr_t)(M > 1 ? lda : 0) | (uintptr_t)(N > 1 ? ldb : 0)) & 15) == 0;
+}
 
 Plan plan(int M, int N, int K, bool exact, int64_t workspace_bytes)
 {
@@ -525,11 +532,9 @@ Plan plan(int M, int N, int K, bool exact, int64_t workspace_bytes)
 template <typename T>
 hipError_t launch(GemmF8Args& a, int64_t workspace_bytes, hipStream_t s)
 {
-    const uintptr_t bits = reinterpret_cast<uintptr_t>(a.a) | reinterpret_cast<uintptr_t>(a.b) | (uintptr_t)a.K |
-                           (uintptr_t)(a.M > 1 ? a.lda : 0) | (uintptr_t)(a.N > 1 ? a.ldb : 0);
     // (the row scales of a tile are addressed through 32-bit offsets)
     const bool near = (int64_t)a.sa_m * 256 + (int64_t)a.sa_g * (a.groups + 4) < (1 << 29);
-    if((bits & 15) != 0 || a.K == 0 || !near)
+    if(!near || !whole_vectors(a.M, a.N, a.K, a.lda, a.ldb, reinterpret_cast<uintptr_t>(a.a) | reinterpret_cast<uintptr_t>(a.b)))
     {
         a.tiles_m = (a.M + 127) / 128, a.tiles_n = (a.N + 127) / 128;
         hipLaunchKernelGGL((gemm_f8_ragged_kernel<T>), dim3((unsigned)a.tiles_m * (unsigned)a.tiles_n), dim3(256), 0, s, a);
@@ -564,6 +569,15 @@ int64_t gemm_f8_workspace(int M, int N, int K)
 {
     const Plan p = plan(M, N, K, false, INT64_MAX);
     return p.ksplit > 1 ? 4ll * M * N * p.ksplit : 0;
+}
+
+void gemm_f8_plan(int M, int N, int K, int lda, int ldb, int c_type, int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs)
+{
+    constexpr int m[] = {128, 16, 32, 64, 128, 256}, n[] = {128, 16, 32, 128, 128, 256};
+    Plan p{kRagged, 0, 0};
+    if(whole_vectors(M, N, K, lda, ldb, 0))
+        p = plan(M, N, K, c_type == CKX_TYPE_F32, workspace_bytes);
+    *tile_m = m[p.kind + 1], *tile_n = n[p.kind + 1], *k_runs = p.ksplit;
 }
 
 hipError_t gemm_f8_launch(GemmF8Args a, int c_type, int64_t workspace_bytes, hipStream_t s)

@@ -31,6 +31,7 @@ struct GemmF8Args
 };
 bool gemm_f8_fits(int M, int N);
 int64_t gemm_f8_workspace(int M, int N, int K);
+void gemm_f8_plan(int M, int N, int K, int lda, int ldb, int c_type, int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs);
 hipError_t gemm_f8_launch(GemmF8Args a, int c_type, int64_t workspace_bytes, hipStream_t s);
 
 struct TablesArgs

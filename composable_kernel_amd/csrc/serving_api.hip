@@ -167,6 +167,22 @@ int ckx_gemm_f8_blockscale(const void* p_a, const void* p_b, void* p_c, const fl
     return e == hipSuccess ? CKX_OK : ckx::api_hip_fail(e, "gemm_f8_blockscale");
 }
 
+int ckx_gemm_f8_blockscale_plan(int32_t M, int32_t N, int32_t K, int32_t lda, int32_t ldb, int32_t ldc, int c_type,
+                                int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs)
+{
+    if(!tile_m || !tile_n || !k_runs)
+        return api_fail(CKX_INVALID_VALUE, "null result pointer");
+    int st = ckx_gemm_f8_blockscale_is_supported(M, N, K, lda, ldb, ldc, 1, M, 1, 1, c_type);
+    if(st != CKX_OK)
+        return st;
+    if(workspace_bytes < 0)
+        return api_fail(CKX_INVALID_VALUE, "negative size");
+    *tile_m = *tile_n = *k_runs = 0;
+    if(M > 0 && N > 0)
+        ckx::gemm_f8_plan(M, N, K, lda, ldb, c_type, workspace_bytes, tile_m, tile_n, k_runs);
+    return CKX_OK;
+}
+
 int ckx_kv_cache_tables_is_supported(int32_t batch, int32_t num_free, int32_t max_blocks, int32_t stride_table,
                                      int32_t num_slots, int32_t block_size)
 {

@@ -463,6 +463,11 @@ int ckx_gemm_f8_blockscale(const void* p_a, const void* p_b, void* p_c, const fl
                            int32_t M, int32_t N, int32_t K, int32_t lda, int32_t ldb, int32_t ldc, int32_t stride_sa_m,
                            int32_t stride_sa_g, int32_t stride_sb_n, int32_t stride_sb_g, int c_type, void* p_workspace,
                            int64_t workspace_bytes, void* stream);
+/* What a launch with 16-byte aligned A and B, dense scales and this much workspace would use (pure host): the output tile of a
+ * workgroup (16 x 16 and 32 x 32: the direct kernel; 64 x 128, 128 x 128, 256 x 256) and the runs that K is cut into; 0 runs: the
+ * kernel for any K and stride, 128 x 128. Nothing to do (M or N 0): all 0. */
+int ckx_gemm_f8_blockscale_plan(int32_t M, int32_t N, int32_t K, int32_t lda, int32_t ldb, int32_t ldc, int c_type,
+                                int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs);
 
 /* ---- key / value cache in 8 bits -----------------------------------------------------------------
  * Blocks of block_size tokens; the code of token t, head h, element d of block b is

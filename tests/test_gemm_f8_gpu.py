@@ -187,3 +187,64 @@ def test_nan_and_infinite_scales_in_16_bit_outputs(M, out):
     assert bool(c[3].isnan().all()) and not bool(c[5].isfinite().any())
     rest = [i for i in range(M) if i not in (3, 5)]
     assert bool(c[rest].isfinite().all())
+
+
+def on(tile, M, N, K, out, runs=1, workspace=1 << 40):
+    """This problem runs on that tile (the plan of 16-byte aligned operands)."""
+    types = {"f32": ck.capi.TYPE_F32, "f16": ck.capi.TYPE_F16, "bf16": ck.capi.TYPE_BF16}
+    got = ck.capi.gemm_f8_plan(M, N, K, c_type=types[out], workspace_bytes=workspace)
+    assert got[:2] == tile and (got[2] == runs or runs is None and got[2] > 1), got
+
+
+@pytest.mark.parametrize("out", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("M,N,K,tile", [
+    (1, 300, 400, (16, 16)), (16, 130, 272, (16, 16)), (17, 200, 1040, (32, 32)), (32, 47, 144, (32, 32)),
+    (33, 300, 400, (64, 128)), (2001, 1003, 1040, (64, 128)),
+    (1025, 2100, 512, (128, 128)), (2049, 1300, 400, (128, 128)), (1153, 1922, 144, (128, 128)),    # one row, two columns in the last tiles
+    (1300, 2049, 128, (128, 128)), (9001, 1100, 16, (128, 128))])                                   # a single group, of 16 columns
+def test_every_kernel(M, N, K, tile, out):
+    on(tile, M, N, K, out)
+    check(M, N, K, out)
+
+
+@pytest.mark.parametrize("out", ["bf16", "f16"])
+@pytest.mark.parametrize("M,N,K", [(3841, 3844, 144), (3900, 3300, 400), (4000, 3960, 272), (3970, 3970, 16)])
+def test_the_largest_tile(M, N, K, out):
+    """256 x 256, with one row, four columns, and no column of the right half (so no scale of its block either) in the last tiles."""
+    on((256, 256), M, N, K, out)
+    check(M, N, K, out)
+
+
+@pytest.mark.parametrize("M,N,K", [(64, 200, 4096), (130, 128, 8192), (70, 390, 2064), (33, 4096, 11008)])
+@pytest.mark.parametrize("out", ["bf16", "f32"])
+def test_runs_of_k(M, N, K, out):
+    on((64, 128), M, N, K, out, runs=None)
+    check(M, N, K, out)
+    on((64, 128), M, N, K, out, workspace=0)
+
+
+@pytest.mark.parametrize("out", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("M,N,tile", [(1025, 2100, (128, 128)), (3841, 3844, (256, 256))])
+def test_large_tiles_exactly(M, N, tile, out):
+    """Small whole numbers, scales powers of two: every sum is exact, whatever the order; twice the same bits; rows with a NaN or an infinite
+    scale keep it to themselves; the scales' other strides."""
+    if out == "f32" and tile == (256, 256):
+        tile = (128, 128)
+    K, g = 400, sp.gen(M + N)
+    on(tile, M, N, K, out)
+    a, b = (torch.randint(-3, 4, (n, K), generator=g).float().to(torch.float8_e4m3fn) for n in (M, N))
+    sa, sb = (torch.exp2(torch.randint(-2, 3, (n, 4), generator=g).float()) for n in (M, -(-N // 128)))
+    want = sp.gemm(a, b, sa, sb)[0].to(DT[out])
+    got = run(a, b, sa, sb, out)
+    assert torch.equal(got, want) and torch.equal(run(a, b, sa, sb, out, sa_m_fast=False, sb_n_fast=True, pads=(16, 32, 3)), want)
+    a[M - 1, 130], sa[700, 1] = float("nan"), float("inf")
+    got = run(a, b, sa, sb, out)
+    assert bool(got[M - 1].isnan().all()) and not bool(got[700].isfinite().any())
+    rest = torch.ones(M, dtype=torch.bool)
+    rest[[M - 1, 700]] = False
+    assert torch.equal(got[rest], want[rest])
+
+
+@pytest.mark.parametrize("M,N,K,out", [(1025, 2100, 512, "f16"), (1025, 2100, 512, "f32"), (3900, 3300, 400, "f16"), (3900, 3300, 400, "bf16")])
+def test_error_of_large_tiles_in_the_2_norm(M, N, K, out):
+    check_norm(M, N, K, out)

@@ -279,3 +279,22 @@ def test_cache_strides_past_32_bits_are_refused():
     one = blank((2, 1, 16, 64), (1 << 45, 1 << 40, 64, 1), torch.int8)                  # (a single head's stride is never used)
     assert L.ckx_kv_cache_store8_is_supported(C.byref(ck.KvCache8(one, one, scale[:, :1], scale[:, :1]).desc), 4, 64, 64, 64, 64,
                                               capi.TYPE_BF16) == capi.OK
+
+
+def test_gemm_plan():
+    plan = capi.gemm_f8_plan
+    assert plan(1, 11008, 4096) == (16, 16, 1) and plan(32, 11008, 4096) == (32, 32, 1)
+    assert plan(4096, 11008, 4096) == (256, 256, 1) and plan(4096, 11008, 4096, c_type=capi.TYPE_F32) == (128, 128, 1)
+    assert plan(64, 4096, 8192)[2] == 1                                              # (runs of K need their workspace)
+    need = L.ckx_gemm_f8_blockscale_workspace_bytes(64, 4096, 8192)
+    tile, runs = plan(64, 4096, 8192, workspace_bytes=need)[:2], plan(64, 4096, 8192, workspace_bytes=need)[2]
+    assert tile == (64, 128) and runs > 1 and need == 4 * 64 * 4096 * runs
+    for odd in (dict(K=4097), dict(lda=4104), dict(ldb=4104)):
+        assert plan(**{**dict(M=64, N=4096, K=4096), **odd}) == (128, 128, 0)
+    assert plan(1, 4096, 4096, lda=0) == (16, 16, 1)                                  # (a single row's stride is never used)
+    assert plan(0, 8, 16) == plan(8, 0, 16) == (0, 0, 0) and plan(8, 8, 0) == (128, 128, 0)
+    for bad in (dict(M=-1), dict(c_type=capi.TYPE_I8), dict(lda=1), dict(workspace_bytes=-1)):
+        with pytest.raises(capi.CkxError):
+            plan(**{**dict(M=8, N=8, K=16), **bad})
+    one = C.c_int(0)
+    assert L.ckx_gemm_f8_blockscale_plan(8, 8, 16, 16, 16, 8, capi.TYPE_BF16, 0, C.byref(one), C.byref(one), None) == capi.INVALID_VALUE
