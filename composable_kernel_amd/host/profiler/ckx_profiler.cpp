@@ -34,7 +34,9 @@
 // 246-249), extended with the fraction of the MI355X roofline that binds the problem.
 // verify = 1 checks that all instances agree with the first supported one (bit-exact for
 // int8, rtol = atol = 1e-2 for fp16); comparison against the CPU reference is the job of the
-// test-suite, which regenerates these inputs from the same seeds. If the environment variable
+// test-suite, which regenerates these inputs from the same seeds. The 8-bit serving operators have one kernel choice each:
+// there verify = 1 compares a sample of their outputs with plain host forms in 64 bits (ckx/serving_check.hpp), and
+// init = 0 leaves inputs zero, any other fills them with decimal values. If the environment variable
 // CKX_PROFILER_DUMP names a file, the best instance's output tensor is written there.
 #include <cstdlib>
 #include <cstring>
@@ -43,6 +45,7 @@
 
 #include "ckx/device_ops.hpp"
 #include "ckx/host_tensor.hpp"
+#include "ckx/serving_check.hpp"
 #include "ckx/serving_ops.hpp"
 
 using namespace ck;
@@ -901,14 +904,33 @@ void run_one(Op& op, const typename Op::Argument& arg, const char* what, bool ti
 }
 
 template <typename T>
-int profile_gemm_f8_t(bool time_kernel, int M, int N, int K, int nrepeat)
+std::vector<T> from_device(const ckx::DeviceMem& m)
+{
+    std::vector<T> v(m.GetBufferSize() / sizeof(T));
+    m.FromDevice(v.data());
+    return v;
+}
+
+// reports what a check found; whether nothing was wrong
+bool verified(const char* what, std::size_t bad, std::size_t checked)
+{
+    if(bad)
+        std::cout << "Error: " << what << " differs from the plain form in " << bad << " of " << checked << " values" << std::endl;
+    else
+        std::cout << "verified " << what << ": " << checked << " values" << std::endl;
+    return bad == 0;
+}
+
+template <typename T>
+int profile_gemm_f8_t(bool verify, int init, bool time_kernel, int M, int N, int K, int nrepeat)
 {
     const int groups = (K + 127) / 128, nb = (N + 127) / 128;
     std::vector<half_t> x((std::size_t)M * K);
-    ckx::fill_uniform_f16(x, -1.f, 1.f, 0xC0FFEE + 10);
+    if(init)
+        ckx::fill_uniform_f16(x, -1.f, 1.f, 0xC0FFEE + 10);
     // weights: every finite code; scales of 2^-9 ... 2^-6
     std::vector<uint8_t> w((std::size_t)N * K);
-    for(std::size_t i = 0; i < w.size(); ++i)
+    for(std::size_t i = 0; init && i < w.size(); ++i)
     {
         w[i] = (uint8_t)(ckx::splitmix64(0xC0FFEE + 11, i) >> 56);
         w[i] = (w[i] & 127) == 127 ? 0 : w[i];
@@ -934,13 +956,29 @@ int profile_gemm_f8_t(bool time_kernel, int M, int N, int K, int nrepeat)
     if(ws.GetBufferSize() > 0)
         gemm.SetWorkSpacePointer(&arg, ws.GetDeviceBuffer());
     run_one(gemm, arg, "the product", time_kernel, nrepeat, 2.0 * M * N * K, (double)M * K + (double)N * K + 2.0 * M * N, true);
+    const auto out = from_device<T>(dc);
     if(const char* path = std::getenv("CKX_PROFILER_DUMP"))
-    {
-        std::vector<T> out((std::size_t)M * N);
-        dc.FromDevice(out.data());
         ckx::dump_to_file(path, out);
+    bool pass = true;
+    if(verify)
+    {
+        const auto q = from_device<uint8_t>(dq);
+        const auto s = from_device<float>(ds);
+        std::size_t checked = 0;
+        std::size_t bad = ckx::quantise_errors([&](std::size_t m, int k) { return (double)x[m * K + k]; }, q.data(), s.data(), M, K, checked);
+        pass            = verified("DeviceBlockQuantizeF8", bad, checked);
+        checked         = 0;
+        bad             = ckx::gemm_f8_errors(
+            [&](std::size_t m, std::size_t n) {
+                if constexpr(std::is_same_v<T, bhalf_t>)
+                    return (double)ckx::bf16_to_float(out[m * N + n]);
+                else
+                    return (double)out[m * N + n];
+            },
+            q.data(), w.data(), s.data(), sw.data(), M, N, K, std::is_same_v<T, bhalf_t> ? 0x1p-8 : 0x1p-11, checked);
+        pass = verified("DeviceGemmBlockScaleF8", bad, checked) && pass;
     }
-    return 0;
+    return pass ? 0 : 1;
 }
 
 int profile_gemm_f8(int argc, char* argv[])
@@ -954,12 +992,12 @@ int profile_gemm_f8(int argc, char* argv[])
     const int M = std::atoi(argv[7]), N = std::atoi(argv[8]), K = std::atoi(argv[9]), nrepeat = argc > 10 ? std::atoi(argv[10]) : 10;
     if(M < 1 || N < 1 || K < 1)
         throw std::runtime_error("M, N and K are at least 1");
-    return std::atoi(argv[2]) == 2 ? profile_gemm_f8_t<bhalf_t>(std::atoi(argv[6]), M, N, K, nrepeat)
-                                   : profile_gemm_f8_t<half_t>(std::atoi(argv[6]), M, N, K, nrepeat);
+    auto* run = std::atoi(argv[2]) == 2 ? &profile_gemm_f8_t<bhalf_t> : &profile_gemm_f8_t<half_t>;
+    return run(std::atoi(argv[3]) != 0, std::atoi(argv[4]), std::atoi(argv[6]) != 0, M, N, K, nrepeat);
 }
 
 template <bool Causal>
-int profile_attention8_t(int type, bool time_kernel, int B, int ctx, int fresh, int heads, int kv_heads, int D, int bs, int nrepeat)
+int profile_attention8_t(int type, bool verify, int init, bool time_kernel, int B, int ctx, int fresh, int heads, int kv_heads, int D, int bs, int nrepeat)
 {
     const int width = (ctx + fresh + bs - 1) / bs, blocks = B * width;
     const std::size_t codes = (std::size_t)blocks * kv_heads * bs * D;
@@ -998,7 +1036,8 @@ int profile_attention8_t(int type, bool time_kernel, int B, int ctx, int fresh, 
     };
     auto filled = [&](int n, uint64_t seed) {
         std::vector<half_t> v((std::size_t)B * n * row);
-        ckx::fill_uniform_f16(v, -1.f, 1.f, seed);
+        if(init)
+            ckx::fill_uniform_f16(v, -1.f, 1.f, seed);
         auto m = std::make_unique<ckx::DeviceMem>(v.size() * 2);
         m->ToDevice(v.data());
         return m;
@@ -1016,13 +1055,32 @@ int profile_attention8_t(int type, bool time_kernel, int B, int ctx, int fresh, 
         attention.SetWorkSpacePointer(&arg, ws.GetDeviceBuffer());
     run_one(attention, arg, "the attention", time_kernel, nrepeat, 4.0 * B * fresh * heads * D * (Causal ? ctx + (fresh + 1) / 2.0 : ctx + fresh),
             2.0 * B * (double)(ctx + fresh) * kv_heads * D + 4.0 * B * fresh * heads * D, false);
+    const auto out = from_device<half_t>(dout);
     if(const char* path = std::getenv("CKX_PROFILER_DUMP"))
-    {
-        std::vector<half_t> out((std::size_t)B * fresh * heads * D);
-        dout.FromDevice(out.data());
         ckx::dump_to_file(path, out);
-    }
-    return 0;
+    if(!verify)
+        return 0;
+    const auto k = from_device<uint8_t>(dk), v = from_device<uint8_t>(dv);
+    const auto ks = from_device<float>(dks), vs = from_device<float>(dvs);
+    const auto table = from_device<index_t>(dtable);
+    const auto qkv   = from_device<half_t>(*dqkv);
+    const ckx::Cache8View view{k.data(), v.data(), ks.data(), vs.data(), table.data(), blocks, kv_heads, bs, D, B, width, ctx + fresh,
+                               type == CKX_TYPE_I8};
+    if(!verified("DeviceKvCacheTables", view.sound() ? 0 : 1, (std::size_t)blocks))
+        return 1;
+    const int group = heads / kv_heads;
+    auto at         = [&](int b, int i, int column) { return (double)qkv[((std::size_t)b * fresh + i) * row + column]; };
+    std::size_t checked = 0;
+    std::size_t bad     = ckx::store8_errors(
+        [&](int b, int i, int h, int d, int value) { return at(b, i, (heads + value * kv_heads + h) * D + d); }, view, fresh, checked);
+    bool pass = verified("DeviceKvCacheStore8", bad, checked);
+    checked   = 0;
+    bad       = ckx::attention8_errors(
+        [&](int b, int i, int h, int d) { return at(b, i, h * D + d); },
+        [&](int b, int i, int h, int d) { return (double)out[(((std::size_t)b * fresh + i) * heads + h) * D + d]; }, view, fresh, group,
+        1.0f / std::sqrt((float)D), Causal, checked);
+    pass = verified("DevicePagedAttention8", bad, checked) && pass;
+    return pass ? 0 : 1;
 }
 
 int profile_attention8(int argc, char* argv[])
@@ -1043,7 +1101,7 @@ int profile_attention8(int argc, char* argv[])
     const bool causal = argc > 14 ? std::atoi(argv[14]) != 0 : true;
     const int nrepeat = argc > 15 ? std::atoi(argv[15]) : 10, type = std::atoi(argv[2]) == 2 ? CKX_TYPE_I8 : CKX_TYPE_E4M3;
     auto* run         = causal ? &profile_attention8_t<true> : &profile_attention8_t<false>;
-    return run(type, std::atoi(argv[6]) != 0, p[0], p[1], p[2], p[3], p[4], p[5], p[6], nrepeat);
+    return run(type, std::atoi(argv[3]) != 0, std::atoi(argv[4]), std::atoi(argv[6]) != 0, p[0], p[1], p[2], p[3], p[4], p[5], p[6], nrepeat);
 }
 
 } // namespace

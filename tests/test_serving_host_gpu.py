@@ -67,3 +67,20 @@ def test_paged_attention8(cache, B, ctx, new, heads, kv, D, size, causal, tmp_pa
     got = torch.from_numpy(np.fromfile(dump, np.float16)).view(B * new, heads, D).double()
     bound = sp.attention_bound(o, mag, big, torch.float16, D, ctx + new) + 2.0 ** -25 + sp.small_products(scales[1], code, ctx + new)
     assert bool(((got - o).abs() <= bound).all()), float((got - o).abs().max())
+
+
+@pytest.mark.parametrize("c_type,init,M,N,K", [(1, 1, 3, 300, 1000), (2, 1, 600, 520, 512), (2, 2, 40, 128, 4096), (1, 0, 20, 40, 128)])
+def test_gemm_f8_blockscale_verified(c_type, init, M, N, K, tmp_path):
+    out, dump = _run(["gemm_f8_blockscale", c_type, 1, init, 0, 0, M, N, K], tmp_path)
+    assert f"verified DeviceBlockQuantizeF8: {min(M, 256) * (K + -(-K // 128))} values" in out
+    assert f"verified DeviceGemmBlockScaleF8: {min(M * N, 4096)} values" in out and "Error" not in out and "Perf" not in out
+    assert bool(np.fromfile(dump, np.int16).any()) == (init > 0)
+
+
+@pytest.mark.parametrize("cache,init,time,B,ctx,new,heads,kv,D,size,causal", [
+    (1, 1, 0, 3, 500, 1, 8, 2, 128, 16, 1), (2, 1, 1, 2, 33, 90, 4, 4, 64, 32, 1), (1, 1, 1, 2, 20, 70, 6, 2, 80, 16, 0), (2, 0, 0, 2, 5, 3, 4, 2, 64, 16, 1)])
+def test_paged_attention8_verified(cache, init, time, B, ctx, new, heads, kv, D, size, causal, tmp_path):
+    out, dump = _run(["paged_attention8", cache, 1, init, 0, time, B, ctx, new, heads, kv, D, size, causal, 2], tmp_path)
+    assert "verified DeviceKvCacheTables" in out and f"verified DeviceKvCacheStore8: {2 * min(B * new, 512) * kv * D} values" in out
+    assert f"verified DevicePagedAttention8: {min(B * new * heads, 256) * D} values" in out and "Error" not in out
+    assert bool(np.fromfile(dump, np.int16).any()) == (init > 0)
