@@ -58,10 +58,10 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_rows_kernel(AttentionArg
     const bool row_live = rt < p.tile_tokens && tile.first + rt < tile.q_len && rh < p.group;
     const int head      = kvh * p.group + rh;
     const int64_t token = tile.q0 + tile.first + rt;
-    const int behind    = tile.q_len - 1 - (tile.first + rt); // query tokens behind the row's
+    const int behind    = tile.of - 1 - (tile.first + rt); // query tokens behind the row's
     const int see       = row_live ? (p.causal ? tile.kv - behind : tile.kv) : 0;
     const int last      = min(tile.first + p.tile_tokens, tile.q_len) - 1;
-    const int most      = max(p.causal ? tile.kv - (tile.q_len - 1 - last) : tile.kv, 0); // what the tile's furthest row sees
+    const int most      = max(p.causal ? tile.kv - (tile.of - 1 - last) : tile.kv, 0); // what the tile's furthest row sees
 
     // the share: whole steps of 32 tokens; the wave's turns among them
     const int steps = (most + 31) / 32, per = (steps + p.splits - 1) / p.splits;

@@ -75,7 +75,8 @@ __device__ __forceinline__ void transpose4(uint32_t a, uint32_t b, uint32_t c, u
 // tiles begin at cu[b] / tile_tokens + b (cu[b] with one token a tile), which leaves every sequence enough of them.
 struct TileOf
 {
-    int b, q0, q_len, first; // sequence, its first row of q, its query tokens, the tile's first token among them
+    int b, q0, q_len, first; // sequence, its first row of q, its query tokens as far as q reaches, the tile's first token among them
+    int of;                  // all its query tokens: what their places are counted by
     int kv;                  // cached tokens, as far as the table reaches
     bool live;
 };
@@ -83,7 +84,7 @@ __device__ __forceinline__ TileOf tile_of(const AttentionArgs& p, int tile)
 {
     const int lane = threadIdx.x & 63;
     TileOf t;
-    t.b = 0, t.live = false, t.q0 = t.q_len = t.first = t.kv = 0;
+    t.b = 0, t.live = false, t.q0 = t.q_len = t.of = t.first = t.kv = 0;
     for(int b0 = 0; b0 < p.batch; b0 += 64)
     {
         // all three at once: what the sequence's lane has is handed on, not loaded again
@@ -95,7 +96,8 @@ __device__ __forceinline__ TileOf tile_of(const AttentionArgs& p, int tile)
         {
             t.b     = b0 + n - 1;
             t.q0    = __builtin_amdgcn_readlane(c, n - 1);
-            t.q_len = min(max(__builtin_amdgcn_readlane(end, n - 1), t.q0), p.tokens) - t.q0;
+            t.of    = max(__builtin_amdgcn_readlane(end, n - 1), t.q0) - t.q0;
+            t.q_len = min(t.of, p.tokens - t.q0);
             t.first = (tile - __builtin_amdgcn_readlane(start, n - 1)) * p.tile_tokens;
             t.live  = t.first >= 0 && t.first < t.q_len;
             t.kv    = min(max(__builtin_amdgcn_readlane(kv, n - 1), 0), p.max_blocks << p.block_shift);

@@ -68,9 +68,9 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
     const bool row_live = rt < p.tile_tokens && tile.first + rt < tile.q_len && rh < p.group;
     const int head      = kvh * p.group + rh;
     const int64_t token = tile.q0 + tile.first + rt;
-    const int see       = row_live ? (p.causal ? tile.kv - (tile.q_len - 1 - (tile.first + rt)) : tile.kv) : 0;
+    const int see       = row_live ? (p.causal ? tile.kv - (tile.of - 1 - (tile.first + rt)) : tile.kv) : 0;
     const int last      = min(tile.first + p.tile_tokens, tile.q_len) - 1;
-    const int most      = max(p.causal ? tile.kv - (tile.q_len - 1 - last) : tile.kv, 0);
+    const int most      = max(p.causal ? tile.kv - (tile.of - 1 - last) : tile.kv, 0);
     // the share of the cached tokens: an even number of steps
     const int all_steps = (most + kStep - 1) / kStep, per = ((all_steps + p.splits - 1) / p.splits + 1) & ~1;
     const int begin = min(split * per, (all_steps + 1) & ~1), steps = min(begin + per, all_steps);

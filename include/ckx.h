@@ -532,7 +532,7 @@ int ckx_kv_cache_store8(const void* p_k, const void* p_v, const int32_t* p_slots
  * and sums are fp32; probability times value scale is rounded to fp16 (relative to the row's largest value scale) before the
  * second product: an error of 2^-11 of each summand and, under 2^-14 of the largest, of 2^-25 of the row's largest value. max_kv_len (an upper bound that a
  * program knows) steers how the work is cut and no result depends on its being right; num_tokens bounds the rows that are
- * read and written. Token and head strides of q and o: elements, multiples of 8, 16-byte aligned.
+ * read and written (a row under it keeps its place among its sequence's). Token and head strides of q and o: elements, multiples of 8, 16-byte aligned.
  * At most 2^31 - 65536 cached tokens a sequence (max_blocks * block_size); what p_kv_lens says beyond the table is not there.
  * Workspace (ckx_paged_attention8_workspace_bytes): required where that is not 0; launches that share one must not overlap. */
 int ckx_paged_attention8_is_supported(const ckx_kv_cache8* cache, int32_t batch, int32_t num_tokens, int32_t num_q_heads,

@@ -334,3 +334,40 @@ def test_scales_of_either_sign(which, news, kvs, D, code):
     if which == "both":
         p.scale = -p.scale
         p.check()
+
+
+@pytest.mark.parametrize("news,kvs,heads,H,D,rows", [([2, 5], [40, 300], 8, 2, 64, 4), ([1, 4, 3], [9, 20, 33], 4, 1, 128, 3),
+                                                     ([60, 70], [90, 400], 8, 2, 64, 83), ([150], [1500], 4, 1, 128, 101), ([40, 40], [40, 64], 8, 8, 64, 80)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_fewer_rows_than_the_sequences_have(news, kvs, heads, H, D, rows, causal):
+    """num_tokens ends inside a sequence: its rows up to there keep their places in it, the others are neither read nor written."""
+    p = Problem(news, kvs, heads, H, D, 16, causal=causal)
+    cache, (kc, vc, ks, vs) = [x.cuda() for x in p.cache], p.cache
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    table, cu, kv = p.table.cuda(), i32(p.cu), i32(kvs)
+    q, o = p.q.cuda(), torch.full((p.T, heads, D), 5.0, dtype=torch.bfloat16, device="cuda")
+    q[rows:] = float("nan")
+    op = ck.DevicePagedAttention8("bf16", Causal=causal)
+    arg = op.MakeArgumentPointer(q, o, table, cu, kv, ck.KvCache8(*cache), len(news), rows, heads, max(kvs), table.shape[1], table.shape[1],
+                                 q.stride()[:2], o.stride()[:2], ck.Scale(p.scale))
+    need = op.GetWorkSpaceSize(arg)
+    if need:
+        op.SetWorkSpacePointer(arg, torch.full((need,), 0x7F, device="cuda", dtype=torch.uint8))
+    op.MakeInvokerPointer().Run(arg, ck.StreamConfig(torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert bool((o[rows:] == 5).all())
+    want, mag, big = sp.attention(p.q, p.table, p.cu, kvs, kc, vc, ks, vs, p.scale, causal)
+    bound = sp.attention_bound(want, mag, big, torch.bfloat16, D, max(kvs))
+    assert bool(((o.cpu().double() - want).abs() <= bound)[:rows].all())
+
+
+@pytest.mark.parametrize("heads,H,D,size", [(8, 2, 64, 16), (4, 4, 128, 32)])
+@pytest.mark.parametrize("most", [1, 3, 90])
+def test_many_sequences(most, heads, H, D, size):
+    """Past 64, 128 and 192 sequences, some without queries, some without cached tokens, rows in front of the first sequence."""
+    g = sp.gen(most + heads)
+    B = 200 if most < 90 else 130
+    news = torch.randint(0, most + 1, (B,), generator=g).tolist()
+    kvs = [n + int(torch.randint(0, 60, (1,), generator=g)) if b % 7 else 0 for b, n in enumerate(news)]
+    p = Problem(news, kvs, heads, H, D, size, spare=5)
+    p.check()
