@@ -1,11 +1,13 @@
 // Activations to e4m3 in groups of 128 columns (formula: include/ckx.h, ckx_quantize_blocks_f8).
 //
-// One pass over x: 16 lanes hold the 128 values of a group, eight each, so that the group's maximum crosses four lane
-// exchanges and the codes leave from the registers they were read into. Memory bounds it: 2 (or 4) bytes read and 1 written
-// per value, and 1/32 byte of scales. bf16 8192 x 11008: 55.6 us, 4.9 TB/s, what a large copy reaches (53.2 with one
-// multiplication in place of the exact quotient); fp32 11886 x 3388 43.5 us, element by element at K's end only (107 where every
-// row went that way); 1 x 4096: the launch. Rows at any address take the same wide accesses. A workgroup takes 16 rows x 512 columns, 16 lanes a row: the scales of a group's 16 rows are
-// written as one 64-byte piece where the scales' rows are next to each other.
+// One pass over x: 16 lanes hold the 128 values of a group, eight each, so that the group's maximum crosses four lane exchanges
+// and the codes leave from the registers they were read into. A workgroup takes 16 rows x 512 columns, 16 lanes a row: the scales
+// of a group's 16 rows are written as one 64-byte piece where the scales' rows are next to each other. Rows at any address take
+// the same wide accesses; only K's end goes element by element.
+// Memory bounds it: 2 (or 4) bytes read and 1 written per value, and 1/32 byte of scales. bf16 8192 x 11008: 55.6 us, 4.9 TB/s of
+// both together; reads alone (6.35 TB/s on this card) and writes alone (5.2) would take 46. The exact quotient costs 2.4 of it
+// (53.2 with one multiplication in its place). fp32 11886 x 3388 43.5 us (107 where every row went element by element). 1 x 4096:
+// the launch.
 #include "f8.hpp"
 #include "serving.hpp"
 

@@ -1,14 +1,15 @@
 // GEMM with e4m3 operands and a scale for each block of 128 (formula: include/ckx.h, ckx_gemm_f8_blockscale).
 //
-// 16-bit outputs: one matrix instruction covers a group: v_mfma_f32_16x16x128_f8f6f4 multiplies 16 rows by 16 columns over 128 bytes of K, so
-// its result, started from zero, is the group's sum, and acc += (sa * sb) * result is one multiply-add per value and group. The
-// instruction is issued as D^T = B_frag x A_frag: a lane then holds one row m and four consecutive columns of a 16 x 16 tile, so
-// that the row's scale is one register, and the rows of B are permuted in LDS (b_row_to_col) so that four tiles leave the lane
-// with 16 consecutive columns. That instruction adds the products of eight neighbours of K on a grid 2^-13 of the power of two under
-// the largest among them (measured: what lies under it is cut towards zero; 1.5e-5 of C in the 2-norm for normal codes, where the
-// output's own rounding is 2^-11 or 2^-8 of each value). It goes by the products, not by their sum: where large ones cancel it is more than the
-// rounding, and the callers are told so. fp32 outputs take the codes converted to fp16 (exact) through v_mfma_f32_16x16x32_f16, whose
-// sums are fp32, at half the rate.
+// 16-bit outputs: one matrix instruction covers a group: v_mfma_f32_16x16x128_f8f6f4 multiplies 16 rows by 16 columns over 128
+// bytes of K, so its result, started from zero, is the group's sum, and acc += (sa * sb) * result is one multiply-add per value
+// and group. The instruction is issued as D^T = B_frag x A_frag: a lane then holds one row m and four consecutive columns of a 16
+// x 16 tile, so that the row's scale is one register, and the rows of B are permuted in LDS (b_row_to_col) so that four tiles
+// leave the lane with 16 consecutive columns.
+// That instruction adds the products of eight neighbours of K on a grid 2^-13 of the power of two under the largest among them
+// (measured: what lies under it is cut towards zero; 1.5e-5 of C in the 2-norm for normal codes, where the output's own rounding
+// is 2^-11 or 2^-8 of each value). It goes by the products, not by their sum: where large ones cancel it is more than the
+// rounding, and the callers are told so. fp32 outputs take the codes converted to fp16 (exact) through v_mfma_f32_16x16x32_f16,
+// whose sums are fp32: 4096 x 11008 x 4096 432 us, where 16-bit outputs take 178.
 #include "f8.hpp"
 #include "serving.hpp"
 
@@ -73,7 +74,9 @@ __device__ __forceinline__ void store_cols16(T* row, int n0, int N, const f32x4 
     }
 }
 
-// Any K, leading dimension and address: 128 x 128 tiles, four waves of 64 x 64, the operands through registers into LDS.
+// Any K, leading dimension and address: 128 x 128 tiles, four waves of 64 x 64, the operands through registers into LDS. What bounds it
+// are the loads, one group ahead and byte by byte behind the last whole 16 of K: 4096 x 11008 x 4100 807 us (the kernels below, K 4096: 178),
+// and with few rows its few workgroups: 1 x 11008 x 4100 87 us, 9 times the direct kernel's time for K 4096.
 template <typename T>
 __global__ __launch_bounds__(256) void gemm_f8_ragged_kernel(GemmF8Args p)
 {
@@ -170,12 +173,12 @@ __global__ __launch_bounds__(256) void gemm_f8_ragged_kernel(GemmF8Args p)
     }
 }
 
-// BM x BN tiles, WM x WN waves, NST stages of operands in LDS: the loads of a group are asked for NST - 1 groups ahead.
-// 256 x 256 and 128 x 128 in two stages (133 KB; 67 KB, two workgroups a CU) where there are tiles enough, 64 x 128 in four otherwise:
-// the time from a load to its data, about 1.1 us, is then spread over three groups instead of one. What bounds the large tiles is the
-// multiply-adds that wait for each matrix result, beside the matrix instructions, and the clock: 4096 x 11008 x 4096 176 to 181 us,
-// 2.1 PFLOP/s, 8192 x 8192 x 8192 2.4 (plan() has the steps of each tile).
-//
+// BM x BN tiles, WM x WN waves, NST stages of operands in LDS: the loads of a group are asked for NST - 1 groups ahead. 256 x 256
+// and 128 x 128 in two stages (133 KB; 67 KB, two workgroups a CU) where there are tiles enough, 64 x 128 in four otherwise: the
+// time from a load to its data, about 1.1 us, is then spread over three groups instead of one. What bounds the large tiles is the
+// multiply-adds that wait for each matrix result, beside the matrix instructions, and the clock: 4096 x 11008 x 4096 176 to 181
+// us, 2.1 PFLOP/s (matrix cores busy 46 % of the launch, vector instructions active 35 %, no LDS conflicts), 8192 x 8192 x 8192
+// 2.4 (plan() has the steps of each tile).
 // The direct loads are inline assembly: the compiler, told of them, would wait for all of them before every LDS read of another
 // stage. Its own LDS reads it waits for itself; the wait for the direct loads stands in front of the barrier.
 template <typename T, int BM, int BN, int WM, int WN, int NST>
@@ -200,8 +203,8 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_f8_tile_kernel(GemmF8Args p)
         make_rsrc(p.sa + (int64_t)m0 * p.sa_m, ((uint32_t)(rows - 1) * p.sa_m + (uint32_t)(p.groups - 1) * p.sa_g + 1) * 4);
     const uint32_t base = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
 
-    // a load fills eight rows, chunk c of row r at c ^ (r & 7). B's rows lie in b_row_to_col's order: within a wave's rows, eight rows
-    // on are 32 columns on, sixteen are 4
+    // a load fills eight rows, chunk c of row r at c ^ (r & 7). B's rows lie in b_row_to_col's order: within a wave's rows, eight
+    // rows on are 32 columns on, sixteen are 4
     const int kc      = ((lane & 7) ^ (lane >> 3)) * 16;
     const int row0_a = wave * NLA * 8 + (lane >> 3), row0_b = wave * NLB * 8 + (lane >> 3);
     const uint32_t oa = (uint32_t)row0_a * p.lda + kc, ob = b_row_to_col((uint32_t)row0_b) * p.ldb + kc;
@@ -483,8 +486,11 @@ hipError_t launch_direct(GemmF8Args& a, hipStream_t s)
 //   64 x 128, four stages    0.49, one workgroup a CU        512 x 4096: 19.4 us (128 x 128: 21.8, 256 x 256: 49.6)
 //   128 x 128, two stages    0.58, two a CU 1.0              1024 x 4096: 23.7 (35.9, 50.1), 2048 x 4096: 35.5 (69.4, 52.4)
 //   256 x 256, two stages    1.42, all CUs busy 1.75         4096 x 4096: 61.0 (140, 68.0), 8192 x 8192 x 8192: 460 (1068, 566)
-// and about 4 us around the steps. A run costs 3 us more and its sums' way to the workspace and back.
-// Up to 32 rows the direct kernel: one row of 11008 x 4096 9.7 us (the weights' 9.1), 64 x 128 tiles 18.5.
+// and about 4 us around the steps. A run costs 3 us more and its sums' way to the workspace and back. Between the direct kernel and the
+// large tiles that leaves 1.6 to 3.2 times what the bytes or operations take: the loads of 64 x 128 tiles and of few 128 x 128 ones are
+// longer than a step, and runs of K pay a second launch (64 x 11008 x 4096 16.3 us, 128 x 4096 x 11008 20.8, 1024 x 4096 x 4096 25.5).
+// Up to 32 rows the direct kernel: one row of 11008 x 4096 9.7 us (reading the weights alone 8.7), 64 x 128 tiles 18.5; 16 rows 13.3, and
+// past 16 the tiles draw level: 17 rows 14.9, 32 rows 17.7, 33 rows (tiles, two runs of K) 14.6.
 struct Plan
 {
     int kind; // 0: direct, up to 16 rows; 1: direct, up to 32; 2, 3, 4: the tiles above; kRagged

@@ -132,7 +132,7 @@ __global__ __launch_bounds__(kTablesThreads) void kv_tables_kernel(TablesArgs p)
 // the older codes if the scale grew, and a pass that writes the codes. Which runs begin among a wave's
 // `span` tokens comes out of one comparison of neighbouring slots, so that no list of runs is needed. The first 16 (32) tokens of
 // a run stay in registers between the passes. Memory bounds it (2 bytes read, 1 written per element): 4 x 4096 tokens of 8 heads of
-// 128 in 19.6 us, 4.1 TB/s; 64 tokens, latency: 5.3 with the launch.
+// 128 in 19.4 us, 4.1 TB/s (13.4 at the rates that reads and writes alone reach); 64 tokens, latency: 5.3 with the launch.
 constexpr int kKept = 4; // vectors a lane keeps
 
 template <typename T, int CODE>

@@ -2,16 +2,21 @@
 // into registers.
 //
 // One workgroup takes 16 query rows (the heads of one group, times as many tokens as fit) and a share of the cached tokens; its
-// waves take 32 tokens each in turn with running maxima and sums of their own and are joined through LDS at the end.
-// Shares of one row are joined by a second launch.
+// waves take 32 tokens each in turn with running maxima and sums of their own and are joined through LDS at the end. Shares of
+// one row are joined by a second launch.
 //   scores   S^T = K Q^T, v_mfma_f32_16x16x32: lane (row l % 16 of q, g = l / 16) gets tokens 4g .. 4g + 3 of each 16
 //   output   O^T = V^T P^T, the same instruction over 32 tokens: the lane's own probabilities are its operand, so V's lanes take tokens
 //            {4g .. 4g + 3, 16 + 4g .. + 3} as well, eight (four) neighbouring elements of d each, transposed by byte permutes
 //            in registers. MFMA j's row c stands for element c * E + j (E elements a lane): the lane ends with a contiguous
 //            stretch of the output row.
-// What bounds it is the cache's bytes: 64 sequences of 8192, 32 / 8 heads of 128, 158 us, 5.1 TB/s; one of 1000 11.3 us, of which the
-// first loads, one behind the other (lengths, table, codes), are about four and the joining launch 3.5. The next 32 tokens' codes (8 KB a wave for heads of 128) are on their way while the present
-// ones are multiplied; block numbers and scales of 32 such turns are fetched at once, a lane each.
+// What bounds it is the cache's bytes: 64 sequences of 8192, 32 / 8 heads of 128, e4m3 157.7 us, 5.1 TB/s (reads alone reach 6.35
+// on this card, 127 us; the waves wait 41 % of their time, vector instructions are active 31 % of the launch, the matrix cores 6
+// %); int8, whose codes take three times the instructions to convert, 180 us. One sequence of 1000 11.2 us, of which the first
+// loads, one behind the other (lengths, table, codes), are about four and the joining launch 3.4. The next 32 tokens' codes (8 KB
+// a wave for heads of 128) are on their way while the present ones are multiplied; block numbers and scales of 32 such turns are
+// fetched at once, a lane each.
+// The number of shares is one for the call. Sequences of very different lengths, enough of them to fill the CUs, leave the
+// longest to one workgroup a head: one of 131072 among 31 of 1000 844 us, where its bytes take 52.
 #include "paged_attention.hpp"
 
 namespace ckx {

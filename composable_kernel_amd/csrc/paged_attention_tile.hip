@@ -1,20 +1,23 @@
 // Attention over the 8-bit cache for prompts: many query rows per sequence, so that the cache is converted once for 128 of them.
 //
 // One workgroup takes 128 query rows (the heads of one group times consecutive tokens), 32 a wave, and walks the cached tokens in
-// steps of 64 with running maxima and sums. The codes of the next step are on their way into registers while one is multiplied; they are
-// converted (keys to the type of q, values to fp16) on their way into LDS, values transposed by byte permutes, two stages, one
-// barrier a step.
+// steps of 64 with running maxima and sums. The codes of the next step are on their way into registers while one is multiplied;
+// they are converted (keys to the type of q, values to fp16) on their way into LDS, values transposed by byte permutes, two
+// stages, one barrier a step.
 //   scores   S^T = K Q^T, v_mfma_f32_32x32x16: lane (row l % 32 of q, h = l / 32) gets tokens 8x + 4h + y (x, y < 4) of each 32
 //   output   O^T = V^T P^T: 16 tokens an instruction, the lane's own probabilities as its operand: slots of half h are tokens
 //            {4h .. 4h + 3, 8 + 4h .. + 3} of each 16, which the values' rows in LDS are ordered by. The rows themselves (elements of
 //            d) are ordered so that a lane ends with 16 neighbouring elements of each 32.
 // LDS rows of 16-byte chunks, chunk c of row r at c ^ (r & 15) (keys of 128), c ^ (r & 7) (keys of 64), c ^ ((r ^ r / 4) & 7)
 // (values): eight neighbouring rows never meet on a bank, neither for the writes nor for the reads.
-// What bounds it are vector instructions: 7 a score (the exponential counts four), about as many cycles as the matrix
-// instructions take, and the two share the SIMD's issue: 4 sequences of 4096 and 1024 new tokens, 32 / 8 heads of 128, int8, 306 us,
-// 0.65 PFLOP/s (counters some steps earlier: matrix instructions busy 33 %, vector instructions 56 %; LDS is read at about 60 % of its
-// rate). Fragments further ahead, and the output's matrix instructions between the exponentials, are level; a copy of the loop without masks gives heads of 64 a tenth and
-// spills at 128.
+// What bounds it are vector instructions: 13 for each of a lane's scores for int8, 11 for e4m3 (heads of 128, counted).
+// Multiply-add, exponential (which takes the time of four), sum, half a conversion and half a maximum are the softmax's. A lane
+// converts 64 codes a step for its 32 scores, 1.5 instructions each for int8 and 0.5 for e4m3, and transposes its values by 16
+// byte permutes. The rest is addresses, scales and masks. The matrix instructions wait for them and hardly run beside them: 4
+// sequences of 4096 and 1024 new tokens, 32 / 8 heads of 128, int8 303 us, 0.66 PFLOP/s, vector instructions active 51 % of the
+// launch, matrix cores busy 27 %; e4m3 284 us, 46 and 28 %. LDS is active 24 % of it, a seventh of that conflicts. Fragments
+// further ahead, and the output's matrix instructions between the exponentials, are level; a copy of the loop without masks gives
+// heads of 64 a tenth and spills at 128.
 #include "paged_attention.hpp"
 
 namespace ckx {
@@ -148,8 +151,9 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
     const int krow = wave * 16 + kt, vrow = (vd & ~31) + (((vd >> 2) & 3) << 3) + (((vd >> 4) & 1) << 2);
     const uint32_t k_write = krow * (DP * 2) + (((kq * (KC / 4)) ^ (krow & (KC - 1))) << 4);
     const uint32_t v_write = K_TILE + vrow * (kStep * 2) + (((2 * wave + vh) ^ ((vrow ^ (vrow >> 2)) & 7)) << 4);
-    // In pieces (2 KB chunks of keys, 4 of values), so that a wave converts the next step's between the matrix instructions of its scores:
-    // heads of 64, 8 x (1024 + 256) 50.9 -> 44.3 us, heads of 128, 4 x (4096 + 1024) 292 -> 285. The stage was last read a step ago.
+    // In pieces (2 KB chunks of keys, 4 of values), so that a wave converts the next step's between the matrix instructions of its
+    // scores: heads of 64, 8 x (1024 + 256) 50.9 -> 44.3 us, heads of 128, 4 x (4096 + 1024) e4m3 292 -> 285. The stage was last read a
+    // step ago.
     uint32_t k_to, v_to, v_lo[4], v_hi[4];
     auto deposit_begin = [&](int step, auto odd) {
         constexpr int S = decltype(odd)::value;
@@ -213,8 +217,8 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
         for(int i = 0; i < 16; ++i)
             o[j][i] = 0.0f;
     float m = -__builtin_inff(), l = 0.0f;
-    // The value scale that the row's sums are relative to, the largest finite one (by its size) that it has seen, and its logarithm; `low`: the least of
-    // them among the wave's rows (steps that all rows see whole leave them one), under which no scale raises any.
+    // The value scale that the row's sums are relative to, the largest finite one (by its size) that it has seen, and its logarithm;
+    // `low`: the least of them among the wave's rows (steps that all rows see whole leave them one), under which no scale raises any.
     constexpr float kLeast = 1.9259299443872359e-34f; // (2^-112: a score's sum relative to it stays finite)
     float top = kLeast, top_log = -112.0f, low = kLeast;
 
@@ -244,8 +248,7 @@ __global__ __launch_bounds__(256, 2) void attention_tile_kernel(AttentionArgs p)
             uint32_t k_at = k_read + (step & 1) * STAGE, v_at = v_read + (step & 1) * STAGE;
             asm volatile("" : "+v"(k_at), "+v"(v_at));
             // The value scales go into the exponent, exp2(score - m + log2(scale / top)), which saves a multiplication a score; the
-            // sum of the probabilities takes them out again, 16 tokens at a time. All scales enter by
-            // their size (negate).
+            // sum of the probabilities takes them out again, 16 tokens at a time. All scales enter by their size (negate).
             const float size = __builtin_fabsf(scale);
             float keep_v     = 1.0f;
             if(__any((lane & 4) && size > low))

@@ -434,10 +434,10 @@ enum
 /* ---- e4m3 codes of activations, one scale per row and group of 128 columns -----------------------
  *   s[m, g] = max(max_{k in g} |x[m, k]|, 2^-100) / 448        (fp32; NaN does not count)
  *   q[m, k] = e4m3(x[m, k] * 448 / max(max |x|, 2^-100))       (the quotient rounded to fp32, then to nearest even)
- * x [M, K] fp32, fp16 or bf16 (x_type), q [M, K] e4m3, rows stride_x / stride_q elements apart; the scale of row m, group g
- * is p_scale[m * stride_scale_m + g * stride_scale_g]: (1, M) is the layout that ckx_gemm_f8_blockscale reads fastest. The last
- * group is short where K is no multiple of 128. A NaN stays NaN; an infinity makes its group's scale infinite, and every
- * value of the group NaN when it is read back. Any K, stride and address; 16-byte aligned rows run on wide loads. */
+ * x [M, K] fp32, fp16 or bf16 (x_type), q [M, K] e4m3, rows stride_x / stride_q elements apart; the scale of row m, group
+ * g is p_scale[m * stride_scale_m + g * stride_scale_g]: (1, M) is the layout that ckx_gemm_f8_blockscale reads fastest.
+ * The last group is short where K is no multiple of 128. A NaN stays NaN; an infinity makes its group's scale infinite,
+ * and every value of the group NaN when it is read back. Any K, stride and address, all on wide accesses. */
 int ckx_quantize_blocks_f8_is_supported(int32_t M, int32_t K, int32_t stride_x, int32_t stride_q, int32_t stride_scale_m,
                                         int32_t stride_scale_g, int x_type);
 int ckx_quantize_blocks_f8(const void* p_x, void* p_q, float* p_scale, int32_t M, int32_t K, int32_t stride_x,
@@ -447,14 +447,15 @@ int ckx_quantize_blocks_f8(const void* p_x, void* p_q, float* p_scale, int32_t M
  *   C[m, n] = round( sum_g sa[m, g] * sb[n / 128, g] * sum_{k in group g} A[m, k] * B[n, k] )
  * A [M, K] row-major, B stored [N, K] (column-major K x N), C [M, N] row-major fp32, fp16 or bf16 (c_type), rounded once.
  * sa[m, g] = p_scale_a[m * stride_sa_m + g * stride_sa_g], sb[j, g] = p_scale_b[j * stride_sb_n + g * stride_sb_g].
- * fp32 outputs: products are exact, sums fp32. 16-bit outputs: so are the sums of groups, scales and eights, but the products of eight
- * neighbours of K (8i ... 8i + 7) are first cut, towards zero, to a grid of 2^-13 of the power of two under the largest of them.
- * A product within 2^5 of the largest loses nothing, another less than 2^-13 of the largest: with normal operands 1.5e-5 of C in
- * the 2-norm. Where large products cancel, the loss is measured by them and not by C: 448 * 448 - 448 * 448 + six times 1 gives
- * 0. A caller with such operands takes fp32 outputs. K == 0 gives zeros. Any stride and address; K <= 2^30, 256 rows of A or of B within 2 GiB, and fewer
- * than 2^23 output tiles (64 x 128; up to 32 rows 32 x 16). K, lda, ldb multiples of 16 with 16-byte aligned A and B
- * run on the vectorised kernels. Workspace (optional, ckx_gemm_f8_blockscale_workspace_bytes; 0 for most problems): lets few
- * output tiles with a long K run side by side. */
+ * fp32 outputs: products are exact, sums fp32. 16-bit outputs: so are the sums of groups, scales and eights, but the
+ * products of eight neighbours of K (8i ... 8i + 7) are first cut, towards zero, to a grid of 2^-13 of the power of two
+ * under the largest of them. A product within 2^5 of the largest loses nothing, another less than 2^-13 of the largest:
+ * with normal operands 1.5e-5 of C in the 2-norm. Where large products cancel, the loss is measured by them and not by C:
+ * 448 * 448 - 448 * 448 + six times 1 gives 0. A caller with such operands takes fp32 outputs.
+ * K == 0 gives zeros. Any stride and address; K <= 2^30, 256 rows of A or of B within 2 GiB, and fewer than 2^23 output
+ * tiles (64 x 128; up to 32 rows 32 x 16). K, lda, ldb multiples of 16 with 16-byte aligned A and B run on the vectorised
+ * kernels. Workspace (optional, ckx_gemm_f8_blockscale_workspace_bytes; 0 for most problems): lets few output tiles with
+ * a long K run side by side. */
 int ckx_gemm_f8_blockscale_is_supported(int32_t M, int32_t N, int32_t K, int32_t lda, int32_t ldb, int32_t ldc,
                                         int32_t stride_sa_m, int32_t stride_sa_g, int32_t stride_sb_n, int32_t stride_sb_g,
                                         int c_type);
@@ -470,12 +471,12 @@ int ckx_gemm_f8_blockscale_plan(int32_t M, int32_t N, int32_t K, int32_t lda, in
                                 int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs);
 
 /* ---- key / value cache in 8 bits -----------------------------------------------------------------
- * Blocks of block_size tokens; the code of token t, head h, element d of block b is
- * p_k[b * stride_block + h * stride_head + t * stride_token + d] (p_v alike), the value it stands for that code times
- * p_k_scale[b * stride_scale + h], a scale of either sign. Slot number = block * block_size + token. e4m3 or int8 codes; head_dim a multiple of
- * 16 up to 128; block_size 16, 32, 64 or 128; strides multiples of 16, p_k and p_v 16-byte aligned, block_size * stride_token under 2 GiB. Codes are finite
- * (ckx_kv_cache_store8 writes no others: it puts a NaN or infinity into the block's scale). Blocks with numbers outside
- * [0, num_blocks) are neither read nor written. */
+ * Blocks of block_size tokens; the code of token t, head h, element d of block b is p_k[b * stride_block + h *
+ * stride_head + t * stride_token + d] (p_v alike), the value it stands for that code times p_k_scale[b * stride_scale +
+ * h], a scale of either sign. Slot number = block * block_size + token. e4m3 or int8 codes; head_dim a multiple of 16 up
+ * to 128; block_size 16, 32, 64 or 128; strides multiples of 16, p_k and p_v 16-byte aligned, block_size * stride_token
+ * under 2 GiB. Codes are finite (ckx_kv_cache_store8 writes no others: it puts a NaN or infinity into the block's scale).
+ * Blocks with numbers outside [0, num_blocks) are neither read nor written. */
 typedef struct ckx_kv_cache8
 {
     void* p_k;
@@ -507,9 +508,10 @@ int ckx_kv_cache_tables(const int32_t* p_context_lens, const int32_t* p_new_lens
                         int32_t block_size, void* stream);
 
 /* New keys and values into the cache. x: p_k / p_v [num_tokens, num_heads, head_dim] fp16 or bf16 (x_type), strides in
- * elements (multiples of 8, 16-byte aligned), at most 2^29 tokens, token t into slot p_slots[t]; slots outside the cache (-1) are skipped. A run =
- * consecutive tokens whose slots lie in one block, slots ascending; a block occurs in one run of a call. With o the place
- * of the run's first token in its block, Q = 448 (e4m3) or 127 (int8), per head, for keys and values alike:
+ * elements (multiples of 8, 16-byte aligned), at most 2^29 tokens, token t into slot p_slots[t]; slots outside the cache
+ * (-1) are skipped. A run = consecutive tokens whose slots lie in one block, slots ascending; a block occurs in one run
+ * of a call. With o the place of the run's first token in its block, Q = 448 (e4m3) or 127 (int8), per head, for keys and
+ * values alike:
  *   new scale = max(max |x| over the run, 2^-100) / Q, or with o > 0 the old scale where its size is at least that
  *   o > 0 and the scale grew: the codes of the tokens before o become round(code * (old / new))
  *   codes of the run: round(x * Q / max(max |x|, 2^-100)) where the run set the scale, round(x / old) where it did not; the
@@ -528,13 +530,20 @@ int ckx_kv_cache_store8(const void* p_k, const void* p_v, const int32_t* p_slots
  * h / (num_q_heads / num_heads).
  *   O[t, h] = sum_j softmax_j(scale * q[t, h] . k[j, h']) * v[j, h']
  * over all cached tokens of the sequence, or with `causal` those up to the token's own place (the last query row sees all
- * of them, the one before it one less). A row that sees nothing is 0. Rows of p_o outside p_cu_q's are left alone. Scores, softmax
- * and sums are fp32; probability times value scale is rounded to fp16 (relative to the row's largest value scale) before the
- * second product: an error of 2^-11 of each summand and, under 2^-14 of the largest, of 2^-25 of the row's largest value. max_kv_len (an upper bound that a
+ * of them, the one before it one less). A row that sees nothing is 0. Rows of p_o outside p_cu_q's are left alone.
+ * Scores, softmax and sums are fp32; probability times value scale is rounded to fp16 (relative to the largest value
+ * scale that the row sees) before the second product: an error of 2^-11 of each summand and, under 2^-14 of the largest,
+ * of 2^-25 of the row's largest value. What a row does not see does not affect it. max_kv_len (an upper bound that a
  * program knows) steers how the work is cut and no result depends on its being right; num_tokens bounds the rows that are
- * read and written (a row under it keeps its place among its sequence's). Token and head strides of q and o: elements, multiples of 8, 16-byte aligned.
- * At most 2^31 - 65536 cached tokens a sequence (max_blocks * block_size); what p_kv_lens says beyond the table is not there.
- * Workspace (ckx_paged_attention8_workspace_bytes): required where that is not 0; launches that share one must not overlap. */
+ * read and written (a row under it keeps its place among its sequence's). Token and head strides of q and o: elements,
+ * multiples of 8, 16-byte aligned.
+ * At most 2^31 - 65536 cached tokens a sequence (max_blocks * block_size); what p_kv_lens says beyond the table is not
+ * there. Workspace (ckx_paged_attention8_workspace_bytes): required where that is not 0; launches that share one must not
+ * overlap.
+ * The kernel (few rows a sequence, or prompts) and the number of shares that the cached tokens are cut into are one for
+ * the call, chosen from num_tokens, batch and max_kv_len, as if all sequences were alike. Single tokens beside a prompt,
+ * and one long sequence among many short ones, are served faster by a call for each kind (31 tokens and a prompt of 512
+ * over 8192 each: 306 us together, 222 apart). */
 int ckx_paged_attention8_is_supported(const ckx_kv_cache8* cache, int32_t batch, int32_t num_tokens, int32_t num_q_heads,
                                       int32_t max_kv_len, int32_t max_blocks, int32_t stride_table, int32_t stride_q_token,
                                       int32_t stride_q_head, int32_t stride_o_token, int32_t stride_o_head, float scale,
