@@ -73,7 +73,8 @@ __device__ __forceinline__ void transpose4(uint32_t a, uint32_t b, uint32_t c, u
 }
 
 // What a tile is about: its sequence, its tokens and how far they see. The sequence is found by all lanes at once: sequence b's
-// tiles begin at cu[b] / tile_tokens + b (cu[b] with one token a tile), which leaves every sequence enough of them.
+// tiles begin at cu[b] / tile_tokens + b (cu[b] with one token a tile), which leaves every sequence enough of them. (64 sequences a
+// round, each waiting for the one before: 1024 of 1000 tokens 493 us, where their bytes take 333.)
 struct TileOf
 {
     int b, q0, q_len, first; // sequence, its first row of q, its query tokens as far as q reaches, the tile's first token among them
