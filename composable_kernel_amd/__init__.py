@@ -14,4 +14,5 @@ from .device_ops import (  # noqa: F401
     DeviceConvNdFwdInt8, DeviceConvNdFwdF16,
     DeviceConv2dFwdBiasActivationF16, DeviceBatchedGemmGemmF16, DeviceBatchedGemmSoftmaxGemmF16,
     KvCache8, DeviceBlockQuantizeF8, DeviceGemmBlockScaleF8, DeviceKvCacheTables, DeviceKvCacheStore8, DevicePagedAttention8,
+    DeviceRouteExperts, DeviceTokenQuantizeI8, DeviceGemmTokenScaleI8, DeviceExpertsGemmI8, DeviceExpertsCombine,
 )

@@ -21,6 +21,7 @@ EPI_BILINEAR, EPI_ADD_ADD_FASTGELU = 8, 9    # fp16 GEMM: alpha * acc + beta * d
  OP_BATCHED_GEMM_SOFTMAX_GEMM) = range(8)
 INSTANCE_AUTO = -1
 TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_E4M3, TYPE_I8 = range(5)   # CKX_TYPE_*: the 8-bit serving operators
+SCORE_SOFTMAX, SCORE_SIGMOID = range(2)   # CKX_SCORE_*
 STATIC_WORKSPACE_BYTES = 32 * 1024 * 1024   # CKX_STATIC_WORKSPACE_BYTES
 
 # every symbol include/ckx.h declares
@@ -42,6 +43,10 @@ SYMBOLS = [
     "ckx_gemm_f8_blockscale_plan",
     "ckx_kv_cache_tables_is_supported", "ckx_kv_cache_tables", "ckx_kv_cache_store8_is_supported", "ckx_kv_cache_store8",
     "ckx_paged_attention8_is_supported", "ckx_paged_attention8", "ckx_paged_attention8_workspace_bytes",
+    "ckx_route_experts_is_supported", "ckx_route_experts", "ckx_route_experts_workspace_bytes",
+    "ckx_quantize_tokens_i8_is_supported", "ckx_quantize_tokens_i8",
+    "ckx_gemm_i8_tokenscale_is_supported", "ckx_gemm_i8_tokenscale", "ckx_gemm_i8_tokenscale_workspace_bytes",
+    "ckx_experts_gemm_i8_is_supported", "ckx_experts_gemm_i8", "ckx_experts_combine_is_supported", "ckx_experts_combine",
     "ckx_gemm_plan", "ckx_conv2d_fwd_plan", "ckx_set_forced_k_runs", "ckx_set_big_tile_waves",
 ]
 
@@ -72,6 +77,18 @@ class KvCache8Desc(C.Structure):
     _fields_ = [("p_k", C.c_void_p), ("p_v", C.c_void_p), ("p_k_scale", C.c_void_p), ("p_v_scale", C.c_void_p)] + [
         (n, C.c_int32) for n in ("type", "num_blocks", "block_size", "num_heads", "head_dim", "stride_head", "stride_token",
                                  "stride_scale")] + [("stride_block", C.c_int64)]
+
+
+class RouteDesc(C.Structure):
+    """ckx_route_desc"""
+    _fields_ = [(n, C.c_int32) for n in ("num_tokens", "num_experts", "top_k", "stride_x", "num_groups", "top_groups", "group_best", "scoring",
+                                         "renormalise", "x_type")] + [("scale", C.c_float)]
+
+
+class ExpertsDesc(C.Structure):
+    """ckx_experts_desc"""
+    _fields_ = [(n, C.c_int32) for n in ("num_rows", "num_rows_a", "num_experts", "N", "K", "stride_a", "stride_b", "stride_c", "rows_per",
+                                         "gated", "c_type", "reserved")] + [("batch_stride_b", C.c_int64)]
 
 
 LAUNCH_FN = C.CFUNCTYPE(C.c_int, C.c_void_p)
@@ -172,6 +189,24 @@ def lib():
     L.ckx_paged_attention8.argtypes = [vp] * 5 + attn + [vp, i64, vp]
     L.ckx_paged_attention8_workspace_bytes.restype = i64
     L.ckx_paged_attention8_workspace_bytes.argtypes = [kvp] + [i32] * 5
+    rp, ep = C.POINTER(RouteDesc), C.POINTER(ExpertsDesc)
+    L.ckx_route_experts_is_supported.argtypes = [rp]
+    L.ckx_route_experts_workspace_bytes.restype = i64
+    L.ckx_route_experts_workspace_bytes.argtypes = [rp]
+    L.ckx_route_experts.argtypes = [vp] * 8 + [rp, vp, i64, vp]
+    tq = [i32] * 4 + [C.c_int]
+    L.ckx_quantize_tokens_i8_is_supported.argtypes = tq
+    L.ckx_quantize_tokens_i8.argtypes = [vp] * 3 + tq + [vp]
+    i8 = [i32] * 6 + [C.c_int] * 2
+    L.ckx_gemm_i8_tokenscale_is_supported.argtypes = i8
+    L.ckx_gemm_i8_tokenscale.argtypes = [vp] * 6 + i8 + [vp, i64, vp]
+    L.ckx_gemm_i8_tokenscale_workspace_bytes.restype = i64
+    L.ckx_gemm_i8_tokenscale_workspace_bytes.argtypes = [i32] * 3 + [C.c_int]
+    L.ckx_experts_gemm_i8_is_supported.argtypes = [ep]
+    L.ckx_experts_gemm_i8.argtypes = [vp] * 8 + [ep, vp]
+    ec = [i32] * 7 + [C.c_int]
+    L.ckx_experts_combine_is_supported.argtypes = ec
+    L.ckx_experts_combine.argtypes = [vp] * 5 + ec + [vp]
     L.ckx_time_launches.argtypes = [LAUNCH_FN, vp, C.c_int, C.c_int, vp, C.POINTER(C.c_float)]
     ip = C.POINTER(C.c_int)
     L.ckx_gemm_plan.argtypes = [C.c_int] + shape + [C.c_int, i32, i64, ip, ip]

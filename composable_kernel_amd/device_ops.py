@@ -841,3 +841,119 @@ class DevicePagedAttention8(_ServingOperator):
 
     def _call(self, a, stream):
         return capi.lib().ckx_paged_attention8(*a.ptrs, *a.dims, a.p_workspace_ or 0, a.workspace_bytes_, C.c_void_p(stream or 0))
+
+
+# ------------------------------------- int8 linear layers and mixtures of experts
+class DeviceRouteExperts(_ServingOperator):
+    """Each token's experts and weights from its logits, and the experts' rows in order (ckx_route_experts). LogitsDataType: "f32", "f16"
+    or "bf16"; Scoring: "softmax" or "sigmoid". p_bias, p_num_tokens and the three tables (p_offsets, p_rows, p_places) may be None."""
+
+    def __init__(self, LogitsDataType="f32", Scoring="softmax", Renormalise=True):
+        super().__init__()
+        self.x, self.x_type = LogitsDataType, _TYPES[LogitsDataType]
+        self.scoring, self.renormalise = {"softmax": capi.SCORE_SOFTMAX, "sigmoid": capi.SCORE_SIGMOID}[Scoring], int(bool(Renormalise))
+
+    def MakeArgumentPointer(self, p_logits, p_bias, p_num_tokens, p_ids, p_weights, p_offsets, p_rows, p_places, NumTokens, NumExperts, TopK,
+                            StrideLogits, NumGroups=1, TopGroups=1, GroupBest=1, weight_element_op=None):
+        if weight_element_op is not None and not isinstance(weight_element_op, (Scale, PassThrough)):
+            raise TypeError("the weights' operation is Scale or PassThrough")
+        scale = weight_element_op.scale if isinstance(weight_element_op, Scale) else 1.0
+        ptrs = (_typed(p_logits, self.x, "logits"), _typed(p_bias, "f32", "bias"), _typed(p_num_tokens, "i32", "number of tokens"),
+                _typed(p_ids, "i32", "ids"), _typed(p_weights, "f32", "weights")) + tuple(
+                    _typed(x, "i32", "tables") for x in (p_offsets, p_rows, p_places))
+        d = capi.RouteDesc(*map(_i32, (NumTokens, NumExperts, TopK, StrideLogits, NumGroups, TopGroups, GroupBest)), self.scoring, self.renormalise,
+                           self.x_type, scale)
+        return _ServingArgument(ptrs, (C.byref(d),))
+
+    def _supported(self, a):
+        return capi.lib().ckx_route_experts_is_supported(*a.dims)
+
+    def GetWorkSpaceSize(self, a):
+        return int(capi.lib().ckx_route_experts_workspace_bytes(*a.dims)) if any(a.ptrs[5:8]) else 0
+
+    def _call(self, a, stream):
+        return capi.lib().ckx_route_experts(*a.ptrs, *a.dims, a.p_workspace_ or 0, a.workspace_bytes_, C.c_void_p(stream or 0))
+
+
+class DeviceTokenQuantizeI8(_ServingOperator):
+    """x [M, K] -> int8 codes [M, K] and one fp32 scale per row (ckx_quantize_tokens_i8). XDataType: "f32", "f16" or "bf16"."""
+
+    def __init__(self, XDataType="bf16"):
+        super().__init__()
+        self.x, self.x_type = XDataType, _TYPES[XDataType]
+
+    def MakeArgumentPointer(self, p_x, p_q, p_scale, M, K, StrideX, StrideQ):
+        return _ServingArgument((_typed(p_x, self.x, "x"), _typed(p_q, "i8", "q"), _typed(p_scale, "f32", "scale")),
+                                (_i32(M), _i32(K), _i32(StrideX), _i32(StrideQ), self.x_type))
+
+    def _supported(self, a):
+        return capi.lib().ckx_quantize_tokens_i8_is_supported(*a.dims)
+
+    def _call(self, a, stream):
+        return capi.lib().ckx_quantize_tokens_i8(*a.ptrs, *a.dims, C.c_void_p(stream or 0))
+
+
+class DeviceGemmTokenScaleI8(_ServingOperator):
+    """C = scale_a[m] * scale_b[n] * (A B^T) + bias[n], int8 operands (ckx_gemm_i8_tokenscale): A [M, K], B [N, K]. Gated: B, scale_b and
+    bias have 2 N rows and C = silu(first half) * second half. p_bias may be None. CDataType: "f32", "f16" or "bf16"."""
+
+    def __init__(self, CDataType="bf16", Gated=False):
+        super().__init__()
+        self.c, self.c_type, self.gated = CDataType, _TYPES[CDataType], int(bool(Gated))
+
+    def MakeArgumentPointer(self, p_a, p_b, p_c, p_scale_a, p_scale_b, p_bias, M, N, K, StrideA, StrideB, StrideC):
+        ptrs = (_typed(p_a, "i8", "A"), _typed(p_b, "i8", "B"), _typed(p_c, self.c, "C"), _typed(p_scale_a, "f32", "scale_a"),
+                _typed(p_scale_b, "f32", "scale_b"), _typed(p_bias, "f32", "bias"))
+        return _ServingArgument(ptrs, tuple(map(_i32, (M, N, K, StrideA, StrideB, StrideC))) + (self.gated, self.c_type))
+
+    def _supported(self, a):
+        return capi.lib().ckx_gemm_i8_tokenscale_is_supported(*a.dims)
+
+    def GetWorkSpaceSize(self, a):
+        return int(capi.lib().ckx_gemm_i8_tokenscale_workspace_bytes(*a.dims[:3], self.gated))
+
+    def _call(self, a, stream):
+        return capi.lib().ckx_gemm_i8_tokenscale(*a.ptrs, *a.dims, a.p_workspace_ or 0, a.workspace_bytes_, C.c_void_p(stream or 0))
+
+
+class DeviceExpertsGemmI8(_ServingOperator):
+    """The product of DeviceGemmTokenScaleI8 for each expert's rows (ckx_experts_gemm_i8): B [experts, N, K] (Gated: 2 N), scale_b and bias
+    [experts, N]; rows p_offsets[e] ... p_offsets[e + 1] - 1 of C are expert e's, row i takes row p_rows[i] / RowsPer of A (p_rows
+    None: row i). p_bias may be None. NumRows: of C; NumRowsA: of A."""
+
+    def __init__(self, CDataType="bf16", Gated=False):
+        super().__init__()
+        self.c, self.c_type, self.gated = CDataType, _TYPES[CDataType], int(bool(Gated))
+
+    def MakeArgumentPointer(self, p_a, p_b, p_c, p_scale_a, p_scale_b, p_bias, p_offsets, p_rows, NumRows, NumRowsA, NumExperts, N, K, StrideA,
+                            StrideB, StrideC, BatchStrideB, RowsPer=1):
+        ptrs = (_typed(p_a, "i8", "A"), _typed(p_b, "i8", "B"), _typed(p_c, self.c, "C"), _typed(p_scale_a, "f32", "scale_a"),
+                _typed(p_scale_b, "f32", "scale_b"), _typed(p_bias, "f32", "bias"), _typed(p_offsets, "i32", "offsets"), _typed(p_rows, "i32", "rows"))
+        d = capi.ExpertsDesc(*map(_i32, (NumRows, NumRowsA, NumExperts, N, K, StrideA, StrideB, StrideC, RowsPer)), self.gated, self.c_type, 0,
+                             int(BatchStrideB))
+        return _ServingArgument(ptrs, (C.byref(d),))
+
+    def _supported(self, a):
+        return capi.lib().ckx_experts_gemm_i8_is_supported(*a.dims)
+
+    def _call(self, a, stream):
+        return capi.lib().ckx_experts_gemm_i8(*a.ptrs, *a.dims, C.c_void_p(stream or 0))
+
+
+class DeviceExpertsCombine(_ServingOperator):
+    """out[t] = add[t] + sum_j weights[t, j] * y[places[t, j]] (ckx_experts_combine); p_add may be None. XDataType: of y, add and out."""
+
+    def __init__(self, XDataType="bf16"):
+        super().__init__()
+        self.x, self.x_type = XDataType, _TYPES[XDataType]
+
+    def MakeArgumentPointer(self, p_y, p_places, p_weights, p_add, p_out, NumTokens, TopK, NumRows, N, StrideY, StrideAdd, StrideOut):
+        ptrs = (_typed(p_y, self.x, "y"), _typed(p_places, "i32", "places"), _typed(p_weights, "f32", "weights"), _typed(p_add, self.x, "add"),
+                _typed(p_out, self.x, "out"))
+        return _ServingArgument(ptrs, tuple(map(_i32, (NumTokens, TopK, NumRows, N, StrideY, StrideAdd, StrideOut))) + (self.x_type,))
+
+    def _supported(self, a):
+        return capi.lib().ckx_experts_combine_is_supported(*a.dims)
+
+    def _call(self, a, stream):
+        return capi.lib().ckx_experts_combine(*a.ptrs, *a.dims, C.c_void_p(stream or 0))

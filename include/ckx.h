@@ -556,6 +556,108 @@ int ckx_paged_attention8(const void* p_q, void* p_o, const int32_t* p_block_tabl
                          int32_t stride_q_token, int32_t stride_q_head, int32_t stride_o_token, int32_t stride_o_head,
                          float scale, int causal, int q_type, void* p_workspace, int64_t workspace_bytes, void* stream);
 
+/* ==== int8 linear layers and mixtures of experts ==================================================
+ * A layer's linear work in 8-bit integers, and what a mixture of experts needs around it: route each token to its experts,
+ * quantise the tokens, multiply each expert's rows, add a token's rows up again. All entry points are asynchronous on
+ * `stream`, allocate nothing, can be captured into a graph, and read the experts' tables and the number of tokens on the
+ * device: a replay sees what they hold then. `stream`'s device has to be the current one. */
+
+/* ---- each token's experts, their weights, and the experts' rows in order ---------------------------
+ * x[t, e]: logits [num_tokens, num_experts] fp32, fp16 or bf16, rows stride_x apart; bias[e] fp32 (p_bias NULL: none).
+ *   available   e is available to t where neither x[t, e] nor bias[e] is NaN or -infinity; +infinity counts as the largest fp32
+ *   score       s[t, e] = softmax over the available experts, or 1 / (1 + exp(-x[t, e]))
+ *   order       by s + bias in 64 bits; without bias by x itself (the same order); ties: the lower number first
+ *   groups      num_groups > 1: experts g * size ... (g + 1) * size - 1 are group g; its value is that of its best available
+ *               expert (group_best 1) or the sum of its two best s + bias (2; one alone counts by itself), in 64 bits. The
+ *               top_groups best groups with an available expert stay; ties: the lower number first
+ *   ids[t, j]   the top_k best available experts of the groups that stay, best first; -1 where there are fewer
+ *   weights     w[t, j] = s[t, ids[t, j]], with `renormalise` divided by their sum over j (0 where that is 0), times scale;
+ *               0 where the id is -1. Computed in 64 bits, rounded once to fp32
+ * The tables (all three or none, NULL) order the pairs t * top_k + j by their experts:
+ *   p_offsets [num_experts + 1]: pairs of the experts before each; the last is the number of all that have an expert
+ *   p_rows    [num_tokens * top_k]: the pairs of expert 0, of expert 1, ..., ascending within each; -1 behind the last
+ *   p_places  [num_tokens * top_k]: where each pair stands in p_rows; -1 for an id of -1
+ * p_num_tokens (NULL: num_tokens): how many tokens there are, on the device, cut to 0 ... num_tokens; the rows behind it
+ * have ids -1, weights 0 and places -1. A rank that holds experts a ... b - 1 hands p_offsets + a and b - a to
+ * ckx_experts_gemm_i8. Up to 1024 experts, top_k up to 32, 64 groups, 2^24 pairs. No output may lie on an input. Workspace
+ * (ckx_route_experts_workspace_bytes): required with tables where that is not 0; launches that share one must not overlap. */
+enum
+{
+    CKX_SCORE_SOFTMAX = 0,
+    CKX_SCORE_SIGMOID = 1
+};
+typedef struct ckx_route_desc
+{
+    int32_t num_tokens, num_experts, top_k;
+    int32_t stride_x;
+    int32_t num_groups, top_groups, group_best; /* 1, 1, 1: no groups */
+    int32_t scoring;                            /* CKX_SCORE_* */
+    int32_t renormalise;                        /* 0 or 1 */
+    int32_t x_type;
+    float scale;
+} ckx_route_desc;
+int ckx_route_experts_is_supported(const ckx_route_desc* desc);
+int64_t ckx_route_experts_workspace_bytes(const ckx_route_desc* desc);
+int ckx_route_experts(const void* p_logits, const float* p_bias, const int32_t* p_num_tokens, int32_t* p_ids, float* p_weights,
+                      int32_t* p_offsets, int32_t* p_rows, int32_t* p_places, const ckx_route_desc* desc, void* p_workspace,
+                      int64_t workspace_bytes, void* stream);
+
+/* ---- int8 codes of activations, one scale per token ------------------------------------------------
+ *   s[m]    = max(max_k |x[m, k]|, 2^-100) / 127                       (fp32)
+ *   q[m, k] = x[m, k] * 127 / max(max_k |x[m, k]|, 2^-100)             (the quotient rounded to fp32, then to nearest even)
+ * x [M, K] fp32, fp16 or bf16 (x_type), q [M, K] int8, rows stride_x / stride_q elements apart. A NaN or infinity makes its
+ * row's scale NaN and its codes 0: every product with the row is NaN. Any K, stride and address. */
+int ckx_quantize_tokens_i8_is_supported(int32_t M, int32_t K, int32_t stride_x, int32_t stride_q, int x_type);
+int ckx_quantize_tokens_i8(const void* p_x, void* p_q, float* p_scale, int32_t M, int32_t K, int32_t stride_x, int32_t stride_q, int x_type,
+                           void* stream);
+
+/* ---- GEMM, int8 operands with a scale for each token and channel -----------------------------------
+ *   D[m, n] = float(sum_k A[m, k] * B[n, k]) * sa[m] * sb[n] + bias[n]
+ *   C[m, n] = round( D[m, n] ),  gated: round( D[m, n] / (1 + exp(-D[m, n])) * D[m, N + n] )
+ * A [M, K] row-major, B stored [N, K] (gated: [2 N, K], the gates' rows before the others; column-major), C [M, N] row-major
+ * fp32, fp16 or bf16 (c_type); sa [M], sb and bias [N] (gated: [2 N]) fp32, p_bias NULL: none. Sums are exact (32-bit), the
+ * rest is fp32 in the order of the formula, C rounded once. K <= 131071. Any stride and address; K, lda, ldb multiples of 16
+ * with 16-byte aligned A and B run on the vectorised kernels. Workspace (optional, ckx_gemm_i8_tokenscale_workspace_bytes; 0
+ * for most problems): lets few output tiles with a long K run side by side. */
+int ckx_gemm_i8_tokenscale_is_supported(int32_t M, int32_t N, int32_t K, int32_t lda, int32_t ldb, int32_t ldc, int gated, int c_type);
+int64_t ckx_gemm_i8_tokenscale_workspace_bytes(int32_t M, int32_t N, int32_t K, int gated);
+int ckx_gemm_i8_tokenscale(const void* p_a, const void* p_b, void* p_c, const float* p_scale_a, const float* p_scale_b, const float* p_bias,
+                           int32_t M, int32_t N, int32_t K, int32_t lda, int32_t ldb, int32_t ldc, int gated, int c_type, void* p_workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/* ---- the same product for each expert's rows -------------------------------------------------------
+ * Rows p_offsets[e] ... p_offsets[e + 1] - 1 of C [num_rows, N] are expert e's (offsets ascend; they are cut to 0 ...
+ * num_rows): row i takes row p_rows[i] / rows_per of A [num_rows_a, K] (p_rows NULL: row i), its scale with it, and B, scales
+ * and biases of expert e: B [num_experts, N, K] (gated: 2 N), experts batch_stride_b elements apart, sb and bias
+ * [num_experts, N] (gated: 2 N). A row number outside A counts as a row of zeros with scale 0. Rows of C that belong to no
+ * expert are left alone. With the tables of ckx_route_experts, p_rows and rows_per = top_k take each pair's token; C's rows
+ * then stand in the order of p_rows. Up to 1024 experts, 2^24 rows; otherwise as ckx_gemm_i8_tokenscale. */
+typedef struct ckx_experts_desc
+{
+    int32_t num_rows, num_rows_a, num_experts;
+    int32_t N, K;
+    int32_t stride_a, stride_b, stride_c;
+    int32_t rows_per;
+    int32_t gated; /* 0 or 1 */
+    int32_t c_type;
+    int32_t reserved;
+    int64_t batch_stride_b;
+} ckx_experts_desc;
+int ckx_experts_gemm_i8_is_supported(const ckx_experts_desc* desc);
+int ckx_experts_gemm_i8(const void* p_a, const void* p_b, void* p_c, const float* p_scale_a, const float* p_scale_b, const float* p_bias,
+                        const int32_t* p_offsets, const int32_t* p_rows, const ckx_experts_desc* desc, void* stream);
+
+/* ---- a token's rows, weighted and added up ---------------------------------------------------------
+ *   out[t, n] = round( add[t, n] + sum_j w[t, j] * y[places[t, j], n] )       (j ascending, fp32; p_add NULL: 0)
+ * y [num_rows, N], add and out [num_tokens, N] fp32, fp16 or bf16 (type), rows stride_* apart; places and w [num_tokens,
+ * top_k] as ckx_route_experts gives them. Places outside y (-1) are skipped; a token with none gets add alone. add may be
+ * out itself (the same address and stride). */
+int ckx_experts_combine_is_supported(int32_t num_tokens, int32_t top_k, int32_t num_rows, int32_t N, int32_t stride_y, int32_t stride_add,
+                                     int32_t stride_out, int type);
+int ckx_experts_combine(const void* p_y, const int32_t* p_places, const float* p_weights, const void* p_add, void* p_out, int32_t num_tokens,
+                        int32_t top_k, int32_t num_rows, int32_t N, int32_t stride_y, int32_t stride_add, int32_t stride_out, int type,
+                        void* stream);
+
 /* ---- timing helper --------------------------------------------------------
  * launch_and_time_kernel (include/ck/device_utility/kernel_launch.hpp:13-74):
  * `fn(user)` is called n_warmup times untimed, then n_repeat times between two
