@@ -14,7 +14,7 @@ namespace ckx {
 
 namespace {
 
-constexpr int kWaves = 16, kThreads = kWaves * 64;
+constexpr int kWaves = 8, kThreads = kWaves * 64; // (16 experts a lane take more registers than 16 waves leave)
 constexpr int kOneGroup = 64, kMostChunks = 256;
 
 // numbers that rise with the value; none of them is 0
@@ -204,34 +204,295 @@ __device__ __forceinline__ void route_token(const RouteArgs& p, int64_t t, int l
     }
 }
 
-// sums of the counts before each expert, over the workgroup: base[e] for e < experts; returns the sum of all
-__device__ __forceinline__ int sums_before(int* base, int count, int experts, int* parts)
+// ---- four tokens a wave: up to 256 experts and 16 picks, groups that are whole lanes -----------------------------------------------
+// Sixteen lanes take a token, EPL experts a lane one after the other. Its values stay what they are, fp32 logits where there is no bias
+// and 64-bit sums otherwise: the largest of 16 values in a lane is 15 instructions, that of a row of lanes four rotations, and the lowest
+// expert of those that hold it another four.
+template <int CTRL>
+__device__ __forceinline__ int row_dpp(int v)
+{
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, false);
+}
+template <int CTRL>
+__device__ __forceinline__ float row_dpp(float v)
+{
+    return __builtin_bit_cast(float, row_dpp<CTRL>(__builtin_bit_cast(int, v)));
+}
+template <int CTRL>
+__device__ __forceinline__ double row_dpp(double v)
+{
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)(uint32_t)row_dpp<CTRL>((int)(uint32_t)b) | (uint64_t)(uint32_t)row_dpp<CTRL>((int)(uint32_t)(b >> 32)) << 32);
+}
+__device__ __forceinline__ float most_of(float a, float b) { return __builtin_fmaxf(a, b); }
+__device__ __forceinline__ double most_of(double a, double b) { return __builtin_fmax(a, b); }
+__device__ __forceinline__ float least_of(float a, float b) { return __builtin_fminf(a, b); }
+__device__ __forceinline__ double least_of(double a, double b) { return __builtin_fmin(a, b); }
+// of the row's sixteen lanes, in all of them (rotations by 8, 4, 2 and 1 lanes)
+template <typename V>
+__device__ __forceinline__ V row_most(V v)
+{
+    v = most_of(v, row_dpp<0x128>(v));
+    v = most_of(v, row_dpp<0x124>(v));
+    v = most_of(v, row_dpp<0x122>(v));
+    return most_of(v, row_dpp<0x121>(v));
+}
+__device__ __forceinline__ int row_least(int v)
+{
+    v = min(v, row_dpp<0x128>(v));
+    v = min(v, row_dpp<0x124>(v));
+    v = min(v, row_dpp<0x122>(v));
+    return min(v, row_dpp<0x121>(v));
+}
+__device__ __forceinline__ double row_sum(double v)
+{
+    v += row_dpp<0x128>(v);
+    v += row_dpp<0x124>(v);
+    v += row_dpp<0x122>(v);
+    return v + row_dpp<0x121>(v);
+}
+
+// exp(x) for |x| <= 600: 2^n times the series of exp over half a step to either side of zero, whose term behind the last kept is under
+// 2^-52 of the sum. A third of the library function's instructions, which has the ends of the range to look after.
+__device__ __forceinline__ double exp_near(double x)
+{
+    const double n = __builtin_rint(x * 1.4426950408889634074);
+    double r       = __builtin_fma(-n, 6.93147180369123816490e-01, x); // (ln 2 in two parts)
+    r              = __builtin_fma(-n, 1.90821492927058770002e-10, r);
+    double y       = 1.0 / 6227020800.0;
+    y              = __builtin_fma(y, r, 1.0 / 479001600.0);
+    y              = __builtin_fma(y, r, 1.0 / 39916800.0);
+    y              = __builtin_fma(y, r, 1.0 / 3628800.0);
+    y              = __builtin_fma(y, r, 1.0 / 362880.0);
+    y              = __builtin_fma(y, r, 1.0 / 40320.0);
+    y              = __builtin_fma(y, r, 1.0 / 5040.0);
+    y              = __builtin_fma(y, r, 1.0 / 720.0);
+    y              = __builtin_fma(y, r, 1.0 / 120.0);
+    y              = __builtin_fma(y, r, 1.0 / 24.0);
+    y              = __builtin_fma(y, r, 1.0 / 6.0);
+    y              = __builtin_fma(y, r, 0.5);
+    y              = __builtin_fma(y, r, 1.0);
+    y              = __builtin_fma(y, r, 1.0);
+    return __builtin_ldexp(y, (int)n);
+}
+// 1 / x for 1 <= x < 2^900: two of Newton's steps from the instruction's estimate
+__device__ __forceinline__ double reciprocal_near(double x)
+{
+    double y = __builtin_amdgcn_rcp(x);
+    y        = __builtin_fma(__builtin_fma(-x, y, 1.0), y, y);
+    return __builtin_fma(__builtin_fma(-x, y, 1.0), y, y);
+}
+
+// the lane's experts [lane * EPL ... ) of a row of logits, -infinity behind the last
+template <typename X, int EPL>
+__device__ __forceinline__ void load_logits(const X* row, int first, int experts, float (&x)[EPL])
+{
+    struct __attribute__((packed)) All
+    {
+        X v[EPL];
+    };
+    if(first + EPL <= experts)
+    {
+        const All a = *reinterpret_cast<const All*>(row + first);
+#pragma unroll
+        for(int i = 0; i < EPL; ++i)
+            x[i] = (float)a.v[i];
+    }
+    else
+#pragma unroll
+        for(int i = 0; i < EPL; ++i)
+            x[i] = first + i < experts ? (float)row[first + i] : -__builtin_inff();
+}
+
+// V: float, there are no biases; double: there are. ALL as above. `live`: of the lane's row of lanes.
+template <typename X, int EPL, typename V, bool ALL>
+__device__ __forceinline__ void route_tokens(const RouteArgs& p, int64_t t, bool live, int lane, const float (&bias)[EPL], int (&ids)[1])
+{
+    constexpr bool WIDE      = sizeof(V) == 8;
+    constexpr float kLargest = 3.402823466e38f;
+    constexpr V kNone        = -(V)__builtin_inff();
+    const int first          = lane * EPL;
+    const X* const row       = reinterpret_cast<const X*>(p.x) + (live ? t : 0) * p.stride_x;
+    float x[EPL];
+    load_logits(row, first, p.experts, x);
+    auto there = [&](int i) { return x[i] > -__builtin_inff(); };
+    float most = -__builtin_inff(), least = 0.0f;
+#pragma unroll
+    for(int i = 0; i < EPL; ++i)
+    {
+        x[i]  = live && x[i] > -__builtin_inff() && bias[i] > -__builtin_inff() ? __builtin_fminf(x[i], kLargest) : -__builtin_inff(); // (a NaN is out)
+        most  = __builtin_fmaxf(most, x[i]);
+        least = __builtin_fminf(least, there(i) ? x[i] : 0.0f);
+    }
+    const float x_max = row_most(most);
+    V value[EPL];          // by which experts are ordered
+    double score[EPL];     // ALL: s, or s + bias
+    double total = 1.0;
+    if constexpr(ALL)
+    {
+        // (differences of 600 and more go to the library's functions)
+        const bool near = p.sigmoid ? __builtin_fmaxf(most, -least) <= 600.0f : least >= x_max - 600.0f && x_max <= 600.0f && x_max >= -600.0f;
+        const bool fast = __ballot(near || !live || x_max == -__builtin_inff()) == ~0ull;
+        double sum      = 0.0;
+#pragma unroll
+        for(int i = 0; i < EPL; ++i)
+        {
+            const double a = !there(i) ? 0.0 : p.sigmoid ? -(double)x[i] : (double)x[i] - (double)x_max;
+            double d       = fast ? exp_near(a) : exp(a);
+            d              = there(i) ? d : 0.0;
+            score[i]       = p.sigmoid ? (fast ? reciprocal_near(1.0 + d) : 1.0 / (1.0 + d)) : d;
+            sum += d;
+        }
+        if(!p.sigmoid)
+        {
+            total = row_sum(sum);
+            total = total > 0.0 ? total : 1.0;
+#pragma unroll
+            for(int i = 0; i < EPL; ++i)
+                score[i] /= total;
+        }
+    }
+#pragma unroll
+    for(int i = 0; i < EPL; ++i)
+    {
+        if constexpr(WIDE)
+        {
+            score[i] += (double)__builtin_fminf(bias[i], kLargest);
+            value[i] = there(i) ? score[i] : kNone;
+        }
+        else
+            value[i] = x[i];
+    }
+    if(p.groups > 1)
+    {
+        // the group's lanes all come to hold its value
+        const int lanes = p.experts / p.groups / EPL, mine = lane / lanes;
+        auto best_two   = [&](auto of) {
+            using S  = decltype(of(0));
+            S a = -(S)__builtin_inff(), b = -(S)__builtin_inff();
+            auto with = [&](S v) {
+                b = most_of(b, least_of(a, v));
+                a = most_of(a, v);
+            };
+#pragma unroll
+            for(int i = 0; i < EPL; ++i)
+                with(of(i));
+            // another lane's two: both go in
+            auto other = [&](S c, S d) {
+                with(c);
+                with(d);
+            };
+            if(lanes > 1)
+                other(row_dpp<0xb1>(a), row_dpp<0xb1>(b)); // the neighbour in a pair of lanes
+            if(lanes > 2)
+                other(row_dpp<0x4e>(a), row_dpp<0x4e>(b)); // the other pair of four
+            if(lanes > 4)
+                other(row_dpp<0x141>(a), row_dpp<0x141>(b)); // eight lanes mirrored: the other four
+            return p.group_best == 2 && b > -(S)__builtin_inff() ? (double)(a + b) : (double)a;
+        };
+        double of;
+        if constexpr(ALL && !WIDE)
+            of = p.group_best == 2 ? best_two([&](int i) { return there(i) ? score[i] : -__builtin_inf(); }) : best_two([&](int i) { return (double)value[i]; });
+        else
+            of = best_two([&](int i) { return value[i]; });
+        bool stays = false;
+        for(int j = 0; j < p.top_groups; ++j)
+        {
+            const double top = row_most(of);
+            const int which  = row_least(of == top ? mine : 64);
+            const bool won   = which == mine && top > -__builtin_inf();
+            stays |= won;
+            of = won ? -__builtin_inf() : of;
+        }
+#pragma unroll
+        for(int i = 0; i < EPL; ++i)
+            value[i] = stays ? value[i] : kNone;
+    }
+    // the picks: lane j keeps the j-th
+    int expert = -1;
+    for(int j = 0; j < p.top_k; ++j)
+    {
+        V best = value[0];
+#pragma unroll
+        for(int i = 1; i < EPL; ++i)
+            best = most_of(best, value[i]);
+        const V top = row_most(best);
+        int at      = kMostExperts;
+#pragma unroll
+        for(int i = EPL - 1; i >= 0; --i)
+            at = value[i] == top ? first + i : at;
+        const int e = row_least(at);
+        if(lane == j && top > kNone)
+            expert = e;
+#pragma unroll
+        for(int i = 0; i < EPL; ++i)
+            value[i] = first + i == e ? kNone : value[i];
+    }
+    double w = 0.0;
+    if(expert >= 0)
+    {
+        const float v  = __builtin_fminf((float)row[expert], kLargest);
+        const double d = exp(p.sigmoid ? -(double)v : (double)v - (double)x_max);
+        w              = p.sigmoid ? 1.0 / (1.0 + d) : d / total;
+    }
+    if(p.renormalise)
+    {
+        const double sum = row_sum(w);
+        w                = sum > 0.0 ? w / sum : 0.0;
+    }
+    ids[0] = expert;
+    if(t < p.tokens && lane < p.top_k)
+    {
+        p.ids[t * p.top_k + lane]     = expert;
+        p.weights[t * p.top_k + lane] = (float)(w * (double)p.scale);
+    }
+}
+
+// whether the kernel of four tokens a wave takes a call, EPL experts a lane
+int row_experts(const RouteArgs& a)
+{
+    int epl = 1;
+    while(epl * 16 < a.experts)
+        epl *= 2;
+    const int size = a.experts / a.groups, lanes = size / epl;
+    const bool whole = a.groups == 1 || (size % epl == 0 && (lanes & (lanes - 1)) == 0 && lanes <= 8);
+    return epl <= 16 && a.top_k <= 16 && whole ? epl : 0;
+}
+
+// base[e]: from the counts of each expert to the sums of those before it, over the workgroup; returns the sum of all
+__device__ __forceinline__ int sums_before(int* base, int experts, int* parts)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int v = count;
+    int all = 0;
+    for(int e0 = 0; e0 < experts; e0 += kThreads)
+    {
+        const int e     = e0 + (int)threadIdx.x;
+        const int count = e < experts ? base[e] : 0;
+        int v           = count;
 #pragma unroll
-    for(int d = 1; d < 64; d *= 2)
-    {
-        const int o = __shfl_up(v, d, 64);
-        v += lane >= d ? o : 0;
+        for(int d = 1; d < 64; d *= 2)
+        {
+            const int o = __shfl_up(v, d, 64);
+            v += lane >= d ? o : 0;
+        }
+        if(lane == 63)
+            parts[wave] = v;
+        __syncthreads();
+        int before = all;
+        for(int w = 0; w < kWaves; ++w)
+        {
+            const int n = parts[w];
+            before += w < wave ? n : 0;
+            all += n;
+        }
+        if(e < experts)
+            base[e] = before + v - count;
+        __syncthreads();
     }
-    if(lane == 63)
-        parts[wave] = v;
-    __syncthreads();
-    int before = 0, all = 0;
-    for(int w = 0; w < kWaves; ++w)
-    {
-        const int n = parts[w];
-        before += w < wave ? n : 0;
-        all += n;
-    }
-    if((int)threadIdx.x < experts)
-        base[threadIdx.x] = before + v - count;
-    __syncthreads();
     return all;
 }
 
-// the pairs [from, to) to their places: base[e] is where the next row of expert e goes. 1024 pairs at a time, 64 a wave; cells:
+// the pairs [from, to) to their places: base[e] is where the next row of expert e goes. 512 pairs at a time, 64 a wave; cells:
 // [kWaves][experts] numbers.
 __device__ __forceinline__ void place_pairs(const RouteArgs& p, int64_t from, int64_t to, int* base, int* cells)
 {
@@ -254,16 +515,19 @@ __device__ __forceinline__ void place_pairs(const RouteArgs& p, int64_t from, in
         if(e >= 0 && rank == 0)
             cells[wave * p.experts + e] = (int)__builtin_popcountll(same);
         __syncthreads();
-        if((int)threadIdx.x < p.experts)
+        for(int x = threadIdx.x; x < p.experts; x += kThreads)
         {
-            int next = base[threadIdx.x];
+            int n[kWaves], next = base[x];
+#pragma unroll
+            for(int w = 0; w < kWaves; ++w)
+                n[w] = cells[w * p.experts + x];
+#pragma unroll
             for(int w = 0; w < kWaves; ++w)
             {
-                const int n                          = cells[w * p.experts + threadIdx.x];
-                cells[w * p.experts + threadIdx.x] = next;
-                next += n;
+                cells[w * p.experts + x] = next;
+                next += n[w];
             }
-            base[threadIdx.x] = next;
+            base[x] = next;
         }
         __syncthreads();
         if(pair < to)
@@ -277,13 +541,13 @@ __device__ __forceinline__ void place_pairs(const RouteArgs& p, int64_t from, in
     }
 }
 
-// LDS: [kWaves][experts] doubles (groups) or numbers (tables)
-template <typename X, int EPL, bool WIDE, bool ALL>
+// ROWS: four tokens a wave. LDS: [kWaves][experts] doubles (one token a wave, groups) or numbers (tables)
+template <typename X, bool ROWS, int EPL, bool WIDE, bool ALL>
 __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs p)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t ckx_route_lds[];
     __shared__ int counts[kMostExperts], parts[kWaves];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & (ROWS ? 15 : 63), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t first = (int64_t)blockIdx.x * p.chunk_tokens;
     const int64_t last  = first + p.chunk_tokens < p.tokens ? first + p.chunk_tokens : p.tokens;
     const int live      = p.live ? max(0, min(*p.live, p.tokens)) : p.tokens;
@@ -295,7 +559,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs p)
     {
         const int e = lane * EPL + i;
         bias[i]     = WIDE && e < p.experts ? p.bias[e] : 0.0f;
-        group[i]    = p.groups > 1 && e < p.experts ? e / (p.experts / p.groups) : 0;
+        group[i]    = !ROWS && p.groups > 1 && e < p.experts ? e / (p.experts / p.groups) : 0;
     }
     if(p.offsets)
     {
@@ -303,32 +567,41 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs p)
             counts[e] = 0;
         __syncthreads();
     }
-    for(int64_t t = first + wave; t < last; t += kWaves)
-    {
-        if(t < live)
-            route_token<X, EPL, WIDE, ALL>(p, t, lane, values, bias, group);
-        else if(lane < p.top_k)
-            p.ids[t * p.top_k + lane] = -1, p.weights[t * p.top_k + lane] = 0.0f;
-        if(p.offsets && lane < p.top_k)
+    if constexpr(ROWS)
+        for(int64_t t0 = first + wave * 4; t0 < last; t0 += kWaves * 4)
         {
-            const int e = p.ids[t * p.top_k + lane]; // (the lane's own)
-            if(e >= 0)
-                atomicAdd(&counts[e], 1);
+            const int64_t t = t0 + (threadIdx.x >> 4 & 3);
+            int expert[1];
+            route_tokens<X, EPL, typename std::conditional<WIDE, double, float>::type, ALL>(p, t < last ? t : p.tokens, t < last && t < live, lane, bias, expert);
+            if(p.offsets && expert[0] >= 0)
+                atomicAdd(&counts[expert[0]], 1);
         }
-    }
+    else
+        for(int64_t t = first + wave; t < last; t += kWaves)
+        {
+            if(t < live)
+                route_token<X, EPL, WIDE, ALL>(p, t, lane, values, bias, group);
+            else if(lane < p.top_k)
+                p.ids[t * p.top_k + lane] = -1, p.weights[t * p.top_k + lane] = 0.0f;
+            if(p.offsets && lane < p.top_k)
+            {
+                const int e = p.ids[t * p.top_k + lane]; // (the lane's own)
+                if(e >= 0)
+                    atomicAdd(&counts[e], 1);
+            }
+        }
     if(!p.offsets)
         return;
     __syncthreads();
-    const int count = (int)threadIdx.x < p.experts ? counts[threadIdx.x] : 0;
     if(p.chunks > 1)
     {
-        if((int)threadIdx.x < p.experts)
-            p.ws[(int64_t)blockIdx.x * p.experts + threadIdx.x] = count;
+        for(int e = threadIdx.x; e < p.experts; e += kThreads)
+            p.ws[(int64_t)blockIdx.x * p.experts + e] = counts[e];
         return;
     }
-    const int all = sums_before(counts, count, p.experts, parts);
-    if((int)threadIdx.x < p.experts)
-        p.offsets[threadIdx.x] = counts[threadIdx.x];
+    const int all = sums_before(counts, p.experts, parts);
+    for(int e = threadIdx.x; e < p.experts; e += kThreads)
+        p.offsets[e] = counts[e];
     if(threadIdx.x == 0)
         p.offsets[p.experts] = all;
     const int64_t pairs = (int64_t)p.tokens * p.top_k;
@@ -346,10 +619,9 @@ __global__ __launch_bounds__(kThreads) void route_tables_kernel(RouteArgs p)
     __syncthreads();
     // (threads in rows of `wide`, a chunk each)
     int wide = 64;
-    while(wide < p.experts)
+    while(wide < p.experts && wide < kThreads)
         wide *= 2;
-    const int e = threadIdx.x & (wide - 1);
-    if(e < p.experts)
+    for(int e = threadIdx.x & (wide - 1); e < p.experts; e += wide)
     {
         int before = 0, all = 0;
 #pragma unroll 8
@@ -363,13 +635,12 @@ __global__ __launch_bounds__(kThreads) void route_tables_kernel(RouteArgs p)
         atomicAdd(&totals[e], all);
     }
     __syncthreads();
-    const int total = (int)threadIdx.x < p.experts ? totals[threadIdx.x] : 0;
-    const int all   = sums_before(totals, total, p.experts, parts);
-    if((int)threadIdx.x < p.experts)
+    const int all = sums_before(totals, p.experts, parts);
+    for(int e = threadIdx.x; e < p.experts; e += kThreads)
     {
-        mine[threadIdx.x] += totals[threadIdx.x];
+        mine[e] += totals[e];
         if(blockIdx.x == 0)
-            p.offsets[threadIdx.x] = totals[threadIdx.x];
+            p.offsets[e] = totals[e];
     }
     if(blockIdx.x == 0 && threadIdx.x == 0)
         p.offsets[p.experts] = all;
@@ -388,15 +659,15 @@ hipError_t allow_lds(F* kernel, size_t bytes)
                          : hipSuccess;
 }
 
-template <typename X, int EPL, bool WIDE, bool ALL>
+template <typename X, bool ROWS, int EPL, bool WIDE, bool ALL>
 hipError_t launch(const RouteArgs& a, hipStream_t s)
 {
     const size_t cells = a.offsets ? (size_t)kWaves * a.experts * 4 : 0;
-    const size_t lds   = a.groups > 1 ? (size_t)kWaves * a.experts * 8 : a.chunks == 1 ? cells : 0;
-    hipError_t e       = allow_lds(&route_kernel<X, EPL, WIDE, ALL>, lds);
+    const size_t lds   = !ROWS && a.groups > 1 ? (size_t)kWaves * a.experts * 8 : a.chunks == 1 ? cells : 0;
+    hipError_t e       = allow_lds(&route_kernel<X, ROWS, EPL, WIDE, ALL>, lds);
     if(e != hipSuccess)
         return e;
-    hipLaunchKernelGGL((route_kernel<X, EPL, WIDE, ALL>), dim3(a.chunks), dim3(kThreads), lds, s, a);
+    hipLaunchKernelGGL((route_kernel<X, ROWS, EPL, WIDE, ALL>), dim3(a.chunks), dim3(kThreads), lds, s, a);
     e = hipGetLastError();
     if(e != hipSuccess || a.chunks == 1 || !a.offsets)
         return e;
@@ -406,23 +677,28 @@ hipError_t launch(const RouteArgs& a, hipStream_t s)
     return hipGetLastError();
 }
 
-template <typename X, int EPL>
+template <typename X, bool ROWS, int EPL>
 hipError_t launch_form(const RouteArgs& a, hipStream_t s)
 {
     if(a.bias)
-        return launch<X, EPL, true, true>(a, s);
+        return launch<X, ROWS, EPL, true, true>(a, s);
     const bool all = (a.groups > 1 && a.group_best == 2) || (!a.sigmoid && !a.renormalise);
-    return all ? launch<X, EPL, false, true>(a, s) : launch<X, EPL, false, false>(a, s);
+    return all ? launch<X, ROWS, EPL, false, true>(a, s) : launch<X, ROWS, EPL, false, false>(a, s);
 }
 
 template <typename X>
 hipError_t launch_any(const RouteArgs& a, hipStream_t s)
 {
-    return a.experts <= 64    ? launch_form<X, 1>(a, s)
-           : a.experts <= 128 ? launch_form<X, 2>(a, s)
-           : a.experts <= 256 ? launch_form<X, 4>(a, s)
-           : a.experts <= 512 ? launch_form<X, 8>(a, s)
-                              : launch_form<X, 16>(a, s);
+    switch(row_experts(a))
+    {
+    case 1: return launch_form<X, true, 1>(a, s);
+    case 2: return launch_form<X, true, 2>(a, s);
+    case 4: return launch_form<X, true, 4>(a, s);
+    case 8: return launch_form<X, true, 8>(a, s);
+    case 16: return launch_form<X, true, 16>(a, s);
+    default: break;
+    }
+    return a.experts <= 256 ? launch_form<X, false, 4>(a, s) : launch_form<X, false, 16>(a, s);
 }
 
 void cut(int tokens, int& chunk_tokens, int& chunks)
