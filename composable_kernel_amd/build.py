@@ -62,7 +62,7 @@ def check_compiler():
 
 # kernels whose LDS fragment reads are inline assembly waited for by hand (mangled-name fragments)
 HAND_WAITED_KERNELS = ("gemm_tile_kernel", "gemm_w4_kernel", "gemm_astream_kernel", "conv_patch_kernel", "conv_patch_wide_kernel",
-                       "conv_pointwise_kernel", "conv_window_kernel", "gemm_f8_tile_kernel")
+                       "conv_pointwise_kernel", "conv_window_kernel", "gemm_f8_tile_kernel", "gemm_i8_tile_kernel", "gemm_i8_big_kernel")
 
 
 def vgpr_spills(compiler_output):

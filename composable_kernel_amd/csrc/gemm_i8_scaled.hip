@@ -1,6 +1,6 @@
 // int8 GEMM with a scale for each token and channel, dense and for each expert's rows (formulas: include/ckx.h,
 // ckx_gemm_i8_tokenscale and ckx_experts_gemm_i8).
-#include "gemm_i8_scaled.hpp"
+#include "gemm_i8_big.hpp"
 
 namespace ckx {
 
@@ -39,12 +39,16 @@ __global__ __launch_bounds__(256) void gemm_i8_any_kernel(GemmI8Args p)
     i8_load_scales<GATED>(p, t.expert, n0, BN, tid, 256, sb, bias);
     // a wave fills LDS rows wave * 32 ... + 31 of either tile, eight rows a load; chunk c of row r lies at c ^ (r & 7)
     const int8_t *ra[4], *rb[4];
+    int row[4], m[4];
+#pragma unroll
+    for(int j = 0; j < 4; ++j)
+        row[j] = wave * 32 + j * 8 + (lane >> 3);
+    i8_rows_of_a(p, t, row, m);
 #pragma unroll
     for(int j = 0; j < 4; ++j)
     {
-        const int r = wave * 32 + j * 8 + (lane >> 3);
-        const int m = r < t.rows ? i8_row_of_a(p, t.m0 + r) : -1;
-        ra[j]       = m >= 0 ? p.a + (int64_t)m * p.lda : nullptr;
+        const int r = row[j];
+        ra[j]       = m[j] >= 0 ? p.a + (int64_t)m[j] * p.lda : nullptr;
         bool second;
         const int n = n0 + i8_col_of<GATED>((uint32_t)r, second);
         rb[j]       = n < p.N ? p.b + (int64_t)t.expert * p.batch_b + ((int64_t)n + (second ? p.N : 0)) * p.ldb : nullptr;
@@ -99,9 +103,316 @@ __global__ __launch_bounds__(256) void gemm_i8_any_kernel(GemmI8Args p)
         const int r = wm * 64 + i * 16 + (lane & 15), m = t.m0 + r;
         if(r >= t.rows)
             continue;
-        const int from = i8_row_of_a(p, m);
+        const int from = i8_row_of_a(p, t, r);
         i8_finish<T, GATED>(reinterpret_cast<T*>(p.c) + (int64_t)m * p.ldc, n0 + wn * (GATED ? 32 : 64), p.N, q, acc[i], from >= 0 ? p.sa[from] : 0.0f,
                             sb + wn * 64, bias + wn * 64);
+    }
+}
+
+// BM rows x BN rows of B, WM x WN waves, NST stages of operands in LDS: the loads of a K tile (128) are asked for NST - 1 tiles ahead.
+// The direct loads are inline assembly: the compiler, told of them, would wait for all of them before every LDS read of another
+// stage. Its own LDS reads it waits for itself; the wait for the direct loads stands in front of the barrier.
+// Columns behind K count by A's zeros alone: what B's loads bring there, and the rows of a tile that C does not have, are whatever the
+// resource's bounds let through.
+template <typename T, bool GATED, int BM, int BN, int WM, int WN, int NST>
+__global__ __launch_bounds__(WM* WN * 64) void gemm_i8_tile_kernel(GemmI8Args p)
+{
+    constexpr int NW = WM * WN, MT = BM / WM / 16, NLA = BM / 8 / NW, NLB = BN / 8 / NW, LPT = NLA + NLB, COLS = GATED ? BN / 2 : BN;
+    constexpr int A_TILE = BM * 128, B_AT = NST * A_TILE, B_TILE = BN * 128, S_AT = B_AT + NST * B_TILE;
+    static_assert(BN / WN == 64 && NLA >= 1 && NLB >= 1, "");
+    __shared__ __align__(1024) uint8_t lds[S_AT + (BM + 2 * BN) * 4]; // [A | B | scales of rows, of columns, biases]
+    float* const s_row = reinterpret_cast<float*>(lds + S_AT);
+    float* const s_col = s_row + BM;
+    float* const s_bias = s_col + BN;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WN, wn = wave % WN, q = lane >> 4;
+    I8Tile t;
+    int run = 0;
+    if(p.offsets)
+    {
+        if(!i8_expert_tile(p, (int)blockIdx.x, BM, t))
+            return;
+    }
+    else
+    {
+        int tm; // (a run of K tiles takes the place of a batch)
+        tile_of_block((int)blockIdx.x, p.tiles_m, p.tiles_n, p.ksplit, run, tm, t.tn);
+        t.expert = 0, t.m0 = tm * BM, t.rows = min(BM, p.M - t.m0);
+    }
+    const int g0 = run * p.per, g1 = min(g0 + p.per, p.ksteps);
+    const int n0 = t.tn * COLS;
+    // resources that end with the last byte of what the tile may read; rows are counted from the tile's first, or from the first
+    // of A (gathered) and of the expert's B (its halves lie apart)
+    const int64_t a0 = p.rows ? 0 : t.m0, b0 = GATED ? 0 : n0;
+    const int64_t rows_a = p.rows ? p.rows_a : min((int64_t)t.rows, (int64_t)p.rows_a - t.m0), rows_b = GATED ? 2 * (int64_t)p.N : min(BN, p.N - n0);
+    const __amdgpu_buffer_rsrc_t ra = make_rsrc(p.a + a0 * p.lda, rows_a > 0 ? (uint32_t)((rows_a - 1) * p.lda + p.K) : 0u);
+    const __amdgpu_buffer_rsrc_t rb = make_rsrc(p.b + (int64_t)t.expert * p.batch_b + b0 * p.ldb, (uint32_t)((rows_b - 1) * p.ldb + p.K));
+    const uint32_t base = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
+    // a load fills eight rows, chunk c of row r at c ^ (r & 7)
+    const int kc = ((lane & 7) ^ (lane >> 3)) * 16;
+    uint32_t oa[NLA], ob[NLB];
+#pragma unroll
+    for(int j = 0; j < NLB; ++j)
+    {
+        bool second;
+        const int n = n0 + i8_col_of<GATED>((uint32_t)((wave * NLB + j) * 8 + (lane >> 3)), second);
+        ob[j]       = n < p.N ? (uint32_t)(n - b0 + (second ? p.N : 0)) * (uint32_t)p.ldb + kc : kOutOfRange;
+    }
+    int row[NLA], m[NLA];
+#pragma unroll
+    for(int j = 0; j < NLA; ++j)
+        row[j] = (wave * NLA + j) * 8 + (lane >> 3);
+    i8_rows_of_a(p, t, row, m);
+#pragma unroll
+    for(int j = 0; j < NLA; ++j)
+        oa[j] = m[j] >= 0 ? (uint32_t)(m[j] - a0) * (uint32_t)p.lda + kc : kOutOfRange;
+    auto load16 = [&](const __amdgpu_buffer_rsrc_t& r, uint32_t off, uint32_t k, uint32_t at) {
+        asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(off), "s"(r), "s"(k), "s"(at));
+    };
+    // (tiles behind the last come as zeros: the counts of loads under way stay the same)
+    auto load_all = [&](int g) {
+        const uint32_t k = (uint32_t)g * 128, st = (uint32_t)g % NST;
+        const bool in = (int)k + kc < p.K;
+#pragma unroll
+        for(int j = 0; j < NLA; ++j)
+            load16(ra, in ? oa[j] : kOutOfRange, k, base + st * A_TILE + (wave * NLA + j) * 1024);
+#pragma unroll
+        for(int j = 0; j < NLB; ++j)
+            load16(rb, ob[j], k, base + B_AT + st * B_TILE + (wave * NLB + j) * 1024);
+    };
+    for(int g = g0; g < g0 + NST - 1; ++g)
+        load_all(g);
+    // (behind the first loads: their waits are the compiler's, and count those too)
+    i8_load_scales<GATED>(p, t.expert, n0, BN, tid, NW * 64, s_col, s_bias);
+    for(int r = tid; r < BM; r += NW * 64)
+    {
+        const int m = i8_row_of_a(p, t, r);
+        s_row[r]    = m >= 0 ? p.sa[m] : 0.0f;
+    }
+    i32x4 acc[MT][4];
+#pragma unroll
+    for(int i = 0; i < MT; ++i)
+#pragma unroll
+        for(int j = 0; j < 4; ++j)
+            acc[i][j] = i32x4{0, 0, 0, 0};
+    const int a_row = wm * (BM / WM) + (lane & 15), b_row = wn * 64 + (lane & 15);
+    const int a_lo = a_row * 128 + ((q ^ (a_row & 7)) << 4), b_lo = B_AT + b_row * 128 + ((q ^ (b_row & 7)) << 4);
+    for(int g = g0; g < g1; ++g)
+    {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * LPT) : "memory"); // this tile's
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        load_all(g + NST - 1); // (into the stage that every wave has read before this barrier)
+        const uint8_t* const at = lds + g % NST * A_TILE;
+        const uint8_t* const bt = lds + g % NST * B_TILE;
+#pragma unroll
+        for(int ks = 0; ks < 2; ++ks)
+        {
+            i32x4 bf[4];
+#pragma unroll
+            for(int j = 0; j < 4; ++j)
+                bf[j] = *reinterpret_cast<const i32x4*>(bt + (b_lo ^ (ks * 64)) + j * 2048);
+#pragma unroll
+            for(int i = 0; i < MT; ++i)
+            {
+                const i32x4 af = *reinterpret_cast<const i32x4*>(at + (a_lo ^ (ks * 64)) + i * 2048);
+#pragma unroll
+                for(int j = 0; j < 4; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j], af, acc[i][j], 0, 0, 0);
+            }
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // (no load may land in LDS that is another workgroup's by then)
+    __syncthreads();                                 // (a run without K tiles: the scales)
+#pragma unroll
+    for(int i = 0; i < MT; ++i)
+    {
+        const int r = wm * (BM / WM) + i * 16 + (lane & 15), n = n0 + wn * (GATED ? 32 : 64);
+        if(r >= t.rows)
+            continue;
+        if(p.ksplit > 1)
+        {
+            int* const row = p.ws + ((int64_t)run * p.M + t.m0 + r) * p.N * (GATED ? 2 : 1);
+#pragma unroll
+            for(int h = 0; h < 2; ++h)
+            {
+                const int c = n + 8 * q + (GATED ? 0 : 32 * h);
+                int* const to = row + (GATED && h ? p.N : 0);
+                store_room<4>(to + c, acc[i][2 * h], (p.N - c) * 4, false);
+                store_room<4>(to + c + 4, acc[i][2 * h + 1], (p.N - c - 4) * 4, false);
+            }
+        }
+        else
+            i8_finish<T, GATED>(reinterpret_cast<T*>(p.c) + (int64_t)(t.m0 + r) * p.ldc, n, p.N, q, acc[i], s_row[r], s_col + wn * 64, s_bias + wn * 64);
+    }
+}
+
+// C from the sums of the runs: four columns a thread
+template <typename T, bool GATED>
+__global__ __launch_bounds__(256) void gemm_i8_join_kernel(GemmI8Args p, int quads)
+{
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t m  = id / quads;
+    const int n      = (int)(id - m * quads) * 4;
+    if(m >= p.M)
+        return;
+    const int64_t wide = (int64_t)p.N * (GATED ? 2 : 1);
+    const float sa     = p.sa[m];
+    T* const c         = reinterpret_cast<T*>(p.c) + m * p.ldc + n;
+    float x[2][4];
+#pragma unroll
+    for(int h = 0; h < (GATED ? 2 : 1); ++h)
+    {
+        const int64_t col = n + (h ? p.N : 0);
+        const int* at     = p.ws + m * wide + col;
+        i32x4 v           = {0, 0, 0, 0};
+        for(int r = 0; r < p.ksplit; ++r, at += (int64_t)p.M * wide)
+            if(n + 4 <= p.N)
+                v += load_vec<i32x4>(at);
+            else
+                for(int j = 0; n + j < p.N; ++j)
+                    v[j] += at[j];
+#pragma unroll
+        for(int j = 0; j < 4; ++j)
+            x[h][j] = n + j < p.N ? (float)v[j] * sa * p.sb[col + j] + (p.bias ? p.bias[col + j] : 0.0f) : 0.0f;
+    }
+    typedef T tx4 __attribute__((ext_vector_type(4)));
+    tx4 out;
+#pragma unroll
+    for(int j = 0; j < 4; ++j)
+        out[j] = (T)(GATED ? i8_silu<T>(x[0][j]) * x[1][j] : x[0][j]);
+    if(n + 4 <= p.N)
+        reinterpret_cast<AnyAlign<tx4>*>(c)->v = out;
+    else
+        for(int j = 0; n + j < p.N; ++j)
+            c[j] = out[j];
+}
+
+// Few rows: a workgroup takes MT x NT tiles of 16 x 16 and its NW waves share the K tiles among them, each straight from memory into
+// its registers (the next K tile's 32 bytes a lane and tile row are on their way while one is multiplied); the waves' sums meet in LDS.
+// Nothing waits at a barrier until the end: what a product of few rows needs, which is bound by reading B once. Gated, the tiles of B
+// come in pairs, a gate's and its partner's.
+template <typename T, bool GATED, int MT, int NT, int NW>
+__global__ __launch_bounds__(NW * 64) void gemm_i8_direct_kernel(GemmI8Args p)
+{
+    constexpr int BM = MT * 16, COLS = NT * 16 / (GATED ? 2 : 1);
+    static_assert(!GATED || NT % 2 == 0, "");
+    __shared__ __align__(16) i32x4 sums[NW][MT * NT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = lane & 15, q = lane >> 4;
+    I8Tile t;
+    if(!i8_find_tile(p, (int)blockIdx.x, BM, t))
+        return;
+    const int n0 = t.tn * COLS;
+    const int64_t a0 = p.rows ? 0 : t.m0, b0 = GATED ? 0 : n0;
+    const int64_t rows_a = p.rows ? p.rows_a : min((int64_t)t.rows, (int64_t)p.rows_a - t.m0), rows_b = GATED ? 2 * (int64_t)p.N : min(COLS, p.N - n0);
+    const __amdgpu_buffer_rsrc_t ra = make_rsrc(p.a + a0 * p.lda, rows_a > 0 ? (uint32_t)((rows_a - 1) * p.lda + p.K) : 0u);
+    const __amdgpu_buffer_rsrc_t rb = make_rsrc(p.b + (int64_t)t.expert * p.batch_b + b0 * p.ldb, (uint32_t)((rows_b - 1) * p.ldb + p.K));
+    struct Step
+    {
+        i32x4 a[MT][2], b[NT][2];
+    };
+    uint32_t oa[MT], ob[NT];
+#pragma unroll
+    for(int j = 0; j < NT; ++j)
+    {
+        const int n = n0 + (GATED ? j / 2 : j) * 16 + r;
+        ob[j]       = n < p.N ? (uint32_t)(n - b0 + (GATED && (j & 1) ? p.N : 0)) * (uint32_t)p.ldb + q * 16 : kOutOfRange;
+    }
+    int row[MT], m[MT];
+#pragma unroll
+    for(int i = 0; i < MT; ++i)
+        row[i] = i * 16 + r;
+    i8_rows_of_a(p, t, row, m);
+#pragma unroll
+    for(int i = 0; i < MT; ++i)
+        oa[i] = m[i] >= 0 ? (uint32_t)(m[i] - a0) * (uint32_t)p.lda + q * 16 : kOutOfRange;
+    auto load = [&](Step& x, int g) {
+#pragma unroll
+        for(int h = 0; h < 2; ++h)
+        {
+            const int k        = g * 128 + h * 64;
+            const uint32_t out = k + q * 16 < p.K ? 0u : kOutOfRange; // (columns behind K, and tiles behind the last)
+#pragma unroll
+            for(int j = 0; j < NT; ++j)
+                x.b[j][h] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rb, (int)(ob[j] | out), k, 0));
+#pragma unroll
+            for(int i = 0; i < MT; ++i)
+                x.a[i][h] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(ra, (int)(oa[i] | out), k, 0));
+        }
+    };
+    i32x4 acc[MT][NT];
+#pragma unroll
+    for(int i = 0; i < MT; ++i)
+#pragma unroll
+        for(int j = 0; j < NT; ++j)
+            acc[i][j] = i32x4{0, 0, 0, 0};
+    auto multiply = [&](const Step& x) {
+#pragma unroll
+        for(int h = 0; h < 2; ++h)
+#pragma unroll
+            for(int i = 0; i < MT; ++i)
+#pragma unroll
+                for(int j = 0; j < NT; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.b[j][h], x.a[i][h], acc[i][j], 0, 0, 0);
+    };
+    Step x, y;
+    if(wave < p.ksteps)
+        load(x, wave);
+    for(int g = wave; g < p.ksteps; g += 2 * NW)
+    {
+        if(g + NW < p.ksteps)
+            load(y, g + NW);
+        multiply(x);
+        if(g + 2 * NW < p.ksteps)
+            load(x, g + 2 * NW);
+        if(g + NW < p.ksteps)
+            multiply(y);
+    }
+#pragma unroll
+    for(int i = 0; i < MT; ++i)
+#pragma unroll
+        for(int j = 0; j < NT; ++j)
+            sums[wave][i * NT + j][lane] = acc[i][j];
+    __syncthreads();
+    constexpr int PER = GATED ? 2 : 1;
+    const int64_t at_b = (int64_t)t.expert * p.N * PER;
+    for(int tile = wave; tile < MT * NT / PER; tile += NW)
+    {
+        const int i = tile / (NT / PER), j = tile % (NT / PER);
+        const int m = i * 16 + r, n = n0 + j * 16 + 4 * q;
+        if(m >= t.rows || n >= p.N)
+            continue;
+        const int from = i8_row_of_a(p, t, m);
+        const float sa = from >= 0 ? p.sa[from] : 0.0f;
+        float d[PER][4];
+#pragma unroll
+        for(int h = 0; h < PER; ++h)
+        {
+            i32x4 v = sums[0][i * NT + j * PER + h][lane];
+#pragma unroll
+            for(int w = 1; w < NW; ++w)
+                v += sums[w][i * NT + j * PER + h][lane];
+#pragma unroll
+            for(int e = 0; e < 4; ++e)
+            {
+                const int64_t k = at_b + (h ? p.N : 0) + min(n + e, p.N - 1);
+                d[h][e]         = (float)v[e] * sa * p.sb[k] + (p.bias ? p.bias[k] : 0.0f);
+            }
+        }
+        typedef T tx4 __attribute__((ext_vector_type(4)));
+        T* const c = reinterpret_cast<T*>(p.c) + (int64_t)(t.m0 + m) * p.ldc + n;
+        tx4 out;
+#pragma unroll
+        for(int e = 0; e < 4; ++e)
+            out[e] = (T)(GATED ? i8_silu<T>(d[0][e]) * d[PER - 1][e] : d[0][e]);
+        if(n + 4 <= p.N)
+            reinterpret_cast<AnyAlign<tx4>*>(c)->v = out;
+        else
+#pragma unroll
+            for(int e = 0; e < 3; ++e)
+                if(n + e < p.N)
+                    c[e] = out[e];
     }
 }
 
@@ -111,11 +422,133 @@ int64_t most_tiles_m(const GemmI8Args& a, int BM)
     return a.offsets ? a.M / BM + (a.experts < a.M ? a.experts : a.M) : ((int64_t)a.M + BM - 1) / BM;
 }
 
+void cut(GemmI8Args& a, int BM, int cols)
+{
+    a.tiles_m = (int)most_tiles_m(a, BM), a.tiles_n = (a.N + cols - 1) / cols;
+}
+template <typename T, bool GATED, int BM, int BN, int WM, int WN, int NST>
+hipError_t launch_tiles(GemmI8Args& a, hipStream_t s)
+{
+    cut(a, BM, GATED ? BN / 2 : BN);
+    hipLaunchKernelGGL((gemm_i8_tile_kernel<T, GATED, BM, BN, WM, WN, NST>), dim3((unsigned)a.tiles_m * (unsigned)a.tiles_n * (unsigned)a.ksplit),
+                       dim3(WM * WN * 64), 0, s, a);
+    hipError_t e = hipGetLastError();
+    if(e != hipSuccess || a.ksplit == 1)
+        return e;
+    const int quads = (a.N + 3) / 4;
+    hipLaunchKernelGGL((gemm_i8_join_kernel<T, GATED>), dim3((unsigned)(((int64_t)a.M * quads + 255) / 256)), dim3(256), 0, s, a, quads);
+    return hipGetLastError();
+}
+template <typename T, bool GATED, int MT, int NT, int NW>
+hipError_t launch_direct(GemmI8Args& a, hipStream_t s)
+{
+    cut(a, MT * 16, NT * 16 / (GATED ? 2 : 1));
+    hipLaunchKernelGGL((gemm_i8_direct_kernel<T, GATED, MT, NT, NW>), dim3((unsigned)a.tiles_m * (unsigned)a.tiles_n), dim3(NW * 64), 0, s, a);
+    return hipGetLastError();
+}
+
+// Which kernel, and into how many runs K is cut. us of a step (a K tile) that one CU's tiles take, as measured (rows x 4096 x 4096):
+//   64 x 128, four stages    0.43, all CUs busy 0.50         128 rows 17.7 (in four runs 14.9), 512: 20.1
+//   128 x 128, two stages    0.52 to 0.65, two a CU 0.98     512: 22.3, 1024: 24.5, 2048: 34.8 (64 x 128: 36.2, 70.9; 256 x 256: 38.7, 39.7)
+//   256 x 256, four waves    1.05, all CUs busy 1.47         4096: 51.6 (128 x 128 66.3), 4096 x 11008: 145 (213)
+// and about 4 us around the steps. A run costs 3 us more and its sums' way to the workspace and back.
+// Up to 16 rows the direct kernel of one row tile, 11008 x 4096: 1 row 10.4, 16 rows 13.6 (64 x 128 tiles in two runs 14.7); 8 waves where K is
+// long (4096 x 11008: 9.9 where four take 10.7). To 64 rows the direct kernel of two row tiles where its workgroups find a CU each, 4096 x 4096
+// 10.6 us for 32 rows (11.8 in the best runs of tiles), 11008 x 4096 18 (15.6).
+// Experts: by the rows that each has on average, since the host knows no more. Few: the direct kernel reads each expert's matrix once
+// (64 experts of 2816 x 4096 gated, 4 rows each: 129 us, 128 x 128 tiles 153; 8 rows: 152, 153); many: 256 x 256 tiles (128 rows: 209, 227;
+// 64 rows: 174, 194). K moves both borders: what a tile's beginning and end take, and what a workgroup reads again, weigh less beside a long one.
+struct Plan
+{
+    int kind; // below
+    int ksplit, per;
+};
+enum
+{
+    kAny     = 0,
+    kDirect1 = 1, // 16 x 16, four waves
+    kDirect8 = 2, // the same, eight waves
+    kDirect2 = 3, // 32 x 32
+    kTile64  = 4, // 64 x 128
+    kTile128 = 5, // 128 x 128
+    kTile256 = 6  // 256 x 256
+};
+
+// whether the kernels of 16-byte vectors take a call: K, strides and addresses in whole vectors, and what a tile may read within 32-bit
+// offsets (rows that are gathered from all of A, the halves of a gated B)
+bool whole_vectors(const GemmI8Args& a)
+{
+    constexpr int64_t kMost = 0x7fff0000;
+    const uint64_t odd      = reinterpret_cast<uintptr_t>(a.a) | reinterpret_cast<uintptr_t>(a.b) | (uint64_t)a.K | (uint64_t)(a.rows_a > 1 ? a.lda : 0) |
+                         (uint64_t)((int64_t)a.N * (a.gated ? 2 : 1) > 1 ? a.ldb : 0) | (uint64_t)(a.experts > 1 ? a.batch_b : 0);
+    const int64_t rows_a = a.rows ? a.rows_a : a.rows_a < 256 ? a.rows_a : 256, rows_b = a.gated ? 2 * (int64_t)a.N : a.N < 256 ? a.N : 256;
+    return a.K > 0 && (odd & 15) == 0 && rows_a * a.lda <= kMost && rows_b * a.ldb <= kMost && a.K <= kMost;
+}
+
+Plan plan(const GemmI8Args& a, int64_t workspace_bytes)
+{
+    const int steps = (int)(((int64_t)a.K + 127) / 128);
+    if(!whole_vectors(a))
+        return Plan{kAny, 1, steps};
+    if(a.offsets)
+    {
+        const double rows = (double)a.M / a.experts;
+        return Plan{rows * 1024 <= a.K ? kDirect1 : rows * a.K >= 1 << 18 ? kTile256 : kTile128, 1, steps};
+    }
+    if(a.M <= 16)
+        return Plan{a.K > 8192 ? kDirect8 : kDirect1, 1, steps};
+    const int64_t wide = (int64_t)a.N * (a.gated ? 2 : 1);
+    auto tiles         = [&](int bm, int bn) { return ((int64_t)a.M + bm - 1) / bm * ((wide + bn - 1) / bn); };
+    auto rounds        = [](int64_t n) { return (double)((n + 255) / 256); };
+    const int64_t big  = tiles(256, 256);
+    const double share = (double)big / (256 * rounds(big));
+    Plan best{kTile256, 1, steps};
+    double us    = 2 + rounds(big) * (2 + steps * (1.05 + 0.42 * share * share));
+    auto compare = [&](double t, const Plan& p) {
+        if(t < us)
+            us = t, best = p;
+    };
+    if(a.M <= 64)
+    {
+        const double n = rounds(tiles(32, 32));
+        compare(3.4 + steps * 0.2 * n * (n > 1 ? 1.13 : 1.0), Plan{kDirect2, 1, steps});
+    }
+    for(int ks = 1; ks <= 16 && ks * 2 <= (steps > 1 ? steps : 2); ++ks)
+    {
+        const int per     = (steps + ks - 1) / ks, runs = (steps + per - 1) / per;
+        const double sums = runs > 1 ? 4.0 * a.M * wide * runs : 0.0, join = runs > 1 ? 3 + 2 * sums / 4e6 : 0.0;
+        if(sums > (double)workspace_bytes)
+            continue;
+        const int64_t n64 = tiles(64, 128) * runs, n128 = tiles(128, 128) * runs, rest = n128 % 512;
+        compare(3.5 + join + per * (n64 < 256 ? 0.43 + 0.07 * (double)n64 / 256 : 0.50) * rounds(n64), Plan{kTile64, runs, per});
+        compare(3.5 + join + per * (0.98 * (double)(n128 / 512) + (rest == 0 ? 0.0 : rest > 256 ? 0.98 : 0.52 + 0.13 * (double)rest / 256)),
+                Plan{kTile128, runs, per});
+    }
+    return best;
+}
+
+template <typename T>
+constexpr int type_of()
+{
+    return sizeof(T) == 4 ? CKX_TYPE_F32 : std::is_same<T, _Float16>::value ? CKX_TYPE_F16 : CKX_TYPE_BF16;
+}
+
 template <typename T, bool GATED>
 hipError_t launch(GemmI8Args& a, int64_t workspace_bytes, hipStream_t s)
 {
-    constexpr int COLS = GATED ? 64 : 128;
-    a.tiles_m = (int)most_tiles_m(a, 128), a.tiles_n = (a.N + COLS - 1) / COLS;
+    const Plan w = plan(a, workspace_bytes);
+    a.ksplit = w.ksplit, a.per = w.per;
+    switch(w.kind)
+    {
+    case kDirect1: return launch_direct<T, GATED, 1, GATED ? 2 : 1, 4>(a, s);
+    case kDirect8: return launch_direct<T, GATED, 1, GATED ? 2 : 1, 8>(a, s);
+    case kDirect2: return launch_direct<T, GATED, 2, 2, 8>(a, s);
+    case kTile64: return launch_tiles<T, GATED, 64, 128, 2, 2, 4>(a, s);
+    case kTile128: return launch_tiles<T, GATED, 128, 128, 4, 2, 2>(a, s);
+    case kTile256: return gemm_i8_big_launch(a, type_of<T>(), most_tiles_m(a, 256), s);
+    default: break;
+    }
+    cut(a, 128, GATED ? 64 : 128);
     hipLaunchKernelGGL((gemm_i8_any_kernel<T, GATED>), dim3((unsigned)a.tiles_m * (unsigned)a.tiles_n), dim3(256), 0, s, a);
     return hipGetLastError();
 }
@@ -128,17 +561,32 @@ hipError_t launch_form(GemmI8Args& a, int64_t workspace_bytes, hipStream_t s)
 
 } // namespace
 
+// a launch has fewer than 2^32 threads, 512 a workgroup at most: one for 64 x 128 outputs, for 16 rows and 8 columns of few rows
 bool gemm_i8_scaled_fits(int M, int N, int gated, int experts)
 {
     GemmI8Args a{};
     a.M = M, a.experts = experts;
-    const int most  = 0; // (offsets alone say that there are experts)
-    a.offsets       = experts ? &most : nullptr;
-    const int cols  = gated ? 64 : 128;
-    return most_tiles_m(a, 128) * (((int64_t)N + cols - 1) / cols) < (1ll << 32) / 512;
+    const int none     = 0;
+    a.offsets          = experts ? &none : nullptr; // (says that there are experts)
+    const bool few     = experts || M <= 64;
+    const int64_t wide = (int64_t)N * (gated ? 2 : 1);
+    return most_tiles_m(a, few ? 16 : 64) * (wide / (few ? 16 : 128) + 2) < (1ll << 32) / 512;
 }
 
-int64_t gemm_i8_scaled_workspace(int, int, int, int) { return 0; }
+int64_t gemm_i8_scaled_workspace(int M, int N, int K, int gated)
+{
+    GemmI8Args a{};
+    a.M = a.rows_a = M, a.N = N, a.K = (K + 15) / 16 * 16, a.gated = gated, a.lda = a.ldb = a.K;
+    const Plan w = plan(a, INT64_MAX);
+    return w.ksplit > 1 ? 4ll * M * N * (gated ? 2 : 1) * w.ksplit : 0;
+}
+
+void gemm_i8_scaled_plan(const GemmI8Args& a, int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs)
+{
+    constexpr int m[] = {128, 16, 16, 32, 64, 128, 256}, n[] = {128, 16, 16, 32, 128, 128, 256};
+    const Plan w      = plan(a, workspace_bytes);
+    *tile_m = m[w.kind], *tile_n = n[w.kind] * (a.gated && w.kind <= kDirect8 && w.kind != kAny ? 2 : 1), *k_runs = w.kind == kAny ? 0 : w.ksplit;
+}
 
 hipError_t gemm_i8_scaled_launch(GemmI8Args a, int c_type, int64_t workspace_bytes, hipStream_t s)
 {

@@ -101,18 +101,32 @@ __device__ __forceinline__ bool i8_find_tile(const GemmI8Args& p, int block, int
     t.expert = 0, t.m0 = tm * BM, t.rows = min(BM, p.M - t.m0);
     return true;
 }
-// row of A that row m of C takes; -1: none, a row of zeros
-__device__ __forceinline__ int i8_row_of_a(const GemmI8Args& p, int m)
+// rows of A that rows r[...] of a tile take; -1: none (behind the tile's last, or a row of zeros). The numbers are asked for all at once.
+template <int N>
+__device__ __forceinline__ void i8_rows_of_a(const GemmI8Args& p, const I8Tile& t, const int (&r)[N], int (&m)[N])
 {
-    if(!p.offsets)
-        return m;
-    int r = m;
+#pragma unroll
+    for(int j = 0; j < N; ++j)
+        m[j] = t.m0 + min(r[j], t.rows - 1);
     if(p.rows)
     {
-        r = p.rows[m];
-        r = r < 0 ? -1 : (int)((uint32_t)r / (uint32_t)p.rows_per);
+#pragma unroll
+        for(int j = 0; j < N; ++j)
+            m[j] = p.rows[m[j]];
+#pragma unroll
+        for(int j = 0; j < N; ++j)
+            m[j] = m[j] < 0 ? -1 : (int)((uint32_t)m[j] / (uint32_t)p.rows_per);
     }
-    return r < p.rows_a ? r : -1;
+#pragma unroll
+    for(int j = 0; j < N; ++j)
+        m[j] = r[j] < t.rows && m[j] < p.rows_a ? m[j] : -1;
+}
+__device__ __forceinline__ int i8_row_of_a(const GemmI8Args& p, const I8Tile& t, int r)
+{
+    const int one[1] = {r};
+    int m[1];
+    i8_rows_of_a(p, t, one, m);
+    return m[0];
 }
 
 // x / (1 + exp(-x)): 16-bit outputs take the fast exponential and reciprocal, whose errors (a few 2^-24 of the value for |x| under 80)

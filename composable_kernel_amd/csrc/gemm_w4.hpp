@@ -29,15 +29,23 @@ namespace ckx {
 // like the FUSED variants of the tile kernel.
 // EPI (int8, plain epilogues): the requant form as a compile-time constant, so that the last K tile's loop, which stores
 // finished fragment rows between its MFMAs, carries no branch on it.
-template <int DT, bool FUSED = false, int EPI = EPI_PASSTHROUGH>
+// EXT (int8): where the tiles, the rows of A and B and the epilogue come from something else than a GemmArgs (gemm_i8_big.hip); GemmArgs
+// then gives K alone, the operands and their row strides.
+struct W4Plain
+{
+    static constexpr bool kExt = false;
+    static constexpr int kBytes = 0;
+};
+template <int DT, bool FUSED = false, int EPI = EPI_PASSTHROUGH, typename EXT = W4Plain>
 struct GemmW4
 {
     static_assert(!FUSED || DT == DT_F16, "D-operand epilogues: fp16");
+    static_assert(!EXT::kExt || (DT == DT_I8 && !FUSED && EPI == EPI_PASSTHROUGH), "");
     static_assert(EPI == EPI_PASSTHROUGH || (DT == DT_I8 && (EPI == EPI_REQUANT_CK || EPI == EPI_REQUANT_RND)), "");
     static constexpr int BM = 256, BN = 256, BKB = 128, NW = 4, NT = NW * 64, NST = 2;
     static constexpr int ES     = DT == DT_I8 ? 1 : 2;
     static constexpr int A_TILE = BM * BKB, B_TILE = BN * BKB, STAGE = A_TILE + B_TILE;
-    static constexpr int LUT    = DT == DT_I8 ? 256 : 0;
+    static constexpr int LUT    = EXT::kExt ? EXT::kBytes : DT == DT_I8 ? 256 : 0;
     static constexpr int LDS    = NST * STAGE + LUT;
     static constexpr int MT = 8, NB = 8;  // A fragments (16 rows each) and B fragments (16 columns each) of a wave per k-step
     static constexpr int NLA = 8, NLB = 8, LPT = NLA + NLB; // 16-byte direct loads per thread and K tile
@@ -166,7 +174,7 @@ struct GemmW4
     // interleave the two stores' 16-byte pieces.
     __device__ static __forceinline__ uint32_t row_to_col(uint32_t r)
     {
-        if constexpr(DT == DT_I8)
+        if constexpr(DT == DT_I8 && !EXT::kExt)
             return b_row_to_col(r);
         else
         {
@@ -201,7 +209,7 @@ struct GemmW4
         store_room<1>(crow + n0, pk, N - n0, nt);
     }
 
-    __device__ static __forceinline__ void run(const GemmArgs& p, uint8_t* smem)
+    __device__ static __forceinline__ void run(const GemmArgs& p, uint8_t* smem, EXT ext = EXT{})
     {
         const int tid  = threadIdx.x;
         const int lane = tid & 63;
@@ -215,10 +223,12 @@ struct GemmW4
         // all zeros if need be)
         const int nk = nk_real > (FUSED ? 0 : 1) ? nk_real : (FUSED ? 1 : 2);
 
-        const __amdgpu_buffer_rsrc_t rsrc_a =
-            make_rsrc(reinterpret_cast<const uint8_t*>(p.a) - kImmBias, p.a_bytes + (uint32_t)kImmBias);
-        const __amdgpu_buffer_rsrc_t rsrc_b =
-            make_rsrc(reinterpret_cast<const uint8_t*>(p.b) - kImmBias, p.b_bytes + (uint32_t)kImmBias);
+        __amdgpu_buffer_rsrc_t rsrc_a, rsrc_b; // (EXT: of each tile)
+        if constexpr(!EXT::kExt)
+        {
+            rsrc_a = make_rsrc(reinterpret_cast<const uint8_t*>(p.a) - kImmBias, p.a_bytes + (uint32_t)kImmBias);
+            rsrc_b = make_rsrc(reinterpret_cast<const uint8_t*>(p.b) - kImmBias, p.b_bytes + (uint32_t)kImmBias);
+        }
         const uint32_t smem_lds = (uint32_t)(uintptr_t)(lds_ptr_t)smem;
         if constexpr(DT == DT_I8 && EPI == EPI_REQUANT_RND) // (visible to every wave after the first barrier of the K loop)
             requant_lut_fill(smem + NST * STAGE, p.scale_relu, tid, NT);
@@ -238,13 +248,38 @@ struct GemmW4
 
         const bool nt     = p.nt_store != 0;
 
-        for(int unit = (int)blockIdx.x; unit < ntiles; unit += (int)gridDim.x)
+        for(int unit = (int)blockIdx.x; EXT::kExt || unit < ntiles; unit += (int)gridDim.x)
         {
-            int tm, tn, bi;
-            tile_of_block(unit, p.tiles_m, p.tiles_n, nbatch, bi, tm, tn);
+            int tm = 0, tn = 0, bi = 0;
+            if constexpr(EXT::kExt)
+            {
+                if(!ext.find(unit))
+                    return;
+                rsrc_a = make_rsrc(ext.a() - kImmBias, ext.a_bytes() + (uint32_t)kImmBias);
+                rsrc_b = make_rsrc(ext.b() - kImmBias, ext.b_bytes() + (uint32_t)kImmBias);
+            }
+            else
+                tile_of_block(unit, p.tiles_m, p.tiles_n, nbatch, bi, tm, tn);
             const uint32_t a_batch = (uint32_t)((long)bi * p.bsa * ES), b_batch = (uint32_t)((long)bi * p.bsb * ES);
             uint8_t* const c_batch = reinterpret_cast<uint8_t*>(p.c) + (size_t)bi * p.bsc * ES;
             uint32_t a_off[NLA], b_off[NLB];
+            if constexpr(EXT::kExt)
+            {
+                int rows[NLA], at[NLA];
+#pragma unroll
+                for(int j = 0; j < NLA; ++j)
+                    rows[j] = (wave * NLA + j) * 8 + (lane >> 3);
+                ext.rows_of_a(rows, at);
+#pragma unroll
+                for(int j = 0; j < NLA; ++j)
+                {
+                    const uint32_t bias = kb + (uint32_t)(kImmBias - (j & 3) * 1024);
+                    const int b         = ext.row_of_b((uint32_t)rows[j]);
+                    a_off[j]            = at[j] >= 0 ? (uint32_t)at[j] + bias : kOutOfRange;
+                    b_off[j]            = b >= 0 ? (uint32_t)b + bias : kOutOfRange;
+                }
+            }
+            else
 #pragma unroll
             for(int j = 0; j < NLA; ++j)
             {
@@ -281,6 +316,8 @@ struct GemmW4
             // ordered against loads: drained here, so that the counted wait below sees loads only.
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __builtin_amdgcn_s_barrier();
+            if constexpr(EXT::kExt)
+                ext.ask(tid);
             static_for<NST>([&](auto st_c) {
                 const uint32_t oob = k_oob_of(decltype(st_c)::value);
                 static_for<LPT>([&](auto s_c) {
@@ -291,6 +328,8 @@ struct GemmW4
                     load_slot(s_c, std::true_type{}, (uint32_t)decltype(st_c)::value * BKB, oob);
                 });
             });
+            if constexpr(EXT::kExt)
+                ext.fill(smem + NST * STAGE, tid); // (read behind the K loop's barriers)
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LPT) : "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
@@ -413,6 +452,19 @@ struct GemmW4
                 const int m     = tm * BM + wm * 128 + 16 * i + (lane & 15);
                 const int nb    = tn * BN + wn * 128 + 16 * (lane >> 4); // first column of group 0; group 1 is 64 further
                 using in_vgpr   = std::integral_constant<bool, (i == MT - 1)>;
+                if constexpr(EXT::kExt)
+                {
+#pragma unroll
+                    for(int g = (G < 0 ? 0 : G); g < (G < 0 ? 2 : G + 1); ++g)
+                    {
+                        if constexpr(G < 0)
+                            ext.fetch(smem + NST * STAGE, i, g, wm, wn, lane);
+                        acc_t v[4];
+                        fetch_acc(in_vgpr{}, acc[i], g, v);
+                        ext.store(i, g, wm, wn, lane, v);
+                    }
+                    return;
+                }
                 if constexpr(DT == DT_I8 && EPI == EPI_REQUANT_RND)
                 {
                     // the values go through the table behind ONE wait per call (both column groups where the caller
@@ -612,9 +664,13 @@ struct GemmW4
                 // inline-assembly MFMAs are invisible to the compiler's hazard handling)
                 static_for<MT - 2>([&](auto r_c) {
                     using fi_c = integral_constant<int, decltype(r_c)::value + 2>;
+                    if constexpr(EXT::kExt) // (the scales of a store are read in front of the MFMAs before it)
+                        ext.fetch(smem + NST * STAGE, decltype(r_c)::value, 0, wm, wn, lane);
                     row_mfmas(fi_c{}, integral_constant<int, 0>{}, integral_constant<int, 0>{});
                     __builtin_amdgcn_sched_barrier(0);
                     store_row(r_c, integral_constant<int, 0>{});
+                    if constexpr(EXT::kExt)
+                        ext.fetch(smem + NST * STAGE, decltype(r_c)::value, 1, wm, wn, lane);
                     __builtin_amdgcn_sched_barrier(0);
                     row_mfmas(fi_c{}, integral_constant<int, 0>{}, integral_constant<int, 1>{});
                     row_mfmas(fi_c{}, integral_constant<int, 1>{}, integral_constant<int, 0>{});
