@@ -7,6 +7,30 @@ namespace ckx {
 
 namespace {
 
+constexpr int kBatch = 8; // rows that are under way together
+
+// numbers that are the same for all lanes, through the scalar cache
+template <typename T>
+using Uniform = const __attribute__((address_space(4))) T*;
+
+template <typename T>
+struct Eight // consecutive elements, as they lie in memory
+{
+    u32x4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p)
+    {
+#pragma unroll
+        for(int i = 0; i < (int)(sizeof(T) / 2); ++i)
+            w[i] = load_vec<u32x4>(p + i * (16 / (int)sizeof(T)));
+    }
+    __device__ __forceinline__ float operator[](int i) const
+    {
+        typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+        constexpr int PER = 16 / (int)sizeof(T);
+        return (float)__builtin_bit_cast(vec, w[i / PER])[i % PER];
+    }
+};
+
 template <typename T>
 __global__ __launch_bounds__(256) void experts_combine_kernel(CombineArgs p, int col_tiles, int64_t tiles)
 {
@@ -14,45 +38,65 @@ __global__ __launch_bounds__(256) void experts_combine_kernel(CombineArgs p, int
     {
         const int64_t t = tile / col_tiles;
         const int64_t n = ((tile - t * col_tiles) * 256 + threadIdx.x) * 8;
-        if(n >= p.N)
-            continue;
-        const bool whole = n + 8 <= p.N;
-        auto load = [&](const T* row, float(&v)[8]) {
-            if(whole)
-                load8(row + n, v);
-            else
+        const Uniform<int> places    = (Uniform<int>)(p.places + t * p.top_k);
+        const Uniform<float> weights = (Uniform<float>)(p.weights + t * p.top_k);
+        const T* const y             = reinterpret_cast<const T*>(p.y) + n;
+        const T* const add           = reinterpret_cast<const T*>(p.add) + t * p.sadd + n;
+        T* const out                 = reinterpret_cast<T*>(p.out) + t * p.sout + n;
+        if(n + 8 <= p.N)
+        {
+            float sum[8] = {};
+            Eight<T> a;
+            if(p.add)
+                a.load(add);
+            for(int j0 = 0; j0 < p.top_k; j0 += kBatch)
+            {
+                // the rows of a batch are all asked for before the first is used
+                Eight<T> v[kBatch];
+                int row[kBatch];
+                float w[kBatch];
+#pragma unroll
+                for(int j = 0; j < kBatch; ++j)
+                {
+                    const int at = j0 + j < p.top_k ? j0 + j : j0;
+                    row[j]       = j0 + j < p.top_k ? places[at] : -1;
+                    w[j]         = weights[at];
+                }
+#pragma unroll
+                for(int j = 0; j < kBatch; ++j)
+                    if((unsigned)row[j] < (unsigned)p.rows)
+                        v[j].load(y + (int64_t)row[j] * p.sy);
+                if(j0 == 0 && p.add)
+#pragma unroll
+                    for(int i = 0; i < 8; ++i)
+                        sum[i] = a[i];
+#pragma unroll
+                for(int j = 0; j < kBatch; ++j)
+                    if((unsigned)row[j] < (unsigned)p.rows)
+#pragma unroll
+                        for(int i = 0; i < 8; ++i)
+                            sum[i] = __builtin_fmaf(w[j], v[j][i], sum[i]);
+            }
+            if(p.top_k == 0 && p.add)
 #pragma unroll
                 for(int i = 0; i < 8; ++i)
-                    v[i] = n + i < p.N ? (float)row[n + i] : 0.0f;
-        };
-        float sum[8] = {};
-        if(p.add)
-            load(reinterpret_cast<const T*>(p.add) + t * p.sadd, sum);
-        for(int j = 0; j < p.top_k; ++j)
-        {
-            const int row = p.places[t * p.top_k + j];
-            if((unsigned)row >= (unsigned)p.rows)
-                continue;
-            const float w = p.weights[t * p.top_k + j];
-            float v[8];
-            load(reinterpret_cast<const T*>(p.y) + (int64_t)row * p.sy, v);
+                    sum[i] = a[i];
+            typedef T tx8 __attribute__((ext_vector_type(8)));
+            tx8 o;
 #pragma unroll
             for(int i = 0; i < 8; ++i)
-                sum[i] = __builtin_fmaf(w, v[i], sum[i]);
-        }
-        T* const out = reinterpret_cast<T*>(p.out) + t * p.sout + n;
-        typedef T tx8 __attribute__((ext_vector_type(8)));
-        tx8 o;
-#pragma unroll
-        for(int i = 0; i < 8; ++i)
-            o[i] = (T)sum[i];
-        if(whole)
+                o[i] = (T)sum[i];
             reinterpret_cast<AnyAlign<tx8>*>(out)->v = o;
+        }
         else
-#pragma unroll
-            for(int i = 0; i < 7; ++i)
-                if(n + i < p.N)
-                    out[i] = o[i];
+            for(int i = 0; n + i < p.N; ++i) // the row's end, one thread
+            {
+                float sum = p.add ? (float)add[i] : 0.0f;
+                for(int j = 0; j < p.top_k; ++j)
+                    if((unsigned)places[j] < (unsigned)p.rows)
+                        sum = __builtin_fmaf(weights[j], (float)y[(int64_t)places[j] * p.sy + i], sum);
+                out[i] = (T)sum;
+            }
     }
 }
 

@@ -252,31 +252,37 @@ __device__ __forceinline__ double row_sum(double v)
     return v + row_dpp<0x121>(v);
 }
 
-// exp(x) for |x| <= 600: 2^n times the series of exp over half a step to either side of zero, whose term behind the last kept is under
-// 2^-52 of the sum. A third of the library function's instructions, which has the ends of the range to look after.
-__device__ __forceinline__ double exp_near(double x)
+// x[i] = exp(x[i]) in 64 bits: 2^n times the series of exp over half a step to either side of zero, whose term behind the last kept is
+// under 2^-52 of the sum. Coefficient by coefficient over all of them, so that each is in a register once and no sum waits for the last;
+// the library's function takes three times the instructions, one value after the other.
+template <int N>
+__device__ __forceinline__ void exp_all(double (&x)[N])
 {
-    const double n = __builtin_rint(x * 1.4426950408889634074);
-    double r       = __builtin_fma(-n, 6.93147180369123816490e-01, x); // (ln 2 in two parts)
-    r              = __builtin_fma(-n, 1.90821492927058770002e-10, r);
-    double y       = 1.0 / 6227020800.0;
-    y              = __builtin_fma(y, r, 1.0 / 479001600.0);
-    y              = __builtin_fma(y, r, 1.0 / 39916800.0);
-    y              = __builtin_fma(y, r, 1.0 / 3628800.0);
-    y              = __builtin_fma(y, r, 1.0 / 362880.0);
-    y              = __builtin_fma(y, r, 1.0 / 40320.0);
-    y              = __builtin_fma(y, r, 1.0 / 5040.0);
-    y              = __builtin_fma(y, r, 1.0 / 720.0);
-    y              = __builtin_fma(y, r, 1.0 / 120.0);
-    y              = __builtin_fma(y, r, 1.0 / 24.0);
-    y              = __builtin_fma(y, r, 1.0 / 6.0);
-    y              = __builtin_fma(y, r, 0.5);
-    y              = __builtin_fma(y, r, 1.0);
-    y              = __builtin_fma(y, r, 1.0);
-    return __builtin_ldexp(y, (int)n);
+    constexpr double c[] = {1.0 / 479001600.0, 1.0 / 39916800.0, 1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0, 1.0 / 720.0,
+                            1.0 / 120.0,       1.0 / 24.0,       1.0 / 6.0,       0.5,            1.0,           1.0};
+    double y[N];
+    int n[N];
+#pragma unroll
+    for(int i = 0; i < N; ++i)
+    {
+        x[i]           = __builtin_fmin(__builtin_fmax(x[i], -745.2), 709.78); // (exp of less is 0; of more: the callers look)
+        const double m = __builtin_rint(x[i] * 1.4426950408889634074);
+        x[i]           = __builtin_fma(-m, 6.93147180369123816490e-01, x[i]); // (ln 2 in two parts)
+        x[i]           = __builtin_fma(-m, 1.90821492927058770002e-10, x[i]);
+        n[i]           = (int)m;
+        y[i]           = 1.0 / 6227020800.0;
+    }
+#pragma unroll
+    for(int k = 0; k < 13; ++k)
+#pragma unroll
+        for(int i = 0; i < N; ++i)
+            y[i] = __builtin_fma(y[i], x[i], c[k]);
+#pragma unroll
+    for(int i = 0; i < N; ++i)
+        x[i] = __builtin_ldexp(y[i], n[i]);
 }
-// 1 / x for 1 <= x < 2^900: two of Newton's steps from the instruction's estimate
-__device__ __forceinline__ double reciprocal_near(double x)
+// 1 / x for x >= 1: two of Newton's steps from the instruction's estimate
+__device__ __forceinline__ double reciprocal(double x)
 {
     double y = __builtin_amdgcn_rcp(x);
     y        = __builtin_fma(__builtin_fma(-x, y, 1.0), y, y);
@@ -316,40 +322,46 @@ __device__ __forceinline__ void route_tokens(const RouteArgs& p, int64_t t, bool
     float x[EPL];
     load_logits(row, first, p.experts, x);
     auto there = [&](int i) { return x[i] > -__builtin_inff(); };
-    float most = -__builtin_inff(), least = 0.0f;
+    float most = -__builtin_inff();
 #pragma unroll
     for(int i = 0; i < EPL; ++i)
     {
-        x[i]  = live && x[i] > -__builtin_inff() && bias[i] > -__builtin_inff() ? __builtin_fminf(x[i], kLargest) : -__builtin_inff(); // (a NaN is out)
-        most  = __builtin_fmaxf(most, x[i]);
-        least = __builtin_fminf(least, there(i) ? x[i] : 0.0f);
+        x[i] = __builtin_fminf(live && there(i) && bias[i] > -__builtin_inff() ? x[i] : -__builtin_inff(), kLargest); // (a NaN is out)
+        most = __builtin_fmaxf(most, x[i]);
     }
     const float x_max = row_most(most);
-    V value[EPL];          // by which experts are ordered
-    double score[EPL];     // ALL: s, or s + bias
+    V value[EPL];      // by which experts are ordered
+    double score[EPL]; // ALL: s, or s + bias
     double total = 1.0;
     if constexpr(ALL)
     {
-        // (differences of 600 and more go to the library's functions)
-        const bool near = p.sigmoid ? __builtin_fmaxf(most, -least) <= 600.0f : least >= x_max - 600.0f && x_max <= 600.0f && x_max >= -600.0f;
-        const bool fast = __ballot(near || !live || x_max == -__builtin_inff()) == ~0ull;
-        double sum      = 0.0;
+        // (-infinity, which is out, goes the way of a number: to 0 or behind its own check)
+        const double at = p.sigmoid ? 0.0 : (double)__builtin_fmaxf(x_max, -kLargest), sign = p.sigmoid ? -1.0 : 1.0;
 #pragma unroll
         for(int i = 0; i < EPL; ++i)
+            score[i] = sign * (double)__builtin_fmaxf(x[i], -kLargest) - at;
+        exp_all(score);
+        if(p.sigmoid)
         {
-            const double a = !there(i) ? 0.0 : p.sigmoid ? -(double)x[i] : (double)x[i] - (double)x_max;
-            double d       = fast ? exp_near(a) : exp(a);
-            d              = there(i) ? d : 0.0;
-            score[i]       = p.sigmoid ? (fast ? reciprocal_near(1.0 + d) : 1.0 / (1.0 + d)) : d;
-            sum += d;
-        }
-        if(!p.sigmoid)
-        {
-            total = row_sum(sum);
-            total = total > 0.0 ? total : 1.0;
 #pragma unroll
             for(int i = 0; i < EPL; ++i)
-                score[i] /= total;
+                score[i] = x[i] < -709.78f ? 0.0 : reciprocal(1.0 + score[i]); // (the exponential is past the range)
+        }
+        else
+        {
+            double sum = 0.0;
+#pragma unroll
+            for(int i = 0; i < EPL; ++i)
+            {
+                score[i] = there(i) ? score[i] : 0.0;
+                sum += score[i];
+            }
+            total            = row_sum(sum);
+            total            = total > 0.0 ? total : 1.0;
+            const double one = reciprocal(total); // (at least 1, the largest's own)
+#pragma unroll
+            for(int i = 0; i < EPL; ++i)
+                score[i] *= one;
         }
     }
 #pragma unroll
@@ -552,13 +564,14 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs p)
     const int64_t last  = first + p.chunk_tokens < p.tokens ? first + p.chunk_tokens : p.tokens;
     const int live      = p.live ? max(0, min(*p.live, p.tokens)) : p.tokens;
     double* const values = reinterpret_cast<double*>(ckx_route_lds) + wave * p.experts;
-    float bias[EPL];
+    float bias[EPL] = {};
     int group[EPL];
+    if constexpr(WIDE)
+        load_logits(p.bias, lane * EPL, p.experts, bias);
 #pragma unroll
     for(int i = 0; i < EPL; ++i)
     {
         const int e = lane * EPL + i;
-        bias[i]     = WIDE && e < p.experts ? p.bias[e] : 0.0f;
         group[i]    = !ROWS && p.groups > 1 && e < p.experts ? e / (p.experts / p.groups) : 0;
     }
     if(p.offsets)
@@ -617,22 +630,34 @@ __global__ __launch_bounds__(kThreads) void route_tables_kernel(RouteArgs p)
     for(int e = threadIdx.x; e < p.experts; e += kThreads)
         mine[e] = totals[e] = 0;
     __syncthreads();
-    // (threads in rows of `wide`, a chunk each)
-    int wide = 64;
-    while(wide < p.experts && wide < kThreads)
+    // (threads in rows of `wide`, a chunk each, four experts a thread)
+    int wide = 16;
+    while(wide * 4 < p.experts)
         wide *= 2;
-    for(int e = threadIdx.x & (wide - 1); e < p.experts; e += wide)
+    const int e0 = (threadIdx.x & (wide - 1)) * 4, per = kThreads / wide;
+    if(e0 < p.experts)
     {
-        int before = 0, all = 0;
+        const int left = p.experts - e0;
+        i32x4 before = {0, 0, 0, 0}, all = {0, 0, 0, 0};
 #pragma unroll 8
-        for(int c = threadIdx.x / wide; c < p.chunks; c += kThreads / wide)
+        for(int c = threadIdx.x / wide; c < p.chunks; c += per)
         {
-            const int n = p.ws[(int64_t)c * p.experts + e];
-            before += c < (int)blockIdx.x ? n : 0;
+            const int* at = p.ws + (int64_t)c * p.experts + e0;
+            i32x4 n       = {0, 0, 0, 0};
+            if(left >= 4)
+                n = load_vec<i32x4>(at);
+            else
+                n = i32x4{at[0], left > 1 ? at[1] : 0, left > 2 ? at[2] : 0, 0};
+            before += c < (int)blockIdx.x ? n : i32x4{0, 0, 0, 0};
             all += n;
         }
-        atomicAdd(&mine[e], before);
-        atomicAdd(&totals[e], all);
+#pragma unroll
+        for(int i = 0; i < 4; ++i)
+            if(i < left)
+            {
+                atomicAdd(&mine[e0 + i], before[i]);
+                atomicAdd(&totals[e0 + i], all[i]);
+            }
     }
     __syncthreads();
     const int all = sums_before(totals, p.experts, parts);
