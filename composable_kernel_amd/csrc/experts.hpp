@@ -17,7 +17,7 @@ struct RouteArgs
     int* ids;
     float* weights;
     int *offsets, *rows, *places; // null: no tables
-    int* ws;                      // [chunks][experts] counts
+    void* ws;                     // [chunks][experts] counts
     int tokens, experts, top_k, groups, top_groups, group_best, stride_x;
     int sigmoid, renormalise;
     float scale;

@@ -129,7 +129,7 @@ int ckx_route_experts(const void* p_logits, const float* p_bias, const int32_t* 
         return api_fail(CKX_INVALID_VALUE, "the workspace must be 16-byte aligned");
     ckx::RouteArgs a{};
     a.x = p_logits, a.bias = p_bias, a.live = p_num_tokens, a.ids = p_ids, a.weights = p_weights;
-    a.offsets = p_offsets, a.rows = p_rows, a.places = p_places, a.ws = static_cast<int*>(p_workspace);
+    a.offsets = p_offsets, a.rows = p_rows, a.places = p_places, a.ws = p_workspace;
     a.tokens = d->num_tokens, a.experts = d->num_experts, a.top_k = d->top_k, a.groups = d->num_groups;
     a.top_groups = d->top_groups, a.group_best = d->group_best, a.stride_x = d->stride_x;
     a.sigmoid = d->scoring == CKX_SCORE_SIGMOID, a.renormalise = d->renormalise, a.scale = d->scale;
