@@ -13,7 +13,8 @@ struct I8Big
 {
     static constexpr bool kExt  = true;
     static constexpr int kTile  = 256, kCols = GATED ? 128 : 256;
-    static constexpr int kBytes = 3 * kTile * 4; // scales of the tile's rows, of its columns, biases
+    static constexpr int kLists = 3 * kTile * 4;              // scales of the tile's rows, of its columns, biases
+    static constexpr int kBytes = kLists + 3 * kMostExperts * 4; // the experts' tiles
     const GemmI8Args& p;
     I8Tile t{};
     int n0 = 0;
@@ -22,12 +23,19 @@ struct I8Big
     const float* s_bias = nullptr;
 
     __device__ __forceinline__ explicit I8Big(const GemmI8Args& args) : p(args) {}
-    __device__ __forceinline__ bool find(int unit)
+    __device__ __forceinline__ void begin(uint8_t* lds) const
     {
-        if(!p.offsets && unit >= p.tiles_m * p.tiles_n)
+        if(!p.offsets)
+            return;
+        i8_list_tiles(p, kTile, reinterpret_cast<uint32_t*>(lds + kLists));
+        __syncthreads();
+    }
+    __device__ __forceinline__ bool find(int unit, const uint8_t* lds)
+    {
+        if(p.offsets ? !i8_listed_tile(p, unit, kTile, reinterpret_cast<const uint32_t*>(lds + kLists), t) : unit >= p.tiles_m * p.tiles_n)
             return false;
-        if(!i8_find_tile(p, unit, kTile, t))
-            return false;
+        if(!p.offsets)
+            i8_find_tile(p, unit, kTile, t);
         n0 = t.tn * kCols;
         return true;
     }

@@ -31,23 +31,29 @@ struct I8Tile
 // The tiles of a launch: a dense product's in the order of tile_of_block; the experts' by the rows that offsets give them now, dealt to
 // the XCDs alike, each expert's tiles next to each other. False: there is no tile for this workgroup. The same for every lane.
 __device__ __forceinline__ int i8_first_row(const GemmI8Args& p, int e) { return min(max(p.offsets[e], 0), p.M); }
-__device__ __forceinline__ bool i8_expert_tile(const GemmI8Args& p, int block, int BM, I8Tile& t)
+// rows and tiles of the lane's expert of e0 ... e0 + 63, and the sum of the tiles up to it, `before` those of the experts before e0
+__device__ __forceinline__ void i8_expert_tiles(const GemmI8Args& p, int e0, int BM, uint32_t before, int& lo, int& n, uint32_t& tiles, uint32_t& upto)
 {
-    const int lane = threadIdx.x & 63;
-    uint32_t all   = 0;
-    for(int e0 = 0; e0 < p.experts; e0 += 64)
+    const int lane = threadIdx.x & 63, e = e0 + lane;
+    lo = n = 0;
+    if(e < p.experts)
     {
-        const int e = e0 + lane;
-        int n       = 0;
-        if(e < p.experts)
-            n = max(i8_first_row(p, e + 1) - i8_first_row(p, e), 0);
-        uint32_t tiles = (uint32_t)(n + BM - 1) / (uint32_t)BM;
-#pragma unroll
-        for(int d = 1; d < 64; d *= 2)
-            tiles += (uint32_t)__shfl_xor((int)tiles, d, 64);
-        all += tiles;
+        lo = i8_first_row(p, e);
+        n  = max(i8_first_row(p, e + 1) - lo, 0);
     }
-    all                 = (uint32_t)__builtin_amdgcn_readfirstlane((int)all);
+    tiles = (uint32_t)(n + BM - 1) / (uint32_t)BM;
+    upto  = tiles;
+#pragma unroll
+    for(int d = 1; d < 64; d *= 2)
+    {
+        const uint32_t o = (uint32_t)__shfl_up((int)upto, d, 64);
+        upto += lane >= d ? o : 0;
+    }
+    upto += before;
+}
+// the tile among `all` of a column of tiles that workgroup `block` takes, and its column
+__device__ __forceinline__ bool i8_place_of(const GemmI8Args& p, int block, uint32_t all, uint32_t& tm, int& tn)
+{
     const uint64_t nall = (uint64_t)all * (uint32_t)p.tiles_n;
     if((uint64_t)(uint32_t)block >= nall)
         return false;
@@ -57,38 +63,74 @@ __device__ __forceinline__ bool i8_expert_tile(const GemmI8Args& p, int block, i
     constexpr uint32_t GM = 4;
     const uint32_t group = id / (GM * (uint32_t)p.tiles_n), first = group * GM, in = id - group * GM * (uint32_t)p.tiles_n;
     const uint32_t size  = min(GM, all - first);
-    uint32_t tm          = first + in % size;
-    t.tn                 = (int)(in / size);
-    uint32_t before      = 0;
+    tm                   = first + in % size;
+    tn                   = (int)(in / size);
+    return true;
+}
+__device__ __forceinline__ bool i8_expert_tile(const GemmI8Args& p, int block, int BM, I8Tile& t)
+{
+    int lo, n;
+    uint32_t tiles, upto, all = 0, tm;
     for(int e0 = 0; e0 < p.experts; e0 += 64)
     {
-        const int e = e0 + lane;
-        int lo = 0, n = 0;
-        if(e < p.experts)
-        {
-            lo = i8_first_row(p, e);
-            n  = max(i8_first_row(p, e + 1) - lo, 0);
-        }
-        const uint32_t tiles = (uint32_t)(n + BM - 1) / (uint32_t)BM;
-        uint32_t upto        = tiles;
-#pragma unroll
-        for(int d = 1; d < 64; d *= 2)
-        {
-            const uint32_t o = (uint32_t)__shfl_up((int)upto, d, 64);
-            upto += lane >= d ? o : 0;
-        }
-        upto += before;
+        i8_expert_tiles(p, e0, BM, all, lo, n, tiles, upto);
+        all = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    }
+    if(!i8_place_of(p, block, all, tm, t.tn))
+        return false;
+    uint32_t before = 0;
+    for(int e0 = 0; e0 < p.experts; e0 += 64)
+    {
+        if(p.experts > 64) // (otherwise they are at hand)
+            i8_expert_tiles(p, e0, BM, before, lo, n, tiles, upto);
         const uint64_t who = __ballot(tm < upto);
         if(who)
         {
             const int w  = (int)__builtin_ctzll(who);
-            const int in_e = ((int)tm - __builtin_amdgcn_readlane((int)(upto - tiles), w)) * BM;
+            const int in = ((int)tm - __builtin_amdgcn_readlane((int)(upto - tiles), w)) * BM;
             t.expert = e0 + w;
-            t.m0     = __builtin_amdgcn_readlane(lo, w) + in_e;
-            t.rows   = min(BM, __builtin_amdgcn_readlane(n, w) - in_e);
+            t.m0     = __builtin_amdgcn_readlane(lo, w) + in;
+            t.rows   = min(BM, __builtin_amdgcn_readlane(n, w) - in);
             return true;
         }
         before = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    }
+    return false; // (not reached)
+}
+// the same for a workgroup that takes one tile after another: the sums, and the experts' first rows and their numbers, in LDS (3 * experts
+// numbers)
+__device__ __forceinline__ void i8_list_tiles(const GemmI8Args& p, int BM, uint32_t* list)
+{
+    const int lane = threadIdx.x & 63;
+    uint32_t all   = 0;
+    for(int e0 = 0; e0 < p.experts; e0 += 64) // (every wave for itself, the same numbers)
+    {
+        int lo, n;
+        uint32_t tiles, upto;
+        i8_expert_tiles(p, e0, BM, all, lo, n, tiles, upto);
+        if(e0 + lane < p.experts)
+            list[e0 + lane] = upto, list[p.experts + e0 + lane] = (uint32_t)lo, list[2 * p.experts + e0 + lane] = (uint32_t)n;
+        all = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    }
+}
+__device__ __forceinline__ bool i8_listed_tile(const GemmI8Args& p, int block, int BM, const uint32_t* list, I8Tile& t)
+{
+    const int lane = threadIdx.x & 63;
+    uint32_t tm;
+    if(!i8_place_of(p, block, (uint32_t)__builtin_amdgcn_readfirstlane((int)list[p.experts - 1]), tm, t.tn))
+        return false;
+    for(int e0 = 0; e0 < p.experts; e0 += 64)
+    {
+        const uint64_t who = __ballot(tm < list[min(e0 + lane, p.experts - 1)]);
+        if(who)
+        {
+            const int e       = min(e0 + (int)__builtin_ctzll(who), p.experts - 1);
+            const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane(e > 0 ? (int)list[e - 1] : 0);
+            const int lo = __builtin_amdgcn_readfirstlane((int)list[p.experts + e]), n = __builtin_amdgcn_readfirstlane((int)list[2 * p.experts + e]);
+            const int in = (int)(tm - at) * BM;
+            t.expert = e, t.m0 = lo + in, t.rows = min(BM, n - in);
+            return true;
+        }
     }
     return false; // (not reached)
 }

@@ -247,13 +247,15 @@ struct GemmW4
         const uint32_t fb[2] = {smem_lds + B_AT(0) + frag_part(wn * 128, 0), smem_lds + B_AT(0) + frag_part(wn * 128, 1)};
 
         const bool nt     = p.nt_store != 0;
+        if constexpr(EXT::kExt)
+            ext.begin(smem + NST * STAGE);
 
         for(int unit = (int)blockIdx.x; EXT::kExt || unit < ntiles; unit += (int)gridDim.x)
         {
             int tm = 0, tn = 0, bi = 0;
             if constexpr(EXT::kExt)
             {
-                if(!ext.find(unit))
+                if(!ext.find(unit, smem + NST * STAGE))
                     return;
                 rsrc_a = make_rsrc(ext.a() - kImmBias, ext.a_bytes() + (uint32_t)kImmBias);
                 rsrc_b = make_rsrc(ext.b() - kImmBias, ext.b_bytes() + (uint32_t)kImmBias);
