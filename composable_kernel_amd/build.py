@@ -102,20 +102,20 @@ W4_AGPRS_FUSED_MAX = 232
 
 
 def w4_register_faults(compiler_output):
-    """(kernel, what) for every gemm_w4_kernel of the resource-usage report that uses scratch memory or another number of
-    AccVGPRs than the source ties."""
+    """(kernel, what) for every kernel on the four-wave body (gemm_w4_kernel, gemm_i8_big_kernel) of the resource-usage report that uses
+    scratch memory or another number of AccVGPRs than the source ties."""
     bad, name = [], None
     for line in compiler_output.splitlines():
         if "Function Name:" in line:
             name = line.split("Function Name:", 1)[1].split("[", 1)[0].strip()
-            name = name if "gemm_w4_kernel" in name else None
+            name = name if "gemm_w4_kernel" in name or "gemm_i8_big_kernel" in name else None
         elif name and "ScratchSize [bytes/lane]:" in line:
             n = int(line.split("ScratchSize [bytes/lane]:", 1)[1].split("[", 1)[0])
             if n:
                 bad.append((name, f"{n} bytes of scratch per lane"))
         elif name and "AGPRs:" in line:
             n = int(line.split("AGPRs:", 1)[1].split("[", 1)[0])
-            fused = "ILi1ELb1E" in name      # <DT_F16, FUSED = true, ...>
+            fused = "gemm_w4_kernelILi1ELb1E" in name      # <DT_F16, FUSED = true, ...>
             if (n != W4_AGPRS and not fused) or (fused and not W4_AGPRS <= n <= W4_AGPRS_FUSED_MAX):
                 bad.append((name, f"{n} AccVGPRs"))
     return bad

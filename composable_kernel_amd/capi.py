@@ -45,8 +45,8 @@ SYMBOLS = [
     "ckx_paged_attention8_is_supported", "ckx_paged_attention8", "ckx_paged_attention8_workspace_bytes",
     "ckx_route_experts_is_supported", "ckx_route_experts", "ckx_route_experts_workspace_bytes",
     "ckx_quantize_tokens_i8_is_supported", "ckx_quantize_tokens_i8",
-    "ckx_gemm_i8_tokenscale_is_supported", "ckx_gemm_i8_tokenscale", "ckx_gemm_i8_tokenscale_workspace_bytes",
-    "ckx_experts_gemm_i8_is_supported", "ckx_experts_gemm_i8", "ckx_experts_combine_is_supported", "ckx_experts_combine",
+    "ckx_gemm_i8_tokenscale_is_supported", "ckx_gemm_i8_tokenscale", "ckx_gemm_i8_tokenscale_workspace_bytes", "ckx_gemm_i8_tokenscale_plan",
+    "ckx_experts_gemm_i8_is_supported", "ckx_experts_gemm_i8", "ckx_experts_gemm_i8_plan", "ckx_experts_combine_is_supported", "ckx_experts_combine",
     "ckx_gemm_plan", "ckx_conv2d_fwd_plan", "ckx_set_forced_k_runs", "ckx_set_big_tile_waves",
 ]
 
@@ -202,6 +202,8 @@ def lib():
     L.ckx_gemm_i8_tokenscale.argtypes = [vp] * 6 + i8 + [vp, i64, vp]
     L.ckx_gemm_i8_tokenscale_workspace_bytes.restype = i64
     L.ckx_gemm_i8_tokenscale_workspace_bytes.argtypes = [i32] * 3 + [C.c_int]
+    L.ckx_gemm_i8_tokenscale_plan.argtypes = i8 + [i64] + [C.POINTER(C.c_int)] * 3
+    L.ckx_experts_gemm_i8_plan.argtypes = [ep, C.c_int] + [C.POINTER(C.c_int)] * 3
     L.ckx_experts_gemm_i8_is_supported.argtypes = [ep]
     L.ckx_experts_gemm_i8.argtypes = [vp] * 8 + [ep, vp]
     ec = [i32] * 7 + [C.c_int]
@@ -253,6 +255,22 @@ def gemm_f8_plan(M, N, K, lda=None, ldb=None, ldc=None, c_type=TYPE_BF16, worksp
     out = [C.c_int(0) for _ in range(3)]
     check(lib().ckx_gemm_f8_blockscale_plan(M, N, K, K if lda is None else lda, K if ldb is None else ldb, N if ldc is None else ldc, c_type,
                                             int(workspace_bytes), *map(C.byref, out)))
+    return tuple(x.value for x in out)
+
+
+def gemm_i8_plan(M, N, K, lda=None, ldb=None, ldc=None, gated=False, c_type=TYPE_BF16, workspace_bytes=0):
+    """(rows of A, rows of B, K runs) of a workgroup of this token-scaled int8 GEMM (ckx_gemm_i8_tokenscale_plan); 0 runs: the kernel for any K
+    and stride."""
+    out = [C.c_int(0) for _ in range(3)]
+    check(lib().ckx_gemm_i8_tokenscale_plan(M, N, K, K if lda is None else lda, K if ldb is None else ldb, N if ldc is None else ldc, int(gated), c_type,
+                                            int(workspace_bytes), *map(C.byref, out)))
+    return tuple(x.value for x in out)
+
+
+def experts_gemm_i8_plan(desc, gathered=True):
+    """As gemm_i8_plan, of the experts' GEMM that an ExpertsDesc describes (ckx_experts_gemm_i8_plan)."""
+    out = [C.c_int(0) for _ in range(3)]
+    check(lib().ckx_experts_gemm_i8_plan(C.byref(desc), int(gathered), *map(C.byref, out)))
     return tuple(x.value for x in out)
 
 

@@ -49,6 +49,14 @@ int check_product(int32_t N, int32_t K, int32_t ldb, int gated, int c_type)
     return CKX_OK;
 }
 
+ckx::GemmI8Args product_of(const ckx_experts_desc& d)
+{
+    ckx::GemmI8Args a{};
+    a.experts = d.num_experts, a.rows_a = d.num_rows_a, a.rows_per = d.rows_per, a.batch_b = d.batch_stride_b;
+    a.M = d.num_rows, a.N = d.N, a.K = d.K, a.lda = d.stride_a, a.ldb = d.stride_b, a.ldc = d.stride_c, a.gated = d.gated;
+    return a;
+}
+
 } // namespace
 
 extern "C" {
@@ -211,6 +219,24 @@ int ckx_gemm_i8_tokenscale(const void* p_a, const void* p_b, void* p_c, const fl
     return e == hipSuccess ? CKX_OK : ckx::api_hip_fail(e, "gemm_i8_tokenscale");
 }
 
+int ckx_gemm_i8_tokenscale_plan(int32_t M, int32_t N, int32_t K, int32_t lda, int32_t ldb, int32_t ldc, int gated, int c_type,
+                                int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs)
+{
+    if(!tile_m || !tile_n || !k_runs)
+        return api_fail(CKX_INVALID_VALUE, "null result pointer");
+    int st = ckx_gemm_i8_tokenscale_is_supported(M, N, K, lda, ldb, ldc, gated, c_type);
+    if(st != CKX_OK)
+        return st;
+    if(workspace_bytes < 0)
+        return api_fail(CKX_INVALID_VALUE, "negative size");
+    *tile_m = *tile_n = *k_runs = 0;
+    ckx::GemmI8Args a{};
+    a.rows_a = M, a.rows_per = 1, a.M = M, a.N = N, a.K = K, a.lda = lda, a.ldb = ldb, a.ldc = ldc, a.gated = gated;
+    if(M > 0 && N > 0)
+        ckx::gemm_i8_scaled_plan(a, workspace_bytes, tile_m, tile_n, k_runs);
+    return CKX_OK;
+}
+
 int ckx_experts_gemm_i8_is_supported(const ckx_experts_desc* d)
 {
     if(!d)
@@ -246,13 +272,29 @@ int ckx_experts_gemm_i8(const void* p_a, const void* p_b, void* p_c, const float
     if(!aligned(p_c, size_of(d->c_type)) || !aligned(p_scale_a, 4) || !aligned(p_scale_b, 4) || !aligned(p_bias, 4) || !aligned(p_offsets, 4) ||
        !aligned(p_rows, 4))
         return api_fail(CKX_UNSUPPORTED, "operands must be aligned to their element size");
-    ckx::GemmI8Args a{};
+    ckx::GemmI8Args a = product_of(*d);
     a.a = static_cast<const int8_t*>(p_a), a.b = static_cast<const int8_t*>(p_b), a.c = p_c;
     a.sa = p_scale_a, a.sb = p_scale_b, a.bias = p_bias, a.offsets = p_offsets, a.rows = p_rows;
-    a.experts = d->num_experts, a.rows_a = d->num_rows_a, a.rows_per = d->rows_per, a.batch_b = d->batch_stride_b;
-    a.M = d->num_rows, a.N = d->N, a.K = d->K, a.lda = d->stride_a, a.ldb = d->stride_b, a.ldc = d->stride_c, a.gated = d->gated;
     hipError_t e = ckx::gemm_i8_scaled_launch(a, d->c_type, 0, (hipStream_t)stream);
     return e == hipSuccess ? CKX_OK : ckx::api_hip_fail(e, "experts_gemm_i8");
+}
+
+int ckx_experts_gemm_i8_plan(const ckx_experts_desc* d, int gathered, int* tile_m, int* tile_n, int* k_runs)
+{
+    if(!tile_m || !tile_n || !k_runs)
+        return api_fail(CKX_INVALID_VALUE, "null result pointer");
+    int st = ckx_experts_gemm_i8_is_supported(d);
+    if(st != CKX_OK)
+        return st;
+    if(gathered != 0 && gathered != 1)
+        return api_fail(CKX_INVALID_VALUE, "gathered is 0 or 1");
+    *tile_m = *tile_n = *k_runs = 0;
+    ckx::GemmI8Args a = product_of(*d);
+    const int32_t none = 0; // (says that there are tables; the plan reads none)
+    a.offsets = &none, a.rows = gathered ? &none : nullptr;
+    if(d->num_rows > 0 && d->num_experts > 0 && d->N > 0)
+        ckx::gemm_i8_scaled_plan(a, 0, tile_m, tile_n, k_runs);
+    return CKX_OK;
 }
 
 int ckx_experts_combine_is_supported(int32_t num_tokens, int32_t top_k, int32_t num_rows, int32_t N, int32_t stride_y, int32_t stride_add,
@@ -283,6 +325,8 @@ int ckx_experts_combine(const void* p_y, const int32_t* p_places, const float* p
     if(!aligned(p_y, size_of(type)) || !aligned(p_add, size_of(type)) || !aligned(p_out, size_of(type)) || !aligned(p_places, 4) ||
        !aligned(p_weights, 4))
         return api_fail(CKX_UNSUPPORTED, "operands must be aligned to their element size");
+    if(p_add && p_add == p_out && num_tokens > 1 && stride_add != stride_out)
+        return api_fail(CKX_INVALID_VALUE, "add is out, with another stride");
     const ckx::CombineArgs a{p_y, p_places, p_weights, p_add, p_out, num_tokens, top_k, num_rows, N, stride_y, stride_add, stride_out};
     hipError_t e = ckx::combine_launch(a, type, (hipStream_t)stream);
     return e == hipSuccess ? CKX_OK : ckx::api_hip_fail(e, "experts_combine");

@@ -561,16 +561,17 @@ hipError_t launch_form(GemmI8Args& a, int64_t workspace_bytes, hipStream_t s)
 
 } // namespace
 
-// a launch has fewer than 2^32 threads, 512 a workgroup at most: one for 64 x 128 outputs, for 16 rows and 8 columns of few rows
+// a launch has fewer than 2^32 threads, 512 a workgroup at most: one for 64 x 128 outputs (experts: 128 x 128), and where the rows are
+// few (experts: under 128 each, which K <= 131071 makes of the plan's border) for 16 x 16
 bool gemm_i8_scaled_fits(int M, int N, int gated, int experts)
 {
     GemmI8Args a{};
     a.M = M, a.experts = experts;
     const int none     = 0;
     a.offsets          = experts ? &none : nullptr; // (says that there are experts)
-    const bool few     = experts || M <= 64;
+    const bool few     = experts ? M < (int64_t)experts * 128 : M <= 64;
     const int64_t wide = (int64_t)N * (gated ? 2 : 1);
-    return most_tiles_m(a, few ? 16 : 64) * (wide / (few ? 16 : 128) + 2) < (1ll << 32) / 512;
+    return most_tiles_m(a, few ? 16 : experts ? 128 : 64) * (wide / (few ? 16 : 128) + 2) < (1ll << 32) / 512;
 }
 
 int64_t gemm_i8_scaled_workspace(int M, int N, int K, int gated)

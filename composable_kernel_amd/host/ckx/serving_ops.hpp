@@ -1,5 +1,5 @@
-// C++ operators of the 8-bit serving path (include/ckx.h): block quantiser, block-scaled GEMM, cache tables, cache store and paged
-// attention. Same conduct as the operators of device_ops.hpp: MakeArgument / MakeArgumentPointer, IsSupportedArgument,
+// C++ operators of the 8-bit serving path (include/ckx.h): block quantiser, block-scaled GEMM, cache tables, cache store, paged
+// attention; experts' router, token quantiser, token-scaled int8 GEMM, the experts' GEMM and the weighted sum of their rows. Same conduct as the operators of device_ops.hpp: MakeArgument / MakeArgumentPointer, IsSupportedArgument,
 // MakeInvoker()->Run. Types as template parameters: float, half_t, bhalf_t; codes are f8_t (e4m3) or int8_t.
 #pragma once
 
@@ -150,6 +150,94 @@ struct PagedAttention8Argument : public BaseArgument
     }
 };
 
+struct RouteExpertsArgument : public BaseArgument
+{
+    const void* p_logits;
+    const float* p_bias;
+    const index_t* p_num_tokens;
+    index_t* p_ids;
+    float* p_weights;
+    index_t *p_offsets, *p_rows, *p_places;
+    ckx_route_desc desc;
+    int64_t WorkSpaceSize() const { return p_offsets || p_rows || p_places ? ckx_route_experts_workspace_bytes(&desc) : 0; }
+    static int Supported(const RouteExpertsArgument& a, int) { return ckx_route_experts_is_supported(&a.desc); }
+    static int Launch(const RouteExpertsArgument& a, int, void* stream)
+    {
+        return ckx_route_experts(a.p_logits, a.p_bias, a.p_num_tokens, a.p_ids, a.p_weights, a.p_offsets, a.p_rows, a.p_places, &a.desc,
+                                 a.p_workspace_, a.p_workspace_ ? a.WorkSpaceSize() : 0, stream);
+    }
+};
+
+struct TokenQuantizeI8Argument : public BaseArgument
+{
+    const void* p_x;
+    int8_t* p_q;
+    float* p_scale;
+    index_t M, K, StrideX, StrideQ;
+    int type;
+    static int Supported(const TokenQuantizeI8Argument& a, int)
+    {
+        return ckx_quantize_tokens_i8_is_supported(a.M, a.K, a.StrideX, a.StrideQ, a.type);
+    }
+    static int Launch(const TokenQuantizeI8Argument& a, int, void* stream)
+    {
+        return ckx_quantize_tokens_i8(a.p_x, a.p_q, a.p_scale, a.M, a.K, a.StrideX, a.StrideQ, a.type, stream);
+    }
+};
+
+struct GemmTokenScaleI8Argument : public BaseArgument
+{
+    const int8_t *p_a, *p_b;
+    void* p_c;
+    const float *p_scale_a, *p_scale_b, *p_bias;
+    index_t M, N, K, StrideA, StrideB, StrideC;
+    int gated, type;
+    int64_t WorkSpaceSize() const { return ckx_gemm_i8_tokenscale_workspace_bytes(M, N, K, gated); }
+    static int Supported(const GemmTokenScaleI8Argument& a, int)
+    {
+        return ckx_gemm_i8_tokenscale_is_supported(a.M, a.N, a.K, a.StrideA, a.StrideB, a.StrideC, a.gated, a.type);
+    }
+    static int Launch(const GemmTokenScaleI8Argument& a, int, void* stream)
+    {
+        return ckx_gemm_i8_tokenscale(a.p_a, a.p_b, a.p_c, a.p_scale_a, a.p_scale_b, a.p_bias, a.M, a.N, a.K, a.StrideA, a.StrideB,
+                                      a.StrideC, a.gated, a.type, a.p_workspace_, a.p_workspace_ ? a.WorkSpaceSize() : 0, stream);
+    }
+};
+
+struct ExpertsGemmI8Argument : public BaseArgument
+{
+    const int8_t *p_a, *p_b;
+    void* p_c;
+    const float *p_scale_a, *p_scale_b, *p_bias;
+    const index_t *p_offsets, *p_rows;
+    ckx_experts_desc desc;
+    static int Supported(const ExpertsGemmI8Argument& a, int) { return ckx_experts_gemm_i8_is_supported(&a.desc); }
+    static int Launch(const ExpertsGemmI8Argument& a, int, void* stream)
+    {
+        return ckx_experts_gemm_i8(a.p_a, a.p_b, a.p_c, a.p_scale_a, a.p_scale_b, a.p_bias, a.p_offsets, a.p_rows, &a.desc, stream);
+    }
+};
+
+struct ExpertsCombineArgument : public BaseArgument
+{
+    const void* p_y;
+    const index_t* p_places;
+    const float* p_weights;
+    const void* p_add;
+    void* p_out;
+    index_t NumTokens, TopK, NumRows, N, StrideY, StrideAdd, StrideOut;
+    int type;
+    static int Supported(const ExpertsCombineArgument& a, int)
+    {
+        return ckx_experts_combine_is_supported(a.NumTokens, a.TopK, a.NumRows, a.N, a.StrideY, a.StrideAdd, a.StrideOut, a.type);
+    }
+    static int Launch(const ExpertsCombineArgument& a, int, void* stream)
+    {
+        return ckx_experts_combine(a.p_y, a.p_places, a.p_weights, a.p_add, a.p_out, a.NumTokens, a.TopK, a.NumRows, a.N, a.StrideY,
+                                   a.StrideAdd, a.StrideOut, a.type, stream);
+    }
+};
+
 template <typename Argument>
 using ServingOperatorOf = ServingOperator<Argument, &Argument::Supported, &Argument::Launch>;
 
@@ -247,6 +335,108 @@ struct DevicePagedAttention8 : public detail::ServingOperatorOf<detail::PagedAtt
         return a ? (size_t)a->WorkSpaceSize() : 0;
     }
     std::string GetTypeString() const override { return "DevicePagedAttention8<auto>"; }
+};
+
+enum struct ExpertScoring
+{
+    Softmax = CKX_SCORE_SOFTMAX,
+    Sigmoid = CKX_SCORE_SIGMOID
+};
+
+// each token's experts and weights, and the experts' rows in order; p_bias, p_num_tokens and the three tables may be null
+template <typename LogitsDataType, ExpertScoring Scoring = ExpertScoring::Softmax, bool Renormalise = true>
+struct DeviceRouteExperts : public detail::ServingOperatorOf<detail::RouteExpertsArgument>
+{
+    static Argument MakeArgument(const LogitsDataType* p_logits, const float* p_bias, const index_t* p_num_tokens, index_t* p_ids,
+                                 float* p_weights, index_t* p_offsets, index_t* p_rows, index_t* p_places, index_t NumTokens,
+                                 index_t NumExperts, index_t TopK, index_t StrideLogits, index_t NumGroups = 1, index_t TopGroups = 1,
+                                 index_t GroupBest = 1, element_wise::Scale weight_element_op = {})
+    {
+        Argument a;
+        a.p_logits = p_logits, a.p_bias = p_bias, a.p_num_tokens = p_num_tokens, a.p_ids = p_ids, a.p_weights = p_weights;
+        a.p_offsets = p_offsets, a.p_rows = p_rows, a.p_places = p_places;
+        a.desc = ckx_route_desc{NumTokens, NumExperts, TopK, StrideLogits, NumGroups, TopGroups, GroupBest, (int32_t)Scoring,
+                                Renormalise ? 1 : 0, detail::ckx_type<LogitsDataType>(), weight_element_op.scale_};
+        return a;
+    }
+    size_t GetWorkSpaceSize(const BaseArgument* p) const override
+    {
+        const auto* a = dynamic_cast<const Argument*>(p);
+        return a ? (size_t)a->WorkSpaceSize() : 0;
+    }
+    std::string GetTypeString() const override { return "DeviceRouteExperts<auto>"; }
+};
+
+// x [M, K] -> int8 codes and one fp32 scale per row
+template <typename XDataType>
+struct DeviceTokenQuantizeI8 : public detail::ServingOperatorOf<detail::TokenQuantizeI8Argument>
+{
+    static Argument MakeArgument(const XDataType* p_x, int8_t* p_q, float* p_scale, index_t M, index_t K, index_t StrideX, index_t StrideQ)
+    {
+        Argument a;
+        a.p_x = p_x, a.p_q = p_q, a.p_scale = p_scale, a.M = M, a.K = K, a.StrideX = StrideX, a.StrideQ = StrideQ;
+        a.type = detail::ckx_type<XDataType>();
+        return a;
+    }
+    std::string GetTypeString() const override { return "DeviceTokenQuantizeI8<auto>"; }
+};
+
+// C [M, N] = scale_a[m] * scale_b[n] * (A B^T) + bias[n]: A [M, K], B [N, K] int8; Gated: B, scale_b and bias of 2 N rows, C = silu(first
+// half) * second half. p_bias may be null
+template <typename CDataType, bool Gated = false>
+struct DeviceGemmTokenScaleI8 : public detail::ServingOperatorOf<detail::GemmTokenScaleI8Argument>
+{
+    static Argument MakeArgument(const int8_t* p_a, const int8_t* p_b, CDataType* p_c, const float* p_scale_a, const float* p_scale_b,
+                                 const float* p_bias, index_t M, index_t N, index_t K, index_t StrideA, index_t StrideB, index_t StrideC)
+    {
+        Argument a;
+        a.p_a = p_a, a.p_b = p_b, a.p_c = p_c, a.p_scale_a = p_scale_a, a.p_scale_b = p_scale_b, a.p_bias = p_bias;
+        a.M = M, a.N = N, a.K = K, a.StrideA = StrideA, a.StrideB = StrideB, a.StrideC = StrideC;
+        a.gated = Gated ? 1 : 0, a.type = detail::ckx_type<CDataType>();
+        return a;
+    }
+    size_t GetWorkSpaceSize(const BaseArgument* p) const override
+    {
+        const auto* a = dynamic_cast<const Argument*>(p);
+        return a ? (size_t)a->WorkSpaceSize() : 0;
+    }
+    std::string GetTypeString() const override { return "DeviceGemmTokenScaleI8<auto>"; }
+};
+
+// the same product for each expert's rows: B [NumExperts, N, K]; p_bias and p_rows may be null
+template <typename CDataType, bool Gated = false>
+struct DeviceExpertsGemmI8 : public detail::ServingOperatorOf<detail::ExpertsGemmI8Argument>
+{
+    static Argument MakeArgument(const int8_t* p_a, const int8_t* p_b, CDataType* p_c, const float* p_scale_a, const float* p_scale_b,
+                                 const float* p_bias, const index_t* p_offsets, const index_t* p_rows, index_t NumRows, index_t NumRowsA,
+                                 index_t NumExperts, index_t N, index_t K, index_t StrideA, index_t StrideB, index_t StrideC,
+                                 int64_t BatchStrideB, index_t RowsPer = 1)
+    {
+        Argument a;
+        a.p_a = p_a, a.p_b = p_b, a.p_c = p_c, a.p_scale_a = p_scale_a, a.p_scale_b = p_scale_b, a.p_bias = p_bias;
+        a.p_offsets = p_offsets, a.p_rows = p_rows;
+        a.desc = ckx_experts_desc{NumRows, NumRowsA, NumExperts, N, K, StrideA, StrideB, StrideC, RowsPer, Gated ? 1 : 0,
+                                  detail::ckx_type<CDataType>(), 0, BatchStrideB};
+        return a;
+    }
+    std::string GetTypeString() const override { return "DeviceExpertsGemmI8<auto>"; }
+};
+
+// out [t] = add [t] + sum over j of weights [t, j] * y [places [t, j]]; p_add may be null, or p_out
+template <typename XDataType>
+struct DeviceExpertsCombine : public detail::ServingOperatorOf<detail::ExpertsCombineArgument>
+{
+    static Argument MakeArgument(const XDataType* p_y, const index_t* p_places, const float* p_weights, const XDataType* p_add,
+                                 XDataType* p_out, index_t NumTokens, index_t TopK, index_t NumRows, index_t N, index_t StrideY,
+                                 index_t StrideAdd, index_t StrideOut)
+    {
+        Argument a;
+        a.p_y = p_y, a.p_places = p_places, a.p_weights = p_weights, a.p_add = p_add, a.p_out = p_out;
+        a.NumTokens = NumTokens, a.TopK = TopK, a.NumRows = NumRows, a.N = N, a.StrideY = StrideY, a.StrideAdd = StrideAdd;
+        a.StrideOut = StrideOut, a.type = detail::ckx_type<XDataType>();
+        return a;
+    }
+    std::string GetTypeString() const override { return "DeviceExpertsCombine<auto>"; }
 };
 
 } // namespace device

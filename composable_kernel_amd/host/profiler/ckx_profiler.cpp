@@ -28,6 +28,11 @@
 //   ckx_profiler paged_attention8 <cache 1:e4m3 2:int8> <verify> <init> <log> <time> Batch Context New QHeads KvHeads HeadDim
 //                     BlockSize [causal 0|1] [nrepeat]   (a step of a decoder: DeviceKvCacheTables, DeviceKvCacheStore8,
 //                     DevicePagedAttention8, fp16; the cached tokens are stored by a step of their own first)
+//   ckx_profiler gemm_i8_tokenscale <c type 1:fp16 2:bf16> <verify> <init> <log> <time> M N K [gated 0|1] [nrepeat]
+//                     (fp16 activations through DeviceTokenQuantizeI8, then DeviceGemmTokenScaleI8)
+//   ckx_profiler experts_i8 <scores 1:softmax 2:sigmoid> <verify> <init> <log> <time> Tokens Experts TopK Hidden Inner [nrepeat]
+//                     (a mixture of experts from its logits to its output, fp16: DeviceRouteExperts, DeviceTokenQuantizeI8, the gated
+//                     DeviceExpertsGemmI8 of Inner columns, DeviceTokenQuantizeI8, DeviceExpertsGemmI8, DeviceExpertsCombine)
 //
 // Every instance of the family is run (DeviceOperationInstanceFactory), one "Perf:" line each
 // and a final "Best Perf:" line, in the reference's format (profile_gemm_impl.hpp:176-177,
@@ -35,7 +40,7 @@
 // verify = 1 checks that all instances agree with the first supported one (bit-exact for
 // int8, rtol = atol = 1e-2 for fp16); comparison against the CPU reference is the job of the
 // test-suite, which regenerates these inputs from the same seeds. The 8-bit serving operators have one kernel choice each:
-// there verify = 1 compares a sample of their outputs with plain host forms in 64 bits (ckx/serving_check.hpp), and
+// there verify = 1 compares a sample of their outputs with plain host forms in 64 bits (ckx/serving_check.hpp, experts_check.hpp), and
 // init = 0 leaves inputs zero, any other fills them with decimal values. If the environment variable
 // CKX_PROFILER_DUMP names a file, the best instance's output tensor is written there.
 #include <cstdlib>
@@ -44,6 +49,7 @@
 #include <iostream>
 
 #include "ckx/device_ops.hpp"
+#include "ckx/experts_check.hpp"
 #include "ckx/host_tensor.hpp"
 #include "ckx/serving_check.hpp"
 #include "ckx/serving_ops.hpp"
@@ -1104,6 +1110,211 @@ int profile_attention8(int argc, char* argv[])
     return run(type, std::atoi(argv[3]) != 0, std::atoi(argv[4]), std::atoi(argv[6]) != 0, p[0], p[1], p[2], p[3], p[4], p[5], p[6], nrepeat);
 }
 
+// int8 weights: every code; scales of 2^-15 ... 2^-12
+std::vector<int8_t> i8_weights(std::size_t n, int init, uint64_t seed)
+{
+    std::vector<int8_t> w(n);
+    for(std::size_t i = 0; init && i < n; ++i)
+        w[i] = (int8_t)(ckx::splitmix64(seed, i) >> 56);
+    return w;
+}
+std::vector<float> i8_scales(std::size_t n, uint64_t seed)
+{
+    std::vector<float> s(n);
+    for(std::size_t i = 0; i < n; ++i)
+        s[i] = 1.0f / (float)(4096 << (ckx::splitmix64(seed, i) >> 62));
+    return s;
+}
+template <typename T>
+double value_of(T x)
+{
+    if constexpr(std::is_same_v<T, bhalf_t>)
+        return (double)ckx::bf16_to_float(x);
+    else
+        return (double)x;
+}
+
+template <typename T, bool Gated>
+int profile_gemm_i8_t(bool verify, int init, bool time_kernel, int M, int N, int K, int nrepeat)
+{
+    const std::size_t wide = (std::size_t)N * (Gated ? 2 : 1);
+    std::vector<half_t> x((std::size_t)M * K);
+    if(init)
+        ckx::fill_uniform_f16(x, -1.f, 1.f, 0xC0FFEE + 15);
+    const auto w  = i8_weights(wide * K, init, 0xC0FFEE + 16);
+    const auto sw = i8_scales(wide, 0xC0FFEE + 17);
+    ckx::DeviceMem dx(x.size() * 2), dq(x.size()), ds((std::size_t)M * 4), dw(w.size()), dsw(sw.size() * 4), dc((std::size_t)M * N * sizeof(T));
+    dx.ToDevice(x.data());
+    dw.ToDevice(w.data());
+    dsw.ToDevice(sw.data());
+    device::DeviceTokenQuantizeI8<half_t> quantize;
+    run_one(quantize,
+            quantize.MakeArgument(static_cast<const half_t*>(dx.GetDeviceBuffer()), static_cast<int8_t*>(dq.GetDeviceBuffer()),
+                                  static_cast<float*>(ds.GetDeviceBuffer()), M, K, K, K),
+            "the quantiser", time_kernel, nrepeat, 3.0 * M * K, 3.0 * M * K + 4.0 * M, false);
+    device::DeviceGemmTokenScaleI8<T, Gated> gemm;
+    auto arg = gemm.MakeArgument(static_cast<const int8_t*>(dq.GetDeviceBuffer()), static_cast<const int8_t*>(dw.GetDeviceBuffer()),
+                                 static_cast<T*>(dc.GetDeviceBuffer()), static_cast<const float*>(ds.GetDeviceBuffer()),
+                                 static_cast<const float*>(dsw.GetDeviceBuffer()), nullptr, M, N, K, K, K, N);
+    ckx::DeviceMem ws(gemm.GetWorkSpaceSize(&arg));
+    if(ws.GetBufferSize() > 0)
+        gemm.SetWorkSpacePointer(&arg, ws.GetDeviceBuffer());
+    run_one(gemm, arg, "the product", time_kernel, nrepeat, 2.0 * M * wide * K, (double)M * K + (double)wide * K + 2.0 * M * N, true);
+    const auto out = from_device<T>(dc);
+    if(const char* path = std::getenv("CKX_PROFILER_DUMP"))
+        ckx::dump_to_file(path, out);
+    if(!verify)
+        return 0;
+    const auto q = from_device<int8_t>(dq);
+    const auto s = from_device<float>(ds);
+    std::size_t checked = 0;
+    std::size_t bad = ckx::token_quantise_errors([&](std::size_t m, int k) { return (double)x[m * K + k]; }, q.data(), s.data(), M, K, checked);
+    bool pass       = verified("DeviceTokenQuantizeI8", bad, checked);
+    checked         = 0;
+    bad             = ckx::gemm_i8_errors([&](std::size_t m, std::size_t n) { return value_of(out[m * N + n]); },
+                                      [](std::size_t m, std::size_t& row, std::size_t& expert) { row = m, expert = 0; },
+                                      ckx::GemmI8View{q.data(), w.data(), s.data(), sw.data(), M, N, K, Gated},
+                                      std::is_same_v<T, bhalf_t> ? 0x1p-8 : 0x1p-11, checked);
+    pass = verified("DeviceGemmTokenScaleI8", bad, checked) && pass;
+    return pass ? 0 : 1;
+}
+
+int profile_gemm_i8(int argc, char* argv[])
+{
+    if(argc < 10)
+    {
+        std::printf("arg1: tensor operation (gemm_i8_tokenscale)\narg2: type of C (1: fp16, 2: bf16)\narg3: verification\n"
+                    "arg4: initialization\narg5: print tensor value\narg6: time kernel\narg7 to 9: M, N, K\narg10: gated (0 | 1)\n"
+                    "last: nrepeat\n");
+        return 1;
+    }
+    const int M = std::atoi(argv[7]), N = std::atoi(argv[8]), K = std::atoi(argv[9]), nrepeat = argc > 11 ? std::atoi(argv[11]) : 10;
+    if(M < 1 || N < 1 || K < 1)
+        throw std::runtime_error("M, N and K are at least 1");
+    const bool gated = argc > 10 && std::atoi(argv[10]) != 0, bf16 = std::atoi(argv[2]) == 2;
+    auto* run = gated ? (bf16 ? &profile_gemm_i8_t<bhalf_t, true> : &profile_gemm_i8_t<half_t, true>)
+                      : (bf16 ? &profile_gemm_i8_t<bhalf_t, false> : &profile_gemm_i8_t<half_t, false>);
+    return run(std::atoi(argv[3]) != 0, std::atoi(argv[4]), std::atoi(argv[6]) != 0, M, N, K, nrepeat);
+}
+
+template <device::ExpertScoring Scoring>
+int profile_experts_i8_t(bool verify, int init, bool time_kernel, int T, int E, int k, int hidden, int inner, int nrepeat)
+{
+    const int pairs = T * k;
+    std::vector<half_t> logits((std::size_t)T * E), x((std::size_t)T * hidden);
+    if(init)
+    {
+        ckx::fill_uniform_f16(logits, -4.f, 4.f, 0xC0FFEE + 18);
+        ckx::fill_uniform_f16(x, -1.f, 1.f, 0xC0FFEE + 19);
+    }
+    const auto up = i8_weights((std::size_t)E * 2 * inner * hidden, init, 0xC0FFEE + 20), down = i8_weights((std::size_t)E * hidden * inner, init, 0xC0FFEE + 21);
+    const auto s_up = i8_scales((std::size_t)E * 2 * inner, 0xC0FFEE + 22), s_down = i8_scales((std::size_t)E * hidden, 0xC0FFEE + 23);
+    auto sent = [](const auto& v) {
+        auto m = std::make_unique<ckx::DeviceMem>(v.size() * sizeof(v[0]));
+        m->ToDevice(v.data());
+        return m;
+    };
+    auto dlogits = sent(logits), dx = sent(x), dup = sent(up), ddown = sent(down), dsup = sent(s_up), dsdown = sent(s_down);
+    ckx::DeviceMem dids((std::size_t)pairs * 4), dweights((std::size_t)pairs * 4), doffsets((std::size_t)(E + 1) * 4), drows((std::size_t)pairs * 4),
+        dplaces((std::size_t)pairs * 4), dq(x.size()), ds((std::size_t)T * 4), dh((std::size_t)pairs * inner * 2), dqh((std::size_t)pairs * inner),
+        dsh((std::size_t)pairs * 4), dy((std::size_t)pairs * hidden * 2), dout(x.size() * 2);
+    auto ints   = [](ckx::DeviceMem& m) { return static_cast<index_t*>(m.GetDeviceBuffer()); };
+    auto floats = [](ckx::DeviceMem& m) { return static_cast<float*>(m.GetDeviceBuffer()); };
+    auto halves = [](ckx::DeviceMem& m) { return static_cast<half_t*>(m.GetDeviceBuffer()); };
+    auto codes  = [](ckx::DeviceMem& m) { return static_cast<int8_t*>(m.GetDeviceBuffer()); };
+    device::DeviceRouteExperts<half_t, Scoring> route;
+    auto rarg = route.MakeArgument(halves(*dlogits), nullptr, nullptr, ints(dids), floats(dweights), ints(doffsets), ints(drows), ints(dplaces), T, E, k, E);
+    ckx::DeviceMem ws(route.GetWorkSpaceSize(&rarg));
+    if(ws.GetBufferSize() > 0)
+        route.SetWorkSpacePointer(&rarg, ws.GetDeviceBuffer());
+    run_one(route, rarg, "the router", time_kernel, nrepeat, (double)T * E, 2.0 * T * E + 16.0 * pairs, false);
+    device::DeviceTokenQuantizeI8<half_t> quantize;
+    run_one(quantize, quantize.MakeArgument(halves(*dx), codes(dq), floats(ds), T, hidden, hidden, hidden), "the quantiser", time_kernel, nrepeat,
+            3.0 * T * hidden, 3.0 * T * hidden, false);
+    const double used = std::min(E, pairs); // experts' matrices that are read
+    device::DeviceExpertsGemmI8<half_t, true> gemm_up;
+    run_one(gemm_up,
+            gemm_up.MakeArgument(codes(dq), codes(*dup), halves(dh), floats(ds), floats(*dsup), nullptr, ints(doffsets), ints(drows), pairs, T, E, inner,
+                                 hidden, hidden, hidden, inner, (int64_t)2 * inner * hidden, k),
+            "the experts' first product", time_kernel, nrepeat, 4.0 * pairs * inner * hidden,
+            used * 2 * inner * hidden + (double)T * hidden + 2.0 * pairs * inner, true);
+    run_one(quantize, quantize.MakeArgument(halves(dh), codes(dqh), floats(dsh), pairs, inner, inner, inner), "the quantiser", time_kernel, nrepeat,
+            3.0 * pairs * inner, 3.0 * pairs * inner, false);
+    device::DeviceExpertsGemmI8<half_t> gemm_down;
+    run_one(gemm_down,
+            gemm_down.MakeArgument(codes(dqh), codes(*ddown), halves(dy), floats(dsh), floats(*dsdown), nullptr, ints(doffsets), nullptr, pairs, pairs, E,
+                                   hidden, inner, inner, inner, hidden, (int64_t)hidden * inner),
+            "the experts' second product", time_kernel, nrepeat, 2.0 * pairs * hidden * inner,
+            used * hidden * inner + (double)pairs * inner + 2.0 * pairs * hidden, true);
+    device::DeviceExpertsCombine<half_t> combine;
+    run_one(combine,
+            combine.MakeArgument(halves(dy), ints(dplaces), floats(dweights), nullptr, halves(dout), T, k, pairs, hidden, hidden, 0, hidden),
+            "the weighted sum", time_kernel, nrepeat, 2.0 * pairs * hidden, 2.0 * (pairs + (double)T) * hidden, false);
+    const auto out = from_device<half_t>(dout);
+    if(const char* path = std::getenv("CKX_PROFILER_DUMP"))
+        ckx::dump_to_file(path, out);
+    if(!verify)
+        return 0;
+    const auto ids = from_device<index_t>(dids), offsets = from_device<index_t>(doffsets), rows = from_device<index_t>(drows), places = from_device<index_t>(dplaces);
+    const auto weights = from_device<float>(dweights), s = from_device<float>(ds), sh = from_device<float>(dsh);
+    const auto q = from_device<int8_t>(dq), qh = from_device<int8_t>(dqh);
+    const auto h = from_device<half_t>(dh), y = from_device<half_t>(dy);
+    bool pass    = true;
+    auto check   = [&](const char* what, auto errors) {
+        std::size_t checked = 0;
+        const std::size_t bad = errors(checked);
+        pass                  = verified(what, bad, checked) && pass;
+        return bad == 0;
+    };
+    if(!check("DeviceRouteExperts", [&](std::size_t& n) {
+           return ckx::route_errors([&](std::size_t t, int e) { return (double)logits[t * E + e]; },
+                                    ckx::RouteView{ids.data(), offsets.data(), rows.data(), places.data(), weights.data(), T, E, k,
+                                                   Scoring == device::ExpertScoring::Sigmoid, true},
+                                    n);
+       }))
+        return 1; // (the tables are indices below)
+    auto expert_of = [&](std::size_t i) { return (std::size_t)ids[rows[i]]; };
+    check("DeviceTokenQuantizeI8", [&](std::size_t& n) {
+        return ckx::token_quantise_errors([&](std::size_t m, int j) { return (double)x[m * hidden + j]; }, q.data(), s.data(), T, hidden, n);
+    });
+    check("DeviceExpertsGemmI8, gated", [&](std::size_t& n) {
+        return ckx::gemm_i8_errors([&](std::size_t m, std::size_t j) { return (double)h[m * inner + j]; },
+                                   [&](std::size_t m, std::size_t& row, std::size_t& expert) { row = rows[m] / k, expert = expert_of(m); },
+                                   ckx::GemmI8View{q.data(), up.data(), s.data(), s_up.data(), pairs, inner, hidden, true}, 0x1p-11, n);
+    });
+    check("DeviceTokenQuantizeI8", [&](std::size_t& n) {
+        return ckx::token_quantise_errors([&](std::size_t m, int j) { return (double)h[m * inner + j]; }, qh.data(), sh.data(), pairs, inner, n);
+    });
+    check("DeviceExpertsGemmI8", [&](std::size_t& n) {
+        return ckx::gemm_i8_errors([&](std::size_t m, std::size_t j) { return (double)y[m * hidden + j]; },
+                                   [&](std::size_t m, std::size_t& row, std::size_t& expert) { row = m, expert = expert_of(m); },
+                                   ckx::GemmI8View{qh.data(), down.data(), sh.data(), s_down.data(), pairs, hidden, inner, false}, 0x1p-11, n);
+    });
+    check("DeviceExpertsCombine", [&](std::size_t& n) {
+        return ckx::combine_errors([&](std::size_t t, std::size_t j) { return (double)out[t * hidden + j]; },
+                                   [&](std::size_t i, std::size_t j) { return (double)y[i * hidden + j]; }, places.data(), weights.data(), T, k, pairs, hidden,
+                                   0x1p-11, n);
+    });
+    return pass ? 0 : 1;
+}
+
+int profile_experts_i8(int argc, char* argv[])
+{
+    if(argc < 12)
+    {
+        std::printf("arg1: tensor operation (experts_i8)\narg2: scores (1: softmax, 2: sigmoid)\narg3: verification\narg4: initialization\n"
+                    "arg5: print tensor value\narg6: time kernel\narg7 to 11: Tokens, Experts, TopK, Hidden, Inner\nlast: nrepeat\n");
+        return 1;
+    }
+    int p[5];
+    for(int i = 0; i < 5; ++i)
+        p[i] = std::atoi(argv[7 + i]);
+    if(*std::min_element(p, p + 5) < 1 || p[2] > p[1])
+        throw std::runtime_error("sizes are at least 1, TopK at most Experts");
+    auto* run = std::atoi(argv[2]) == 2 ? &profile_experts_i8_t<device::ExpertScoring::Sigmoid> : &profile_experts_i8_t<device::ExpertScoring::Softmax>;
+    return run(std::atoi(argv[3]) != 0, std::atoi(argv[4]), std::atoi(argv[6]) != 0, p[0], p[1], p[2], p[3], p[4], argc > 12 ? std::atoi(argv[12]) : 10);
+}
+
 } // namespace
 
 int main(int argc, char* argv[])
@@ -1140,6 +1351,10 @@ int main(int argc, char* argv[])
             return profile_gemm_f8(argc, argv);
         if(argc >= 2 && std::strcmp(argv[1], "paged_attention8") == 0)
             return profile_attention8(argc, argv);
+        if(argc >= 2 && std::strcmp(argv[1], "gemm_i8_tokenscale") == 0)
+            return profile_gemm_i8(argc, argv);
+        if(argc >= 2 && std::strcmp(argv[1], "experts_i8") == 0)
+            return profile_experts_i8(argc, argv);
         std::printf("arg1: tensor operation (gemm: GEMM\n"
                     "                        conv2d_fwd: NHWC/KYXC/NHWK forward convolution\n"
                     "                        batched_gemm_gemm: batched fused GEMM+GEMM\n"
@@ -1151,7 +1366,9 @@ int main(int argc, char* argv[])
                     "                        gemm_splitk: Split-K GEMM\n"
                     "                        gemm_bias_relu: GEMM+Bias+ReLU\n"
                     "                        gemm_f8_blockscale: quantiser and GEMM, e4m3 with a scale for each block of 128\n"
-                    "                        paged_attention8: tables, store and attention over a cache of 8-bit blocks)\n");
+                    "                        paged_attention8: tables, store and attention over a cache of 8-bit blocks\n"
+                    "                        gemm_i8_tokenscale: quantiser and GEMM, int8 with a scale for each token and channel\n"
+                    "                        experts_i8: a mixture of experts in int8)\n");
         return 1;
     }
     catch(const std::exception& e)

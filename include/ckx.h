@@ -560,7 +560,8 @@ int ckx_paged_attention8(const void* p_q, void* p_o, const int32_t* p_block_tabl
  * A layer's linear work in 8-bit integers, and what a mixture of experts needs around it: route each token to its experts,
  * quantise the tokens, multiply each expert's rows, add a token's rows up again. All entry points are asynchronous on
  * `stream`, allocate nothing, can be captured into a graph, and read the experts' tables and the number of tokens on the
- * device: a replay sees what they hold then. `stream`'s device has to be the current one. */
+ * device: a replay sees what they hold then. `stream`'s device has to be the current one. No output lies on an input, but
+ * where a line below allows it. */
 
 /* ---- each token's experts, their weights, and the experts' rows in order ---------------------------
  * x[t, e]: logits [num_tokens, num_experts] fp32, fp16 or bf16, rows stride_x apart; bias[e] fp32 (p_bias NULL: none).
@@ -624,6 +625,11 @@ int64_t ckx_gemm_i8_tokenscale_workspace_bytes(int32_t M, int32_t N, int32_t K, 
 int ckx_gemm_i8_tokenscale(const void* p_a, const void* p_b, void* p_c, const float* p_scale_a, const float* p_scale_b, const float* p_bias,
                            int32_t M, int32_t N, int32_t K, int32_t lda, int32_t ldb, int32_t ldc, int gated, int c_type, void* p_workspace,
                            int64_t workspace_bytes, void* stream);
+/* What a launch with 16-byte aligned A and B and this much workspace would use (pure host): the rows of A and of B that a workgroup
+ * takes (16 x 16, gated 16 x 32, and 32 x 32: straight from memory; 64 x 128, 128 x 128, 256 x 256) and the runs that K is cut into;
+ * 0 runs: the kernel for any K and stride, 128 x 128. Nothing to do (M or N 0): all 0. */
+int ckx_gemm_i8_tokenscale_plan(int32_t M, int32_t N, int32_t K, int32_t lda, int32_t ldb, int32_t ldc, int gated, int c_type,
+                                int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs);
 
 /* ---- the same product for each expert's rows -------------------------------------------------------
  * Rows p_offsets[e] ... p_offsets[e + 1] - 1 of C [num_rows, N] are expert e's (offsets ascend; they are cut to 0 ...
@@ -646,6 +652,8 @@ typedef struct ckx_experts_desc
 int ckx_experts_gemm_i8_is_supported(const ckx_experts_desc* desc);
 int ckx_experts_gemm_i8(const void* p_a, const void* p_b, void* p_c, const float* p_scale_a, const float* p_scale_b, const float* p_bias,
                         const int32_t* p_offsets, const int32_t* p_rows, const ckx_experts_desc* desc, void* stream);
+/* as ckx_gemm_i8_tokenscale_plan; gathered: whether there are p_rows */
+int ckx_experts_gemm_i8_plan(const ckx_experts_desc* desc, int gathered, int* tile_m, int* tile_n, int* k_runs);
 
 /* ---- a token's rows, weighted and added up ---------------------------------------------------------
  *   out[t, n] = round( add[t, n] + sum_j w[t, j] * y[places[t, j], n] )       (j ascending, fp32; p_add NULL: 0)
