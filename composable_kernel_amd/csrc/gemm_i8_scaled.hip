@@ -109,23 +109,28 @@ __global__ __launch_bounds__(256) void gemm_i8_any_kernel(GemmI8Args p)
     }
 }
 
-// BM rows x BN rows of B, WM x WN waves, NST stages of operands in LDS: the loads of a K tile (128) are asked for NST - 1 tiles ahead.
+// BM rows x BN rows of B, WM x WN x KH waves, NST stages of operands in LDS: the loads of a K tile (128) are asked for NST - 1 tiles
+// ahead. LDS bounds the steps (rows x columns of a step: what the waves read and the loads write, at 128 bytes a clock: 64 x 128
+// 0.23 us at 2.4 GHz, 128 x 128 0.31 with waves of 64 x 64, 0.42 with 32 x 64), and with one wave a SIMD its latency would. So KH = 2 waves
+// share an output, one for each half of a K tile, where one workgroup fits a CU, and with more than two stages the next tile's fragments are
+// read while the present are multiplied: 64 x 128 from 0.43 to 0.29 us a step (128 rows of 4096 x 4096: 17.5 to 13.5).
 // The direct loads are inline assembly: the compiler, told of them, would wait for all of them before every LDS read of another
 // stage. Its own LDS reads it waits for itself; the wait for the direct loads stands in front of the barrier.
 // Columns behind K count by A's zeros alone: what B's loads bring there, and the rows of a tile that C does not have, are whatever the
 // resource's bounds let through.
-template <typename T, bool GATED, int BM, int BN, int WM, int WN, int NST>
-__global__ __launch_bounds__(WM* WN * 64) void gemm_i8_tile_kernel(GemmI8Args p)
+template <typename T, bool GATED, int BM, int BN, int WM, int WN, int KH, int NST>
+__global__ __launch_bounds__(WM* WN* KH * 64) void gemm_i8_tile_kernel(GemmI8Args p)
 {
-    constexpr int NW = WM * WN, MT = BM / WM / 16, NLA = BM / 8 / NW, NLB = BN / 8 / NW, LPT = NLA + NLB, COLS = GATED ? BN / 2 : BN;
+    constexpr int NW = WM * WN * KH, MT = BM / WM / 16, NG = BN / WN / 64, NLA = BM / 8 / NW, NLB = BN / 8 / NW, LPT = NLA + NLB, COLS = GATED ? BN / 2 : BN;
     constexpr int A_TILE = BM * 128, B_AT = NST * A_TILE, B_TILE = BN * 128, S_AT = B_AT + NST * B_TILE;
-    static_assert(BN / WN == 64 && NLA >= 1 && NLB >= 1, "");
-    __shared__ __align__(1024) uint8_t lds[S_AT + (BM + 2 * BN) * 4]; // [A | B | scales of rows, of columns, biases]
+    static_assert(BN / WN % 64 == 0 && BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "");
+    static_assert(KH == 1 || (MT % 2 == 0 && WM * WN * MT * NG * 4096 <= S_AT), "");
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[]; // [A | B | scales of rows, of columns, biases]
     float* const s_row = reinterpret_cast<float*>(lds + S_AT);
     float* const s_col = s_row + BM;
     float* const s_bias = s_col + BN;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave / WN, wn = wave % WN, q = lane >> 4;
+    const int kh = wave / (WM * WN), wm = wave / WN % WM, wn = wave % WN, q = lane >> 4;
     I8Tile t;
     int run = 0;
     if(p.offsets)
@@ -189,61 +194,131 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_i8_tile_kernel(GemmI8Args p)
         const int m = i8_row_of_a(p, t, r);
         s_row[r]    = m >= 0 ? p.sa[m] : 0.0f;
     }
-    i32x4 acc[MT][4];
+    i32x4 acc[MT][NG][4];
 #pragma unroll
     for(int i = 0; i < MT; ++i)
 #pragma unroll
-        for(int j = 0; j < 4; ++j)
-            acc[i][j] = i32x4{0, 0, 0, 0};
-    const int a_row = wm * (BM / WM) + (lane & 15), b_row = wn * 64 + (lane & 15);
+        for(int j = 0; j < NG * 4; ++j)
+            acc[i][j / 4][j % 4] = i32x4{0, 0, 0, 0};
+    const int a_row = wm * (BM / WM) + (lane & 15), b_row = wn * NG * 64 + (lane & 15);
     const int a_lo = a_row * 128 + ((q ^ (a_row & 7)) << 4), b_lo = B_AT + b_row * 128 + ((q ^ (b_row & 7)) << 4);
-    for(int g = g0; g < g1; ++g)
+    struct Fragments
     {
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 2) * LPT) : "memory"); // this tile's
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        load_all(g + NST - 1); // (into the stage that every wave has read before this barrier)
+        i32x4 a[2 / KH][MT], b[2 / KH][NG * 4];
+    };
+    auto read = [&](Fragments& f, int g) {
         const uint8_t* const at = lds + g % NST * A_TILE;
         const uint8_t* const bt = lds + g % NST * B_TILE;
 #pragma unroll
-        for(int ks = 0; ks < 2; ++ks)
+        for(int s = 0; s < 2 / KH; ++s)
         {
-            i32x4 bf[4];
+            const int half = (KH > 1 ? kh : s) * 64;
 #pragma unroll
-            for(int j = 0; j < 4; ++j)
-                bf[j] = *reinterpret_cast<const i32x4*>(bt + (b_lo ^ (ks * 64)) + j * 2048);
+            for(int j = 0; j < NG * 4; ++j)
+                f.b[s][j] = *reinterpret_cast<const i32x4*>(bt + (b_lo ^ half) + j * 2048);
 #pragma unroll
             for(int i = 0; i < MT; ++i)
-            {
-                const i32x4 af = *reinterpret_cast<const i32x4*>(at + (a_lo ^ (ks * 64)) + i * 2048);
+                f.a[s][i] = *reinterpret_cast<const i32x4*>(at + (a_lo ^ half) + i * 2048);
+        }
+    };
+    auto multiply = [&](const Fragments& f) {
 #pragma unroll
-                for(int j = 0; j < 4; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j], af, acc[i][j], 0, 0, 0);
-            }
+        for(int s = 0; s < 2 / KH; ++s)
+#pragma unroll
+            for(int i = 0; i < MT; ++i)
+#pragma unroll
+                for(int j = 0; j < NG * 4; ++j)
+                    acc[i][j / 4][j % 4] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.b[s][j], f.a[s][i], acc[i][j / 4][j % 4], 0, 0, 0);
+    };
+    // until all of the workgroup's loads but those of `tiles` tiles have landed
+    auto landed = [&](auto tiles) {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(decltype(tiles)::value * LPT) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    if constexpr(NST > 2)
+    {
+        // the fragments of a tile are read while the one before is multiplied
+        Fragments x, y;
+        auto step = [&](const Fragments& now, Fragments& next, int g) {
+            landed(std::integral_constant<int, NST - 3>());
+            load_all(g + NST - 1); // (into the stage of the tile before, which every wave has multiplied before this barrier)
+            read(next, g + 1);
+            multiply(now);
+        };
+        landed(std::integral_constant<int, NST - 2>());
+        read(x, g0);
+        for(int g = g0; g < g1; g += 2)
+        {
+            step(x, y, g);
+            if(g + 1 < g1)
+                step(y, x, g + 1);
         }
     }
+    else
+        for(int g = g0; g < g1; ++g)
+        {
+            landed(std::integral_constant<int, NST - 2>());
+            load_all(g + NST - 1); // (into the stage that every wave has read before this barrier)
+            Fragments f;
+            read(f, g);
+            multiply(f);
+        }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); // (no load may land in LDS that is another workgroup's by then)
     __syncthreads();                                 // (a run without K tiles: the scales)
-#pragma unroll
-    for(int i = 0; i < MT; ++i)
+    constexpr int MINE = MT / KH;                    // fragment rows that the wave finishes
+    i32x4 sum[MINE][NG][4];
+    if constexpr(KH > 1)
     {
-        const int r = wm * (BM / WM) + i * 16 + (lane & 15), n = n0 + wn * (GATED ? 32 : 64);
+        // each of the two waves of an output hands the other half of its sums over
+        i32x4* const there = reinterpret_cast<i32x4*>(lds) + ((wm * WN + wn) * KH + kh) * (MINE * NG * 4 * 64) + lane;
+        i32x4* const here  = reinterpret_cast<i32x4*>(lds) + ((wm * WN + wn) * KH + 1 - kh) * (MINE * NG * 4 * 64) + lane;
+#pragma unroll
+        for(int i = 0; i < MINE; ++i)
+#pragma unroll
+            for(int j = 0; j < NG * 4; ++j)
+            {
+                here[(i * NG * 4 + j) * 64] = kh ? acc[i][j / 4][j % 4] : acc[MINE + i][j / 4][j % 4];
+                sum[i][j / 4][j % 4]        = kh ? acc[MINE + i][j / 4][j % 4] : acc[i][j / 4][j % 4];
+            }
+        __syncthreads();
+#pragma unroll
+        for(int i = 0; i < MINE; ++i)
+#pragma unroll
+            for(int j = 0; j < NG * 4; ++j)
+                sum[i][j / 4][j % 4] += there[(i * NG * 4 + j) * 64];
+    }
+    else
+#pragma unroll
+        for(int i = 0; i < MINE; ++i)
+#pragma unroll
+            for(int j = 0; j < NG * 4; ++j)
+                sum[i][j / 4][j % 4] = acc[i][j / 4][j % 4];
+#pragma unroll
+    for(int i = 0; i < MINE; ++i)
+    {
+        const int r = wm * (BM / WM) + (kh * MINE + i) * 16 + (lane & 15);
         if(r >= t.rows)
             continue;
-        if(p.ksplit > 1)
-        {
-            int* const row = p.ws + ((int64_t)run * p.M + t.m0 + r) * p.N * (GATED ? 2 : 1);
 #pragma unroll
-            for(int h = 0; h < 2; ++h)
+        for(int g = 0; g < NG; ++g)
+        {
+            const int at = wn * NG + g, n = n0 + at * (GATED ? 32 : 64);
+            if(p.ksplit > 1)
             {
-                const int c = n + 8 * q + (GATED ? 0 : 32 * h);
-                int* const to = row + (GATED && h ? p.N : 0);
-                store_room<4>(to + c, acc[i][2 * h], (p.N - c) * 4, false);
-                store_room<4>(to + c + 4, acc[i][2 * h + 1], (p.N - c - 4) * 4, false);
+                int* const row = p.ws + ((int64_t)run * p.M + t.m0 + r) * p.N * (GATED ? 2 : 1);
+#pragma unroll
+                for(int h = 0; h < 2; ++h)
+                {
+                    const int c = n + 8 * q + (GATED ? 0 : 32 * h);
+                    int* const to = row + (GATED && h ? p.N : 0);
+                    store_room<4>(to + c, sum[i][g][2 * h], (p.N - c) * 4, false);
+                    store_room<4>(to + c + 4, sum[i][g][2 * h + 1], (p.N - c - 4) * 4, false);
+                }
             }
+            else
+                i8_finish<T, GATED>(reinterpret_cast<T*>(p.c) + (int64_t)(t.m0 + r) * p.ldc, n, p.N, q, sum[i][g], s_row[r], s_col + at * 64, s_bias + at * 64);
         }
-        else
-            i8_finish<T, GATED>(reinterpret_cast<T*>(p.c) + (int64_t)(t.m0 + r) * p.ldc, n, p.N, q, acc[i], s_row[r], s_col + wn * 64, s_bias + wn * 64);
     }
 }
 
@@ -426,13 +501,17 @@ void cut(GemmI8Args& a, int BM, int cols)
 {
     a.tiles_m = (int)most_tiles_m(a, BM), a.tiles_n = (a.N + cols - 1) / cols;
 }
-template <typename T, bool GATED, int BM, int BN, int WM, int WN, int NST>
+template <typename T, bool GATED, int BM, int BN, int WM, int WN, int KH, int NST>
 hipError_t launch_tiles(GemmI8Args& a, hipStream_t s)
 {
+    constexpr int kLds = NST * (BM + BN) * 128 + (BM + 2 * BN) * 4;
+    auto* const kernel = &gemm_i8_tile_kernel<T, GATED, BM, BN, WM, WN, KH, NST>;
+    hipError_t e       = kLds > 65536 ? hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kLds) : hipSuccess;
+    if(e != hipSuccess)
+        return e;
     cut(a, BM, GATED ? BN / 2 : BN);
-    hipLaunchKernelGGL((gemm_i8_tile_kernel<T, GATED, BM, BN, WM, WN, NST>), dim3((unsigned)a.tiles_m * (unsigned)a.tiles_n * (unsigned)a.ksplit),
-                       dim3(WM * WN * 64), 0, s, a);
-    hipError_t e = hipGetLastError();
+    hipLaunchKernelGGL(kernel, dim3((unsigned)a.tiles_m * (unsigned)a.tiles_n * (unsigned)a.ksplit), dim3(WM * WN * KH * 64), kLds, s, a);
+    e = hipGetLastError();
     if(e != hipSuccess || a.ksplit == 1)
         return e;
     const int quads = (a.N + 3) / 4;
@@ -448,10 +527,11 @@ hipError_t launch_direct(GemmI8Args& a, hipStream_t s)
 }
 
 // Which kernel, and into how many runs K is cut. us of a step (a K tile) that one CU's tiles take, as measured (rows x 4096 x 4096):
-//   64 x 128, four stages    0.43, all CUs busy 0.50         128 rows 17.7 (in four runs 14.9), 512: 20.1
-//   128 x 128, two stages    0.52 to 0.65, two a CU 0.98     512: 22.3, 1024: 24.5, 2048: 34.8 (64 x 128: 36.2, 70.9; 256 x 256: 38.7, 39.7)
+//   64 x 128, four stages    0.29, all CUs busy 0.33         128 rows 13.5, 512: 15.6
+//   128 x 128, four stages   0.37, all CUs busy 0.44         512: 18.7, 1024: 22.4, 2048: 43 (64 x 128: 28.8, 55)
+//   128 x 128, two stages    0.57 to 0.63, two a CU 0.93 to 0.98     512: 22.4, 1024: 25, 2048: 35 to 38 (256 x 256: 39, 44)
 //   256 x 256, four waves    1.05, all CUs busy 1.47         4096: 51.6 (128 x 128 66.3), 4096 x 11008: 145 (213)
-// and about 4 us around the steps. A run costs 3 us more and its sums' way to the workspace and back.
+// and about 4 us around the steps, which a second round pays again where a CU holds one workgroup. A run costs 3 us more and its sums' way to the workspace and back.
 // Up to 16 rows the direct kernel of one row tile, 11008 x 4096: 1 row 10.4, 16 rows 13.6 (64 x 128 tiles in two runs 14.7); 8 waves where K is
 // long (4096 x 11008: 9.9 where four take 10.7). To 64 rows the direct kernel of two row tiles where its workgroups find a CU each, 4096 x 4096
 // 10.6 us for 32 rows (11.8 in the best runs of tiles), 11008 x 4096 18 (15.6).
@@ -470,8 +550,9 @@ enum
     kDirect8 = 2, // the same, eight waves
     kDirect2 = 3, // 32 x 32
     kTile64  = 4, // 64 x 128
-    kTile128 = 5, // 128 x 128
-    kTile256 = 6  // 256 x 256
+    kTile128 = 5, // 128 x 128, two workgroups a CU
+    kTile256 = 6, // 256 x 256
+    kDeep128 = 7  // 128 x 128, four stages
 };
 
 // whether the kernels of 16-byte vectors take a call: K, strides and addresses in whole vectors, and what a tile may read within 32-bit
@@ -520,8 +601,10 @@ Plan plan(const GemmI8Args& a, int64_t workspace_bytes)
         if(sums > (double)workspace_bytes)
             continue;
         const int64_t n64 = tiles(64, 128) * runs, n128 = tiles(128, 128) * runs, rest = n128 % 512;
-        compare(3.5 + join + per * (n64 < 256 ? 0.43 + 0.07 * (double)n64 / 256 : 0.50) * rounds(n64), Plan{kTile64, runs, per});
-        compare(3.5 + join + per * (0.98 * (double)(n128 / 512) + (rest == 0 ? 0.0 : rest > 256 ? 0.98 : 0.52 + 0.13 * (double)rest / 256)),
+        const double r64 = rounds(n64), s64 = (double)n64 / (256 * r64), r128 = rounds(n128), s128 = (double)n128 / (256 * r128);
+        compare(join + r64 * (3.9 + 0.5 * s64 + per * (0.285 + 0.045 * s64)), Plan{kTile64, runs, per});
+        compare(join + r128 * (4.8 + 4 * s128 * s128 + per * (0.365 + 0.08 * s128)), Plan{kDeep128, runs, per});
+        compare(3.5 + join + per * (0.98 * (double)(n128 / 512) + (rest == 0 ? 0.0 : rest > 256 ? 0.93 : 0.52 + 0.13 * (double)rest / 256)),
                 Plan{kTile128, runs, per});
     }
     return best;
@@ -543,8 +626,9 @@ hipError_t launch(GemmI8Args& a, int64_t workspace_bytes, hipStream_t s)
     case kDirect1: return launch_direct<T, GATED, 1, GATED ? 2 : 1, 4>(a, s);
     case kDirect8: return launch_direct<T, GATED, 1, GATED ? 2 : 1, 8>(a, s);
     case kDirect2: return launch_direct<T, GATED, 2, 2, 8>(a, s);
-    case kTile64: return launch_tiles<T, GATED, 64, 128, 2, 2, 4>(a, s);
-    case kTile128: return launch_tiles<T, GATED, 128, 128, 4, 2, 2>(a, s);
+    case kTile64: return launch_tiles<T, GATED, 64, 128, 2, 2, 2, 4>(a, s);
+    case kTile128: return launch_tiles<T, GATED, 128, 128, 4, 2, 1, 2>(a, s);
+    case kDeep128: return launch_tiles<T, GATED, 128, 128, 2, 2, 2, 4>(a, s);
     case kTile256: return gemm_i8_big_launch(a, type_of<T>(), most_tiles_m(a, 256), s);
     default: break;
     }
@@ -584,7 +668,7 @@ int64_t gemm_i8_scaled_workspace(int M, int N, int K, int gated)
 
 void gemm_i8_scaled_plan(const GemmI8Args& a, int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs)
 {
-    constexpr int m[] = {128, 16, 16, 32, 64, 128, 256}, n[] = {128, 16, 16, 32, 128, 128, 256};
+    constexpr int m[] = {128, 16, 16, 32, 64, 128, 256, 128}, n[] = {128, 16, 16, 32, 128, 128, 256, 128};
     const Plan w      = plan(a, workspace_bytes);
     *tile_m = m[w.kind], *tile_n = n[w.kind] * (a.gated && w.kind <= kDirect8 && w.kind != kAny ? 2 : 1), *k_runs = w.kind == kAny ? 0 : w.ksplit;
 }
