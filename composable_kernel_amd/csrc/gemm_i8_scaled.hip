@@ -23,7 +23,7 @@ __device__ __forceinline__ i32x4 ragged16(const int8_t* row, int k, int K, bool 
 }
 
 // Any K, leading dimension and address: 128 rows x 128 rows of B, four waves of 64 x 64, the operands through registers into LDS, a K
-// tile of 128 ahead.
+// tile of 128 ahead. 1 / 4096 x 11008 x 4100: 74 / 735 us, where K = 4096 takes 9.7 / 148: a tile waits for its loads at each step.
 template <typename T, bool GATED>
 __global__ __launch_bounds__(256) void gemm_i8_any_kernel(GemmI8Args p)
 {
@@ -110,17 +110,19 @@ __global__ __launch_bounds__(256) void gemm_i8_any_kernel(GemmI8Args p)
 }
 
 // BM rows x BN rows of B, WM x WN x KH waves, NST stages of operands in LDS: the loads of a K tile (128) are asked for NST - 1 tiles
-// ahead. LDS bounds the steps (rows x columns of a step: what the waves read and the loads write, at 128 bytes a clock: 64 x 128
-// 0.23 us at 2.4 GHz, 128 x 128 0.31 with waves of 64 x 64, 0.42 with 32 x 64), and with one wave a SIMD its latency would. So KH = 2 waves
-// share an output, one for each half of a K tile, where one workgroup fits a CU, and with more than two stages the next tile's fragments are
-// read while the present are multiplied: 64 x 128 from 0.43 to 0.29 us a step (128 rows of 4096 x 4096: 17.5 to 13.5).
+// ahead. The way from the L2s into LDS bounds the steps: 70 to 80 GB/s a CU with any of these tiles (64 x 128: 24 KB in 0.29 to 0.33 us, 128
+// x 128: 32 KB in 0.37 to 0.44), while LDS is active for 13 to 20 % of the time and the matrix cores for 16 to 25 %. To get there a SIMD needs two
+// waves, or one's wait for its fragments shows: KH = 2 waves share an output, one for each half of a K tile, where one workgroup fits a CU. With
+// PIPE the next tile's fragments are read while the present are multiplied. Both: 64 x 128 from 0.43 to 0.29 us a step (128 rows of 4096 x 4096
+// 17.5 to 13.5; KH alone 14.0).
 // The direct loads are inline assembly: the compiler, told of them, would wait for all of them before every LDS read of another
 // stage. Its own LDS reads it waits for itself; the wait for the direct loads stands in front of the barrier.
-// Columns behind K count by A's zeros alone: what B's loads bring there, and the rows of a tile that C does not have, are whatever the
-// resource's bounds let through.
+// The bounds of a resource are checked against a lane's offset without the scalar one, which holds K: a lane whose columns lie behind K asks
+// out of range, for A and for B, or it would read behind the last row's end.
 template <typename T, bool GATED, int BM, int BN, int WM, int WN, int KH, int NST>
 __global__ __launch_bounds__(WM* WN* KH * 64) void gemm_i8_tile_kernel(GemmI8Args p)
 {
+    constexpr bool PIPE = NST > 2;
     constexpr int NW = WM * WN * KH, MT = BM / WM / 16, NG = BN / WN / 64, NLA = BM / 8 / NW, NLB = BN / 8 / NW, LPT = NLA + NLB, COLS = GATED ? BN / 2 : BN;
     constexpr int A_TILE = BM * 128, B_AT = NST * A_TILE, B_TILE = BN * 128, S_AT = B_AT + NST * B_TILE;
     static_assert(BN / WN % 64 == 0 && BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "");
@@ -183,7 +185,7 @@ __global__ __launch_bounds__(WM* WN* KH * 64) void gemm_i8_tile_kernel(GemmI8Arg
             load16(ra, in ? oa[j] : kOutOfRange, k, base + st * A_TILE + (wave * NLA + j) * 1024);
 #pragma unroll
         for(int j = 0; j < NLB; ++j)
-            load16(rb, ob[j], k, base + B_AT + st * B_TILE + (wave * NLB + j) * 1024);
+            load16(rb, in ? ob[j] : kOutOfRange, k, base + B_AT + st * B_TILE + (wave * NLB + j) * 1024);
     };
     for(int g = g0; g < g0 + NST - 1; ++g)
         load_all(g);
@@ -236,7 +238,7 @@ __global__ __launch_bounds__(WM* WN* KH * 64) void gemm_i8_tile_kernel(GemmI8Arg
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    if constexpr(NST > 2)
+    if constexpr(PIPE)
     {
         // the fragments of a tile are read while the one before is multiplied
         Fragments x, y;
