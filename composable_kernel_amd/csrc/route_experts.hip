@@ -625,7 +625,8 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs p)
         auto row_of       = [&](int64_t t) { return reinterpret_cast<const X*>(p.x) + (t < last ? t : first) * p.stride_x; };
         float bias[EPL]   = {}, x[EPL];
         int64_t t         = first + wave * 4 + (l64 >> 4);
-        load_logits(row_of(t), lane * EPL, p.experts, x);
+        if(first < last) // (there may be tables to fill and no tokens)
+            load_logits(row_of(t), lane * EPL, p.experts, x);
         if constexpr(WIDE)
             load_logits(p.bias, lane * EPL, p.experts, bias);
         clear();

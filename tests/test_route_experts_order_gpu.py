@@ -56,3 +56,15 @@ def test_counts_that_no_byte_holds(kind, E, k, T, live):
     back = torch.full((T * k,), -1, dtype=torch.int32)
     back[order[:n]] = torch.arange(n, dtype=torch.int32)
     assert torch.equal(places, back)
+
+
+@pytest.mark.parametrize("E,k,bias", [(8, 2, False), (256, 8, True), (300, 32, True), (1024, 1, False)])
+def test_no_tokens(E, k, bias):
+    """The tables of no tokens: no logits are read, the offsets are 0."""
+    offsets = torch.full((E + 2,), 7, dtype=torch.int32, device="cuda")
+    op = ck.DeviceRouteExperts("f32")
+    arg = op.MakeArgumentPointer(None, torch.zeros(E, device="cuda") if bias else None, None, None, None, offsets, None, None, 0, E, k, E)
+    assert op.IsSupportedArgument(arg) and op.GetWorkSpaceSize(arg) == 0
+    op.MakeInvokerPointer().Run(arg, ck.StreamConfig(torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert offsets.tolist() == [0] * (E + 1) + [7]
