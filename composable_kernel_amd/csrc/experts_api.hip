@@ -164,9 +164,9 @@ int ckx_quantize_tokens_i8(const void* p_x, void* p_q, float* p_scale, int32_t M
     int st = ckx_quantize_tokens_i8_is_supported(M, K, stride_x, stride_q, x_type);
     if(st != CKX_OK)
         return st;
-    if(M == 0 || K == 0)
+    if(M == 0)
         return CKX_OK;
-    if(!p_x || !p_q || !p_scale)
+    if((K > 0 && (!p_x || !p_q)) || !p_scale)
         return api_fail(CKX_INVALID_VALUE, "null operand pointer");
     if(!aligned(p_x, size_of(x_type)) || !aligned(p_scale, 4))
         return api_fail(CKX_UNSUPPORTED, "operands must be aligned to their element size");

@@ -59,3 +59,13 @@ def test_values_half_way_between_codes(kind):
     ties = ((x.double() * 127 / amax) % 1 == 0.5).sum()
     assert int(ties) > 100
     check(x, kind)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_rows_of_nothing_have_the_smallest_scale(kind):
+    s = torch.full((6,), 7.0, device="cuda")
+    op = ck.DeviceTokenQuantizeI8(kind)
+    arg = op.MakeArgumentPointer(None, None, s, 5, 0, 0, 0)
+    op.MakeInvokerPointer().Run(arg, ck.StreamConfig(torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    assert s.tolist() == [float(torch.tensor(2.0 ** -100) / 127)] * 5 + [7.0]
