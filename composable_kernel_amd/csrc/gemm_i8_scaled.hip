@@ -112,9 +112,9 @@ __global__ __launch_bounds__(256) void gemm_i8_any_kernel(GemmI8Args p)
 // BM rows x BN rows of B, WM x WN x KH waves, NST stages of operands in LDS: the loads of a K tile (128) are asked for NST - 1 tiles
 // ahead. The way from the L2s into LDS bounds the steps: 70 to 80 GB/s a CU with any of these tiles (64 x 128: 24 KB in 0.29 to 0.33 us, 128
 // x 128: 32 KB in 0.37 to 0.44), while LDS is active for 13 to 20 % of the time and the matrix cores for 16 to 25 %. To get there a SIMD needs two
-// waves, or one's wait for its fragments shows: KH = 2 waves share an output, one for each half of a K tile, where one workgroup fits a CU. With
-// PIPE the next tile's fragments are read while the present are multiplied. Both: 64 x 128 from 0.43 to 0.29 us a step (128 rows of 4096 x 4096
-// 17.5 to 13.5; KH alone 14.0).
+// waves, or one's wait for its fragments shows. Either a CU holds two workgroups (KH = 1), or it holds one and KH = 2 waves share an output, one for
+// each half of a K tile; then the next tile's fragments are read while the present are multiplied. 64 x 128 with both from 0.43 to 0.29 us a step (128
+// rows of 4096 x 4096 17.5 to 13.5; two waves alone 14.0).
 // The direct loads are inline assembly: the compiler, told of them, would wait for all of them before every LDS read of another
 // stage. Its own LDS reads it waits for itself; the wait for the direct loads stands in front of the barrier.
 // The bounds of a resource are checked against a lane's offset without the scalar one, which holds K: a lane whose columns lie behind K asks
@@ -122,7 +122,6 @@ __global__ __launch_bounds__(256) void gemm_i8_any_kernel(GemmI8Args p)
 template <typename T, bool GATED, int BM, int BN, int WM, int WN, int KH, int NST>
 __global__ __launch_bounds__(WM* WN* KH * 64) void gemm_i8_tile_kernel(GemmI8Args p)
 {
-    constexpr bool PIPE = NST > 2;
     constexpr int NW = WM * WN * KH, MT = BM / WM / 16, NG = BN / WN / 64, NLA = BM / 8 / NW, NLB = BN / 8 / NW, LPT = NLA + NLB, COLS = GATED ? BN / 2 : BN;
     constexpr int A_TILE = BM * 128, B_AT = NST * A_TILE, B_TILE = BN * 128, S_AT = B_AT + NST * B_TILE;
     static_assert(BN / WN % 64 == 0 && BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "");
@@ -238,7 +237,7 @@ __global__ __launch_bounds__(WM* WN* KH * 64) void gemm_i8_tile_kernel(GemmI8Arg
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    if constexpr(PIPE)
+    if constexpr(KH > 1)
     {
         // the fragments of a tile are read while the one before is multiplied
         Fragments x, y;
@@ -537,9 +536,11 @@ hipError_t launch_direct(GemmI8Args& a, hipStream_t s)
 // Up to 16 rows the direct kernel of one row tile, 11008 x 4096: 1 row 10.4, 16 rows 13.6 (64 x 128 tiles in two runs 14.7); 8 waves where K is
 // long (4096 x 11008: 9.9 where four take 10.7). To 64 rows the direct kernel of two row tiles where its workgroups find a CU each, 4096 x 4096
 // 10.6 us for 32 rows (11.8 in the best runs of tiles), 11008 x 4096 18 (15.6).
-// Experts: by the rows that each has on average, since the host knows no more. Few: the direct kernel reads each expert's matrix once
-// (64 experts of 2816 x 4096 gated, 4 rows each: 129 us, 128 x 128 tiles 153; 8 rows: 152, 153); many: 256 x 256 tiles (128 rows: 209, 227;
-// 64 rows: 174, 194). K moves both borders: what a tile's beginning and end take, and what a workgroup reads again, weigh less beside a long one.
+// Experts: by the rows that each has on average, since the host knows no more. Few: the direct kernel reads each expert's matrix once (64 experts of
+// 2816 x 4096 gated, a row each: 86 us, 64 x 128 tiles 96; two rows: 103, 112; four: 128, 126; of 4096 x 1408 a row each 44.7, 44.9; two: 59, 51).
+// Many: 256 x 256 tiles (64 rows: 179 us, 64 x 128 tiles 185; 96: 181, 210; of 4096 x 1408 64 rows: 107, 99; 96: 121, 119; 128: 125, 139). What lies
+// between runs on 64 x 128 tiles (8 rows: 137, 128 x 128 tiles of two stages 156; 32: 156, 169). K moves both borders: what a tile's beginning and end
+// take weighs less beside a long one.
 struct Plan
 {
     int kind; // below
@@ -554,7 +555,8 @@ enum
     kTile64  = 4, // 64 x 128
     kTile128 = 5, // 128 x 128, two workgroups a CU
     kTile256 = 6, // 256 x 256
-    kDeep128 = 7  // 128 x 128, four stages
+    kDeep128 = 7, // 128 x 128, four stages
+    kPair64  = 8  // 64 x 128, two workgroups a CU: the experts' form, where the loads of one fill the other's beginning and end
 };
 
 // whether the kernels of 16-byte vectors take a call: K, strides and addresses in whole vectors, and what a tile may read within 32-bit
@@ -576,7 +578,7 @@ Plan plan(const GemmI8Args& a, int64_t workspace_bytes)
     if(a.offsets)
     {
         const double rows = (double)a.M / a.experts;
-        return Plan{rows * 1024 <= a.K ? kDirect1 : rows * a.K >= 1 << 18 ? kTile256 : kTile128, 1, steps};
+        return Plan{rows * 1280 <= a.K ? kDirect1 : rows * (a.K + 2560) >= 426000 ? kTile256 : kPair64, 1, steps};
     }
     if(a.M <= 16)
         return Plan{a.K > 8192 ? kDirect8 : kDirect1, 1, steps};
@@ -630,6 +632,7 @@ hipError_t launch(GemmI8Args& a, int64_t workspace_bytes, hipStream_t s)
     case kDirect2: return launch_direct<T, GATED, 2, 2, 8>(a, s);
     case kTile64: return launch_tiles<T, GATED, 64, 128, 2, 2, 2, 4>(a, s);
     case kTile128: return launch_tiles<T, GATED, 128, 128, 4, 2, 1, 2>(a, s);
+    case kPair64: return launch_tiles<T, GATED, 64, 128, 2, 2, 1, 3>(a, s);
     case kDeep128: return launch_tiles<T, GATED, 128, 128, 2, 2, 2, 4>(a, s);
     case kTile256: return gemm_i8_big_launch(a, type_of<T>(), most_tiles_m(a, 256), s);
     default: break;
@@ -648,14 +651,14 @@ hipError_t launch_form(GemmI8Args& a, int64_t workspace_bytes, hipStream_t s)
 } // namespace
 
 // a launch has fewer than 2^32 threads, 512 a workgroup at most: one for 64 x 128 outputs (experts: 128 x 128), and where the rows are
-// few (experts: under 128 each, which K <= 131071 makes of the plan's border) for 16 x 16
+// few (experts: under 256 each, which the plan's borders stay below) for 16 x 16
 bool gemm_i8_scaled_fits(int M, int N, int gated, int experts)
 {
     GemmI8Args a{};
     a.M = M, a.experts = experts;
     const int none     = 0;
     a.offsets          = experts ? &none : nullptr; // (says that there are experts)
-    const bool few     = experts ? M < (int64_t)experts * 128 : M <= 64;
+    const bool few     = experts ? M < (int64_t)experts * 256 : M <= 64;
     const int64_t wide = (int64_t)N * (gated ? 2 : 1);
     return most_tiles_m(a, few ? 16 : experts ? 128 : 64) * (wide / (few ? 16 : 128) + 2) < (1ll << 32) / 512;
 }
@@ -670,7 +673,7 @@ int64_t gemm_i8_scaled_workspace(int M, int N, int K, int gated)
 
 void gemm_i8_scaled_plan(const GemmI8Args& a, int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs)
 {
-    constexpr int m[] = {128, 16, 16, 32, 64, 128, 256, 128}, n[] = {128, 16, 16, 32, 128, 128, 256, 128};
+    constexpr int m[] = {128, 16, 16, 32, 64, 128, 256, 128, 64}, n[] = {128, 16, 16, 32, 128, 128, 256, 128, 128};
     const Plan w      = plan(a, workspace_bytes);
     *tile_m = m[w.kind], *tile_n = n[w.kind] * (a.gated && w.kind <= kDirect8 && w.kind != kAny ? 2 : 1), *k_runs = w.kind == kAny ? 0 : w.ksplit;
 }

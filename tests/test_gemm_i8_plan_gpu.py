@@ -35,7 +35,7 @@ def test_a_workspace_too_small_for_the_runs_is_left_alone():
 
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("gathered", [False, True])
-@pytest.mark.parametrize("rows,E,N,K,tile", [(20, 16, 100, 2048, 16), (200, 4, 130, 272, 128), (2400, 3, 200, 400, 256), (200, 4, 130, 100, 0)])
+@pytest.mark.parametrize("rows,E,N,K,tile", [(20, 16, 100, 2048, 16), (200, 4, 130, 272, 64), (2400, 3, 200, 400, 256), (200, 4, 130, 100, 0)])
 def test_plan_of_experts(gated, gathered, rows, E, N, K, tile):
     g = ep.gen(rows + N)
     R, wide = 50, N * (1 + gated)
