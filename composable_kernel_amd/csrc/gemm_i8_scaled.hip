@@ -1,5 +1,7 @@
 // int8 GEMM with a scale for each token and channel, dense and for each expert's rows (formulas: include/ckx.h,
 // ckx_gemm_i8_tokenscale and ckx_experts_gemm_i8).
+#include <cmath>
+
 #include "gemm_i8_big.hpp"
 
 namespace ckx {
@@ -536,11 +538,7 @@ hipError_t launch_direct(GemmI8Args& a, hipStream_t s)
 // Up to 16 rows the direct kernel of one row tile, 11008 x 4096: 1 row 10.4, 16 rows 13.6 (64 x 128 tiles in two runs 14.7); 8 waves where K is
 // long (4096 x 11008: 9.9 where four take 10.7). To 64 rows the direct kernel of two row tiles where its workgroups find a CU each, 4096 x 4096
 // 10.6 us for 32 rows (11.8 in the best runs of tiles), 11008 x 4096 18 (15.6).
-// Experts: by the rows that each has on average, since the host knows no more. Few: the direct kernel reads each expert's matrix once (64 experts of
-// 2816 x 4096 gated, a row each: 86 us, 64 x 128 tiles 96; two rows: 103, 112; four: 128, 126; of 4096 x 1408 a row each 44.7, 44.9; two: 59, 51).
-// Many: 256 x 256 tiles (64 rows: 179 us, 64 x 128 tiles 185; 96: 181, 210; of 4096 x 1408 64 rows: 107, 99; 96: 121, 119; 128: 125, 139). What lies
-// between runs on 64 x 128 tiles (8 rows: 137, 128 x 128 tiles of two stages 156; 32: 156, 169). K moves both borders: what a tile's beginning and end
-// take weighs less beside a long one.
+// Experts: experts_plan, by the rows that experts have on average, since the host knows no more.
 struct Plan
 {
     int kind; // below
@@ -556,7 +554,7 @@ enum
     kTile128 = 5, // 128 x 128, two workgroups a CU
     kTile256 = 6, // 256 x 256
     kDeep128 = 7, // 128 x 128, four stages
-    kPair64  = 8  // 64 x 128, two workgroups a CU: the experts' form, where the loads of one fill the other's beginning and end
+    kPair64  = 8  // 64 x 128, two workgroups a CU, for experts: the loads of one fill the other's beginning and end
 };
 
 // whether the kernels of 16-byte vectors take a call: K, strides and addresses in whole vectors, and what a tile may read within 32-bit
@@ -570,16 +568,47 @@ bool whole_vectors(const GemmI8Args& a)
     return a.K > 0 && (odd & 15) == 0 && rows_a * a.lda <= kMost && rows_b * a.ldb <= kMost && a.K <= kMost;
 }
 
+// us = 2 + (work^3 + memory^3)^(1/3): memory the bytes that a launch cannot do without at the rate that the kernel reaches, work its rounds of tiles
+// (slots at a time), each with what a tile's beginning and end take and its K tiles, which take longer the more slots are in use. Fitted to 310 products
+// of 4 to 128 experts, 0.1 to 4800 rows each, K 256 to 4096: on average 2.8 % from the best of the five, where borders by rows and K alone were
+// 18 % and up to 3.3 times (150 rows of 606 x 3080 in each of 8 experts: 13.1 us on 64 x 128 tiles, 32 on 256 x 256). Examples, 64 experts of 2816 x 4096
+// gated: a row each 86 direct, 96 on 64 x 128; 8 rows 151, 137 (128 x 128: 156); 64 rows 185 on 64 x 128, 179 on 256 x 256.
+struct ExpertsCost
+{
+    int kind, rows, cols, slots;
+    double end, step, busy, mb_per_us, uneven;
+};
+constexpr ExpertsCost kExpertsCosts[] = {{kDirect1, 16, 16, 2048, 2.49, 0.04, 0.70, 5.27, -0.61}, {kPair64, 64, 128, 512, 3.88, 0.31, 0.58, 5.96, 0.25},
+                                         {kTile128, 128, 128, 512, 3.33, 0.39, 0.93, 5.87, 0.21}, {kTile256, 256, 256, 256, 8.14, 0.70, 0.81, 6.13, 0.18},
+                                         {kTile64, 64, 128, 256, 3.58, 0.24, 0.26, 5.60, 0.28}};
+Plan experts_plan(const GemmI8Args& a, int steps)
+{
+    const double rows = (double)a.M / a.experts, used = a.experts * (1 - std::exp(-rows)), wide = (double)a.N * (a.gated ? 2 : 1);
+    const double mb   = (used * wide * a.K + (double)(a.rows ? a.rows_a : a.M) * a.K + 2.0 * a.M * a.N) * 1e-6;
+    Plan best{kPair64, 1, steps};
+    double least = 1e300;
+    for(const ExpertsCost& c : kExpertsCosts)
+    {
+        const int cols     = c.cols * (c.kind == kDirect1 && a.gated ? 2 : 1);
+        double tiles       = rows > c.rows / 2 ? a.M / (double)c.rows + 0.5 * a.experts : used; // (an expert's last is half full)
+        tiles              = (tiles > used ? tiles : used);
+        const double n     = (tiles < a.M ? tiles : a.M) * std::ceil(wide / cols) / c.slots;
+        const double turns = n > 1 && n + c.uneven > 1 ? n + c.uneven : 1;
+        const double work = turns * (c.end + steps * (c.step + c.busy * (n < 1 ? n : 1))), memory = mb / c.mb_per_us;
+        const double us   = std::cbrt(work * work * work + memory * memory * memory);
+        if(us < least)
+            least = us, best.kind = c.kind;
+    }
+    return best;
+}
+
 Plan plan(const GemmI8Args& a, int64_t workspace_bytes)
 {
     const int steps = (int)(((int64_t)a.K + 127) / 128);
     if(!whole_vectors(a))
         return Plan{kAny, 1, steps};
     if(a.offsets)
-    {
-        const double rows = (double)a.M / a.experts;
-        return Plan{rows * 1280 <= a.K ? kDirect1 : rows * (a.K + 2560) >= 426000 ? kTile256 : kPair64, 1, steps};
-    }
+        return experts_plan(a, steps);
     if(a.M <= 16)
         return Plan{a.K > 8192 ? kDirect8 : kDirect1, 1, steps};
     const int64_t wide = (int64_t)a.N * (a.gated ? 2 : 1);

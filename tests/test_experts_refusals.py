@@ -248,7 +248,8 @@ def test_plans():
     few = lambda **kw: capi.experts_gemm_i8_plan(experts(**kw))
     assert few(rows=0) == (0, 0, 0) and few(experts=0) == (0, 0, 0)
     assert few(rows=8, K=4096) == (16, 16, 1) and few(rows=8, K=4096, gated=1) == (16, 32, 1)
-    assert few(rows=64, K=512) == (64, 128, 1) and few(rows=1024, K=4096) == (256, 256, 1)
+    assert few(rows=256, N=4096, K=4096)[:2] == (64, 128) and few(rows=512, N=4096, K=512)[:2] == (128, 128)
+    assert few(rows=2048, N=4096, K=4096) == (256, 256, 1)
     assert few(K=136)[2] == 0 and few(batch=96 * 128 + 8)[2] == 0
     # rows gathered from all of A have to lie within 2 GiB, and rows in order need not
     far = experts(rows=2048, rows_a=1 << 20, K=4096)

@@ -35,11 +35,50 @@ def test_a_workspace_too_small_for_the_runs_is_left_alone():
 
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("gathered", [False, True])
-@pytest.mark.parametrize("rows,E,N,K,tile", [(20, 16, 100, 2048, 16), (200, 4, 130, 272, 64), (2400, 3, 200, 400, 256), (200, 4, 130, 100, 0)])
+@pytest.mark.parametrize("rows,E,N,K,tile", [(20, 16, 100, 2048, 16), (200, 4, 130, 272, 16), (2400, 3, 200, 400, 64), (200, 4, 130, 100, 0),
+                                             (400, 8, 2100, 1040, 64), (708, 8, 2100, 272, 128), (6000, 8, 2100, 272, 256)])
 def test_plan_of_experts(gated, gathered, rows, E, N, K, tile):
     g = ep.gen(rows + N)
     R, wide = 50, N * (1 + gated)
     counts = torch.multinomial(torch.tensor([1.0] + [0.2] * (E - 1)), rows, replacement=True, generator=g).bincount(minlength=E)
+    of_experts(g, counts, rows, E, N, K, R, wide, gated, gathered, tile)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("gathered", [False, True])
+@pytest.mark.parametrize("counts", [[0, 1, 255, 256, 257, 0, 5200, 31], [6000, 0, 0, 0, 0, 0, 0, 0], [0, 0, 0, 0, 0, 0, 0, 6000], [128, 129, 127, 512, 513, 511, 4000, 80]])
+def test_experts_of_every_size_on_the_largest_tiles(gated, gathered, counts):
+    of_experts(ep.gen(sum(counts[:5])), torch.tensor(counts), 6000, 8, 2100, 272, 50, 2100 * (1 + gated), gated, gathered, 256)
+
+
+def test_rows_outside_a_and_outside_c_on_the_largest_tiles():
+    """Row numbers that A does not have count as rows of zeros; offsets past C's rows are cut."""
+    rows, E, N, K, R = 6000, 8, 2100, 272, 40
+    g = ep.gen(9)
+    a, sa, b, sb = ep.codes(g, (R, K)), torch.rand(R, generator=g), ep.codes(g, (E, N, K)), torch.rand(E, N, generator=g) / 100
+    pick = torch.randint(-R, 3 * R, (rows,), generator=g, dtype=torch.int32)
+    pick[7] = -2 ** 31
+    offsets = torch.tensor([-5, 700, 700, 2000, 1900, 2500, 3000, 5000, 9000], dtype=torch.int32)
+    desc = capi.ExpertsDesc(rows, R, E, N, K, K, K, N, 1, 0, capi.TYPE_F32, 0, N * K)
+    assert capi.experts_gemm_i8_plan(desc, True)[0] == 256
+    c = torch.full((rows + 3, N), 55.0, device="cuda")
+    op = ck.DeviceExpertsGemmI8("f32")
+    arg = op.MakeArgumentPointer(a.cuda(), b.cuda(), c, sa.cuda(), sb.cuda(), None, offsets.cuda(), pick.cuda(), rows, R, E, N, K, K, K, N, N * K)
+    op.MakeInvokerPointer().Run(arg, stream())
+    torch.cuda.synchronize()
+    c = c.cpu()
+    assert bool((c[rows:] == 55).all())
+    for e, (i, j) in enumerate([(0, 700), (700, 700), (700, 2000), (2000, 1900), (2000, 2500), (2500, 3000), (3000, 5000), (5000, 6000)]):
+        if e in (2, 4) or i >= j:                    # (rows that two experts claim are either's)
+            continue
+        from_ = pick[i:j].long()
+        there = (from_ >= 0) & (from_ < R)
+        at = from_.clamp(0, R - 1)
+        want, bound = ep.scaled(a[at] * there[:, None], b[e], sa[at] * there, sb[e], None, False, torch.float32)
+        ep.near(c[i:j], want, bound, e)
+
+
+def of_experts(g, counts, rows, E, N, K, R, wide, gated, gathered, tile):
     offsets = torch.cat([torch.zeros(1, dtype=torch.long), counts.cumsum(0)]).int()
     b, sb, bias = ep.codes(g, (E, wide, K)), (0.5 + torch.rand(E, wide, generator=g)) / 60 / K ** 0.5, ep.normal(g, (E, wide))
     pick = torch.randint(0, R * 2, (rows,), generator=g, dtype=torch.int32)
