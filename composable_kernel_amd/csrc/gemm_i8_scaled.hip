@@ -534,10 +534,12 @@ hipError_t launch_direct(GemmI8Args& a, hipStream_t s)
 //   128 x 128, four stages   0.37, all CUs busy 0.44         512: 18.7, 1024: 22.4, 2048: 43 (64 x 128: 28.8, 55)
 //   128 x 128, two stages    0.57 to 0.63, two a CU 0.93 to 0.98     512: 22.4, 1024: 25, 2048: 35 to 38 (256 x 256: 39, 44)
 //   256 x 256, four waves    1.05, all CUs busy 1.47         4096: 51.6 (128 x 128 66.3), 4096 x 11008: 145 (213)
-// and about 4 us around the steps, which a second round pays again where a CU holds one workgroup. A run costs 3 us more and its sums' way to the workspace and back.
+// and about 4 us around the steps, which a second round pays again where a CU holds one workgroup. Runs cost 4 us more and their sums' way to the workspace
+// and back.
 // Up to 16 rows the direct kernel of one row tile, 11008 x 4096: 1 row 10.4, 16 rows 13.6 (64 x 128 tiles in two runs 14.7); 8 waves where K is
 // long (4096 x 11008: 9.9 where four take 10.7). To 64 rows the direct kernel of two row tiles where its workgroups find a CU each, 4096 x 4096
-// 10.6 us for 32 rows (11.8 in the best runs of tiles), 11008 x 4096 18 (15.6).
+// 10.6 us for 32 rows (11.8 in the best runs of tiles), 11008 x 4096 18 (15.6). To 128 rows the direct kernel of one row tile where N is short (its
+// cost: TileCost): 102 rows of 343 x 2176 gated 6.4 us (six runs of 64 x 128 tiles 18.4), 80 of 640 x 6544 7.1 (13.7).
 // Experts: experts_plan, by the rows that experts have on average, since the host knows no more.
 struct Plan
 {
@@ -573,12 +575,18 @@ bool whole_vectors(const GemmI8Args& a)
 // of 4 to 128 experts, 0.1 to 4800 rows each, K 256 to 4096: on average 2.8 % from the best of the five, where borders by rows and K alone were
 // 18 % and up to 3.3 times (150 rows of 606 x 3080 in each of 8 experts: 13.1 us on 64 x 128 tiles, 32 on 256 x 256). Examples, 64 experts of 2816 x 4096
 // gated: a row each 86 direct, 96 on 64 x 128; 8 rows 151, 137 (128 x 128: 156); 64 rows 185 on 64 x 128, 179 on 256 x 256.
-struct ExpertsCost
+struct TileCost
 {
     int kind, rows, cols, slots;
     double end, step, busy, mb_per_us, uneven;
+    double us(double tiles, int steps, double mb) const
+    {
+        const double n = tiles / slots, turns = n > 1 && n + uneven > 1 ? n + uneven : 1;
+        const double work = turns * (end + steps * (step + busy * (n < 1 ? n : 1))), memory = mb / mb_per_us;
+        return 2 + std::cbrt(work * work * work + memory * memory * memory);
+    }
 };
-constexpr ExpertsCost kExpertsCosts[] = {{kDirect1, 16, 16, 2048, 2.49, 0.04, 0.70, 5.27, -0.61}, {kPair64, 64, 128, 512, 3.88, 0.31, 0.58, 5.96, 0.25},
+constexpr TileCost kExpertsCosts[] = {{kDirect1, 16, 16, 2048, 2.49, 0.04, 0.70, 5.27, -0.61}, {kPair64, 64, 128, 512, 3.88, 0.31, 0.58, 5.96, 0.25},
                                          {kTile128, 128, 128, 512, 3.33, 0.39, 0.93, 5.87, 0.21}, {kTile256, 256, 256, 256, 8.14, 0.70, 0.81, 6.13, 0.18},
                                          {kTile64, 64, 128, 256, 3.58, 0.24, 0.26, 5.60, 0.28}};
 Plan experts_plan(const GemmI8Args& a, int steps)
@@ -587,15 +595,12 @@ Plan experts_plan(const GemmI8Args& a, int steps)
     const double mb   = (used * wide * a.K + (double)(a.rows ? a.rows_a : a.M) * a.K + 2.0 * a.M * a.N) * 1e-6;
     Plan best{kPair64, 1, steps};
     double least = 1e300;
-    for(const ExpertsCost& c : kExpertsCosts)
+    for(const TileCost& c : kExpertsCosts)
     {
-        const int cols     = c.cols * (c.kind == kDirect1 && a.gated ? 2 : 1);
-        double tiles       = rows > c.rows / 2 ? a.M / (double)c.rows + 0.5 * a.experts : used; // (an expert's last is half full)
-        tiles              = (tiles > used ? tiles : used);
-        const double n     = (tiles < a.M ? tiles : a.M) * std::ceil(wide / cols) / c.slots;
-        const double turns = n > 1 && n + c.uneven > 1 ? n + c.uneven : 1;
-        const double work = turns * (c.end + steps * (c.step + c.busy * (n < 1 ? n : 1))), memory = mb / c.mb_per_us;
-        const double us   = std::cbrt(work * work * work + memory * memory * memory);
+        const int cols = c.cols * (c.kind == kDirect1 && a.gated ? 2 : 1);
+        double tiles   = rows > c.rows / 2 ? a.M / (double)c.rows + 0.5 * a.experts : used; // (an expert's last is half full)
+        tiles          = (tiles > used ? tiles : used);
+        const double us = c.us((tiles < a.M ? tiles : a.M) * std::ceil(wide / cols), steps, mb);
         if(us < least)
             least = us, best.kind = c.kind;
     }
@@ -622,6 +627,12 @@ Plan plan(const GemmI8Args& a, int64_t workspace_bytes)
         if(t < us)
             us = t, best = p;
     };
+    if(a.M <= 128)
+    {
+        constexpr TileCost direct{kDirect1, 16, 16, 2048, 1.27, 0.08, 0.57, 5.3, 0.22};
+        compare(direct.us((double)tiles(16, a.gated ? 32 : 16), steps, ((double)wide * a.K + (double)a.M * a.K + 2.0 * a.M * a.N) * 1e-6),
+                Plan{a.K > 8192 ? kDirect8 : kDirect1, 1, steps});
+    }
     if(a.M <= 64)
     {
         const double n = rounds(tiles(32, 32));
@@ -630,7 +641,7 @@ Plan plan(const GemmI8Args& a, int64_t workspace_bytes)
     for(int ks = 1; ks <= 16 && ks * 2 <= (steps > 1 ? steps : 2); ++ks)
     {
         const int per     = (steps + ks - 1) / ks, runs = (steps + per - 1) / per;
-        const double sums = runs > 1 ? 4.0 * a.M * wide * runs : 0.0, join = runs > 1 ? 3 + 2 * sums / 4e6 : 0.0;
+        const double sums = runs > 1 ? 4.0 * a.M * wide * runs : 0.0, join = runs > 1 ? 4 + 2 * sums / 4e6 : 0.0;
         if(sums > (double)workspace_bytes)
             continue;
         const int64_t n64 = tiles(64, 128) * runs, n128 = tiles(128, 128) * runs, rest = n128 % 512;
@@ -687,7 +698,7 @@ bool gemm_i8_scaled_fits(int M, int N, int gated, int experts)
     a.M = M, a.experts = experts;
     const int none     = 0;
     a.offsets          = experts ? &none : nullptr; // (says that there are experts)
-    const bool few     = experts ? M < (int64_t)experts * 256 : M <= 64;
+    const bool few     = experts ? M < (int64_t)experts * 256 : M <= 128;
     const int64_t wide = (int64_t)N * (gated ? 2 : 1);
     return most_tiles_m(a, few ? 16 : experts ? 128 : 64) * (wide / (few ? 16 : 128) + 2) < (1ll << 32) / 512;
 }
