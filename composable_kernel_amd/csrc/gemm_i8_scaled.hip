@@ -573,7 +573,7 @@ bool whole_vectors(const GemmI8Args& a)
 // us = 2 + (work^3 + memory^3)^(1/3): memory the bytes that a launch cannot do without at the rate that the kernel reaches, work its rounds of tiles
 // (slots at a time), each with what a tile's beginning and end take and its K tiles, which take longer the more slots are in use. Fitted to 310 products
 // of 4 to 128 experts, 0.1 to 4800 rows each, K 256 to 4096: on average 2.8 % from the best of the five, where borders by rows and K alone were
-// 18 % and up to 3.3 times (150 rows of 606 x 3080 in each of 8 experts: 13.1 us on 64 x 128 tiles, 32 on 256 x 256). Examples, 64 experts of 2816 x 4096
+// 18 % and up to 3.3 times (519 rows of 512 x 1040 in each of 4 experts: 10.4 us on 64 x 128 tiles, 23.4 on 256 x 256). Examples, 64 experts of 2816 x 4096
 // gated: a row each 86 direct, 96 on 64 x 128; 8 rows 151, 137 (128 x 128: 156); 64 rows 185 on 64 x 128, 179 on 256 x 256.
 struct TileCost
 {

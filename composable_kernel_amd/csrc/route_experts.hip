@@ -7,7 +7,7 @@
 // The tables are a stable counting sort of the tokens * top_k pairs. For few tokens one workgroup does all of it; otherwise
 // each workgroup leaves the counts of its tokens in the workspace and a second launch adds them up and places the pairs. Nothing in it depends on
 // the order in which waves run.
-// 16384 tokens of 256 experts, sigmoid, biases, groups, eight each: 27.4 us, of them 19 for the scores and picks (1683 vector instructions a wave of
+// 16384 tokens of 256 experts, sigmoid, biases, groups, eight each: 27.4 to 30 us, of them 19 to 21 for the scores and picks (1690 vector instructions a wave of
 // four tokens, 40 % of the cycles, the rest their order) and 8.5 for the tables; 64 experts 14.2, one token 5.7 with its launch.
 #include "experts.hpp"
 #include "f8.hpp"
@@ -625,8 +625,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(RouteArgs p)
         auto row_of       = [&](int64_t t) { return reinterpret_cast<const X*>(p.x) + (t < last ? t : first) * p.stride_x; };
         float bias[EPL]   = {}, x[EPL];
         int64_t t         = first + wave * 4 + (l64 >> 4);
-        if(first < last) // (there may be tables to fill and no tokens)
-            load_logits(row_of(t), lane * EPL, p.experts, x);
+        load_logits(row_of(t), lane * EPL, p.experts, x);
         if constexpr(WIDE)
             load_logits(p.bias, lane * EPL, p.experts, bias);
         clear();
@@ -850,6 +849,9 @@ int64_t route_workspace(int tokens, int experts)
 
 hipError_t route_launch(RouteArgs a, int x_type, hipStream_t s)
 {
+    // tables of no tokens: the kernel asks for a first row of logits all the same and looks at none of it; the offsets have the room
+    if(a.tokens == 0)
+        a.x = a.offsets;
     cut(a.tokens, a.experts, a.chunk_tokens, a.chunks);
     return x_type == CKX_TYPE_F32 ? launch_any<float>(a, s) : x_type == CKX_TYPE_F16 ? launch_any<_Float16>(a, s) : launch_any<__bf16>(a, s);
 }
