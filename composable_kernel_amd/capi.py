@@ -259,8 +259,8 @@ def gemm_f8_plan(M, N, K, lda=None, ldb=None, ldc=None, c_type=TYPE_BF16, worksp
 
 
 def gemm_i8_plan(M, N, K, lda=None, ldb=None, ldc=None, gated=False, c_type=TYPE_BF16, workspace_bytes=0):
-    """(rows of A, rows of B, K runs) of a workgroup of this token-scaled int8 GEMM (ckx_gemm_i8_tokenscale_plan); 0 runs: the kernel for any K
-    and stride."""
+    """(rows of A, rows of B, K runs) of a workgroup of this token-scaled int8 GEMM (ckx_gemm_i8_tokenscale_plan); 0 runs: the kernels for any
+    K and stride."""
     out = [C.c_int(0) for _ in range(3)]
     check(lib().ckx_gemm_i8_tokenscale_plan(M, N, K, K if lda is None else lda, K if ldb is None else ldb, N if ldc is None else ldc, int(gated), c_type,
                                             int(workspace_bytes), *map(C.byref, out)))

@@ -8,24 +8,22 @@ namespace ckx {
 
 namespace {
 
-// 16 bytes at column k of a row, zeros behind column K, any alignment
-__device__ __forceinline__ i32x4 ragged16(const int8_t* row, int k, int K, bool live)
+// 16 bytes of which `left` are there, zeros behind them, any alignment
+__device__ __forceinline__ i32x4 ragged16(const int8_t* at, int left)
 {
-    if(live && k + 16 <= K)
-        return load_vec<i32x4>(row + k);
+    if(left >= 16)
+        return load_vec<i32x4>(at);
     uint32_t w[4] = {0, 0, 0, 0};
-    if(live)
-    {
 #pragma unroll
-        for(int i = 0; i < 16; ++i)
-            if(k + i < K)
-                w[i >> 2] |= (uint32_t)(uint8_t)row[k + i] << (8 * (i & 3));
-    }
+    for(int i = 0; i < 16; ++i)
+        if(i < left)
+            w[i >> 2] |= (uint32_t)(uint8_t)at[i] << (8 * (i & 3));
     return i32x4{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
 }
 
 // Any K, leading dimension and address: 128 rows x 128 rows of B, four waves of 64 x 64, the operands through registers into LDS, a K
-// tile of 128 ahead. 1 / 4096 x 11008 x 4100: 74 / 735 us, where K = 4096 takes 9.7 / 148: a tile waits for its loads at each step.
+// tile of 128 ahead: asked for in front of the products, put into LDS behind them. 128 / 4096 x 11008 x 4100: 40 / 317 us, where K = 4096 takes 14.5 / 148:
+// unaligned vectors through registers.
 template <typename T, bool GATED>
 __global__ __launch_bounds__(256) void gemm_i8_any_kernel(GemmI8Args p)
 {
@@ -39,7 +37,8 @@ __global__ __launch_bounds__(256) void gemm_i8_any_kernel(GemmI8Args p)
         return;
     const int n0 = t.tn * (GATED ? BN / 2 : BN);
     i8_load_scales<GATED>(p, t.expert, n0, BN, tid, 256, sb, bias);
-    // a wave fills LDS rows wave * 32 ... + 31 of either tile, eight rows a load; chunk c of row r lies at c ^ (r & 7)
+    // a wave fills LDS rows wave * 32 ... + 31 of either tile, eight rows a load; chunk c of row r lies at c ^ (r & 7). Rows that are not there
+    // take another's place: C does not have them, or their scale is 0
     const int8_t *ra[4], *rb[4];
     int row[4], m[4];
 #pragma unroll
@@ -49,21 +48,35 @@ __global__ __launch_bounds__(256) void gemm_i8_any_kernel(GemmI8Args p)
 #pragma unroll
     for(int j = 0; j < 4; ++j)
     {
-        const int r = row[j];
-        ra[j]       = m[j] >= 0 ? p.a + (int64_t)m[j] * p.lda : nullptr;
         bool second;
-        const int n = n0 + i8_col_of<GATED>((uint32_t)r, second);
-        rb[j]       = n < p.N ? p.b + (int64_t)t.expert * p.batch_b + ((int64_t)n + (second ? p.N : 0)) * p.ldb : nullptr;
+        const int n = min(n0 + i8_col_of<GATED>((uint32_t)row[j], second), p.N - 1), kc = ((lane & 7) ^ (row[j] & 7)) * 16;
+        rb[j]       = p.b + (int64_t)t.expert * p.batch_b + ((int64_t)n + (second ? p.N : 0)) * p.ldb + kc;
+        ra[j]       = m[j] >= 0 ? p.a + (int64_t)m[j] * p.lda + kc : rb[j];
     }
-    auto load = [&](int stage, int g) {
+    struct Rows
+    {
+        i32x4 a[4], b[4];
+    };
+    auto fetch = [&](Rows& x, int g) {
+        if((g + 1) * 128 <= p.K)
+        {
+#pragma unroll
+            for(int j = 0; j < 4; ++j)
+                x.a[j] = load_vec<i32x4>(ra[j] + g * 128), x.b[j] = load_vec<i32x4>(rb[j] + g * 128);
+        }
+        else
+#pragma unroll
+            for(int j = 0; j < 4; ++j)
+            {
+                const int left = p.K - g * 128 - ((lane & 7) ^ (row[j] & 7)) * 16;
+                x.a[j] = ragged16(ra[j] + g * 128, left), x.b[j] = ragged16(rb[j] + g * 128, left);
+            }
+    };
+    auto put = [&](const Rows& x, int stage) {
+        uint8_t* const at = &lds[stage][0][wave * 4096 + lane * 16];
 #pragma unroll
         for(int j = 0; j < 4; ++j)
-        {
-            const int r = wave * 32 + j * 8 + (lane >> 3), k = g * 128 + ((lane & 7) ^ (r & 7)) * 16;
-            uint8_t* const at = &lds[stage][0][(wave * 32 + j * 8) * 128 + lane * 16];
-            *reinterpret_cast<i32x4*>(at)        = ragged16(ra[j], k, p.K, ra[j] != nullptr);
-            *reinterpret_cast<i32x4*>(at + TILE) = ragged16(rb[j], k, p.K, rb[j] != nullptr);
-        }
+            *reinterpret_cast<i32x4*>(at + j * 1024) = x.a[j], *reinterpret_cast<i32x4*>(at + j * 1024 + TILE) = x.b[j];
     };
     i32x4 acc[4][4];
 #pragma unroll
@@ -71,13 +84,17 @@ __global__ __launch_bounds__(256) void gemm_i8_any_kernel(GemmI8Args p)
 #pragma unroll
         for(int j = 0; j < 4; ++j)
             acc[i][j] = i32x4{0, 0, 0, 0};
+    Rows next;
     if(p.ksteps > 0)
-        load(0, 0);
+    {
+        fetch(next, 0);
+        put(next, 0);
+    }
     for(int g = 0; g < p.ksteps; ++g)
     {
         __syncthreads();
         if(g + 1 < p.ksteps)
-            load((g + 1) & 1, g + 1);
+            fetch(next, g + 1);
 #pragma unroll
         for(int ks = 0; ks < 2; ++ks)
         {
@@ -97,6 +114,8 @@ __global__ __launch_bounds__(256) void gemm_i8_any_kernel(GemmI8Args p)
                     acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j], af, acc[i][j], 0, 0, 0);
             }
         }
+        if(g + 1 < p.ksteps)
+            put(next, (g + 1) & 1); // (every wave has read it before this step's barrier)
     }
     __syncthreads(); // (K = 0: the scales)
 #pragma unroll
@@ -369,8 +388,8 @@ __global__ __launch_bounds__(256) void gemm_i8_join_kernel(GemmI8Args p, int qua
 // Few rows: a workgroup takes MT x NT tiles of 16 x 16 and its NW waves share the K tiles among them, each straight from memory into
 // its registers (the next K tile's 32 bytes a lane and tile row are on their way while one is multiplied); the waves' sums meet in LDS.
 // Nothing waits at a barrier until the end: what a product of few rows needs, which is bound by reading B once. Gated, the tiles of B
-// come in pairs, a gate's and its partner's.
-template <typename T, bool GATED, int MT, int NT, int NW>
+// come in pairs, a gate's and its partner's. ANY: any K, stride and address, 1 / 16 x 11008 x 4100 16 us.
+template <typename T, bool GATED, int MT, int NT, int NW, bool ANY>
 __global__ __launch_bounds__(NW * 64) void gemm_i8_direct_kernel(GemmI8Args p)
 {
     constexpr int BM = MT * 16, COLS = NT * 16 / (GATED ? 2 : 1);
@@ -391,10 +410,12 @@ __global__ __launch_bounds__(NW * 64) void gemm_i8_direct_kernel(GemmI8Args p)
         i32x4 a[MT][2], b[NT][2];
     };
     uint32_t oa[MT], ob[NT];
+    const int8_t *pa[MT], *pb[NT]; // (ANY)
 #pragma unroll
     for(int j = 0; j < NT; ++j)
     {
         const int n = n0 + (GATED ? j / 2 : j) * 16 + r;
+        pb[j]       = p.b + (int64_t)t.expert * p.batch_b + (int64_t)(min(n, p.N - 1) + (GATED && (j & 1) ? p.N : 0)) * p.ldb + q * 16;
         ob[j]       = n < p.N ? (uint32_t)(n - b0 + (GATED && (j & 1) ? p.N : 0)) * (uint32_t)p.ldb + q * 16 : kOutOfRange;
     }
     int row[MT], m[MT];
@@ -404,8 +425,38 @@ __global__ __launch_bounds__(NW * 64) void gemm_i8_direct_kernel(GemmI8Args p)
     i8_rows_of_a(p, t, row, m);
 #pragma unroll
     for(int i = 0; i < MT; ++i)
+    {
+        pa[i] = m[i] >= 0 ? p.a + (int64_t)m[i] * p.lda + q * 16 : pb[0]; // (a row that is not there: C does not have it, or its scale is 0)
         oa[i] = m[i] >= 0 ? (uint32_t)(m[i] - a0) * (uint32_t)p.lda + q * 16 : kOutOfRange;
+    }
     auto load = [&](Step& x, int g) {
+        if constexpr(ANY)
+        {
+            auto from = [&](auto whole, const int8_t* at, int h) {
+                const int k = g * 128 + h * 64;
+                if constexpr(decltype(whole)::value)
+                    return load_vec<i32x4>(at + k);
+                else
+                    return ragged16(at + k, p.K - k - q * 16);
+            };
+            auto both = [&](auto whole) {
+#pragma unroll
+                for(int h = 0; h < 2; ++h)
+                {
+#pragma unroll
+                    for(int j = 0; j < NT; ++j)
+                        x.b[j][h] = from(whole, pb[j], h);
+#pragma unroll
+                    for(int i = 0; i < MT; ++i)
+                        x.a[i][h] = from(whole, pa[i], h);
+                }
+            };
+            if((g + 1) * 128 <= p.K)
+                both(std::true_type{});
+            else
+                both(std::false_type{});
+        }
+        else
 #pragma unroll
         for(int h = 0; h < 2; ++h)
         {
@@ -521,11 +572,11 @@ hipError_t launch_tiles(GemmI8Args& a, hipStream_t s)
     hipLaunchKernelGGL((gemm_i8_join_kernel<T, GATED>), dim3((unsigned)(((int64_t)a.M * quads + 255) / 256)), dim3(256), 0, s, a, quads);
     return hipGetLastError();
 }
-template <typename T, bool GATED, int MT, int NT, int NW>
+template <typename T, bool GATED, int MT, int NT, int NW, bool ANY = false>
 hipError_t launch_direct(GemmI8Args& a, hipStream_t s)
 {
     cut(a, MT * 16, NT * 16 / (GATED ? 2 : 1));
-    hipLaunchKernelGGL((gemm_i8_direct_kernel<T, GATED, MT, NT, NW>), dim3((unsigned)a.tiles_m * (unsigned)a.tiles_n), dim3(NW * 64), 0, s, a);
+    hipLaunchKernelGGL((gemm_i8_direct_kernel<T, GATED, MT, NT, NW, ANY>), dim3((unsigned)a.tiles_m * (unsigned)a.tiles_n), dim3(NW * 64), 0, s, a);
     return hipGetLastError();
 }
 
@@ -548,7 +599,7 @@ struct Plan
 };
 enum
 {
-    kAny     = 0,
+    kAny     = 0, // 128 x 128, any K, stride and address
     kDirect1 = 1, // 16 x 16, four waves
     kDirect8 = 2, // the same, eight waves
     kDirect2 = 3, // 32 x 32
@@ -556,7 +607,8 @@ enum
     kTile128 = 5, // 128 x 128, two workgroups a CU
     kTile256 = 6, // 256 x 256
     kDeep128 = 7, // 128 x 128, four stages
-    kPair64  = 8  // 64 x 128, two workgroups a CU, for experts: the loads of one fill the other's beginning and end
+    kPair64  = 8, // 64 x 128, two workgroups a CU, for experts: the loads of one fill the other's beginning and end
+    kAnyFew  = 9  // 16 x 16, any K, stride and address
 };
 
 // whether the kernels of 16-byte vectors take a call: K, strides and addresses in whole vectors, and what a tile may read within 32-bit
@@ -611,7 +663,12 @@ Plan plan(const GemmI8Args& a, int64_t workspace_bytes)
 {
     const int steps = (int)(((int64_t)a.K + 127) / 128);
     if(!whole_vectors(a))
-        return Plan{kAny, 1, steps};
+    {
+        // (11008 x 4100: 16 rows 16 us on 16 x 16 tiles, 33 on 128 x 128; 32: 27, 34; 48: 38, 35; 64 experts of 2816 x 4100, 8 rows each: 201, 200)
+        const double rows = (double)a.M / (a.offsets ? a.experts : 1);
+        const int64_t n16 = most_tiles_m(a, 16) * ((a.N + 15) / 16);
+        return Plan{a.K > 0 && (rows <= (a.offsets ? 8 : 16) || (rows <= 48 && n16 <= 2048)) ? kAnyFew : kAny, 1, steps};
+    }
     if(a.offsets)
         return experts_plan(a, steps);
     if(a.M <= 16)
@@ -672,6 +729,7 @@ hipError_t launch(GemmI8Args& a, int64_t workspace_bytes, hipStream_t s)
     case kDirect2: return launch_direct<T, GATED, 2, 2, 8>(a, s);
     case kTile64: return launch_tiles<T, GATED, 64, 128, 2, 2, 2, 4>(a, s);
     case kTile128: return launch_tiles<T, GATED, 128, 128, 4, 2, 1, 2>(a, s);
+    case kAnyFew: return launch_direct<T, GATED, 1, GATED ? 2 : 1, 4, true>(a, s);
     case kPair64: return launch_tiles<T, GATED, 64, 128, 2, 2, 1, 3>(a, s);
     case kDeep128: return launch_tiles<T, GATED, 128, 128, 2, 2, 2, 4>(a, s);
     case kTile256: return gemm_i8_big_launch(a, type_of<T>(), most_tiles_m(a, 256), s);
@@ -713,9 +771,10 @@ int64_t gemm_i8_scaled_workspace(int M, int N, int K, int gated)
 
 void gemm_i8_scaled_plan(const GemmI8Args& a, int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs)
 {
-    constexpr int m[] = {128, 16, 16, 32, 64, 128, 256, 128, 64}, n[] = {128, 16, 16, 32, 128, 128, 256, 128, 128};
+    constexpr int m[] = {128, 16, 16, 32, 64, 128, 256, 128, 64, 16}, n[] = {128, 16, 16, 32, 128, 128, 256, 128, 128, 16};
     const Plan w      = plan(a, workspace_bytes);
-    *tile_m = m[w.kind], *tile_n = n[w.kind] * (a.gated && w.kind <= kDirect8 && w.kind != kAny ? 2 : 1), *k_runs = w.kind == kAny ? 0 : w.ksplit;
+    const bool any = w.kind == kAny || w.kind == kAnyFew, few = w.kind == kDirect1 || w.kind == kDirect8 || w.kind == kAnyFew;
+    *tile_m = m[w.kind], *tile_n = n[w.kind] * (a.gated && few ? 2 : 1), *k_runs = any ? 0 : w.ksplit;
 }
 
 hipError_t gemm_i8_scaled_launch(GemmI8Args a, int c_type, int64_t workspace_bytes, hipStream_t s)

@@ -627,7 +627,7 @@ int ckx_gemm_i8_tokenscale(const void* p_a, const void* p_b, void* p_c, const fl
                            int64_t workspace_bytes, void* stream);
 /* What a launch with 16-byte aligned A and B and this much workspace would use (pure host): the rows of A and of B that a workgroup
  * takes (16 x 16, gated 16 x 32, and 32 x 32: straight from memory; 64 x 128, 128 x 128, 256 x 256) and the runs that K is cut into;
- * 0 runs: the kernel for any K and stride, 128 x 128. Nothing to do (M or N 0): all 0. */
+ * 0 runs: the kernels for any K and stride, 16 x 16 and 128 x 128. Nothing to do (M or N 0): all 0. */
 int ckx_gemm_i8_tokenscale_plan(int32_t M, int32_t N, int32_t K, int32_t lda, int32_t ldb, int32_t ldc, int gated, int c_type,
                                 int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs);
 

@@ -14,7 +14,7 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("M,N,K,tile,runs", [(16, 100, 272, 16, 1), (13, 40, 9216, 16, 1), (40, 200, 1040, 16, 1), (62, 2000, 1040, 32, 1), (200, 130, 16384, 64, 2), (150, 4096, 256, 128, 1), (300, 4096, 1024, 64, 1),
-                                             (1000, 4100, 512, 128, 1), (2050, 4100, 512, 256, 1), (30, 64, 100, 128, 0)])
+                                             (1000, 4100, 512, 128, 1), (2050, 4100, 512, 256, 1), (30, 64, 100, 16, 0), (60, 64, 100, 128, 0), (1, 500, 4099, 16, 0), (130, 300, 4099, 128, 0)])
 def test_plan(kind, gated, M, N, K, tile, runs):
     N = N // 2 if gated and M > 100 else N
     need = capi.lib().ckx_gemm_i8_tokenscale_workspace_bytes(M, N, K, int(gated))
