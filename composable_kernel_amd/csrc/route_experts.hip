@@ -331,7 +331,7 @@ __device__ __forceinline__ void group_two(V& best, V& next, int lanes)
 template <typename V, int EPL>
 __device__ __forceinline__ V group_value(const RouteArgs& p, const V (&v)[EPL], int lanes)
 {
-    constexpr V kNone = -(V)__builtin_inff();
+    constexpr V kNone = -(V)__builtin_inff(), kLowest = (V)-3.402823466e38f;
     V best = kNone, next = kNone;
 #pragma unroll
     for(int i = 0; i < EPL; ++i)
@@ -340,7 +340,9 @@ __device__ __forceinline__ V group_value(const RouteArgs& p, const V (&v)[EPL], 
         best = most_of(best, v[i]);
     }
     group_two(best, next, lanes);
-    return p.group_best == 2 && next > kNone ? best + next : best;
+    // (two biases near the type's lowest value, as masks have them, are past it together: the group is there all the same. Its order among such
+    // groups is in doubt, since the room that their sums are given is infinite)
+    return p.group_best == 2 && next > kNone ? most_of(best + next, kLowest) : best;
 }
 
 // WIDE and ALL as above; `live`: of the lane's row of lanes. Scores in fp32 find the token's experts; those, one a lane, are computed in
