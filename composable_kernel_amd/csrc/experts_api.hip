@@ -135,6 +135,14 @@ int ckx_route_experts(const void* p_logits, const float* p_bias, const int32_t* 
         return api_fail(CKX_UNSUPPORTED, "the workspace is smaller than ckx_route_experts_workspace_bytes");
     if(need > 0 && !aligned(p_workspace, 16))
         return api_fail(CKX_INVALID_VALUE, "the workspace must be 16-byte aligned");
+    // (the second launch takes its counts as places, and the ids as numbers of experts)
+    const Span ws{p_workspace, need};
+    for(const Span& x : in)
+        if(ws.meets(x))
+            return api_fail(CKX_INVALID_VALUE, "the workspace lies on an input");
+    for(const Span& x : out)
+        if(ws.meets(x))
+            return api_fail(CKX_INVALID_VALUE, "the workspace lies on an output");
     ckx::RouteArgs a{};
     a.x = p_logits, a.bias = p_bias, a.live = p_num_tokens, a.ids = p_ids, a.weights = p_weights;
     a.offsets = p_offsets, a.rows = p_rows, a.places = p_places, a.ws = p_workspace;

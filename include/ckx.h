@@ -561,7 +561,7 @@ int ckx_paged_attention8(const void* p_q, void* p_o, const int32_t* p_block_tabl
  * quantise the tokens, multiply each expert's rows, add a token's rows up again. All entry points are asynchronous on
  * `stream`, allocate nothing, can be captured into a graph, and read the experts' tables and the number of tokens on the
  * device: a replay sees what they hold then. `stream`'s device has to be the current one. No output lies on an input, but
- * where a line below allows it. */
+ * where a line below allows it, and no workspace on either. */
 
 /* ---- each token's experts, their weights, and the experts' rows in order ---------------------------
  * x[t, e]: logits [num_tokens, num_experts] fp32, fp16 or bf16, rows stride_x apart; bias[e] fp32 (p_bias NULL: none).
