@@ -46,7 +46,8 @@ SYMBOLS = [
     "ckx_route_experts_is_supported", "ckx_route_experts", "ckx_route_experts_workspace_bytes",
     "ckx_quantize_tokens_i8_is_supported", "ckx_quantize_tokens_i8",
     "ckx_gemm_i8_tokenscale_is_supported", "ckx_gemm_i8_tokenscale", "ckx_gemm_i8_tokenscale_workspace_bytes", "ckx_gemm_i8_tokenscale_plan",
-    "ckx_experts_gemm_i8_is_supported", "ckx_experts_gemm_i8", "ckx_experts_gemm_i8_plan", "ckx_experts_combine_is_supported", "ckx_experts_combine",
+    "ckx_gemm_i8_tokenscale_kernel_name", "ckx_experts_gemm_i8_is_supported", "ckx_experts_gemm_i8", "ckx_experts_gemm_i8_plan",
+    "ckx_experts_gemm_i8_kernel_name", "ckx_experts_combine_is_supported", "ckx_experts_combine",
     "ckx_gemm_plan", "ckx_conv2d_fwd_plan", "ckx_set_forced_k_runs", "ckx_set_big_tile_waves",
 ]
 
@@ -203,7 +204,11 @@ def lib():
     L.ckx_gemm_i8_tokenscale_workspace_bytes.restype = i64
     L.ckx_gemm_i8_tokenscale_workspace_bytes.argtypes = [i32] * 3 + [C.c_int]
     L.ckx_gemm_i8_tokenscale_plan.argtypes = i8 + [i64] + [C.POINTER(C.c_int)] * 3
+    L.ckx_gemm_i8_tokenscale_kernel_name.restype = C.c_char_p
+    L.ckx_gemm_i8_tokenscale_kernel_name.argtypes = i8 + [i64]
     L.ckx_experts_gemm_i8_plan.argtypes = [ep, C.c_int] + [C.POINTER(C.c_int)] * 3
+    L.ckx_experts_gemm_i8_kernel_name.restype = C.c_char_p
+    L.ckx_experts_gemm_i8_kernel_name.argtypes = [ep, C.c_int]
     L.ckx_experts_gemm_i8_is_supported.argtypes = [ep]
     L.ckx_experts_gemm_i8.argtypes = [vp] * 8 + [ep, vp]
     ec = [i32] * 7 + [C.c_int]
@@ -272,6 +277,19 @@ def experts_gemm_i8_plan(desc, gathered=True):
     out = [C.c_int(0) for _ in range(3)]
     check(lib().ckx_experts_gemm_i8_plan(C.byref(desc), int(gathered), *map(C.byref, out)))
     return tuple(x.value for x in out)
+
+
+def gemm_i8_kernel(M, N, K, lda=None, ldb=None, ldc=None, gated=False, c_type=TYPE_BF16, workspace_bytes=0):
+    """The kernel that gemm_i8_plan describes, by name (ckx_gemm_i8_tokenscale_kernel_name)."""
+    gemm_i8_plan(M, N, K, lda, ldb, ldc, gated, c_type, workspace_bytes)     # (refusals, with their status)
+    return lib().ckx_gemm_i8_tokenscale_kernel_name(M, N, K, K if lda is None else lda, K if ldb is None else ldb, N if ldc is None else ldc, int(gated),
+                                                    c_type, int(workspace_bytes)).decode()
+
+
+def experts_gemm_i8_kernel(desc, gathered=True):
+    """As gemm_i8_kernel, of the experts' GEMM that an ExpertsDesc describes (ckx_experts_gemm_i8_kernel_name)."""
+    experts_gemm_i8_plan(desc, gathered)
+    return lib().ckx_experts_gemm_i8_kernel_name(C.byref(desc), int(gathered)).decode()
 
 
 def conv2d_fwd_plan(op, desc, epilogue=EPI_PASSTHROUGH, workspace_bytes=0, instance=INSTANCE_AUTO):

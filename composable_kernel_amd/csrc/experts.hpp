@@ -53,7 +53,8 @@ struct GemmI8Args
 };
 bool gemm_i8_scaled_fits(int M, int N, int gated, int experts);
 int64_t gemm_i8_scaled_workspace(int M, int N, int K, int gated);
-void gemm_i8_scaled_plan(const GemmI8Args& a, int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs);
+// the kernel's name (include/ckx.h), and what a workgroup takes
+const char* gemm_i8_scaled_plan(const GemmI8Args& a, int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs);
 hipError_t gemm_i8_scaled_launch(GemmI8Args a, int c_type, int64_t workspace_bytes, hipStream_t s);
 
 struct CombineArgs

@@ -57,6 +57,43 @@ ckx::GemmI8Args product_of(const ckx_experts_desc& d)
     return a;
 }
 
+// what the queries answer; `name` of the kernel: empty where there is nothing to do
+int plan_of_product(int32_t M, int32_t N, int32_t K, int32_t lda, int32_t ldb, int32_t ldc, int gated, int c_type, int64_t workspace_bytes, int* tile_m,
+                    int* tile_n, int* k_runs, const char*& name)
+{
+    if(!tile_m || !tile_n || !k_runs)
+        return api_fail(CKX_INVALID_VALUE, "null result pointer");
+    int st = ckx_gemm_i8_tokenscale_is_supported(M, N, K, lda, ldb, ldc, gated, c_type);
+    if(st != CKX_OK)
+        return st;
+    if(workspace_bytes < 0)
+        return api_fail(CKX_INVALID_VALUE, "negative size");
+    *tile_m = *tile_n = *k_runs = 0, name = "";
+    ckx::GemmI8Args a{};
+    a.rows_a = M, a.rows_per = 1, a.M = M, a.N = N, a.K = K, a.lda = lda, a.ldb = ldb, a.ldc = ldc, a.gated = gated;
+    if(M > 0 && N > 0)
+        name = ckx::gemm_i8_scaled_plan(a, workspace_bytes, tile_m, tile_n, k_runs);
+    return CKX_OK;
+}
+
+int plan_of_experts(const ckx_experts_desc* d, int gathered, int* tile_m, int* tile_n, int* k_runs, const char*& name)
+{
+    if(!tile_m || !tile_n || !k_runs)
+        return api_fail(CKX_INVALID_VALUE, "null result pointer");
+    int st = ckx_experts_gemm_i8_is_supported(d);
+    if(st != CKX_OK)
+        return st;
+    if(gathered != 0 && gathered != 1)
+        return api_fail(CKX_INVALID_VALUE, "gathered is 0 or 1");
+    *tile_m = *tile_n = *k_runs = 0, name = "";
+    ckx::GemmI8Args a = product_of(*d);
+    const int32_t none = 0; // (says that there are tables; the plan reads none)
+    a.offsets = &none, a.rows = gathered ? &none : nullptr;
+    if(d->num_rows > 0 && d->num_experts > 0 && d->N > 0)
+        name = ckx::gemm_i8_scaled_plan(a, 0, tile_m, tile_n, k_runs);
+    return CKX_OK;
+}
+
 } // namespace
 
 extern "C" {
@@ -230,19 +267,16 @@ int ckx_gemm_i8_tokenscale(const void* p_a, const void* p_b, void* p_c, const fl
 int ckx_gemm_i8_tokenscale_plan(int32_t M, int32_t N, int32_t K, int32_t lda, int32_t ldb, int32_t ldc, int gated, int c_type,
                                 int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs)
 {
-    if(!tile_m || !tile_n || !k_runs)
-        return api_fail(CKX_INVALID_VALUE, "null result pointer");
-    int st = ckx_gemm_i8_tokenscale_is_supported(M, N, K, lda, ldb, ldc, gated, c_type);
-    if(st != CKX_OK)
-        return st;
-    if(workspace_bytes < 0)
-        return api_fail(CKX_INVALID_VALUE, "negative size");
-    *tile_m = *tile_n = *k_runs = 0;
-    ckx::GemmI8Args a{};
-    a.rows_a = M, a.rows_per = 1, a.M = M, a.N = N, a.K = K, a.lda = lda, a.ldb = ldb, a.ldc = ldc, a.gated = gated;
-    if(M > 0 && N > 0)
-        ckx::gemm_i8_scaled_plan(a, workspace_bytes, tile_m, tile_n, k_runs);
-    return CKX_OK;
+    const char* name = nullptr;
+    return plan_of_product(M, N, K, lda, ldb, ldc, gated, c_type, workspace_bytes, tile_m, tile_n, k_runs, name);
+}
+
+const char* ckx_gemm_i8_tokenscale_kernel_name(int32_t M, int32_t N, int32_t K, int32_t lda, int32_t ldb, int32_t ldc, int gated, int c_type,
+                                               int64_t workspace_bytes)
+{
+    int m, n, runs;
+    const char* name = nullptr;
+    return plan_of_product(M, N, K, lda, ldb, ldc, gated, c_type, workspace_bytes, &m, &n, &runs, name) == CKX_OK ? name : nullptr;
 }
 
 int ckx_experts_gemm_i8_is_supported(const ckx_experts_desc* d)
@@ -289,20 +323,15 @@ int ckx_experts_gemm_i8(const void* p_a, const void* p_b, void* p_c, const float
 
 int ckx_experts_gemm_i8_plan(const ckx_experts_desc* d, int gathered, int* tile_m, int* tile_n, int* k_runs)
 {
-    if(!tile_m || !tile_n || !k_runs)
-        return api_fail(CKX_INVALID_VALUE, "null result pointer");
-    int st = ckx_experts_gemm_i8_is_supported(d);
-    if(st != CKX_OK)
-        return st;
-    if(gathered != 0 && gathered != 1)
-        return api_fail(CKX_INVALID_VALUE, "gathered is 0 or 1");
-    *tile_m = *tile_n = *k_runs = 0;
-    ckx::GemmI8Args a = product_of(*d);
-    const int32_t none = 0; // (says that there are tables; the plan reads none)
-    a.offsets = &none, a.rows = gathered ? &none : nullptr;
-    if(d->num_rows > 0 && d->num_experts > 0 && d->N > 0)
-        ckx::gemm_i8_scaled_plan(a, 0, tile_m, tile_n, k_runs);
-    return CKX_OK;
+    const char* name = nullptr;
+    return plan_of_experts(d, gathered, tile_m, tile_n, k_runs, name);
+}
+
+const char* ckx_experts_gemm_i8_kernel_name(const ckx_experts_desc* d, int gathered)
+{
+    int m, n, runs;
+    const char* name = nullptr;
+    return plan_of_experts(d, gathered, &m, &n, &runs, name) == CKX_OK ? name : nullptr;
 }
 
 int ckx_experts_combine_is_supported(int32_t num_tokens, int32_t top_k, int32_t num_rows, int32_t N, int32_t stride_y, int32_t stride_add,

@@ -769,12 +769,15 @@ int64_t gemm_i8_scaled_workspace(int M, int N, int K, int gated)
     return w.ksplit > 1 ? 4ll * M * N * (gated ? 2 : 1) * w.ksplit : 0;
 }
 
-void gemm_i8_scaled_plan(const GemmI8Args& a, int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs)
+const char* gemm_i8_scaled_plan(const GemmI8Args& a, int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs)
 {
     constexpr int m[] = {128, 16, 16, 32, 64, 128, 256, 128, 64, 16}, n[] = {128, 16, 16, 32, 128, 128, 256, 128, 128, 16};
-    const Plan w      = plan(a, workspace_bytes);
+    constexpr const char* names[] = {"any128x128",   "direct16x16", "direct16x16 eight waves", "direct32x32",        "tile64x128",
+                                     "tile128x128 two a CU", "tile256x256", "tile128x128", "tile64x128 two a CU", "any16x16"};
+    const Plan w   = plan(a, workspace_bytes);
     const bool any = w.kind == kAny || w.kind == kAnyFew, few = w.kind == kDirect1 || w.kind == kDirect8 || w.kind == kAnyFew;
     *tile_m = m[w.kind], *tile_n = n[w.kind] * (a.gated && few ? 2 : 1), *k_runs = any ? 0 : w.ksplit;
+    return names[w.kind];
 }
 
 hipError_t gemm_i8_scaled_launch(GemmI8Args a, int c_type, int64_t workspace_bytes, hipStream_t s)

@@ -630,6 +630,11 @@ int ckx_gemm_i8_tokenscale(const void* p_a, const void* p_b, void* p_c, const fl
  * 0 runs: the kernels for any K and stride, 16 x 16 and 128 x 128. Nothing to do (M or N 0): all 0. */
 int ckx_gemm_i8_tokenscale_plan(int32_t M, int32_t N, int32_t K, int32_t lda, int32_t ldb, int32_t ldc, int gated, int c_type,
                                 int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs);
+/* That kernel's name, empty where there is nothing to do, NULL where the call is refused: "direct16x16", "direct16x16 eight waves" (a long K),
+ * "direct32x32", "tile64x128", "tile128x128", either with " two a CU" (smaller workgroups, two of which share a CU), "tile256x256", "any16x16",
+ * "any128x128". For tests: several share what ckx_gemm_i8_tokenscale_plan tells. */
+const char* ckx_gemm_i8_tokenscale_kernel_name(int32_t M, int32_t N, int32_t K, int32_t lda, int32_t ldb, int32_t ldc, int gated, int c_type,
+                                               int64_t workspace_bytes);
 
 /* ---- the same product for each expert's rows -------------------------------------------------------
  * Rows p_offsets[e] ... p_offsets[e + 1] - 1 of C [num_rows, N] are expert e's (offsets ascend; they are cut to 0 ...
@@ -652,8 +657,9 @@ typedef struct ckx_experts_desc
 int ckx_experts_gemm_i8_is_supported(const ckx_experts_desc* desc);
 int ckx_experts_gemm_i8(const void* p_a, const void* p_b, void* p_c, const float* p_scale_a, const float* p_scale_b, const float* p_bias,
                         const int32_t* p_offsets, const int32_t* p_rows, const ckx_experts_desc* desc, void* stream);
-/* as ckx_gemm_i8_tokenscale_plan; gathered: whether there are p_rows */
+/* as ckx_gemm_i8_tokenscale_plan and _kernel_name; gathered: whether there are p_rows */
 int ckx_experts_gemm_i8_plan(const ckx_experts_desc* desc, int gathered, int* tile_m, int* tile_n, int* k_runs);
+const char* ckx_experts_gemm_i8_kernel_name(const ckx_experts_desc* desc, int gathered);
 
 /* ---- a token's rows, weighted and added up ---------------------------------------------------------
  *   out[t, n] = round( add[t, n] + sum_j w[t, j] * y[places[t, j], n] )       (j ascending, fp32; p_add NULL: 0)

@@ -1,0 +1,41 @@
+"""Which kernel a token-scaled int8 product is given, by name (pure host logic)."""
+import ctypes as C
+
+import pytest
+
+from composable_kernel_amd import capi
+
+NAMES = {"direct16x16": (16, 16), "direct16x16 eight waves": (16, 16), "direct32x32": (32, 32), "tile64x128": (64, 128), "tile128x128": (128, 128),
+         "tile128x128 two a CU": (128, 128), "tile256x256": (256, 256), "any16x16": (16, 16), "any128x128": (128, 128)}
+
+
+@pytest.mark.parametrize("M,N,K,gated,name", [
+    (1, 4096, 4096, False, "direct16x16"), (16, 4096, 16384, True, "direct16x16 eight waves"), (40, 4096, 4096, False, "direct32x32"),
+    (512, 4096, 4096, False, "tile64x128"), (1024, 4096, 4096, False, "tile128x128"), (2048, 4096, 128, False, "tile128x128 two a CU"),
+    (8192, 8192, 8192, False, "tile256x256"), (8, 64, 100, False, "any16x16"), (200, 64, 100, True, "any128x128")])
+def test_dense(M, N, K, gated, name):
+    assert capi.gemm_i8_kernel(M, N, K, gated=gated) == name
+    m, n, runs = capi.gemm_i8_plan(M, N, K, gated=gated)
+    assert (m, n) == (NAMES[name][0], NAMES[name][1] * (2 if gated and NAMES[name] == (16, 16) else 1))
+
+
+def experts(rows, E, N, K, gated=0):
+    return capi.ExpertsDesc(rows, rows, E, N, K, K, K, N, 1, gated, capi.TYPE_BF16, 0, N * K)
+
+
+@pytest.mark.parametrize("desc,name", [
+    (experts(8, 8, 96, 4096), "direct16x16"), (experts(300, 3, 1030, 1040), "tile64x128"), (experts(512, 64, 4096, 4096), "tile64x128 two a CU"),
+    (experts(2000, 3, 1030, 400), "tile128x128 two a CU"), (experts(16384, 8, 4096, 4096), "tile256x256"), (experts(8, 8, 64, 100), "any16x16")])
+def test_experts(desc, name):
+    assert capi.experts_gemm_i8_kernel(desc) == name
+
+
+def test_nothing_to_do_and_refusals():
+    L = capi.lib()
+    assert capi.gemm_i8_kernel(0, 8, 16) == "" and capi.experts_gemm_i8_kernel(experts(0, 8, 64, 128)) == ""
+    assert L.ckx_gemm_i8_tokenscale_kernel_name(4, 8, 256, 255, 256, 8, 0, capi.TYPE_BF16, 0) is None and "leading dimension" in capi.last_error()
+    assert L.ckx_gemm_i8_tokenscale_kernel_name(4, 8, 256, 256, 256, 8, 0, capi.TYPE_BF16, -1) is None
+    assert L.ckx_experts_gemm_i8_kernel_name(None, 0) is None
+    assert L.ckx_experts_gemm_i8_kernel_name(C.byref(experts(8, 8, 64, 128)), 2) is None
+    with pytest.raises(capi.CkxError):
+        capi.gemm_i8_kernel(4, 8, 256, lda=255)
