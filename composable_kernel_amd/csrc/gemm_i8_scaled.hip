@@ -610,6 +610,29 @@ enum
     kPair64  = 8, // 64 x 128, two workgroups a CU, for experts: the loads of one fill the other's beginning and end
     kAnyFew  = 9  // 16 x 16, any K, stride and address
 };
+// of each kind: a workgroup's rows of A and of B (16 x 16, gated: twice as many of B), its threads
+struct Shape
+{
+    const char* name;
+    int rows, cols, threads;
+};
+constexpr Shape kShapes[] = {{"any128x128", 128, 128, 256},
+                             {"direct16x16", 16, 16, 256},
+                             {"direct16x16 eight waves", 16, 16, 512},
+                             {"direct32x32", 32, 32, 512},
+                             {"tile64x128", 64, 128, 512},
+                             {"tile128x128 two a CU", 128, 128, 512},
+                             {"tile256x256", 256, 256, 256},
+                             {"tile128x128", 128, 128, 512},
+                             {"tile64x128 two a CU", 64, 128, 256},
+                             {"any16x16", 16, 16, 256}};
+int rows_of_b(const GemmI8Args& a, int kind) { return kShapes[kind].cols * (a.gated && kShapes[kind].cols == 16 ? 2 : 1); }
+// a launch has fewer than 2^32 threads (256 x 256 tiles: a workgroup a CU)
+bool launch_fits(const GemmI8Args& a, int kind, int runs)
+{
+    const int64_t wide = (int64_t)a.N * (a.gated ? 2 : 1), cols = rows_of_b(a, kind);
+    return kind == kTile256 || most_tiles_m(a, kShapes[kind].rows) * ((wide + cols - 1) / cols) * runs < (1ll << 32) / kShapes[kind].threads;
+}
 
 // whether the kernels of 16-byte vectors take a call: K, strides and addresses in whole vectors, and what a tile may read within 32-bit
 // offsets (rows that are gathered from all of A, the halves of a gated B)
@@ -629,7 +652,7 @@ bool whole_vectors(const GemmI8Args& a)
 // gated: a row each 86 direct, 96 on 64 x 128; 8 rows 151, 137 (128 x 128: 156); 64 rows 185 on 64 x 128, 179 on 256 x 256.
 struct TileCost
 {
-    int kind, rows, cols, slots;
+    int kind, slots;
     double end, step, busy, mb_per_us, uneven;
     double us(double tiles, int steps, double mb) const
     {
@@ -638,19 +661,21 @@ struct TileCost
         return 2 + std::cbrt(work * work * work + memory * memory * memory);
     }
 };
-constexpr TileCost kExpertsCosts[] = {{kDirect1, 16, 16, 2048, 2.49, 0.04, 0.70, 5.27, -0.61}, {kPair64, 64, 128, 512, 3.88, 0.31, 0.58, 5.96, 0.25},
-                                         {kTile128, 128, 128, 512, 3.33, 0.39, 0.93, 5.87, 0.21}, {kTile256, 256, 256, 256, 8.14, 0.70, 0.81, 6.13, 0.18},
-                                         {kTile64, 64, 128, 256, 3.58, 0.24, 0.26, 5.60, 0.28}};
+constexpr TileCost kExpertsCosts[] = {{kDirect1, 2048, 2.49, 0.04, 0.70, 5.27, -0.61}, {kPair64, 512, 3.88, 0.31, 0.58, 5.96, 0.25},
+                                      {kTile128, 512, 3.33, 0.39, 0.93, 5.87, 0.21}, {kTile256, 256, 8.14, 0.70, 0.81, 6.13, 0.18},
+                                      {kTile64, 256, 3.58, 0.24, 0.26, 5.60, 0.28}};
 Plan experts_plan(const GemmI8Args& a, int steps)
 {
     const double rows = (double)a.M / a.experts, used = a.experts * (1 - std::exp(-rows)), wide = (double)a.N * (a.gated ? 2 : 1);
     const double mb   = (used * wide * a.K + (double)(a.rows ? a.rows_a : a.M) * a.K + 2.0 * a.M * a.N) * 1e-6;
-    Plan best{kPair64, 1, steps};
+    Plan best{kTile256, 1, steps};
     double least = 1e300;
     for(const TileCost& c : kExpertsCosts)
     {
-        const int cols = c.cols * (c.kind == kDirect1 && a.gated ? 2 : 1);
-        double tiles   = rows > c.rows / 2 ? a.M / (double)c.rows + 0.5 * a.experts : used; // (an expert's last is half full)
+        if(!launch_fits(a, c.kind, 1))
+            continue;
+        const int high = kShapes[c.kind].rows, cols = rows_of_b(a, c.kind);
+        double tiles   = rows > high / 2 ? a.M / (double)high + 0.5 * a.experts : used; // (an expert's last is half full)
         tiles          = (tiles > used ? tiles : used);
         const double us = c.us((tiles < a.M ? tiles : a.M) * std::ceil(wide / cols), steps, mb);
         if(us < least)
@@ -681,12 +706,12 @@ Plan plan(const GemmI8Args& a, int64_t workspace_bytes)
     Plan best{kTile256, 1, steps};
     double us    = 2 + rounds(big) * (2 + steps * (1.05 + 0.42 * share * share));
     auto compare = [&](double t, const Plan& p) {
-        if(t < us)
+        if(t < us && launch_fits(a, p.kind, p.ksplit))
             us = t, best = p;
     };
     if(a.M <= 128)
     {
-        constexpr TileCost direct{kDirect1, 16, 16, 2048, 1.27, 0.08, 0.57, 5.3, 0.22};
+        constexpr TileCost direct{kDirect1, 2048, 1.27, 0.08, 0.57, 5.3, 0.22};
         compare(direct.us((double)tiles(16, a.gated ? 32 : 16), steps, ((double)wide * a.K + (double)a.M * a.K + 2.0 * a.M * a.N) * 1e-6),
                 Plan{a.K > 8192 ? kDirect8 : kDirect1, 1, steps});
     }
@@ -749,7 +774,7 @@ hipError_t launch_form(GemmI8Args& a, int64_t workspace_bytes, hipStream_t s)
 } // namespace
 
 // a launch has fewer than 2^32 threads, 512 a workgroup at most: one for 64 x 128 outputs (experts: 128 x 128), and where the rows are
-// few (experts: under 256 each, which the plan's borders stay below) for 16 x 16
+// few for 16 x 16. What is left then has a kernel always; plan() takes none whose launch does not fit (a short N has many tiles of few columns)
 bool gemm_i8_scaled_fits(int M, int N, int gated, int experts)
 {
     GemmI8Args a{};
@@ -771,13 +796,9 @@ int64_t gemm_i8_scaled_workspace(int M, int N, int K, int gated)
 
 const char* gemm_i8_scaled_plan(const GemmI8Args& a, int64_t workspace_bytes, int* tile_m, int* tile_n, int* k_runs)
 {
-    constexpr int m[] = {128, 16, 16, 32, 64, 128, 256, 128, 64, 16}, n[] = {128, 16, 16, 32, 128, 128, 256, 128, 128, 16};
-    constexpr const char* names[] = {"any128x128",   "direct16x16", "direct16x16 eight waves", "direct32x32",        "tile64x128",
-                                     "tile128x128 two a CU", "tile256x256", "tile128x128", "tile64x128 two a CU", "any16x16"};
-    const Plan w   = plan(a, workspace_bytes);
-    const bool any = w.kind == kAny || w.kind == kAnyFew, few = w.kind == kDirect1 || w.kind == kDirect8 || w.kind == kAnyFew;
-    *tile_m = m[w.kind], *tile_n = n[w.kind] * (a.gated && few ? 2 : 1), *k_runs = any ? 0 : w.ksplit;
-    return names[w.kind];
+    const Plan w = plan(a, workspace_bytes);
+    *tile_m = kShapes[w.kind].rows, *tile_n = rows_of_b(a, w.kind), *k_runs = w.kind == kAny || w.kind == kAnyFew ? 0 : w.ksplit;
+    return kShapes[w.kind].name;
 }
 
 hipError_t gemm_i8_scaled_launch(GemmI8Args a, int c_type, int64_t workspace_bytes, hipStream_t s)

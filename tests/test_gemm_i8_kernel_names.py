@@ -1,5 +1,6 @@
 """Which kernel a token-scaled int8 product is given, by name (pure host logic)."""
 import ctypes as C
+import random
 
 import pytest
 
@@ -39,3 +40,35 @@ def test_nothing_to_do_and_refusals():
     assert L.ckx_experts_gemm_i8_kernel_name(C.byref(experts(8, 8, 64, 128)), 2) is None
     with pytest.raises(capi.CkxError):
         capi.gemm_i8_kernel(4, 8, 256, lda=255)
+
+
+THREADS = {"any128x128": 256, "direct16x16": 256, "direct16x16 eight waves": 512, "direct32x32": 512, "tile64x128": 512, "tile128x128 two a CU": 512,
+           "tile128x128": 512, "tile64x128 two a CU": 256, "any16x16": 256}
+
+
+def test_launches_of_the_largest_problems():
+    """Whatever problem is supported, the launch of its kernel has fewer than 2^32 threads."""
+    rng, some = random.Random(5), 0
+    for _ in range(30000):
+        gated, E = rng.random() < 0.5, int(2 ** rng.uniform(0, 10)) if rng.random() < 0.6 else 0
+        most = 24 if E else 31
+        M = min(2 ** most, int(2 ** rng.uniform(most - 12, most + 0.01)))
+        if rng.random() < 0.3:
+            M = int(2 ** rng.uniform(0, most - 12))
+        N = min(2 ** 30 - 1, int(2 ** min(30.0, rng.uniform(0, 40 - M.bit_length()))))
+        K = min(131071, int(2 ** rng.uniform(0, 17))) // 16 * 16 + (1 if rng.random() < 0.1 else 0)
+        if E:
+            desc = experts(M, E, N, K, int(gated))
+            if capi.lib().ckx_experts_gemm_i8_is_supported(C.byref(desc)) != capi.OK:
+                continue
+            name, (m, n, runs) = capi.experts_gemm_i8_kernel(desc, False), capi.experts_gemm_i8_plan(desc, False)
+        else:
+            ws = 2 ** 62 if rng.random() < 0.5 else 0
+            if M == 2 ** 31 or capi.lib().ckx_gemm_i8_tokenscale_is_supported(M, N, K, K, K, N, int(gated), capi.TYPE_BF16) != capi.OK:
+                continue
+            name, (m, n, runs) = capi.gemm_i8_kernel(M, N, K, gated=gated, workspace_bytes=ws), capi.gemm_i8_plan(M, N, K, gated=gated, workspace_bytes=ws)
+        rows = M // m + min(E, M) if E else -(-M // m)
+        threads = rows * -(-N * (1 + gated) // n) * max(1, runs) * THREADS.get(name, 0)
+        assert threads < 2 ** 32, (E, M, N, K, gated, name, runs)
+        some += threads > 2 ** 30
+    assert some > 100
