@@ -587,9 +587,9 @@ hipError_t launch_direct(GemmI8Args& a, hipStream_t s)
 //   256 x 256, four waves    1.05, all CUs busy 1.47         4096: 51.6 (128 x 128 66.3), 4096 x 11008: 145 (213)
 // and about 4 us around the steps, which a second round pays again where a CU holds one workgroup. Runs cost 4 us more and their sums' way to the workspace
 // and back.
-// Up to 16 rows the direct kernel of one row tile, 11008 x 4096: 1 row 10.4, 16 rows 13.6 (64 x 128 tiles in two runs 14.7); 8 waves where K is
+// Up to 16 rows the direct kernel of one row tile, 11008 x 4096: 1 row 9.7 to 10.2, 16 rows 13.7 to 14.0 (64 x 128 tiles in two runs 14.7); 8 waves where K is
 // long (4096 x 11008: 9.9 where four take 10.7). To 64 rows the direct kernel of two row tiles where its workgroups find a CU each, 4096 x 4096
-// 10.6 us for 32 rows (11.8 in the best runs of tiles), 11008 x 4096 18 (15.6). To 128 rows the direct kernel of one row tile where N is short (its
+// 10.5 us for 32 rows (11.8 in the best runs of tiles), 11008 x 4096 18 (13.5). To 128 rows the direct kernel of one row tile where N is short (its
 // cost: TileCost): 102 rows of 343 x 2176 gated 6.4 us (six runs of 64 x 128 tiles 18.4), 80 of 640 x 6544 7.1 (13.7).
 // Experts: experts_plan, by the rows that experts have on average, since the host knows no more.
 struct Plan
@@ -649,7 +649,9 @@ bool whole_vectors(const GemmI8Args& a)
 // (slots at a time), each with what a tile's beginning and end take and its K tiles, which take longer the more slots are in use. Fitted to 310 products
 // of 4 to 128 experts, 0.1 to 4800 rows each, K 256 to 4096: on average 2.8 % from the best of the five, where borders by rows and K alone were
 // 18 % and up to 3.3 times (519 rows of 512 x 1040 in each of 4 experts: 10.4 us on 64 x 128 tiles, 23.4 on 256 x 256). Examples, 64 experts of 2816 x 4096
-// gated: a row each 86 direct, 96 on 64 x 128; 8 rows 151, 137 (128 x 128: 156); 64 rows 185 on 64 x 128, 179 on 256 x 256.
+// gated: a row each 86 direct, 96 on 64 x 128; 8 rows 151, 137 (128 x 128: 156); 64 rows 185 on 64 x 128, 179 on 256 x 256. Where a call has fewer rows than M (a
+// rank's slice of the offsets, a padded step) the choice is that of M: 8 of 64 such experts, 512 tokens of eight rows each 44 us, 31.5 with the slice's 533 rows alone; 64 tokens
+// 21.9, 23.6.
 struct TileCost
 {
     int kind, slots;

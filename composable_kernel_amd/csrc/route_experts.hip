@@ -348,7 +348,8 @@ __device__ __forceinline__ V group_value(const RouteArgs& p, const V (&v)[EPL], 
 // WIDE and ALL as above; `live`: of the lane's row of lanes. Scores in fp32 find the token's experts; those, one a lane, are computed in
 // 64 bits (their weights need that anyway), one more than asked for, and put in order by them; the last that counts has to lie further above
 // the next expert, and the groups that stay above the others, than the fp32 scores may be off. Where one does not, the row is `in_doubt`,
-// nothing is written, and the wave takes the token by itself (route_token, 4.5 us at the end of a launch).
+// nothing is written, and the wave takes the token by itself (route_token): one 4.5 us at the end of a launch; all of 16384 tokens of 256 experts (a peaked softmax with
+// biases of zero) 51 us, none 28.
 // How far: sigmoid, with t = exp(-x) off by (|x| + 3) 2^-24 of itself (x log2 e rounded, the power of two, its rounding) and s (1 - s) |x|
 // under 0.23, s is off by less than 4 * 2^-24; softmax, p |x - max| under 0.37, and the sum of at most 16 + 4 terms in a row off by 20 *
 // 2^-24: 27 * 2^-24; and half a step each for the biases' and the groups' sums.

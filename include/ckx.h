@@ -642,7 +642,8 @@ const char* ckx_gemm_i8_tokenscale_kernel_name(int32_t M, int32_t N, int32_t K, 
  * and biases of expert e: B [num_experts, N, K] (gated: 2 N), experts batch_stride_b elements apart, sb and bias
  * [num_experts, N] (gated: 2 N). A row number outside A counts as a row of zeros with scale 0. Rows of C that belong to no
  * expert are left alone. With the tables of ckx_route_experts, p_rows and rows_per = top_k take each pair's token; C's rows
- * then stand in the order of p_rows. Up to 1024 experts, 2^24 rows; otherwise as ckx_gemm_i8_tokenscale. */
+ * then stand in the order of p_rows. The kernel is chosen for num_rows / num_experts rows an expert, all the host knows: num_rows should be near
+ * the rows that there are. Up to 1024 experts, 2^24 rows; otherwise as ckx_gemm_i8_tokenscale. */
 typedef struct ckx_experts_desc
 {
     int32_t num_rows, num_rows_a, num_experts;
